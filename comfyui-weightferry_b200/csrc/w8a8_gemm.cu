@@ -26,13 +26,10 @@
 // memory and returns. Every TMA load here is a plain per-CTA load of this GPU's own memory.
 
 #include "wf_common.cuh"
-
-#include <cuda.h>
+#include "wf_tcgen05.cuh"
 
 #include <atomic>
 #include <cstdlib>
-#include <mutex>
-#include <utility>
 
 namespace wf {
 namespace {
@@ -46,7 +43,6 @@ constexpr int EPI_THREADS = 256;
 constexpr int TMEM_COLS = 512;
 constexpr int OUT_BYTES = 8 * 2 * 2048;  // per epilogue warp two 32 x 32 bf16 output chunks
 constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + OUT_BYTES + 1024 + 256;  // ring, output chunks, slack, barriers
-constexpr uint64_t kWaitLimitNs = 2000000000ull;
 
 // instruction descriptor of kind::i8: D int32 (bits 4-5 = 2), A and B signed int8 (bits 7-9, 10-12 = 1), both
 // K-major, N >> 3 at bits 17-22, M >> 4 at bits 24-28
@@ -57,52 +53,6 @@ __device__ int g_gemm_status;  // 0 ok; 1 producer wait expired; 2 MMA wait expi
 // runs out and the abort path is exercised (wf_w8a8_gemm_set_wait_limit). The drain waits of the abort path keep
 // kWaitLimitNs.
 __device__ unsigned long long g_wait_limit_ns = kWaitLimitNs;
-
-__device__ __forceinline__ uint32_t smem_u32(const void *p) {
-    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-
-__device__ __forceinline__ uint64_t global_ns() {
-    uint64_t t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
-
-__device__ __forceinline__ void mbar_init(uint32_t a, uint32_t count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(a), "r"(count) : "memory");
-}
-__device__ __forceinline__ void mbar_expect_tx(uint32_t a, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(a), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void mbar_complete_tx(uint32_t a, uint32_t bytes) {  // bytes that will never arrive
-    asm volatile("mbarrier.complete_tx.shared::cta.b64 [%0], %1;" ::"r"(a), "r"(bytes) : "memory");
-}
-// bounded wait (kWaitLimitNs) for the phase of the given parity, for the drains of the abort path
-__device__ __forceinline__ void mbar_drain_wait(uint32_t a, uint32_t parity);
-__device__ __forceinline__ void mbar_arrive(uint32_t a) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(a) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {  // an arrive on a barrier anywhere in the cluster
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
-__device__ __forceinline__ bool mbar_try(uint32_t a, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(a), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-
-__device__ __forceinline__ void mbar_drain_wait(uint32_t a, uint32_t parity) {
-    if (mbar_try(a, parity)) return;  // the usual case; a read of the global timer costs ~0.2 us
-    const uint64_t t0 = global_ns();
-    while (!mbar_try(a, parity) && global_ns() - t0 < kWaitLimitNs) {
-    }
-}
 
 // Wait for the phase of the given parity, at most g_wait_limit_ns; gives up early when another role aborted.
 __device__ __forceinline__ bool mbar_wait(uint32_t a, uint32_t parity, volatile int *abort_flag, int code) {
@@ -125,24 +75,6 @@ __device__ __forceinline__ bool mbar_wait(uint32_t a, uint32_t parity, volatile 
     }
 }
 
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap *map, int c0, int c1, uint32_t mbar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(mbar)
-        : "memory");
-}
-
-// shared-memory matrix descriptor: K-major, 128-byte swizzle, rows 128 B apart, 8-row groups 1024 B apart
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr) {
-    uint64_t d = 0;
-    d |= static_cast<uint64_t>((addr >> 4) & 0x3FFFu);        // start address
-    d |= static_cast<uint64_t>(1u) << 16;                      // leading byte offset (16 B; unused when swizzled)
-    d |= static_cast<uint64_t>(1024u >> 4) << 32;              // stride byte offset
-    d |= static_cast<uint64_t>(1u) << 46;                      // descriptor version (Blackwell)
-    d |= static_cast<uint64_t>(2u) << 61;                      // SWIZZLE_128B
-    return d;
-}
-
 __device__ __forceinline__ void mma_i8(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t accumulate) {
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
@@ -150,78 +82,6 @@ __device__ __forceinline__ void mma_i8(uint32_t d_tmem, uint64_t a, uint64_t b, 
         "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
         ::"r"(d_tmem), "l"(a), "l"(b), "r"(kIdesc), "r"(accumulate)
         : "memory");
-}
-
-__device__ __forceinline__ void mma_commit(uint32_t mbar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(mbar)
-                 : "memory");
-}
-
-// Programmatic dependent launch: the kernel is launched while the previous kernel of the stream (the quantiser that
-// writes xq / xs) may still run, so its set-up (barriers, tensor memory, cluster sync) overlaps that kernel's tail;
-// every thread waits here for the previous grid's completion and memory before it touches global memory. Without a
-// programmatic launch this returns at once.
-__device__ __forceinline__ void wait_prior_grid() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
-__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-// tcgen05.ld of 32 consecutive columns of this thread's lane; the registers are valid only after tmem_wait32 on
-// the same array (the wait names them as operands, so no use can be scheduled before it)
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr)
-        : "memory");
-}
-
-__device__ __forceinline__ void tmem_wait32(uint32_t (&r)[32]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
-                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
-                   "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]),
-                   "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]),
-                   "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
-                 :
-                 : "memory");
-}
-
-__device__ __forceinline__ void tma_store_2d(const CUtensorMap *map, uint32_t src, int c0, int c1) {
-    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];"
-                 ::"l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(src)
-                 : "memory");
-}
-__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void bulk_wait_read1() { asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory"); }
-// every output store of this thread has finished reading its shared-memory source (the stores themselves complete
-// with the grid, before any later kernel of the stream -- or a programmatic dependent past griddepcontrol.wait --
-// can read the output)
-__device__ __forceinline__ void bulk_wait_read_all() {
-    asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-}
-__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-
-// Output tile `tile` -> (tile row, tile column). group_m == 0: tiles walk down the M direction first (column by
-// column); group_m > 0: bands of group_m tile rows, each walked column by column, so that the tiles in flight at once
-// share fewer operand rows and columns.
-__device__ __forceinline__ void tile_coords(int tile, int tiles_m, int tiles_n, int group_m, int &mi, int &ni) {
-    if (group_m <= 0) {
-        mi = tile % tiles_m;
-        ni = tile / tiles_m;
-        return;
-    }
-    const int band = tile / (group_m * tiles_n);
-    const int first = band * group_m;
-    const int rows = min(tiles_m - first, group_m);
-    const int r = tile - band * group_m * tiles_n;
-    mi = first + r % rows;
-    ni = r / rows;
 }
 
 // w_s of 32 output columns starting at col0 (a multiple of 32; N is a multiple of 8, so each group of 8 columns is
@@ -545,29 +405,8 @@ constexpr int B2_STAGE = 128 * BK;          // 16 KB: this CTA's 128 rows of wq
 constexpr int STAGE2 = A2_STAGE + B2_STAGE; // 32 KB
 constexpr int SMEM2_BYTES = S2 * STAGE2 + OUT_BYTES + 1024 + 256;
 constexpr uint32_t kIdesc2 = (2u << 4) | (1u << 7) | (1u << 10) | ((256u >> 3) << 17) | ((256u >> 4) << 24);
-constexpr uint32_t kPeerBitMask = 0xFEFFFFFFu;  // clears the CTA-rank bit of a cluster shared address
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
-    uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-    return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap *map, int c0, int c1,
-                                                 uint32_t leader_mbar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
-        "[%0], [%1, {%2, %3}], [%4];"
-        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(leader_mbar)
-        : "memory");
-}
+
 __device__ __forceinline__ void mma_i8_pair(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t accumulate) {
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
@@ -576,11 +415,6 @@ __device__ __forceinline__ void mma_i8_pair(uint32_t d_tmem, uint64_t a, uint64_
         ::"r"(d_tmem), "l"(a), "l"(b), "r"(kIdesc2), "r"(accumulate)
         : "memory");
 }
-__device__ __forceinline__ void mma_commit_pair(uint32_t cluster_mbar) {
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(cluster_mbar)
-                 : "memory");
-}
-
 template <bool RES>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 w8a8_gemm_2sm_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b,
@@ -761,46 +595,6 @@ w8a8_gemm_2sm_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_con
 }
 
 // ---------------------------------------------------------------------------------------------- host
-using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
-                                 const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
-                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiled encoder() {
-    static EncodeTiled fn = nullptr;
-    static std::once_flag once;
-    std::call_once(once, [] {
-        void *p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<EncodeTiled>(p);
-    });
-    return fn;
-}
-
-// WEIGHTFERRY_PDL=0 launches the GEMM as a plain kernel instead of a programmatic dependent
-bool use_pdl() {
-    static const bool pdl = env_digit("WEIGHTFERRY_PDL", 1) != 0;
-    return pdl;
-}
-
-// a kernel launch as a programmatic dependent of the previous one in the stream (WEIGHTFERRY_PDL=0: a plain launch)
-template <typename... KArgs, typename... Args>
-cudaError_t launch_dependent(void (*kern)(KArgs...), int grid, int threads, size_t smem, cudaStream_t stream,
-                             Args &&...args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(grid), 1, 1);
-    cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = use_pdl() ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
-}
-
 // WEIGHTFERRY_W8A8_GROUP_M: tile rows per band of the tile order (0 or unset: down M first)
 int tile_group_m() {
     static const int g = [] {
