@@ -66,6 +66,32 @@ SIGNATURES = {
     "wf_gated_residual": (ctypes.c_int, [ctypes.c_void_p] * 4 + [ctypes.c_int64] * 3 + [ctypes.c_void_p]),
     "wf_hbm_probe": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]),
     "wf_w8a8_linear_noalloc": (ctypes.c_int, [ctypes.c_void_p] * 4 + [ctypes.c_int64] * 3 + [ctypes.c_void_p]),
+    "wf_linear": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
+                                 ctypes.c_int, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64,
+                                 ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int]
+                  + [ctypes.c_int64] * 3 + [ctypes.c_int, ctypes.c_void_p]),
+    "wf_linear_backward_act_workspace": (ctypes.c_int64, [ctypes.c_int64] * 3),
+    "wf_linear_backward_act": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64,
+                                              ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_int64,
+                                              ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p,
+                                              ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.c_void_p,
+                                              ctypes.c_int64, ctypes.c_void_p]),
+    "wf_linear_backward_input": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64] * 3 + [ctypes.c_int64] * 3
+                                 + [ctypes.c_int, ctypes.c_void_p]),
+    "wf_linear_backward_weight": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64] * 3 + [ctypes.c_int64] * 3
+                                  + [ctypes.c_int, ctypes.c_void_p]),
+    "wf_linear_status": (ctypes.c_int, [ctypes.POINTER(ctypes.c_int)]),
+    "wf_copy_rows16": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p] + [ctypes.c_int64] * 3
+                       + [ctypes.c_void_p]),
+    "wf_layer_norm": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int,
+                                     ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p]
+                      + [ctypes.c_int64] * 3 + [ctypes.c_float, ctypes.c_int, ctypes.c_void_p]),
+    "wf_layer_norm_backward_workspace": (ctypes.c_int64, [ctypes.c_int64] * 3),
+    "wf_layer_norm_backward": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64,
+                                              ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p,
+                                              ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p]
+                               + [ctypes.c_int64] * 3 + [ctypes.c_int, ctypes.c_void_p, ctypes.c_int64,
+                                                         ctypes.c_void_p]),
 }
 
 

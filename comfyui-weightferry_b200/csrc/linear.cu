@@ -1,0 +1,489 @@
+// The dense linear layer of 16-bit weights for sm_100a: matrix products on tcgen05 tensor cores with the bias, the
+// activation and the gated residual in the epilogue, and the two products of its backward pass.
+//
+//   forward    z = x W^T + b,  y = r + g[row / rows_per_group] * act(z)        x [m, k], W [n, k]
+//   backward   dx = dz W,  dW = dz^T x                                          dz [m, n] (linear_grad.cu)
+//
+// All three are D[i, j] = sum_c A[i, c] B[j, c] with A and B read as they lie in memory: an operand whose contraction
+// index c is the contiguous one ("c-major": x and W of the forward pass, dz of dx) or whose row index is ("row-major":
+// W of dx, dz and x of dW). The tensor core takes both from shared memory, so nothing is transposed first. Products are
+// summed in float32 in tensor memory; the epilogue works in float32 and rounds once, to the output's type.
+
+#include "wf_act.cuh"
+#include "wf_rows.cuh"
+#include "wf_tcgen05.cuh"
+
+#include <algorithm>
+#include <atomic>
+
+namespace wf {
+namespace {
+
+constexpr int BC = 64;  // contraction values of a stage: 128 bytes of 16-bit values, one swizzle row
+
+__device__ int g_linear_status;  // 0 ok; 1 producer wait expired; 2 MMA wait expired; 3 epilogue wait expired
+
+// Wait for the phase of the given parity, at most kWaitLimitNs; gives up early when another role aborted.
+__device__ __forceinline__ bool pipe_wait(uint32_t a, uint32_t parity, volatile int *abort_flag, int code) {
+    if (mbar_try(a, parity)) return true;
+    const uint64_t t0 = global_ns();
+    while (true) {
+#pragma unroll 1
+        for (int i = 0; i < 32; ++i)
+            if (mbar_try(a, parity)) return true;
+        if (*abort_flag) return false;
+        if (global_ns() - t0 > kWaitLimitNs) {
+            *abort_flag = 1;
+            atomicCAS(&g_linear_status, 0, code);
+            return false;
+        }
+    }
+}
+
+// Shared-memory matrix descriptor of a row-major operand: 64 rows (128 bytes) of one contraction index side by side,
+// 128-byte swizzle; 8 contraction indexes 1024 B apart, blocks of 64 rows `block` B apart.
+__device__ __forceinline__ uint64_t smem_desc_rows(uint32_t addr, uint32_t block) {
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((addr >> 4) & 0x3FFFu);
+    d |= static_cast<uint64_t>(block >> 4) << 16;   // leading byte offset: from 64 rows to the next 64
+    d |= static_cast<uint64_t>(1024u >> 4) << 32;   // stride byte offset: from 8 contraction indexes to the next 8
+    d |= static_cast<uint64_t>(1u) << 46;
+    d |= static_cast<uint64_t>(2u) << 61;
+    return d;
+}
+
+// descriptor of the operand at addr for contraction indexes 16 step .. 16 step + 15 of a stage
+template <bool ROWS>
+__device__ __forceinline__ uint64_t operand_desc(uint32_t addr, int step) {
+    return ROWS ? smem_desc_rows(addr + 2048u * step, BC * 128u) : smem_desc(addr + 32u * step);
+}
+
+// instruction descriptor of kind::f16: D float32 (bits 4-5 = 1), A and B f16 (0) or bf16 (1) at bits 7-9 and 10-12,
+// row-major A / B at bits 15 / 16, N >> 3 at bits 17-22, M >> 4 at bits 24-28
+constexpr uint32_t f16_idesc(bool bf16, bool a_rows, bool b_rows, int m, int n) {
+    return (1u << 4) | (static_cast<uint32_t>(bf16) << 7) | (static_cast<uint32_t>(bf16) << 10) |
+           (static_cast<uint32_t>(a_rows) << 15) | (static_cast<uint32_t>(b_rows) << 16) |
+           (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+}
+
+__device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// tcgen05.ld of 16 consecutive columns of this thread's lane
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+
+// What the epilogue does with z = D + bias: saved (for the backward pass) as keep says, then out = r + g * act(z).
+enum { KEEP_NONE = 0, KEEP_F16 = 1, KEEP_F32 = 2, KEEP_SAME = 3 };
+struct Epilogue {
+    const void *bias;   // [n] or null
+    const void *gate;   // [groups, n] or null
+    const void *resid;  // [m, ld_resid] or null
+    void *out;          // [m, ld_out]
+    void *kept;         // [m, ld_kept] or null
+    int64_t ld_resid, ld_out, ld_kept, rows_per_group;
+    int act, keep;
+    bool vec;  // every pointer 8-byte aligned and every row pitch (n too, where it is one) a multiple of 4 values
+};
+
+// float32 -> f16, clamped to f16's range: the kept z is read by the slopes alone, which are constant out there, and
+// f16's 11 bits keep a bf16 layer's gradients as exact as their own rounding
+__device__ __forceinline__ __half to_half_sat(float v) {
+    return __float2half_rn(v != v ? v : fminf(fmaxf(v, -65504.f), 65504.f));
+}
+
+template <int ACT>
+__device__ __forceinline__ void act4(float (&v)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = act<ACT>(v[i]);
+}
+__device__ __forceinline__ void apply_act4(int kind, float (&v)[4]) {
+    switch (kind) {
+        case WF_ACT_RELU: act4<WF_ACT_RELU>(v); break;
+        case WF_ACT_SILU: act4<WF_ACT_SILU>(v); break;
+        case WF_ACT_GELU: act4<WF_ACT_GELU>(v); break;
+        case WF_ACT_GELU_TANH: act4<WF_ACT_GELU_TANH>(v); break;
+        default: break;
+    }
+}
+
+// four neighbouring values of a row, those at and past n as 0
+template <int T>
+__device__ __forceinline__ void load4(float (&v)[4], const void *row, int col, int n, bool vec) {
+    if (vec && col + 4 <= n) {
+        const uint2 q = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(row) + col);
+        const float2 a = unpack2<T>(q.x), b = unpack2<T>(q.y);
+        v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = col + i < n ? load1<T>(row, col + i) : 0.f;
+    }
+}
+template <int T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if constexpr (T == WF_BF16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    } else {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+}
+template <int T>
+__device__ __forceinline__ void store4(void *row, int col, int n, bool vec, const float (&v)[4]) {
+    if (vec && col + 4 <= n) {
+        *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(row) + col) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (col + i < n) store1<T>(row, col + i, v[i]);
+    }
+}
+
+// the epilogue of four neighbouring outputs of one row
+template <int T>
+__device__ __forceinline__ void finish4(const Epilogue &e, float (&v)[4], int row, int col, int n) {
+    if (e.bias != nullptr) {
+        float b[4];
+        load4<T>(b, e.bias, col, n, e.vec);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] += b[i];
+    }
+    if (e.keep != KEEP_NONE) {
+        if (e.keep == KEEP_F16) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (col + i < n) static_cast<__half *>(e.kept)[row * e.ld_kept + col + i] = to_half_sat(v[i]);
+        } else if (e.keep == KEEP_F32) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (col + i < n) static_cast<float *>(e.kept)[row * e.ld_kept + col + i] = v[i];
+        } else {
+            store4<T>(row_of<T>(e.kept, row, e.ld_kept), col, n, e.vec, v);
+        }
+    }
+    apply_act4(e.act, v);
+    if (e.gate != nullptr) {
+        float g[4];
+        load4<T>(g, row_of<T>(e.gate, row / e.rows_per_group, n), col, n, e.vec);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] *= g[i];
+    }
+    if (e.resid != nullptr) {
+        float r[4];
+        load4<T>(r, row_of<T>(e.resid, row, e.ld_resid), col, n, e.vec);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] += r[i];
+    }
+    store4<T>(row_of<T>(e.out, row, e.ld_out), col, n, e.vec, v);
+}
+
+// ------------------------------------------------------------------------------------------------ few-rows kernel
+// One 128-column x NT-row tile of D for each cluster of S CTAs. The columns j (the layer's output features) take the
+// tensor core's 128 lanes and the few rows i its N, so a product of a handful of rows reads the weight once and wastes
+// no more than NT - m rows. The CTAs of a cluster share the contraction, and their float32 parts are added through
+// distributed shared memory in rank order (the same bits every time): with few tiles every SM still reads weights. Warp
+// 4 loads tiles by TMA into a ring, warp 5 issues the MMAs, warps 0-3 move the accumulator to shared memory, and all
+// threads finish the CTA's share of the rows.
+constexpr int TILE_J = 128;
+constexpr int TILE_THREADS = 192;
+template <int NT>
+struct TileShape {
+    static constexpr int p_bytes = TILE_J * BC * 2, q_bytes = NT * BC * 2, stage = p_bytes + q_bytes;
+    static constexpr int stages = NT <= 32 ? 5 : NT <= 64 ? 4 : 3;  // about 100 KB: two CTAs an SM
+    static constexpr int smem = stages * stage + 1024 + 128;
+    static constexpr int tmem_cols = NT < 32 ? 32 : NT;
+    static_assert(NT * TILE_J * 4 <= stages * stage, "the float32 tile reuses the ring");
+};
+
+template <bool P_ROWS, bool Q_ROWS, int NT, int T>
+__global__ void __launch_bounds__(TILE_THREADS)
+linear_tile_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
+                   const __grid_constant__ Epilogue epi, int m, int n, int c, int tiles_q, int split) {
+    using S = TileShape<NT>;
+    constexpr uint32_t idesc = f16_idesc(T == WF_BF16, P_ROWS, Q_ROWS, TILE_J, NT);
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t *bars = reinterpret_cast<uint64_t *>(ring + S::stages * S::stage);
+    __shared__ uint32_t s_tmem_base;
+    __shared__ int s_abort;
+    const uint32_t ring0 = smem_u32(ring), full0 = smem_u32(bars), empty0 = full0 + 8 * S::stages,
+                   done = empty0 + 8 * S::stages;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = split > 1 ? static_cast<int>(cluster_rank()) : 0;
+    const int tile = blockIdx.x / split;
+    const int j0 = tile / tiles_q * TILE_J, i0 = tile % tiles_q * NT;
+    const int steps = (c + BC - 1) / BC;
+    const int c_lo = static_cast<int>(static_cast<int64_t>(steps) * rank / split);
+    const int c_hi = static_cast<int>(static_cast<int64_t>(steps) * (rank + 1) / split);
+
+    if (threadIdx.x == 0) {
+        s_abort = 0;
+        for (int s = 0; s < S::stages; ++s) {
+            mbar_init(full0 + 8 * s, 1);
+            mbar_init(empty0 + 8 * s, 1);
+        }
+        mbar_init(done, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fence_async_smem();
+    }
+    if (warp == 5) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                     ::"r"(smem_u32(&s_tmem_base)), "r"(S::tmem_cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = s_tmem_base;
+    wait_prior_grid();
+    volatile int *abort_flag = &s_abort;
+
+    if (warp == 4) {
+        if (lane == 0) {
+            int stage = 0;
+            uint32_t phase = 0;
+            int issued = 0;
+            for (int s = c_lo; s < c_hi; ++s, ++issued) {
+                if (!pipe_wait(empty0 + 8 * stage, phase ^ 1u, abort_flag, 1)) break;
+                const uint32_t bar = full0 + 8 * stage, p = ring0 + stage * S::stage, q = p + S::p_bytes;
+                mbar_expect_tx(bar, S::stage);
+                if constexpr (P_ROWS) {
+                    for (int h = 0; h < TILE_J / 64; ++h) tma_load_2d(p + h * BC * 128, &map_p, j0 + 64 * h, s * BC, bar);
+                } else {
+                    tma_load_2d(p, &map_p, s * BC, j0, bar);
+                }
+                if constexpr (Q_ROWS) {
+                    for (int h = 0; h < NT / 64; ++h) tma_load_2d(q + h * BC * 128, &map_q, i0 + 64 * h, s * BC, bar);
+                } else {
+                    tma_load_2d(q, &map_q, s * BC, i0, bar);
+                }
+                if (++stage == S::stages) stage = 0, phase ^= 1u;
+            }
+            // every load has landed before the CTA leaves or reuses the ring: only the last use of a stage can be
+            // outstanding, and only after an abort
+            for (int s = 0; s < S::stages && s < issued; ++s)
+                mbar_drain_wait(full0 + 8 * s, static_cast<uint32_t>((issued - 1 - s) / S::stages) & 1u);
+        }
+        __syncwarp();
+    } else if (warp == 5) {
+        if (lane == 0) {
+            int stage = 0;
+            uint32_t phase = 0;
+            for (int s = c_lo; s < c_hi; ++s) {
+                if (!pipe_wait(full0 + 8 * stage, phase, abort_flag, 2)) break;
+                fence_after();
+                const uint32_t p = ring0 + stage * S::stage, q = p + S::p_bytes;
+#pragma unroll
+                for (int k = 0; k < BC / 16; ++k)
+                    mma_f16(tmem, operand_desc<P_ROWS>(p, k), operand_desc<Q_ROWS>(q, k), idesc, s > c_lo || k > 0);
+                mma_commit(empty0 + 8 * stage);
+                if (++stage == S::stages) stage = 0, phase ^= 1u;
+            }
+            mma_commit(done);  // the accumulator is complete
+            mbar_drain_wait(done, 0);
+        }
+        __syncwarp();
+    } else {
+        // lane w * 32 + l of tensor memory is column j0 + 32 w + l; its NT rows go to part[row][column]
+        const bool ok = __all_sync(0xFFFFFFFFu, pipe_wait(done, 0, abort_flag, 3) && !*abort_flag);
+        fence_after();
+        if (ok) {
+            float *part = reinterpret_cast<float *>(ring);
+#pragma unroll
+            for (int t = 0; t < NT; t += 16) {
+                uint32_t r[16];
+                tmem_ld16(tmem + (static_cast<uint32_t>(warp * 32) << 16) + t, r);
+#pragma unroll
+                for (int u = 0; u < 16; ++u) part[(t + u) * TILE_J + warp * 32 + lane] = __uint_as_float(r[u]);
+            }
+        }
+    }
+    fence_before();
+    __syncthreads();
+    if (split > 1) cluster_sync();
+    fence_after();
+    if (warp == 5)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::tmem_cols) : "memory");
+    // this CTA finishes rows t_lo .. t_hi of the tile, a row a warp, four columns a lane
+    const int t_lo = NT * rank / split, t_hi = min(NT * (rank + 1) / split, m - i0);
+    for (int t = t_lo + warp; t < t_hi; t += TILE_THREADS / 32) {
+        const uint32_t at = ring0 + static_cast<uint32_t>(t * TILE_J + lane * 4) * 4u;
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int r = 0; r < split; ++r) {
+            const float4 p = ld_cluster4(split > 1 ? map_to_rank(at, r) : at);
+            v[0] += p.x, v[1] += p.y, v[2] += p.z, v[3] += p.w;
+        }
+        const int col = j0 + lane * 4;
+        if (col < n) finish4<T>(epi, v, i0 + t, col, n);
+    }
+    if (split > 1) cluster_sync();  // no CTA leaves while another reads its part
+}
+
+// ------------------------------------------------------------------------------------------------------------- host
+// a 16-bit matrix of `rows` rows of `cols` values, `ld` apart, as boxes of box_rows x 64 values with 128-byte swizzle
+// and zeros outside
+int operand_map(CUtensorMap *map, const void *base, int64_t rows, int64_t cols, int64_t ld, int box_rows) {
+    EncodeTiled enc = encoder();
+    if (enc == nullptr) return WF_ERR_DEVICE;
+    cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+    cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * 2};
+    cuuint32_t box[2] = {64, static_cast<cuuint32_t>(box_rows)};
+    cuuint32_t estr[2] = {1, 1};
+    CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, const_cast<void *>(base), dims, strides, box, estr,
+                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? WF_OK : WF_ERR_ARG;
+}
+
+// D [m, n] = A B^T: a is [m, c] (or [c, m] where it is row-major), b is [n, c] (or [c, n])
+struct Product {
+    const void *a, *b;
+    int64_t lda, ldb, m, n, c;
+};
+
+template <bool A_ROWS, bool B_ROWS, int NT, int T>
+int launch_tile(const Product &p, const Epilogue &e, int split, int dev, cudaStream_t stream) {
+    using S = TileShape<NT>;
+    constexpr auto kern = linear_tile_kernel<B_ROWS, A_ROWS, NT, T>;
+    static std::atomic<bool> ready[64];  // any host thread may launch first
+    if (!ready[dev].load(std::memory_order_acquire)) {
+        const cudaError_t e0 = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::smem);
+        if (e0 != cudaSuccess) return static_cast<int>(e0);
+        ready[dev].store(true, std::memory_order_release);
+    }
+    CUtensorMap mp, mq;
+    int rc = B_ROWS ? operand_map(&mp, p.b, p.c, p.n, p.ldb, BC) : operand_map(&mp, p.b, p.n, p.c, p.ldb, TILE_J);
+    if (rc == WF_OK) rc = A_ROWS ? operand_map(&mq, p.a, p.c, p.m, p.lda, BC) : operand_map(&mq, p.a, p.m, p.c, p.lda, NT);
+    if (rc != WF_OK) return rc;
+    const int64_t tiles_q = (p.m + NT - 1) / NT, tiles = (p.n + TILE_J - 1) / TILE_J * tiles_q;
+    if (tiles * split > (1ll << 31) - 1) return WF_ERR_ARG;
+    const cudaError_t err = launch_dependent_clusters(
+        kern, dim3(static_cast<unsigned>(tiles * split)), split > 1 ? split : 0, TILE_THREADS, S::smem, stream, mp, mq, e,
+        static_cast<int>(p.m), static_cast<int>(p.n), static_cast<int>(p.c), static_cast<int>(tiles_q), split);
+    return static_cast<int>(err != cudaSuccess ? err : cudaGetLastError());
+}
+
+template <bool A_ROWS, bool B_ROWS, int T>
+int dispatch(const Product &p, const Epilogue &e, cudaStream_t stream) {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64) return WF_ERR_DEVICE;
+    const int nt = A_ROWS ? (p.m <= 64 ? 64 : 128) : p.m <= 16 ? 16 : p.m <= 32 ? 32 : p.m <= 64 ? 64 : 128;
+    const int64_t tiles = (p.n + TILE_J - 1) / TILE_J * ((p.m + nt - 1) / nt), steps = (p.c + BC - 1) / BC;
+    int split = 1;
+    while (split < 8 && tiles * split * 2 <= 2 * device_sm_count() && steps >= split * 4) split *= 2;
+    if constexpr (!A_ROWS) {
+        if (nt == 16) return launch_tile<A_ROWS, B_ROWS, 16, T>(p, e, split, dev, stream);
+        if (nt == 32) return launch_tile<A_ROWS, B_ROWS, 32, T>(p, e, split, dev, stream);
+    }
+    if (nt == 64) return launch_tile<A_ROWS, B_ROWS, 64, T>(p, e, split, dev, stream);
+    return launch_tile<A_ROWS, B_ROWS, 128, T>(p, e, split, dev, stream);
+}
+
+// what TMA asks of an operand: a 16-byte aligned base and row pitch
+bool operand_ok(const void *p, int64_t cols, int64_t ld) {
+    return p != nullptr && aligned_to(p, 16) && ld >= cols && ld % 8 == 0;
+}
+
+bool sizes_ok(int64_t m, int64_t n, int64_t k) {
+    constexpr int64_t most = 1ll << 30;
+    return m >= 0 && n >= 0 && k >= 1 && m <= most && n <= most && k <= most;
+}
+
+bool vec4_ok(const void *p, int64_t ld) { return p == nullptr || (aligned_to(p, 8) && ld % 4 == 0); }
+
+template <bool A_ROWS, bool B_ROWS>
+int run_product(const Product &p, Epilogue &e, int type, cudaStream_t stream) {
+    e.vec = vec4_ok(e.bias, 0) && vec4_ok(e.gate, p.n) && vec4_ok(e.resid, e.ld_resid) && vec4_ok(e.out, e.ld_out) &&
+            (e.keep != KEEP_SAME || vec4_ok(e.kept, e.ld_kept));
+    const int rc = check_device();
+    if (rc != WF_OK) return rc;
+    return type == WF_BF16 ? dispatch<A_ROWS, B_ROWS, WF_BF16>(p, e, stream) : dispatch<A_ROWS, B_ROWS, WF_F16>(p, e, stream);
+}
+
+}  // namespace
+}  // namespace wf
+
+extern "C" WF_API int wf_linear(const void *x, int64_t ldx, const void *w, int64_t ldw, const void *bias, int act,
+                                const void *gate, int64_t rows_per_group, const void *resid, int64_t ld_resid, void *y,
+                                int64_t ldy, void *z, int64_t ldz, int z_type, int64_t m, int64_t n, int64_t k, int type,
+                                wf_stream_t stream) {
+    using namespace wf;
+    if (type != WF_BF16 && type != WF_F16) return WF_ERR_UNSUPPORTED;
+    if (act < WF_ACT_NONE || act > WF_ACT_GELU_TANH) return WF_ERR_UNSUPPORTED;
+    if (!sizes_ok(m, n, k)) return WF_ERR_ARG;
+    if (m == 0 || n == 0) return WF_OK;
+    if (!operand_ok(x, k, ldx) || !operand_ok(w, k, ldw) || !y || ldy < n || (gate && rows_per_group < 1) ||
+        (resid && ld_resid < n) || !aligned_to(y, 2) || !aligned_to(bias, 2) || !aligned_to(gate, 2) || !aligned_to(resid, 2))
+        return WF_ERR_ARG;
+    int keep = KEEP_NONE;
+    if (z != nullptr) {
+        if (z_type != WF_F32 && z_type != WF_F16 && z_type != type) return WF_ERR_UNSUPPORTED;
+        if (ldz < n || !aligned_to(z, dtype_size(z_type))) return WF_ERR_ARG;
+        keep = z_type == WF_F32 ? KEEP_F32 : z_type == WF_F16 && type != WF_F16 ? KEEP_F16 : KEEP_SAME;
+    }
+    Product p{x, w, ldx, ldw, m, n, k};
+    Epilogue e{bias, gate, resid, y, z, ld_resid, ldy, ldz, rows_per_group, act, keep, false};
+    return run_product<false, false>(p, e, type, reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" WF_API int wf_linear_backward_input(const void *dz, int64_t lddz, const void *w, int64_t ldw, void *dx,
+                                               int64_t lddx, int64_t m, int64_t n, int64_t k, int type,
+                                               wf_stream_t stream) {
+    using namespace wf;
+    if (type != WF_BF16 && type != WF_F16) return WF_ERR_UNSUPPORTED;
+    if (!sizes_ok(m, k, n)) return WF_ERR_ARG;
+    if (m == 0 || k == 0) return WF_OK;
+    if (!operand_ok(dz, n, lddz) || !operand_ok(w, k, ldw) || !dx || lddx < k || !aligned_to(dx, 2)) return WF_ERR_ARG;
+    Product p{dz, w, lddz, ldw, m, k, n};
+    Epilogue e{nullptr, nullptr, nullptr, dx, nullptr, 0, lddx, 0, 1, WF_ACT_NONE, KEEP_NONE, false};
+    return run_product<false, true>(p, e, type, reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" WF_API int wf_linear_backward_weight(const void *dz, int64_t lddz, const void *x, int64_t ldx, void *dw,
+                                                int64_t lddw, int64_t m, int64_t n, int64_t k, int type,
+                                                wf_stream_t stream) {
+    using namespace wf;
+    if (type != WF_BF16 && type != WF_F16) return WF_ERR_UNSUPPORTED;
+    if (!sizes_ok(n, k, m)) return WF_ERR_ARG;
+    if (n == 0 || k == 0) return WF_OK;
+    if (!operand_ok(dz, n, lddz) || !operand_ok(x, k, ldx) || !dw || lddw < k || !aligned_to(dw, 2)) return WF_ERR_ARG;
+    Product p{dz, x, lddz, ldx, n, k, m};
+    Epilogue e{nullptr, nullptr, nullptr, dw, nullptr, 0, lddw, 0, 1, WF_ACT_NONE, KEEP_NONE, false};
+    return run_product<true, true>(p, e, type, reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" WF_API int wf_linear_status(int *status) {
+    if (status == nullptr) return WF_ERR_ARG;
+    int v = 0;
+    const cudaError_t e = cudaMemcpyFromSymbol(&v, wf::g_linear_status, sizeof(int));
+    if (e != cudaSuccess) return static_cast<int>(e);
+    if (v != 0) {
+        const int zero = 0;
+        cudaMemcpyToSymbol(wf::g_linear_status, &zero, sizeof(int));
+    }
+    *status = v;
+    return WF_OK;
+}

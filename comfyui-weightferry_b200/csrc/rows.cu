@@ -1,0 +1,101 @@
+// The sum of partial column sums (see wf_rows.cuh) and the copy of rows to an aligned row pitch.
+
+#include "wf_rows.cuh"
+
+namespace wf {
+namespace {
+
+struct ReduceArgs {
+    const float *part[2];
+    void *out[2];
+    int64_t groups, parts, d;
+};
+
+// Block (x, y, z): columns 32 x .. 32 x + 31 of groups y, y + gridDim.y, ... of sum z. Eight warps take every eighth
+// part, then their sums are added in warp order: a fixed order for a given shape. A few MB at most; bound by latency.
+template <int T>
+__global__ void __launch_bounds__(256) reduce_partials_kernel(const __grid_constant__ ReduceArgs a) {
+    __shared__ float red[8][33];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t col = static_cast<int64_t>(blockIdx.x) * 32 + lane;
+    const float *part = a.part[blockIdx.z];
+    void *out = a.out[blockIdx.z];
+    wait_prior_grid();
+    if (out == nullptr) return;
+    for (int64_t g = blockIdx.y; g < a.groups; g += gridDim.y) {
+        float s = 0.f;
+        if (col < a.d)
+#pragma unroll 8
+            for (int64_t p = warp; p < a.parts; p += 8) s += part[(g * a.parts + p) * a.d + col];
+        red[warp][lane] = s;
+        __syncthreads();
+        if (warp == 0 && col < a.d) {
+#pragma unroll
+            for (int w = 1; w < 8; ++w) s += red[w][lane];
+            store1<T>(row_of<T>(out, g, a.d), col, s);
+        }
+        __syncthreads();
+    }
+}
+
+}  // namespace
+
+int reduce_partials(const float *part0, void *out0, const float *part1, void *out1, int64_t groups, int64_t parts,
+                    int64_t d, int type, cudaStream_t stream) {
+    if (out0 == nullptr && out1 == nullptr) return WF_OK;
+    if (out0 == nullptr) {
+        part0 = part1, out0 = out1;
+        out1 = nullptr;
+    }
+    ReduceArgs a{{part0, part1}, {out0, out1}, groups, parts, d};
+    const dim3 grid(static_cast<unsigned>((d + 31) / 32), static_cast<unsigned>(std::min<int64_t>(groups, 32768)),
+                    out1 != nullptr ? 2 : 1);
+    if (type == WF_F32) return launch_rows(reduce_partials_kernel<WF_F32>, grid, 256, stream, a);
+    if (type == WF_BF16) return launch_rows(reduce_partials_kernel<WF_BF16>, grid, 256, stream, a);
+    return launch_rows(reduce_partials_kernel<WF_F16>, grid, 256, stream, a);
+}
+
+namespace {
+
+struct CopyRowsArgs {
+    const uint16_t *src;
+    uint16_t *dst;
+    int64_t rows, cols, lds, ldd;
+};
+
+// Rows of 16-bit values to another row pitch: a warp a row, neighbouring values in neighbouring lanes (the source may
+// have any 2-byte alignment).
+__global__ void __launch_bounds__(256) copy_rows_kernel(const __grid_constant__ CopyRowsArgs a) {
+    const int64_t per = (a.cols + 255) / 256;  // pieces of 256 values a row
+    const int64_t step = static_cast<int64_t>(gridDim.x) * 8;
+    wait_prior_grid();
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); i < a.rows * per; i += step) {
+        const int64_t row = i / per, col = i % per * 256 + (threadIdx.x & 31);
+        const uint16_t *s = a.src + row * a.lds + col;
+        uint16_t *d = a.dst + row * a.ldd + col;
+        uint16_t v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (col + 32 * j < a.cols) v[j] = s[32 * j];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (col + 32 * j < a.cols) d[32 * j] = v[j];
+    }
+}
+
+}  // namespace
+}  // namespace wf
+
+extern "C" WF_API int wf_copy_rows16(const void *src, int64_t ld_src, void *dst, int64_t ld_dst, int64_t rows,
+                                     int64_t cols, wf_stream_t stream) {
+    using namespace wf;
+    if (rows < 0 || cols < 0 || ld_src < cols || ld_dst < cols) return WF_ERR_ARG;
+    if (rows == 0 || cols == 0) return WF_OK;
+    if (!src || !dst || !aligned_to(src, 2) || !aligned_to(dst, 2)) return WF_ERR_ARG;
+    const int rc = check_device();
+    if (rc != WF_OK) return rc;
+    CopyRowsArgs a{static_cast<const uint16_t *>(src), static_cast<uint16_t *>(dst), rows, cols, ld_src, ld_dst};
+    const int64_t need = (rows * ((cols + 255) / 256) + 7) / 8;
+    const int grid = static_cast<int>(std::min<int64_t>(need, wave_ctas_at<copy_rows_kernel>(256)));
+    return launch_rows(copy_rows_kernel, dim3(grid), 256, reinterpret_cast<cudaStream_t>(stream), a);
+}
