@@ -341,6 +341,367 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_const
     if (split > 1) cluster_sync();  // no CTA leaves while another reads its part
 }
 
+// ------------------------------------------------------------------------------------------------- many-rows kernel
+// One 256 x 256 tile of D for each pair of CTAs (a cluster of 2 on neighbouring SMs), persistent. tcgen05.mma
+// cta_group::2 (M = 256, N = 256, K = 16), issued by one thread of the even CTA, reads rows 0..127 of the A tile and
+// columns 0..127 of the B tile from the even CTA's shared memory and the other halves from the odd CTA's; each CTA's
+// tensor memory holds its 128 rows x 256 columns, twice, so that the next tile's MMAs run while this one is written
+// out. Warp 8 loads (six 32 KB stages), warp 9 of the even CTA issues, warps 0..7 are the epilogue: a warp takes 32
+// rows and 128 columns of the accumulator in chunks of 32 x 32, which leave through a swizzled 2 KB buffer and one TMA
+// store each (plain stores where the output's pitch or base is not a multiple of 16 bytes).
+constexpr int PAIR_STAGES = 6;
+constexpr int PAIR_THREADS = 320;
+constexpr int PAIR_EPI_THREADS = 256;
+constexpr int PAIR_HALF = 128 * BC * 2;            // 16 KB: this CTA's 128 rows of A or columns of B
+constexpr int PAIR_STAGE = 2 * PAIR_HALF;
+constexpr int PAIR_OUT = 8 * 2 * 2048;             // two chunks an epilogue warp
+constexpr int kBand = 8;                           // tile rows of a band of the tile order
+constexpr int PAIR_SMEM = PAIR_STAGES * PAIR_STAGE + PAIR_OUT + 1024 + 256;
+
+__device__ __forceinline__ void mma_f16_pair(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// 32 neighbouring 16-bit values of a row in 16 registers, those at and past n as 0; vec: 16-byte aligned, n % 8 == 0
+__device__ __forceinline__ void load32(uint32_t (&w)[16], const void *row, int col, int n, bool vec) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const int c = col + 8 * q;
+        if (vec) {
+            uint4 v = make_uint4(0u, 0u, 0u, 0u);
+            if (c < n) v = __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(row) + c));
+            w[4 * q] = v.x, w[4 * q + 1] = v.y, w[4 * q + 2] = v.z, w[4 * q + 3] = v.w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint16_t *p = static_cast<const uint16_t *>(row) + c + 2 * i;
+                const uint32_t lo = c + 2 * i < n ? p[0] : 0u, hi = c + 2 * i + 1 < n ? p[1] : 0u;
+                w[4 * q + i] = lo | (hi << 16);
+            }
+        }
+    }
+}
+
+template <int ACT>
+__device__ __forceinline__ void act32(float (&v)[32]) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = act<ACT>(v[i]);
+}
+
+// 32 x 32 values (this lane's row in p) to the warp's chunk buffer and out: 16-byte piece j of row r sits at piece
+// j ^ ((r >> 1) & 3). The buffer is used every second time: lane 0 first waits until its last store has been read.
+__device__ __forceinline__ void emit32(const uint32_t (&p)[16], uint32_t buf, int lane, bool tma, const CUtensorMap *map,
+                                       void *out, int64_t ld, int row0, int col0, int m, int n) {
+    if (lane == 0) bulk_wait_read1();
+    __syncwarp();
+    const uint32_t row_addr = buf + 64u * static_cast<uint32_t>(lane), sw = (static_cast<uint32_t>(lane) >> 1) & 3u;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row_addr + 16u * (static_cast<uint32_t>(j) ^ sw)),
+                     "r"(p[4 * j]), "r"(p[4 * j + 1]), "r"(p[4 * j + 2]), "r"(p[4 * j + 3])
+                     : "memory");
+    if (tma) {
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+            tma_store_2d(map, buf, col0, row0);
+            bulk_commit();
+        }
+        return;
+    }
+    __syncwarp();
+    if (col0 + lane < n) {
+        const int rows = min(32, m - row0);
+        uint16_t *dst = static_cast<uint16_t *>(out) + row0 * ld + col0 + lane;
+        for (int r = 0; r < rows; ++r) {
+            uint16_t v;
+            const uint32_t piece = (static_cast<uint32_t>(lane) >> 3) ^ ((static_cast<uint32_t>(r) >> 1) & 3u);
+            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(buf + 64u * r + 16u * piece + 2u * (lane & 7)) : "memory");
+            dst[r * ld] = v;
+        }
+    }
+}
+
+// what one epilogue warp knows of its 32 rows x 128 columns
+struct Warp32 {
+    uint32_t buf;             // its two chunk buffers
+    uint32_t chunks;          // chunks written so far: which buffer is next
+    int lane, row0, m, n;
+    const void *gate, *resid; // this lane's rows (null: none, or a row past m)
+    bool tma_out, tma_kept;
+};
+
+template <int T, bool FULL>
+__device__ __forceinline__ void finish_chunk(const uint32_t (&r)[32], Warp32 &w, const Epilogue &e, const CUtensorMap *map_out,
+                                             const CUtensorMap *map_kept, const uint32_t (&res)[16], int col0) {
+    float v[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+    uint32_t p[16];
+    if constexpr (FULL) {
+        if (e.bias != nullptr) {
+            uint32_t b[16];
+            load32(b, e.bias, col0, w.n, e.vec);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float2 f = unpack2<T>(b[i]);
+                v[2 * i] += f.x;
+                v[2 * i + 1] += f.y;
+            }
+        }
+        if (e.keep == KEEP_F32) {
+            const int row = w.row0 + w.lane;
+            if (row < w.m) {
+                float *dst = static_cast<float *>(e.kept) + row * e.ld_kept + col0;
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    if (col0 + i < w.n) dst[i] = v[i];
+            }
+        } else if (e.keep != KEEP_NONE) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                if (e.keep == KEEP_F16) {
+                    const __half2 h = __halves2half2(to_half_sat(v[2 * i]), to_half_sat(v[2 * i + 1]));
+                    p[i] = *reinterpret_cast<const uint32_t *>(&h);
+                } else {
+                    p[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
+                }
+            }
+            emit32(p, w.buf + 2048u * (w.chunks++ & 1u), w.lane, w.tma_kept, map_kept, e.kept, e.ld_kept, w.row0, col0, w.m, w.n);
+        }
+        switch (e.act) {
+            case WF_ACT_RELU: act32<WF_ACT_RELU>(v); break;
+            case WF_ACT_SILU: act32<WF_ACT_SILU>(v); break;
+            case WF_ACT_GELU: act32<WF_ACT_GELU>(v); break;
+            case WF_ACT_GELU_TANH: act32<WF_ACT_GELU_TANH>(v); break;
+            default: break;
+        }
+        if (w.gate != nullptr) {
+            uint32_t g[16];
+            load32(g, w.gate, col0, w.n, e.vec);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float2 f = unpack2<T>(g[i]);
+                v[2 * i] *= f.x;
+                v[2 * i + 1] *= f.y;
+            }
+        }
+        if (e.resid != nullptr) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float2 f = unpack2<T>(res[i]);
+                v[2 * i] += f.x;
+                v[2 * i + 1] += f.y;
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) p[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
+    emit32(p, w.buf + 2048u * (w.chunks++ & 1u), w.lane, w.tma_out, map_out, e.out, e.ld_out, w.row0, col0, w.m, w.n);
+}
+
+// FULL: the forward pass's epilogue; else D is rounded and stored
+template <bool A_ROWS, bool B_ROWS, int T, bool FULL>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
+linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                   const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_kept,
+                   const __grid_constant__ Epilogue epi, int m, int n, int c, int band, bool tma_out, bool tma_kept) {
+    constexpr uint32_t idesc = f16_idesc(T == WF_BF16, A_ROWS, B_ROWS, 256, 256);
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t *out_chunks = ring + PAIR_STAGES * PAIR_STAGE;
+    uint64_t *bars = reinterpret_cast<uint64_t *>(out_chunks + PAIR_OUT);
+    // full[0..5] (used in the even CTA), empty[0..5], tmem_full[0..1], tmem_empty[0..1] (even CTA), drain
+    __shared__ uint32_t s_tmem_base;
+    __shared__ int s_abort;
+    __shared__ int s_issued[2];  // stage loads issued by this CTA's producer; [1] in the even CTA: the odd CTA's
+    const uint32_t ring0 = smem_u32(ring), full0 = smem_u32(bars), empty0 = full0 + 8 * PAIR_STAGES,
+                   tfull0 = empty0 + 8 * PAIR_STAGES, tempty0 = tfull0 + 16, drain = tempty0 + 16;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank(), peer = rank ^ 1u;
+    const int tiles_m = (m + 255) / 256, tiles_n = (n + 255) / 256, n_tiles = tiles_m * tiles_n;
+    const int steps = (c + BC - 1) / BC;
+    const int cluster_id = blockIdx.x >> 1, n_clusters = gridDim.x >> 1;
+
+    if (threadIdx.x == 0) {
+        s_abort = 0;
+        s_issued[0] = s_issued[1] = 0;
+        for (int s = 0; s < PAIR_STAGES; ++s) {
+            mbar_init(full0 + 8 * s, 1);
+            mbar_init(empty0 + 8 * s, 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(tfull0 + 8 * b, 1);
+            mbar_init(tempty0 + 8 * b, 2 * PAIR_EPI_THREADS);
+        }
+        mbar_init(drain, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fence_async_smem();
+    }
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
+                     ::"r"(smem_u32(&s_tmem_base)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    fence_before();
+    cluster_sync();  // barriers initialised and tensor memory allocated in both CTAs
+    fence_after();
+    const uint32_t tmem = s_tmem_base;
+    wait_prior_grid();
+    volatile int *abort_flag = &s_abort;
+
+    if (warp == 8) {
+        if (lane == 0) {
+            asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_a)) : "memory");
+            asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_b)) : "memory");
+            int stage = 0, issued = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int tile = cluster_id; tile < n_tiles && ok; tile += n_clusters) {
+                int mi, ni;
+                tile_coords(tile, tiles_m, tiles_n, band, mi, ni);
+                const int i0 = mi * 256 + static_cast<int>(rank) * 128, j0 = ni * 256 + static_cast<int>(rank) * 128;
+                for (int s = 0; s < steps; ++s) {
+                    if (!pipe_wait(empty0 + 8 * stage, phase ^ 1u, abort_flag, 1)) { ok = false; break; }
+                    const uint32_t bar = (full0 + 8 * stage) & kPeerBitMask;  // the even CTA's
+                    if (rank == 0) mbar_expect_tx(full0 + 8 * stage, 2 * PAIR_STAGE);
+                    const uint32_t a = ring0 + stage * PAIR_STAGE, b = a + PAIR_HALF;
+                    if constexpr (A_ROWS) {
+                        tma_load_2d_pair(a, &map_a, i0, s * BC, bar);
+                        tma_load_2d_pair(a + BC * 128, &map_a, i0 + 64, s * BC, bar);
+                    } else {
+                        tma_load_2d_pair(a, &map_a, s * BC, i0, bar);
+                    }
+                    if constexpr (B_ROWS) {
+                        tma_load_2d_pair(b, &map_b, j0, s * BC, bar);
+                        tma_load_2d_pair(b + BC * 128, &map_b, j0 + 64, s * BC, bar);
+                    } else {
+                        tma_load_2d_pair(b, &map_b, s * BC, j0, bar);
+                    }
+                    ++issued;
+                    if (++stage == PAIR_STAGES) stage = 0, phase ^= 1u;
+                }
+            }
+            // the count goes to the even CTA, whose full barriers count both CTAs' bytes: it drains (below)
+            if (rank == 0) {
+                s_issued[0] = issued;
+            } else {
+                asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(map_to_rank(smem_u32(&s_issued[1]), 0)), "r"(issued)
+                             : "memory");
+            }
+        }
+        __syncwarp();
+    } else if (warp == 9) {
+        if (lane == 0 && rank == 0) {
+            const uint32_t empty_peer = map_to_rank(empty0, peer), tfull_peer = map_to_rank(tfull0, peer);
+            int stage = 0, acc = 0;
+            uint32_t phase = 0, acc_phase = 0;
+            bool ok = true;
+            for (int tile = cluster_id; tile < n_tiles && ok; tile += n_clusters) {
+                if (!pipe_wait(tempty0 + 8 * acc, acc_phase ^ 1u, abort_flag, 2)) break;
+                fence_after();
+                const uint32_t d = tmem + static_cast<uint32_t>(acc * 256);
+                for (int s = 0; s < steps; ++s) {
+                    if (!pipe_wait(full0 + 8 * stage, phase, abort_flag, 2)) { ok = false; break; }
+                    fence_after();
+                    const uint32_t a = ring0 + stage * PAIR_STAGE, b = a + PAIR_HALF;
+#pragma unroll
+                    for (int k = 0; k < BC / 16; ++k)
+                        mma_f16_pair(d, operand_desc<A_ROWS>(a, k), operand_desc<B_ROWS>(b, k), idesc, s > 0 || k > 0);
+                    mma_commit_pair(empty0 + 8 * stage);
+                    mma_commit_pair(empty_peer + 8 * stage);
+                    if (++stage == PAIR_STAGES) stage = 0, phase ^= 1u;
+                }
+                if (!ok) break;
+                mma_commit_pair(tfull0 + 8 * acc);
+                mma_commit_pair(tfull_peer + 8 * acc);
+                if (++acc == 2) acc = 0, acc_phase ^= 1u;
+            }
+            mma_commit_pair(drain);
+            mbar_drain_wait(drain, 0);
+        }
+        __syncwarp();
+    } else {
+        const int quarter = warp & 3, half = warp >> 2;
+        const uint32_t tempty_leader = map_to_rank(tempty0, 0);
+        Warp32 w;
+        w.buf = smem_u32(out_chunks + warp * 4096);
+        w.chunks = 0;
+        w.lane = lane, w.m = m, w.n = n;
+        w.tma_out = tma_out, w.tma_kept = tma_kept;
+        int acc = 0;
+        uint32_t acc_phase = 0;
+        for (int tile = cluster_id; tile < n_tiles; tile += n_clusters) {
+            int mi, ni;
+            tile_coords(tile, tiles_m, tiles_n, band, mi, ni);
+            w.row0 = mi * 256 + static_cast<int>(rank) * 128 + quarter * 32;
+            const int col0 = ni * 256 + half * 128, row = w.row0 + lane;
+            const bool in = row < m;
+            w.gate = FULL && epi.gate != nullptr && in ? row_of<T>(epi.gate, row / epi.rows_per_group, n) : nullptr;
+            w.resid = FULL && epi.resid != nullptr && in ? row_of<T>(epi.resid, row, epi.ld_resid) : nullptr;
+            if (FULL && w.resid != nullptr && epi.vec && col0 < n)  // the row's span to L2 while the MMAs run
+                asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;"
+                             ::"l"(static_cast<const uint16_t *>(w.resid) + col0), "r"(static_cast<uint32_t>(min(128, n - col0)) * 2u)
+                             : "memory");
+            if (!__all_sync(0xFFFFFFFFu, pipe_wait(tfull0 + 8 * acc, acc_phase, abort_flag, 3))) break;
+            fence_after();
+            const uint32_t taddr = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * 256 + half * 128);
+            uint32_t ra[32], rb[32], res[16];
+            tmem_ld32(taddr, ra);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                uint32_t(&cur)[32] = (q & 1) ? rb : ra;
+                uint32_t(&nxt)[32] = (q & 1) ? ra : rb;
+                if (FULL && epi.resid != nullptr) {
+                    if (w.resid != nullptr) {
+                        load32(res, w.resid, col0 + 32 * q, n, epi.vec);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) res[i] = 0u;
+                    }
+                }
+                tmem_wait32(cur);
+                if (q < 3) {
+                    tmem_ld32(taddr + 32 * (q + 1), nxt);
+                } else {  // the accumulator is in registers: it may be overwritten
+                    fence_before();
+                    mbar_arrive_cluster(tempty_leader + 8 * acc);
+                }
+                finish_chunk<T, FULL>(cur, w, epi, &map_out, &map_kept, res, col0 + 32 * q);
+            }
+            if (++acc == 2) acc = 0, acc_phase ^= 1u;
+        }
+        if (lane == 0) bulk_wait_read_all();
+        __syncwarp();
+    }
+    fence_before();
+    __syncthreads();
+    cluster_sync();  // both CTAs stopped issuing; the odd CTA's load count is in the even CTA's s_issued[1]
+    if (rank == 0 && warp == 8 && lane == 0) {
+        // Every stage load either CTA issued lands before either CTA leaves: only a stage's last use can be outstanding,
+        // and after an abort one CTA may have issued a use that the other did not (its bytes are then made up for).
+        const int n_even = s_issued[0], n_odd = s_issued[1], last = max(n_even, n_odd);
+        for (int s = 0; s < PAIR_STAGES && s < last; ++s) {
+            const int u = s + ((last - 1 - s) / PAIR_STAGES) * PAIR_STAGES;
+            const uint32_t bar = full0 + 8 * s;
+            if (u >= n_even)
+                mbar_expect_tx(bar, PAIR_STAGE);
+            else if (u >= n_odd)
+                mbar_complete_tx(bar, PAIR_STAGE);
+            mbar_drain_wait(bar, static_cast<uint32_t>(u / PAIR_STAGES) & 1u);
+        }
+    }
+    cluster_sync();  // no CTA leaves (or frees tensor memory) while loads into it or the pair's MMAs may still run
+    fence_after();
+    if (warp == 9)
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+}
+
 // ------------------------------------------------------------------------------------------------------------- host
 // a 16-bit matrix of `rows` rows of `cols` values, `ld` apart, as boxes of box_rows x 64 values with 128-byte swizzle
 // and zeros outside
@@ -385,6 +746,70 @@ int launch_tile(const Product &p, const Epilogue &e, int split, int dev, cudaStr
     return static_cast<int>(err != cudaSuccess ? err : cudaGetLastError());
 }
 
+// a 16-bit [rows, cols] output as boxes of 32 x 32 values with 64-byte swizzle
+int output_map(CUtensorMap *map, void *base, int64_t rows, int64_t cols, int64_t ld) {
+    EncodeTiled enc = encoder();
+    if (enc == nullptr) return WF_ERR_DEVICE;
+    cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
+    cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * 2};
+    cuuint32_t box[2] = {32, 32};
+    cuuint32_t estr[2] = {1, 1};
+    CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                     CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? WF_OK : WF_ERR_ARG;
+}
+
+bool vec8_ok(const void *p, int64_t ld) { return p == nullptr || (aligned_to(p, 16) && ld % 8 == 0); }
+
+template <bool A_ROWS, bool B_ROWS, int T>
+int launch_pair(const Product &p, const Epilogue &e0, int dev, cudaStream_t stream) {
+    constexpr bool full = !A_ROWS && !B_ROWS;
+    constexpr auto kern = linear_pair_kernel<A_ROWS, B_ROWS, T, full>;
+    static std::atomic<int> clusters[64];  // resident pairs; any host thread may launch first
+    if (clusters[dev].load(std::memory_order_acquire) == 0) {
+        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, PAIR_SMEM);
+        if (e != cudaSuccess) return static_cast<int>(e);
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(2 * device_sm_count());
+        cfg.blockDim = dim3(PAIR_THREADS);
+        cfg.dynamicSmemBytes = PAIR_SMEM;
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = 2;
+        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        int n = 0;
+        e = cudaOccupancyMaxActiveClusters(&n, kern, &cfg);
+        if (e != cudaSuccess) return static_cast<int>(e);
+        clusters[dev].store(std::max(n, 1), std::memory_order_release);
+    }
+    Epilogue e = e0;
+    // 16-byte accesses to the bias, the gate and the residual
+    e.vec = p.n % 8 == 0 && vec8_ok(e.bias, 0) && vec8_ok(e.gate, p.n) && vec8_ok(e.resid, e.ld_resid);
+    const bool tma_out = vec8_ok(e.out, e.ld_out);
+    const bool tma_kept = (e.keep == KEEP_F16 || e.keep == KEEP_SAME) && vec8_ok(e.kept, e.ld_kept);
+    CUtensorMap ma, mb, mo = {}, mk = {};
+    int rc = A_ROWS ? operand_map(&ma, p.a, p.c, p.m, p.lda, BC) : operand_map(&ma, p.a, p.m, p.c, p.lda, 128);
+    if (rc == WF_OK) rc = B_ROWS ? operand_map(&mb, p.b, p.c, p.n, p.ldb, BC) : operand_map(&mb, p.b, p.n, p.c, p.ldb, 128);
+    if (rc == WF_OK && tma_out) rc = output_map(&mo, e.out, p.m, p.n, e.ld_out);
+    if (rc == WF_OK && tma_kept) rc = output_map(&mk, e.kept, p.m, p.n, e.ld_kept);
+    if (rc != WF_OK) return rc;
+    const int64_t tiles = ((p.m + 255) / 256) * ((p.n + 255) / 256);
+    if (tiles > (1ll << 30)) return WF_ERR_ARG;
+    const int grid = 2 * static_cast<int>(std::min<int64_t>(tiles, clusters[dev].load(std::memory_order_acquire)));
+    const cudaError_t err = launch_dependent(kern, dim3(grid), PAIR_THREADS, PAIR_SMEM, stream, ma, mb, mo, mk, e,
+                                             static_cast<int>(p.m), static_cast<int>(p.n), static_cast<int>(p.c),
+                                             kBand, tma_out, tma_kept);
+    return static_cast<int>(err != cudaSuccess ? err : cudaGetLastError());
+}
+
+bool use_pair(const Product &p) {
+    static const int forced = env_digit("WEIGHTFERRY_LINEAR_PAIR", 2);
+    if (forced < 2) return forced == 1;
+    return ((p.m + 255) / 256) * ((p.n + 255) / 256) >= device_sm_count() / 4;
+}
+
 template <bool A_ROWS, bool B_ROWS, int T>
 int dispatch(const Product &p, const Epilogue &e, cudaStream_t stream) {
     int dev = 0;
@@ -392,6 +817,7 @@ int dispatch(const Product &p, const Epilogue &e, cudaStream_t stream) {
     if (dev < 0 || dev >= 64) return WF_ERR_DEVICE;
     const int nt = A_ROWS ? (p.m <= 64 ? 64 : 128) : p.m <= 16 ? 16 : p.m <= 32 ? 32 : p.m <= 64 ? 64 : 128;
     const int64_t tiles = (p.n + TILE_J - 1) / TILE_J * ((p.m + nt - 1) / nt), steps = (p.c + BC - 1) / BC;
+    if (use_pair(p)) return launch_pair<A_ROWS, B_ROWS, T>(p, e, dev, stream);
     int split = 1;
     while (split < 8 && tiles * split * 2 <= 2 * device_sm_count() && steps >= split * 4) split *= 2;
     if constexpr (!A_ROWS) {
