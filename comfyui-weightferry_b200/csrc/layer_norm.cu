@@ -423,23 +423,26 @@ RowSplit norm_split(int64_t rows, int64_t rows_per_group, int d) {
 }  // namespace
 }  // namespace wf
 
-extern "C" WF_API int wf_layer_norm(const void *x, int64_t ldx, const void *w, const void *b, int w_type, void *y,
-                                    int64_t ldy, float *mean, float *rstd, int64_t rows, int64_t d,
-                                    int64_t rows_per_group, float eps, int type, wf_stream_t stream) {
+extern "C" WF_API int wf_layer_norm(const wf_layer_norm_args *args, wf_stream_t stream) {
     using namespace wf;
-    if (!norm_types_ok(type, w_type)) return WF_ERR_UNSUPPORTED;
-    if (rows < 0 || d < 1 || d > (1 << 30) || rows_per_group < 1 || !(eps >= 0.f) || ldx < d || ldy < d) return WF_ERR_ARG;
-    if ((mean == nullptr) != (rstd == nullptr)) return WF_ERR_ARG;
-    if (rows == 0) return WF_OK;
-    const int e = dtype_size(type), we = dtype_size(w_type);
-    if (!x || !y || !aligned_to(x, e) || !aligned_to(y, e) || !aligned_to(w, we) || !aligned_to(b, we)) return WF_ERR_ARG;
+    if (args == nullptr) return WF_ERR_ARG;
+    const wf_layer_norm_args &g = *args;
+    if (!norm_types_ok(g.type, g.w_type)) return WF_ERR_UNSUPPORTED;
+    if (g.rows < 0 || g.d < 1 || g.d > (1 << 30) || g.rows_per_group < 1 || !(g.eps >= 0.f) || g.ldx < g.d || g.ldy < g.d)
+        return WF_ERR_ARG;
+    if ((g.mean == nullptr) != (g.rstd == nullptr)) return WF_ERR_ARG;
+    if (g.rows == 0) return WF_OK;
+    const int e = dtype_size(g.type), we = dtype_size(g.w_type);
+    if (!g.x || !g.y || !aligned_to(g.x, e) || !aligned_to(g.y, e) || !aligned_to(g.w, we) || !aligned_to(g.b, we) ||
+        !aligned_to(g.mean, 4) || !aligned_to(g.rstd, 4))
+        return WF_ERR_ARG;
     const int rc = check_device();
     if (rc != WF_OK) return rc;
-    NormArgs a{x, w, b, y, mean, rstd, rows, ldx, ldy, rows_per_group, static_cast<int>(d), eps};
+    const NormArgs a{g.x, g.w, g.b, g.y, g.mean, g.rstd, g.rows, g.ldx, g.ldy, g.rows_per_group, static_cast<int>(g.d), g.eps};
     const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    if (type == WF_F32) return dispatch_norm<WF_F32, WF_F32>(a, st);
-    if (type == WF_BF16) return w_type == WF_F32 ? dispatch_norm<WF_BF16, WF_F32>(a, st) : dispatch_norm<WF_BF16, WF_BF16>(a, st);
-    return w_type == WF_F32 ? dispatch_norm<WF_F16, WF_F32>(a, st) : dispatch_norm<WF_F16, WF_F16>(a, st);
+    if (g.type == WF_F32) return dispatch_norm<WF_F32, WF_F32>(a, st);
+    if (g.type == WF_BF16) return g.w_type == WF_F32 ? dispatch_norm<WF_BF16, WF_F32>(a, st) : dispatch_norm<WF_BF16, WF_BF16>(a, st);
+    return g.w_type == WF_F32 ? dispatch_norm<WF_F16, WF_F32>(a, st) : dispatch_norm<WF_F16, WF_F16>(a, st);
 }
 
 extern "C" WF_API int64_t wf_layer_norm_backward_workspace(int64_t rows, int64_t d, int64_t rows_per_group) {
@@ -448,33 +451,36 @@ extern "C" WF_API int64_t wf_layer_norm_backward_workspace(int64_t rows, int64_t
     return 2 * norm_split(rows, rows_per_group, static_cast<int>(d)).partial_rows() * d * static_cast<int64_t>(sizeof(float));
 }
 
-extern "C" WF_API int wf_layer_norm_backward(const void *dy, int64_t lddy, const void *x, int64_t ldx, const void *w,
-                                             int w_type, const float *mean, const float *rstd, void *dx, int64_t lddx,
-                                             void *dw, void *db, int64_t rows, int64_t d, int64_t rows_per_group,
-                                             int type, void *workspace, int64_t workspace_bytes, wf_stream_t stream) {
+extern "C" WF_API int wf_layer_norm_backward(const wf_layer_norm_grad_args *args, wf_stream_t stream) {
     using namespace wf;
-    if (!norm_types_ok(type, w_type)) return WF_ERR_UNSUPPORTED;
-    if (rows < 1 || d < 1 || d > (1 << 30) || rows_per_group < 1 || ldx < d || lddy < d || (dx && lddx < d)) return WF_ERR_ARG;
-    const int e = dtype_size(type), we = dtype_size(w_type);
-    if (!x || !dy || !mean || !rstd || !aligned_to(x, e) || !aligned_to(dy, e) || !aligned_to(dx, e) ||
-        !aligned_to(w, we) || !aligned_to(dw, we) || !aligned_to(db, we))
+    if (args == nullptr) return WF_ERR_ARG;
+    const wf_layer_norm_grad_args &g = *args;
+    if (!norm_types_ok(g.type, g.w_type)) return WF_ERR_UNSUPPORTED;
+    if (g.rows < 1 || g.d < 1 || g.d > (1 << 30) || g.rows_per_group < 1 || g.ldx < g.d || g.lddy < g.d ||
+        (g.dx && g.lddx < g.d))
         return WF_ERR_ARG;
-    if (!dx && !dw && !db) return WF_OK;
-    const RowSplit split = norm_split(rows, rows_per_group, static_cast<int>(d));
-    const int64_t half = split.partial_rows() * d;
-    if ((dw || db) && (!workspace || !aligned_to(workspace, 16) ||
-                       workspace_bytes < 2 * half * static_cast<int64_t>(sizeof(float))))
+    const int e = dtype_size(g.type), we = dtype_size(g.w_type);
+    if (!g.x || !g.dy || !g.mean || !g.rstd || !aligned_to(g.x, e) || !aligned_to(g.dy, e) || !aligned_to(g.dx, e) ||
+        !aligned_to(g.w, we) || !aligned_to(g.dw, we) || !aligned_to(g.db, we) || !aligned_to(g.mean, 4) ||
+        !aligned_to(g.rstd, 4))
         return WF_ERR_ARG;
-    const int rc0 = check_device();
-    if (rc0 != WF_OK) return rc0;
-    float *part = static_cast<float *>(workspace);
-    NormGradArgs a{x, w, dy, mean, rstd, dx, dw ? part : nullptr, db ? part + half : nullptr, rows, ldx, lddy, lddx,
-                   split, static_cast<int>(d)};
-    const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    int rc;
-    if (type == WF_F32) rc = dispatch_norm_grad<WF_F32, WF_F32>(a, st);
-    else if (type == WF_BF16) rc = w_type == WF_F32 ? dispatch_norm_grad<WF_BF16, WF_F32>(a, st) : dispatch_norm_grad<WF_BF16, WF_BF16>(a, st);
-    else rc = w_type == WF_F32 ? dispatch_norm_grad<WF_F16, WF_F32>(a, st) : dispatch_norm_grad<WF_F16, WF_F16>(a, st);
+    if (!g.dx && !g.dw && !g.db) return WF_OK;
+    const RowSplit split = norm_split(g.rows, g.rows_per_group, static_cast<int>(g.d));
+    const int64_t half = split.partial_rows() * g.d;
+    if ((g.dw || g.db) && (!g.workspace || !aligned_to(g.workspace, 16) ||
+                           g.workspace_bytes < 2 * half * static_cast<int64_t>(sizeof(float))))
+        return WF_ERR_ARG;
+    int rc = check_device();
     if (rc != WF_OK) return rc;
-    return reduce_partials(a.part_w, dw, a.part_b, db, split.groups, split.partials_per_group(), d, w_type, st);
+    float *part = static_cast<float *>(g.workspace);
+    const NormGradArgs a{g.x, g.w, g.dy, g.mean, g.rstd, g.dx, g.dw ? part : nullptr, g.db ? part + half : nullptr, g.rows,
+                         g.ldx, g.lddy, g.lddx, split, static_cast<int>(g.d)};
+    const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    if (g.type == WF_F32) rc = dispatch_norm_grad<WF_F32, WF_F32>(a, st);
+    else if (g.type == WF_BF16) rc = g.w_type == WF_F32 ? dispatch_norm_grad<WF_BF16, WF_F32>(a, st) : dispatch_norm_grad<WF_BF16, WF_BF16>(a, st);
+    else rc = g.w_type == WF_F32 ? dispatch_norm_grad<WF_F16, WF_F32>(a, st) : dispatch_norm_grad<WF_F16, WF_F16>(a, st);
+    if (rc != WF_OK) return rc;
+    const int64_t parts = split.partials_per_group();
+    return reduce_partials(PartialSum{a.part_w, g.dw, split.groups, parts}, PartialSum{a.part_b, g.db, split.groups, parts},
+                           g.d, g.w_type, st);
 }

@@ -9,6 +9,7 @@
 // Bound by HBM: dy and z in, dz out.
 
 #include "wf_act.cuh"
+#include "wf_linear.cuh"
 #include "wf_rows.cuh"
 
 namespace wf {
@@ -82,12 +83,18 @@ __global__ void __launch_bounds__(256) linear_grad_kernel(const __grid_constant_
             }
             if constexpr (!ZN) load_z<Z>(z, a, row, col, vec);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                float h = 0.f, slope = 1.f;
-                if constexpr (!ZN) act_slope<ACT>(z[j], h, slope);
-                if constexpr (!ZN) dg[j] = fmaf(dy[j], h, dg[j]);
-                dy[j] *= g[j] * slope;
-                db[j] += dy[j];
+            for (int j = 0; j < 8; j += 2) {
+                float h[2], slope[2] = {1.f, 1.f};
+                if constexpr (!ZN) {
+                    const float v[2] = {z[j], z[j + 1]};
+                    act_slope2<ACT>(v, h, slope);
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    if constexpr (!ZN) dg[j + i] = fmaf(dy[j + i], h[i], dg[j + i]);
+                    dy[j + i] *= g[j + i] * slope[i];
+                    db[j + i] += dy[j + i];
+                }
             }
             if (a.dz != nullptr) {
                 void *dr = row_of<T>(a.dz, row, a.lddz);
@@ -142,45 +149,26 @@ int dispatch_grad_type(const LinearGradArgs &a, int act, int z_type, cudaStream_
 }
 
 }  // namespace
-}  // namespace wf
 
-extern "C" WF_API int64_t wf_linear_backward_act_workspace(int64_t m, int64_t n, int64_t rows_per_group) {
-    using namespace wf;
-    if (m < 1 || n < 1 || rows_per_group < 1) return 0;
+// rows of a group as the kernel takes them: all of them where no group matters
+static int64_t grad_group(const wf_linear_grad_args &g) { return g.gate || g.dg ? g.rows_per_group : g.m; }
+
+int64_t linear_grad_workspace(int64_t m, int64_t n, int64_t rows_per_group) {
     const RowSplit s = grad_split(m, n, rows_per_group);
     return (s.blocks() + s.partial_rows()) * n * static_cast<int64_t>(sizeof(float));
 }
 
-extern "C" WF_API int wf_linear_backward_act(const void *dy, int64_t lddy, const void *z, int64_t ldz, int z_type, int act,
-                                             const void *gate, int64_t rows_per_group, void *dz, int64_t lddz, void *db,
-                                             void *dg, int64_t m, int64_t n, int type, void *workspace,
-                                             int64_t workspace_bytes, wf_stream_t stream) {
-    using namespace wf;
-    if (type != WF_BF16 && type != WF_F16) return WF_ERR_UNSUPPORTED;
-    if (act < WF_ACT_NONE || act > WF_ACT_GELU_TANH) return WF_ERR_UNSUPPORTED;
-    if (z != nullptr && z_type != WF_F32 && z_type != WF_F16 && z_type != type) return WF_ERR_UNSUPPORTED;
-    if (m < 1 || n < 1 || m > (1ll << 30) || n > (1ll << 30) || rows_per_group < 1 || !dy || lddy < n ||
-        (z && ldz < n) || (dz && lddz < n) || ((act != WF_ACT_NONE || dg) && !z))
-        return WF_ERR_ARG;
-    if (!aligned_to(dy, 2) || !aligned_to(dz, 2) || !aligned_to(gate, 2) || !aligned_to(db, 2) || !aligned_to(dg, 2) ||
-        (z && !aligned_to(z, dtype_size(z_type))))
-        return WF_ERR_ARG;
-    if (!dz && !db && !dg) return WF_OK;
-    const RowSplit split = grad_split(m, n, rows_per_group);
-    if ((db || dg) && (!workspace || !aligned_to(workspace, 4) ||
-                       workspace_bytes < wf_linear_backward_act_workspace(m, n, rows_per_group)))
-        return WF_ERR_ARG;
-    int rc = check_device();
+int linear_grad(const wf_linear_grad_args &g, void *dz, int64_t lddz, float *part, cudaStream_t stream) {
+    const RowSplit split = grad_split(g.m, g.n, grad_group(g));
+    const bool vec = aligned_to(g.dy, 16) && g.lddy % 8 == 0 && (!dz || (aligned_to(dz, 16) && lddz % 8 == 0)) &&
+                     (!g.z || (aligned_to(g.z, 16) && g.ldz % 8 == 0));
+    LinearGradArgs a{g.dy, g.z, g.gate, dz, g.db ? part : nullptr, g.dg ? part + split.blocks() * g.n : nullptr, g.lddy,
+                     g.ldz, lddz, g.n, split, vec};
+    const int rc = g.type == WF_BF16 ? dispatch_grad_type<WF_BF16>(a, g.act, g.z_type, stream)
+                                     : dispatch_grad_type<WF_F16>(a, g.act, g.z_type, stream);
     if (rc != WF_OK) return rc;
-    float *part = static_cast<float *>(workspace);
-    const bool vec = aligned_to(dy, 16) && lddy % 8 == 0 && (!dz || (aligned_to(dz, 16) && lddz % 8 == 0)) &&
-                     (!z || (aligned_to(z, 16) && ldz % 8 == 0));
-    LinearGradArgs a{dy, z, gate, dz, db ? part : nullptr, dg ? part + split.blocks() * n : nullptr, lddy, ldz, lddz, n,
-                     split, vec};
-    const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    rc = type == WF_BF16 ? dispatch_grad_type<WF_BF16>(a, act, z_type, st) : dispatch_grad_type<WF_F16>(a, act, z_type, st);
-    if (rc != WF_OK) return rc;
-    rc = reduce_partials(a.part_b, db, nullptr, nullptr, 1, split.blocks(), n, type, st);
-    if (rc != WF_OK) return rc;
-    return reduce_partials(a.part_g, dg, nullptr, nullptr, split.groups, split.partials_per_group(), n, type, st);
+    return reduce_partials(PartialSum{a.part_b, g.db, 1, split.blocks()},
+                           PartialSum{a.part_g, g.dg, split.groups, split.partials_per_group()}, g.n, g.type, stream);
 }
+
+}  // namespace wf

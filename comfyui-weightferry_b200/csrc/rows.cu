@@ -6,9 +6,8 @@ namespace wf {
 namespace {
 
 struct ReduceArgs {
-    const float *part[2];
-    void *out[2];
-    int64_t groups, parts, d;
+    PartialSum sum[2];
+    int64_t d;
 };
 
 // Block (x, y, z): columns 32 x .. 32 x + 31 of groups y, y + gridDim.y, ... of sum z. Eight warps take every eighth
@@ -18,21 +17,19 @@ __global__ void __launch_bounds__(256) reduce_partials_kernel(const __grid_const
     __shared__ float red[8][33];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t col = static_cast<int64_t>(blockIdx.x) * 32 + lane;
-    const float *part = a.part[blockIdx.z];
-    void *out = a.out[blockIdx.z];
+    const PartialSum &sum = a.sum[blockIdx.z];
     wait_prior_grid();
-    if (out == nullptr) return;
-    for (int64_t g = blockIdx.y; g < a.groups; g += gridDim.y) {
+    for (int64_t g = blockIdx.y; g < sum.groups; g += gridDim.y) {
         float s = 0.f;
         if (col < a.d)
 #pragma unroll 8
-            for (int64_t p = warp; p < a.parts; p += 8) s += part[(g * a.parts + p) * a.d + col];
+            for (int64_t p = warp; p < sum.parts; p += 8) s += sum.part[(g * sum.parts + p) * a.d + col];
         red[warp][lane] = s;
         __syncthreads();
         if (warp == 0 && col < a.d) {
 #pragma unroll
             for (int w = 1; w < 8; ++w) s += red[w][lane];
-            store1<T>(row_of<T>(out, g, a.d), col, s);
+            store1<T>(row_of<T>(sum.out, g, a.d), col, s);
         }
         __syncthreads();
     }
@@ -40,16 +37,12 @@ __global__ void __launch_bounds__(256) reduce_partials_kernel(const __grid_const
 
 }  // namespace
 
-int reduce_partials(const float *part0, void *out0, const float *part1, void *out1, int64_t groups, int64_t parts,
-                    int64_t d, int type, cudaStream_t stream) {
-    if (out0 == nullptr && out1 == nullptr) return WF_OK;
-    if (out0 == nullptr) {
-        part0 = part1, out0 = out1;
-        out1 = nullptr;
-    }
-    ReduceArgs a{{part0, part1}, {out0, out1}, groups, parts, d};
-    const dim3 grid(static_cast<unsigned>((d + 31) / 32), static_cast<unsigned>(std::min<int64_t>(groups, 32768)),
-                    out1 != nullptr ? 2 : 1);
+int reduce_partials(const PartialSum &s0, const PartialSum &s1, int64_t d, int type, cudaStream_t stream) {
+    if (s0.out == nullptr && s1.out == nullptr) return WF_OK;
+    ReduceArgs a{{s0.out != nullptr ? s0 : s1, s1}, d};
+    const bool both = s0.out != nullptr && s1.out != nullptr;
+    const int64_t groups = both ? std::max(s0.groups, s1.groups) : a.sum[0].groups;
+    const dim3 grid(static_cast<unsigned>((d + 31) / 32), static_cast<unsigned>(std::min<int64_t>(groups, 32768)), both ? 2 : 1);
     if (type == WF_F32) return launch_rows(reduce_partials_kernel<WF_F32>, grid, 256, stream, a);
     if (type == WF_BF16) return launch_rows(reduce_partials_kernel<WF_BF16>, grid, 256, stream, a);
     return launch_rows(reduce_partials_kernel<WF_F16>, grid, 256, stream, a);

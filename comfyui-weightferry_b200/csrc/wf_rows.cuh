@@ -45,10 +45,15 @@ inline RowSplit make_split(int64_t rows, int64_t rows_per_group, int64_t wanted,
     return s;
 }
 
-// For each of n_sums column sums (1 or 2): out[g, c] = sum over p < parts of part[g * parts + p, c], float32 in a fixed
-// order, rounded once to `type`. A null out is skipped. d columns.
-int reduce_partials(const float *part0, void *out0, const float *part1, void *out1, int64_t groups, int64_t parts,
-                    int64_t d, int type, cudaStream_t stream);
+// A column sum whose parts blocks have written: out[g, c] = sum over p < parts of part[g * parts + p, c] for g < groups.
+// A null out: no such sum.
+struct PartialSum {
+    const float *part;
+    void *out;
+    int64_t groups, parts;
+};
+// Up to two of them over d columns in one launch: float32 in a fixed order, rounded once to `type`.
+int reduce_partials(const PartialSum &s0, const PartialSum &s1, int64_t d, int type, cudaStream_t stream);
 
 namespace {
 

@@ -13,27 +13,24 @@ import torch
 from .. import _ext
 
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}  # gelu: the erf form
-
-
-def _p(t):
-    return 0 if t is None else t.data_ptr()
+_CODES = {torch.float16: _ext.WF_F16, torch.bfloat16: _ext.WF_BF16, torch.float32: _ext.WF_F32}
+_TYPES = (torch.bfloat16, torch.float16)
 
 
 def _operand(t):
     """(tensor, row pitch) of a 2-D operand as the tensor cores' loads need it: values of a row side by side, rows a
     multiple of 8 values apart, 16-byte aligned. A tensor that is not so laid out is copied (odd widths, slices)."""
     rows, cols = t.shape
-    if cols > 1 and t.stride(1) != 1:
-        t = t.contiguous()
-    ld = t.stride(0) if rows > 1 else -(-cols // 8) * 8
-    if t.data_ptr() % 16 == 0 and ld % 8 == 0 and ld >= cols and (cols == 1 or t.stride(1) == 1):
-        return t, ld
-    if rows > 1 and t.stride(0) < cols:  # expanded rows
-        t = t.contiguous()
+    s0, s1 = t.stride()
+    if rows == 1:
+        s0 = -(-cols // 8) * 8
+    if (s1 == 1 or cols == 1) and s0 % 8 == 0 and s0 >= cols and t.data_ptr() % 16 == 0:
+        return t, s0
+    t, s0 = _rows(t)
     ld = -(-cols // 8) * 8
     out = torch.empty((rows, ld), dtype=t.dtype, device=t.device)
-    rc = _ext.lib().wf_copy_rows16(t.data_ptr(), t.stride(0) if rows > 1 else cols, out.data_ptr(), ld, rows, cols,
-                                   _ext.stream_of(t.device))
+    with _ext.on_device(t.device):
+        rc = _ext.lib().wf_copy_rows16(t.data_ptr(), s0, out.data_ptr(), ld, rows, cols, _ext.stream_of(t.device))
     _ext.check(rc, "wf_copy_rows16")
     return out[:, :cols], ld
 
@@ -41,73 +38,90 @@ def _operand(t):
 def _rows(t):
     """(tensor, row pitch) of a 2-D buffer whose rows are read value by value: neighbours side by side, any pitch."""
     rows, cols = t.shape
-    if (cols > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < cols):
-        t = t.contiguous()
-    return t, (t.stride(0) if rows > 1 else cols)
+    s0, s1 = t.stride()
+    if rows == 1:
+        s0 = cols
+    if (s1 != 1 and cols > 1) or s0 < cols:
+        return t.contiguous(), cols
+    return t, s0
+
+
+def _group_rows(what, p, m, rows_per_group):
+    """Rows of x to each row of p ([n], or [groups, n]): as given, or all m rows divided evenly."""
+    groups = 1 if p.dim() == 1 else p.shape[0]
+    if rows_per_group is None:
+        if m % groups:
+            raise ValueError(f"{what}: {groups} rows do not divide {m} rows; give rows_per_group")
+        return max(1, m // groups)
+    if rows_per_group < 1 or (m and groups != -(-m // rows_per_group)):
+        raise ValueError(f"{what}: {groups} rows for {m} rows in groups of {rows_per_group}")
+    return rows_per_group
 
 
 def _check(x, weight, bias, activation, residual, gate, rows_per_group):
-    """(m, n, k, groups, rows per group) of a call, or the reason it is refused."""
+    """(m, n, k, rows per group) of a call; raises for one that is refused."""
+    dtype = x.dtype
+    if dtype not in _TYPES:
+        raise TypeError(f"linear: x is {dtype}; bfloat16 or float16 is needed")
     if activation not in ACTIVATIONS:
         raise ValueError(f"linear: activation {activation!r} is not one of {', '.join(ACTIVATIONS)}")
-    if x.dtype not in (torch.bfloat16, torch.float16):
-        raise TypeError(f"linear: x is {x.dtype}; bfloat16 or float16 is needed")
-    operands = [(nm, t) for nm, t in (("x", x), ("weight", weight), ("bias", bias), ("residual", residual), ("gate", gate))
-                if t is not None]
-    for name, t in operands:
-        if t.dtype != x.dtype:
-            raise TypeError(f"linear: {name} is {t.dtype}, x is {x.dtype}")
-    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
-        raise ValueError(f"linear: x {tuple(x.shape)} and weight {tuple(weight.shape)} do not match")
-    n, k = weight.shape
+    rest = [(nm, t) for nm, t in (("weight", weight), ("bias", bias), ("residual", residual), ("gate", gate)) if t is not None]
+    for nm, t in rest:
+        if t.dtype != dtype:
+            raise TypeError(f"linear: {nm} is {t.dtype}, x is {dtype}")
+    shape, w_shape = x.shape, weight.shape
+    if len(shape) < 1 or len(w_shape) != 2 or shape[-1] != w_shape[1]:
+        raise ValueError(f"linear: x {tuple(shape)} and weight {tuple(w_shape)} do not match")
+    n, k = w_shape
     if k < 1:
         raise ValueError("linear: a layer without inputs")
     m = x.numel() // k
-    groups = 1
-    if bias is not None and tuple(bias.shape) != (n,):
+    if bias is not None and bias.shape != (n,):
         raise ValueError(f"linear: bias {tuple(bias.shape)} for {n} outputs")
-    if residual is not None and tuple(residual.shape) != (*x.shape[:-1], n):
-        raise ValueError(f"linear: residual {tuple(residual.shape)} for an output {(*x.shape[:-1], n)}")
-    if gate is None:
-        if rows_per_group is not None:
-            raise ValueError("linear: rows_per_group without a gate")
-        rows_per_group = max(1, m)
-    else:
+    if residual is not None and residual.shape != (*shape[:-1], n):
+        raise ValueError(f"linear: residual {tuple(residual.shape)} for an output {(*shape[:-1], n)}")
+    if gate is not None:
         if gate.dim() not in (1, 2) or gate.shape[-1] != n or (gate.dim() == 2 and gate.shape[0] == 0):
             raise ValueError(f"linear: gate {tuple(gate.shape)} for {n} outputs")
-        groups = 1 if gate.dim() == 1 else gate.shape[0]
-        if rows_per_group is None:
-            if m % groups:
-                raise ValueError(f"linear: {groups} gate rows do not divide {m} rows; give rows_per_group")
-            rows_per_group = max(1, m // groups)
-        elif rows_per_group < 1 or (m and groups != -(-m // rows_per_group)):
-            raise ValueError(f"linear: {groups} gate rows for {m} rows in groups of {rows_per_group}")
-    for name, t in operands:
-        if not t.is_cuda or t.device != x.device:
-            raise ValueError(f"linear: {name} is on {t.device}, x on {x.device}; one CUDA device is needed")
-    return m, n, k, groups, rows_per_group
+        rows_per_group = _group_rows("linear: gate", gate, m, rows_per_group)
+    elif rows_per_group is not None:
+        raise ValueError("linear: rows_per_group without a gate")
+    index = x.get_device()
+    for nm, t in rest:
+        if t.get_device() != index:
+            raise ValueError(f"linear: {nm} is on {t.device}, x on {x.device}")
+    if index < 0:
+        raise ValueError(f"linear: x is on {x.device}; a CUDA device is needed")
+    return m, n, k, rows_per_group or max(1, m)
 
 
-def _forward(x2, w, bias, act, r2, gate, rpg, m, n, k, z=None):
-    """(y [m, n], x's operand, weight's operand); z: a [m, n] tensor for the pre-activation, or None."""
-    y = torch.empty((m, n), dtype=x2.dtype, device=x2.device)
+def _forward(x, weight, bias, act, residual, gate, rpg, m, n, k, kept=None):
+    """(y, x's operand, weight's operand, the pre-activation as type `kept` or None)"""
+    lead = x.shape[:-1]
+    y = x.new_empty((*lead, n))
     if m == 0 or n == 0:
-        return y, x2, w
-    xo, ldx = _operand(x2)
-    wo, ldw = _operand(w)
+        return y, None, None, None
+    xo, ldx = _operand(x if len(lead) == 1 else x.reshape(m, k))
+    wo, ldw = _operand(weight)
+    p_bias = p_gate = p_res = p_z = ldr = ldz = 0
+    z = None
     if bias is not None:
         bias = bias.contiguous()
+        p_bias = bias.data_ptr()
     if gate is not None:
         gate = gate.contiguous()
-    ldr = 0
-    if r2 is not None:
-        r2, ldr = _rows(r2)
-    rc = _ext.lib().wf_linear(xo.data_ptr(), ldx, wo.data_ptr(), ldw, _p(bias), act, _p(gate), rpg, _p(r2), ldr,
-                              y.data_ptr(), n, _p(z), z.stride(0) if z is not None else 0,
-                              _ext.dtype_code(z.dtype) if z is not None else 0, m, n, k, _ext.dtype_code(x2.dtype),
-                              _ext.stream_of(x2.device))
-    _ext.check(rc, "wf_linear")
-    return y, xo, wo
+        p_gate = gate.data_ptr()
+    if residual is not None:
+        residual, ldr = _rows(residual if len(lead) == 1 else residual.reshape(m, n))
+        p_res = residual.data_ptr()
+    if kept is not None:
+        ldz = -(-n // 8) * 8
+        z = torch.empty((m, ldz), dtype=kept, device=x.device)
+        p_z = z.data_ptr()
+    _ext.launch("wf_linear", _ext.LINEAR_ARGS.pack(
+        xo.data_ptr(), wo.data_ptr(), p_bias, p_gate, p_res, y.data_ptr(), p_z, ldx, ldw, ldr, n, ldz, rpg, m, n, k, act,
+        _CODES[x.dtype], _CODES[kept] if kept is not None else 0, 0), x.get_device())
+    return y, xo, wo, z
 
 
 def _kept_dtype(act, need_z, need_gate, dtype):
@@ -121,75 +135,43 @@ def _kept_dtype(act, need_z, need_gate, dtype):
 
 class _Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, residual, gate, act, rpg, m, n, k, groups):
-        need_x, need_w, need_b, need_r, need_g = ctx.needs_input_grad[:5]
-        kept = _kept_dtype(act, need_x or need_w or need_b, need_g, x.dtype)
-        with _ext.on_device(x.device):
-            z = None
-            if kept is not None:
-                z = torch.empty((m, -(-n // 8) * 8), dtype=kept, device=x.device)
-            y, xo, wo = _forward(x.reshape(m, k), weight, bias, act, None if residual is None else residual.reshape(m, n),
-                                 gate, rpg, m, n, k, z)
-        ctx.save_for_backward(xo if need_w else None, wo if need_x else None,
-                              gate if need_x or need_w or need_b else None, z)
-        ctx.sizes = (act, rpg, m, n, k, groups)
-        ctx.shapes = (x.shape, x.dtype, x.device, None if gate is None else gate.shape)
-        return y.view(*x.shape[:-1], n)
+    def forward(ctx, x, weight, bias, residual, gate, act, rpg, m, n, k):
+        need_x, need_w, need_b, _need_r, need_g = ctx.needs_input_grad[:5]
+        need_z = need_x or need_w or need_b
+        y, xo, wo, z = _forward(x, weight, bias, act, residual, gate, rpg, m, n, k,
+                                _kept_dtype(act, need_z, need_g, x.dtype))
+        ctx.save_for_backward(xo if need_w else None, wo if need_x else None, gate if need_z else None, z)
+        ctx.call = (act, rpg, m, n, k, x.shape, x.dtype, x.device, None if gate is None else gate.shape)
+        return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         xo, wo, gate, z = ctx.saved_tensors
-        act, rpg, m, n, k, groups = ctx.sizes
-        x_shape, dtype, device, gate_shape = ctx.shapes
+        act, rpg, m, n, k, x_shape, dtype, device, gate_shape = ctx.call
         need_x, need_w, need_b, need_r, need_g = ctx.needs_input_grad[:5]
-        dx = dw = db = dg = None
-        if m == 0 or n == 0:
-            zeros = dict(dtype=dtype, device=device)
-            return (torch.zeros(x_shape, **zeros) if need_x else None, torch.zeros((n, k), **zeros) if need_w else None,
-                    torch.zeros((n,), **zeros) if need_b else None, dy if need_r else None,
-                    torch.zeros(gate_shape, **zeros) if need_g else None, None, None, None, None, None, None)
-        lib, code, stream = _ext.lib(), _ext.dtype_code(dtype), _ext.stream_of(device)
-        with _ext.on_device(device):
-            dy2, lddy = _rows(dy.reshape(m, n))
-            dz, lddz = None, 0
-            if need_x or need_w:
-                if act == 0 and gate is None:
-                    if dy2.data_ptr() % 16 == 0 and lddy % 8 == 0:
-                        dz, lddz = dy2, lddy
-                make = dz is None
-                if make:
-                    lddz = -(-n // 8) * 8
-                    dz = torch.empty((m, lddz), dtype=dtype, device=device)
-            else:
-                make = False
-            if make or need_b or need_g:
-                if need_b:
-                    db = torch.empty((n,), dtype=dtype, device=device)
-                if need_g:
-                    dg = torch.empty((groups, n), dtype=dtype, device=device)
-                size = lib.wf_linear_backward_act_workspace(m, n, rpg) if need_b or need_g else 0
-                work = torch.empty(size, dtype=torch.uint8, device=device) if size else None
-                gc = None if gate is None else gate.contiguous()
-                rc = lib.wf_linear_backward_act(
-                    dy2.data_ptr(), lddy, _p(z), z.stride(0) if z is not None else 0,
-                    _ext.dtype_code(z.dtype) if z is not None else 0, act, _p(gc), rpg, _p(dz) if make else 0, lddz,
-                    _p(db), _p(dg), m, n, code, _p(work), size, stream)
-                _ext.check(rc, "wf_linear_backward_act")
-            if need_x:
-                dx = torch.empty((m, k), dtype=dtype, device=device)
-                rc = lib.wf_linear_backward_input(dz.data_ptr(), lddz, wo.data_ptr(), wo.stride(0) if n > 1 else -(-k // 8) * 8,
-                                                  dx.data_ptr(), k, m, n, k, code, stream)
-                _ext.check(rc, "wf_linear_backward_input")
-                dx = dx.view(x_shape)
-            if need_w:
-                dw = torch.empty((n, k), dtype=dtype, device=device)
-                rc = lib.wf_linear_backward_weight(dz.data_ptr(), lddz, xo.data_ptr(), xo.stride(0) if m > 1 else -(-k // 8) * 8,
-                                                   dw.data_ptr(), k, m, n, k, code, stream)
-                _ext.check(rc, "wf_linear_backward_weight")
-        if dg is not None:
-            dg = dg.view(gate_shape)
-        return dx, dw, db, dy if need_r else None, dg, None, None, None, None, None, None
+        new = torch.empty if m and n else torch.zeros
+        dx = new(x_shape, dtype=dtype, device=device) if need_x else None
+        dw = new((n, k), dtype=dtype, device=device) if need_w else None
+        db = new((n,), dtype=dtype, device=device) if need_b else None
+        dg = new(gate_shape, dtype=dtype, device=device) if need_g else None
+        if m and n and (need_x or need_w or need_b or need_g):
+            dy2, lddy = _rows(dy if dy.dim() == 2 else dy.reshape(m, n))
+            size = _ext.lib().wf_linear_backward_workspace(m, n, rpg)
+            work = torch.empty(size, dtype=torch.uint8, device=device)
+            if gate is not None:
+                gate = gate.contiguous()
+
+            def at(t):
+                return 0 if t is None else t.data_ptr()
+
+            def pitch(t):  # of an operand of a product, as _operand has it
+                return 0 if t is None else t.stride(0) if t.shape[0] > 1 else -(-k // 8) * 8
+            _ext.launch("wf_linear_backward", _ext.LINEAR_GRAD_ARGS.pack(
+                dy2.data_ptr(), at(xo), at(wo), at(z), at(gate), at(dx), at(dw), at(db), at(dg), work.data_ptr(), lddy,
+                pitch(xo), pitch(wo), 0 if z is None else z.stride(0), k, k, rpg, size, m, n, k, act, _CODES[dtype],
+                0 if z is None else _CODES[z.dtype], 0), device.index)
+        return dx, dw, db, dy if need_r else None, dg, None, None, None, None, None
 
 
 def linear(x, weight, bias=None, activation="none", residual=None, gate=None, rows_per_group=None):
@@ -200,14 +182,12 @@ def linear(x, weight, bias=None, activation="none", residual=None, gate=None, ro
     group may be short). All of one type, bfloat16 or float16, on one CUDA device; any strides (rows whose pitch is a
     multiple of 8 values are read in place, others are copied first). activation: a name of ``ACTIVATIONS``. Returns a
     new contiguous [..., n]. Differentiable once in every tensor."""
-    m, n, k, groups, rpg = _check(x, weight, bias, activation, residual, gate, rows_per_group)
+    m, n, k, rpg = _check(x, weight, bias, activation, residual, gate, rows_per_group)
     act = ACTIVATIONS[activation]
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual, gate)):
-        return _Linear.apply(x, weight, bias, residual, gate, act, rpg, m, n, k, groups)
-    with _ext.on_device(x.device):
-        y, _, _ = _forward(x.reshape(m, k), weight, bias, act, None if residual is None else residual.reshape(m, n), gate,
-                           rpg, m, n, k)
-    return y.view(*x.shape[:-1], n)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or any(
+            t is not None and t.requires_grad for t in (bias, residual, gate))):
+        return _Linear.apply(x, weight, bias, residual, gate, act, rpg, m, n, k)
+    return _forward(x, weight, bias, act, residual, gate, rpg, m, n, k)[0]
 
 
 def status():

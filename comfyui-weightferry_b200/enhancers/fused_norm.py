@@ -11,105 +11,101 @@ It launches on the current stream and allocates with PyTorch's allocator."""
 import torch
 
 from .. import _ext
+from .fused_linear import _CODES, _group_rows, _rows
 
-
-def _p(t):
-    return 0 if t is None else t.data_ptr()
-
-
-def _rows(t):
-    """(tensor, row pitch) of a 2-D tensor with a row's values side by side."""
-    rows, cols = t.shape
-    if (cols > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < cols):
-        t = t.contiguous()
-    return t, (t.stride(0) if rows > 1 else cols)
+_TYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
 def _check(x, weight, bias, eps, rows_per_group):
-    """(rows, width, groups, rows per group) of a call, or the reason it is refused."""
-    if x.dtype not in (torch.bfloat16, torch.float16, torch.float32):
-        raise TypeError(f"layer_norm: x is {x.dtype}; bfloat16, float16 or float32 is needed")
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError(f"layer_norm: x {tuple(x.shape)} has no values to normalise")
+    """(rows, width, rows per group) of a call; raises for one that is refused."""
+    dtype, shape = x.dtype, x.shape
+    if dtype not in _TYPES:
+        raise TypeError(f"layer_norm: x is {dtype}; bfloat16, float16 or float32 is needed")
+    if len(shape) < 1 or shape[-1] < 1:
+        raise ValueError(f"layer_norm: x {tuple(shape)} has no values to normalise")
     if not eps >= 0:
         raise ValueError(f"layer_norm: eps {eps}")
-    d = x.shape[-1]
+    d = shape[-1]
     m = x.numel() // d
+    index = x.get_device()
     p = weight if weight is not None else bias
-    if p is None and rows_per_group is not None:
+    if p is not None:
+        for nm, t in (("weight", weight), ("bias", bias)):
+            if t is None:
+                continue
+            if (t.dtype != dtype and t.dtype != torch.float32) or t.dtype != p.dtype:
+                raise TypeError(f"layer_norm: {nm} is {t.dtype}; {dtype} or float32 is needed, weight and bias alike")
+            if t.dim() not in (1, 2) or t.shape[-1] != d or t.shape != p.shape or t.shape[0] == 0:
+                raise ValueError(f"layer_norm: {nm} {tuple(t.shape)} for rows of {d}")
+            if t.get_device() != index:
+                raise ValueError(f"layer_norm: {nm} is on {t.device}, x on {x.device}")
+        rows_per_group = _group_rows("layer_norm: weight", p, m, rows_per_group)
+    elif rows_per_group is not None:
         raise ValueError("layer_norm: rows_per_group without weight or bias")
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is None:
-            continue
-        if t.dtype not in (x.dtype, torch.float32) or t.dtype != p.dtype:
-            raise TypeError(f"layer_norm: {name} is {t.dtype}; {x.dtype} or float32 is needed, weight and bias alike")
-        if t.dim() not in (1, 2) or t.shape[-1] != d or t.shape != p.shape or t.numel() == 0:
-            raise ValueError(f"layer_norm: {name} {tuple(t.shape)} for rows of {d}")
-        if t.device != x.device:
-            raise ValueError(f"layer_norm: {name} is on {t.device}, x on {x.device}")
-    groups = 1 if p is None or p.dim() == 1 else p.shape[0]
-    if rows_per_group is None:
-        if m % groups:
-            raise ValueError(f"layer_norm: {groups} weight rows do not divide {m} rows; give rows_per_group")
-        rows_per_group = max(1, m // groups)
-    elif rows_per_group < 1 or (m and groups != -(-m // rows_per_group)):
-        raise ValueError(f"layer_norm: {groups} weight rows for {m} rows in groups of {rows_per_group}")
-    if not x.is_cuda:
+    if index < 0:
         raise ValueError(f"layer_norm: x is on {x.device}; a CUDA device is needed")
-    return m, d, groups, rows_per_group
+    return m, d, rows_per_group or max(1, m)
 
 
 def _forward(x, weight, bias, eps, rpg, m, d, keep):
-    """(y like x, x's rows, mean, rstd); mean and rstd None unless they are to be kept."""
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    x2, ldx = _rows(x.reshape(m, d))
-    stats = torch.empty((2, m), dtype=torch.float32, device=x.device) if keep else None
-    weight = None if weight is None else weight.contiguous()
-    bias = None if bias is None else bias.contiguous()
-    p = weight if weight is not None else bias
-    rc = _ext.lib().wf_layer_norm(x2.data_ptr(), ldx, _p(weight), _p(bias), _ext.dtype_code(x.dtype if p is None else p.dtype),
-                                  y.data_ptr(), d, _p(stats), stats[1].data_ptr() if keep else 0, m, d, rpg, float(eps),
-                                  _ext.dtype_code(x.dtype), _ext.stream_of(x.device))
-    _ext.check(rc, "wf_layer_norm")
-    return y, x2, stats
+    """(y, x's rows, their pitch, the statistics [2, m] or None)"""
+    y = x.new_empty(x.shape)
+    if m == 0:
+        return y, None, d, None
+    x2, ldx = _rows(x if x.dim() == 2 else x.reshape(m, d))
+    p_w = p_b = p_mean = 0
+    code = w_code = _CODES[x.dtype]
+    stats = None
+    if bias is not None:
+        bias = bias.contiguous()
+        p_b, w_code = bias.data_ptr(), _CODES[bias.dtype]
+    if weight is not None:
+        weight = weight.contiguous()
+        p_w, w_code = weight.data_ptr(), _CODES[weight.dtype]
+    if keep:
+        stats = torch.empty((2, m), dtype=torch.float32, device=x.device)
+        p_mean = stats.data_ptr()
+    _ext.launch("wf_layer_norm", _ext.LAYER_NORM_ARGS.pack(
+        x2.data_ptr(), p_w, p_b, y.data_ptr(), p_mean, p_mean + 4 * m if keep else 0, ldx, d, m, d, rpg, eps, code, w_code,
+        0), x.get_device())
+    return y, x2, ldx, stats
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, rpg, m, d):
-        with _ext.on_device(x.device):
-            y, x2, stats = _forward(x, weight, bias, eps, rpg, m, d, True)
+        y, x2, ldx, stats = _forward(x, weight, bias, eps, rpg, m, d, True)
         ctx.save_for_backward(x2, weight, stats)
         p = weight if weight is not None else bias
-        ctx.sizes = (rpg, m, d, x.shape, None if p is None else p.shape, x.dtype if p is None else p.dtype)
+        ctx.call = (rpg, m, d, ldx, x.shape, x.dtype, x.device, None if p is None else p.shape,
+                    x.dtype if p is None else p.dtype)
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         x2, weight, stats = ctx.saved_tensors
-        rpg, m, d, shape, p_shape, p_dtype = ctx.sizes
+        rpg, m, d, ldx, shape, dtype, device, p_shape, p_dtype = ctx.call
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        dev = x2.device
-        if m == 0:
-            zeros = dict(dtype=p_dtype, device=dev)
-            return (torch.zeros(shape, dtype=x2.dtype, device=dev) if need_x else None,
-                    torch.zeros(p_shape, **zeros) if need_w else None, torch.zeros(p_shape, **zeros) if need_b else None,
-                    None, None, None, None)
-        lib = _ext.lib()
-        with _ext.on_device(dev):
-            dy2, lddy = _rows(dy.reshape(m, d))
-            _, ldx = _rows(x2)
-            dx = torch.empty(shape, dtype=x2.dtype, device=dev) if need_x else None
-            dw = torch.empty(p_shape, dtype=p_dtype, device=dev) if need_w else None
-            db = torch.empty(p_shape, dtype=p_dtype, device=dev) if need_b else None
-            size = lib.wf_layer_norm_backward_workspace(m, d, rpg) if need_w or need_b else 0
-            work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-            w = None if weight is None else weight.contiguous()
-            rc = lib.wf_layer_norm_backward(dy2.data_ptr(), lddy, x2.data_ptr(), ldx, _p(w), _ext.dtype_code(p_dtype),
-                                            stats.data_ptr(), stats[1].data_ptr(), _p(dx), d, _p(dw), _p(db), m, d, rpg,
-                                            _ext.dtype_code(x2.dtype), _p(work), size, _ext.stream_of(dev))
-            _ext.check(rc, "wf_layer_norm_backward")
+        new = torch.empty if m else torch.zeros
+        dx = new(shape, dtype=dtype, device=device) if need_x else None
+        dw = new(p_shape, dtype=p_dtype, device=device) if need_w else None
+        db = new(p_shape, dtype=p_dtype, device=device) if need_b else None
+        if m:
+            dy2, lddy = _rows(dy if dy.dim() == 2 else dy.reshape(m, d))
+            size, work = 0, None
+            if need_w or need_b:
+                size = _ext.lib().wf_layer_norm_backward_workspace(m, d, rpg)
+                work = torch.empty(size, dtype=torch.uint8, device=device)
+            if weight is not None:
+                weight = weight.contiguous()
+
+            def at(t):
+                return 0 if t is None else t.data_ptr()
+            mean = stats.data_ptr()
+            _ext.launch("wf_layer_norm_backward", _ext.LAYER_NORM_GRAD_ARGS.pack(
+                dy2.data_ptr(), x2.data_ptr(), at(weight), mean, mean + 4 * m, at(dx), at(dw), at(db), at(work), lddy, ldx,
+                d, m, d, rpg, size, _CODES[dtype], _CODES[p_dtype]), device.index)
         return dx, dw, db, None, None, None, None
 
 
@@ -119,8 +115,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-6, rows_per_group=None):
     weight and bias: None, [d], or [groups, d] whose row g holds for rows g * rows_per_group .. of x (rows_per_group: all
     rows divided evenly where it is not given; the last group may be short); of x's type or float32, both alike. Returns a
     new contiguous tensor of x's shape and type. Differentiable once in x, weight and bias."""
-    m, d, _groups, rpg = _check(x, weight, bias, eps, rows_per_group)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+    m, d, rpg = _check(x, weight, bias, eps, rows_per_group)
+    if torch.is_grad_enabled() and (x.requires_grad or any(t is not None and t.requires_grad for t in (weight, bias))):
         return _LayerNorm.apply(x, weight, bias, eps, rpg, m, d)
-    with _ext.on_device(x.device):
-        return _forward(x, weight, bias, eps, rpg, m, d, False)[0]
+    return _forward(x, weight, bias, eps, rpg, m, d, False)[0]

@@ -192,36 +192,39 @@ WF_API int wf_w8a8_linear_noalloc(const void *x, const int8_t *wq, const float *
 /* ---------------------------------------------------------------------------------------- dense linear layer
  * bf16 / f16 weights (what the GGUF dequantisation produces) with the bias, the activation and the gated residual in
  * the product's epilogue, and the backward pass. Row-major matrices of one 16-bit type (`type`: WF_F16 or WF_BF16) with
- * a row pitch in values; the operands of a product (x, w, dz) need 16-byte aligned bases and pitches that are multiples
- * of 8 (wf_copy_rows16 makes such a copy), all other buffers only their element's alignment. No reference counterpart:
- * the reference leaves these layers to PyTorch. */
+ * a row pitch in values; the operands of a product (x, w, and dy where it is one) need 16-byte aligned bases and pitches
+ * that are multiples of 8 (wf_copy_rows16 makes such a copy), all other buffers only their element's alignment. No
+ * reference counterpart: the reference leaves these layers to PyTorch. */
 
 enum { WF_ACT_NONE = 0, WF_ACT_RELU = 1, WF_ACT_SILU = 2, WF_ACT_GELU = 3 /* erf */, WF_ACT_GELU_TANH = 4 };
 
 /* y[r, j] = resid[r, j] + gate[r / rows_per_group, j] * act(z[r, j]), z = x w^T + bias: x [m, k], w [n, k], bias [n],
- * gate [ceil(m / rows_per_group), n], resid and y [m, n]; bias, gate and resid may be NULL (0, 1, 0). float32 throughout,
- * one rounding to y. z (may be NULL) keeps the pre-activation for the backward pass as z_type: WF_F32, `type`, or
- * WF_F16 under bf16 (clamped to f16's range, for the activation's slope only). y may be resid. m, n >= 0, k >= 1. */
-WF_API int wf_linear(const void *x, int64_t ldx, const void *w, int64_t ldw, const void *bias, int act,
-                     const void *gate, int64_t rows_per_group, const void *resid, int64_t ld_resid, void *y,
-                     int64_t ldy, void *z, int64_t ldz, int z_type, int64_t m, int64_t n, int64_t k, int type,
-                     wf_stream_t stream);
+ * gate [ceil(m / rows_per_group), n] contiguous, resid and y [m, n]; bias, gate and resid may be NULL (0, 1, 0). float32
+ * throughout, one rounding to y. z (may be NULL) keeps the pre-activation for the backward pass as z_type: WF_F32,
+ * `type`, or WF_F16 under bf16 (clamped to f16's range, for the activation's slope only). y may be resid. m, n >= 0,
+ * k >= 1. */
+typedef struct wf_linear_args {
+    const void *x, *w, *bias, *gate, *resid;
+    void *y, *z;
+    int64_t ldx, ldw, ld_resid, ldy, ldz, rows_per_group, m, n, k;
+    int32_t act, type, z_type, reserved;
+} wf_linear_args;
+WF_API int wf_linear(const wf_linear_args *args, wf_stream_t stream);
 
-/* The element-wise half of the backward pass: dz = dy * gate * act'(z), db [n] = sum of dz over the rows, dg [groups, n]
- * = sum of dy * act(z) over each group's rows (float32 sums in a fixed order, from unrounded values). dz, db and dg may
- * be NULL; z may be NULL when act is WF_ACT_NONE and dg is NULL. m, n >= 1. db and dg need a workspace of
- * wf_linear_backward_act_workspace bytes (4-byte aligned) for the duration of the call's work on the stream. */
-WF_API int64_t wf_linear_backward_act_workspace(int64_t m, int64_t n, int64_t rows_per_group);
-WF_API int wf_linear_backward_act(const void *dy, int64_t lddy, const void *z, int64_t ldz, int z_type, int act,
-                                  const void *gate, int64_t rows_per_group, void *dz, int64_t lddz, void *db, void *dg,
-                                  int64_t m, int64_t n, int type, void *workspace, int64_t workspace_bytes,
-                                  wf_stream_t stream);
-
-/* dx [m, k] = dz w and dw [n, k] = dz^T x: dz [m, n], w [n, k], x [m, k]. */
-WF_API int wf_linear_backward_input(const void *dz, int64_t lddz, const void *w, int64_t ldw, void *dx, int64_t lddx,
-                                    int64_t m, int64_t n, int64_t k, int type, wf_stream_t stream);
-WF_API int wf_linear_backward_weight(const void *dz, int64_t lddz, const void *x, int64_t ldx, void *dw, int64_t lddw,
-                                     int64_t m, int64_t n, int64_t k, int type, wf_stream_t stream);
+/* The gradients of the forward pass above from dy [m, n] and what it kept: with dz = dy * gate * act'(z),
+ *   dx [m, k] = dz w,  dw [n, k] = dz^T x,  db [n] = sum of dz over the rows,  dg [groups, n] = sum of dy * act(z) over
+ * each group's rows. Each result may be NULL, and so may what it does not need (x without dw, w without dx, z where act
+ * is WF_ACT_NONE and dg NULL). dz is rounded to `type` for the two products; the sums are float32, of unrounded values,
+ * in a fixed order. m, n, k >= 1. workspace (16-byte aligned) holds wf_linear_backward_workspace bytes for the duration
+ * of the call's work on the stream: dz, unless the products can read dy itself, and partial sums. */
+typedef struct wf_linear_grad_args {
+    const void *dy, *x, *w, *z, *gate;
+    void *dx, *dw, *db, *dg, *workspace;
+    int64_t lddy, ldx, ldw, ldz, lddx, lddw, rows_per_group, workspace_bytes, m, n, k;
+    int32_t act, type, z_type, reserved;
+} wf_linear_grad_args;
+WF_API int64_t wf_linear_backward_workspace(int64_t m, int64_t n, int64_t rows_per_group);
+WF_API int wf_linear_backward(const wf_linear_grad_args *args, wf_stream_t stream);
 
 /* Status word of the dense linear layer's kernels, as wf_w8a8_gemm_status. Reading it synchronises and clears it. */
 WF_API int wf_linear_status(int *status);
@@ -237,17 +240,28 @@ WF_API int wf_copy_rows16(const void *src, int64_t ld_src, void *dst, int64_t ld
 
 /* y = (x - mean) * rstd * w + b, rstd = 1 / sqrt(var + eps); w and b may be NULL. mean and rstd [rows] float32 (both or
  * neither NULL) are kept for the backward pass. y may be x. rows >= 0, d >= 1. */
-WF_API int wf_layer_norm(const void *x, int64_t ldx, const void *w, const void *b, int w_type, void *y, int64_t ldy,
-                         float *mean, float *rstd, int64_t rows, int64_t d, int64_t rows_per_group, float eps, int type,
-                         wf_stream_t stream);
+typedef struct wf_layer_norm_args {
+    const void *x, *w, *b;
+    void *y;
+    float *mean, *rstd;
+    int64_t ldx, ldy, rows, d, rows_per_group;
+    float eps;
+    int32_t type, w_type, reserved;
+} wf_layer_norm_args;
+WF_API int wf_layer_norm(const wf_layer_norm_args *args, wf_stream_t stream);
 
-/* dx, and dw and db (of w_type, one row of d a group) of the forward pass above; each may be NULL. rows >= 1. dw and db
- * need a workspace of wf_layer_norm_backward_workspace bytes (16-byte aligned) for the duration of the call's work. */
+/* dx, and dw and db (of w_type, one row of d a group) of the forward pass above from dy and the kept mean and rstd; each
+ * may be NULL. rows >= 1. dw and db need a workspace (16-byte aligned) of wf_layer_norm_backward_workspace bytes for the
+ * duration of the call's work on the stream. */
+typedef struct wf_layer_norm_grad_args {
+    const void *dy, *x, *w;
+    const float *mean, *rstd;
+    void *dx, *dw, *db, *workspace;
+    int64_t lddy, ldx, lddx, rows, d, rows_per_group, workspace_bytes;
+    int32_t type, w_type;
+} wf_layer_norm_grad_args;
 WF_API int64_t wf_layer_norm_backward_workspace(int64_t rows, int64_t d, int64_t rows_per_group);
-WF_API int wf_layer_norm_backward(const void *dy, int64_t lddy, const void *x, int64_t ldx, const void *w, int w_type,
-                                  const float *mean, const float *rstd, void *dx, int64_t lddx, void *dw, void *db,
-                                  int64_t rows, int64_t d, int64_t rows_per_group, int type, void *workspace,
-                                  int64_t workspace_bytes, wf_stream_t stream);
+WF_API int wf_layer_norm_backward(const wf_layer_norm_grad_args *args, wf_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -64,16 +64,21 @@ ARG, UNSUPPORTED = -1, -2
 P = 4096  # an aligned address that no refused call reads
 
 
+def _call(name, layout, fields, kw):
+    assert set(kw) <= set(fields), kw
+    ext = wf("_ext")
+    return getattr(ext.lib(), name)(getattr(ext, layout).pack(*{**fields, **kw}.values()), None)
+
+
 def _linear(**kw):
-    a = dict(x=P, ldx=64, w=P, ldw=64, bias=None, act=0, gate=None, rpg=1, resid=None, ldr=0, y=P, ldy=32, z=None, ldz=0,
-             zt=0, m=4, n=32, k=64, type=1, st=None)
-    a.update(kw)
-    return wf("_ext").lib().wf_linear(*a.values())
+    return _call("wf_linear", "LINEAR_ARGS", dict(
+        x=P, w=P, bias=0, gate=0, resid=0, y=P, z=0, ldx=64, ldw=64, ldr=0, ldy=32, ldz=0, rpg=1, m=4, n=32, k=64, act=0,
+        type=1, zt=0, reserved=0), kw)
 
 
 @pytest.mark.parametrize("kw,rc", [
     (dict(type=2), UNSUPPORTED), (dict(act=5), UNSUPPORTED), (dict(act=-1), UNSUPPORTED), (dict(m=-1), ARG), (dict(k=0), ARG),
-    (dict(n=1 << 31), ARG), (dict(x=None), ARG), (dict(x=P + 8), ARG), (dict(ldx=60), ARG), (dict(ldx=68), ARG),
+    (dict(n=1 << 31), ARG), (dict(x=0), ARG), (dict(x=P + 8), ARG), (dict(ldx=60), ARG), (dict(ldx=68), ARG),
     (dict(ldw=56), ARG), (dict(w=P + 2), ARG), (dict(ldy=31), ARG), (dict(y=P + 1), ARG), (dict(gate=P, rpg=0), ARG),
     (dict(resid=P, ldr=8), ARG), (dict(z=P, ldz=8), ARG), (dict(z=P, ldz=32, zt=3), UNSUPPORTED), (dict(m=0), 0), (dict(n=0), 0),
 ])
@@ -84,19 +89,18 @@ def test_c_linear_refuses(kw, rc):
 def test_c_linear_backward_refuses():
     lib = wf("_ext").lib()
 
-    def grad(dy=P, lddy=32, z=P, ldz=32, zt=0, act=3, gate=None, rpg=4, dz=P, lddz=32, db=None, dg=None, m=4, n=32, type=1,
-             ws=None, size=0):
-        return lib.wf_linear_backward_act(dy, lddy, z, ldz, zt, act, gate, rpg, dz, lddz, db, dg, m, n, type, ws, size, None)
-    assert grad(type=2) == UNSUPPORTED and grad(act=9) == UNSUPPORTED
-    for bad in (dict(m=0), dict(n=0), dict(dy=None), dict(lddy=31), dict(ldz=31), dict(lddz=31), dict(z=None), dict(rpg=0),
-                dict(db=P), dict(dg=P, ws=P, size=4), dict(dy=P + 1), dict(act=0, z=None, dg=P)):
+    def grad(**kw):
+        return _call("wf_linear_backward", "LINEAR_GRAD_ARGS", dict(
+            dy=P, x=P, w=P, z=P, gate=0, dx=P, dw=P, db=0, dg=0, ws=P, lddy=32, ldx=64, ldw=64, ldz=32, lddx=64, lddw=64,
+            rpg=4, size=1 << 20, m=4, n=32, k=64, act=3, type=1, zt=0, reserved=0), kw)
+    assert grad(type=2) == UNSUPPORTED and grad(act=9) == UNSUPPORTED and grad(zt=7) == UNSUPPORTED
+    for bad in (dict(m=0), dict(n=0), dict(k=0), dict(dy=0), dict(lddy=31), dict(ldz=31), dict(z=0), dict(rpg=0), dict(ws=0),
+                dict(size=8), dict(ws=P + 8), dict(dy=P + 1), dict(act=0, z=0, dg=P), dict(w=0), dict(x=0), dict(w=P + 8),
+                dict(ldx=63), dict(ldw=68), dict(lddx=63), dict(lddw=63), dict(dx=P + 1), dict(db=P + 1)):
         assert grad(**bad) == ARG, bad
-    assert grad(dz=None) == 0
-    assert lib.wf_linear_backward_input(P, 32, P, 64, P, 63, 4, 32, 64, 1, None) == ARG
-    assert lib.wf_linear_backward_input(P, 33, P, 64, P, 64, 4, 32, 64, 1, None) == ARG
-    assert lib.wf_linear_backward_input(P, 32, P, 64, P, 64, 4, 32, 64, 2, None) == UNSUPPORTED
-    assert lib.wf_linear_backward_weight(P, 32, P + 4, 64, P, 64, 4, 32, 64, 1, None) == ARG
-    assert lib.wf_linear_backward_weight(P, 32, P, 64, None, 64, 4, 32, 64, 1, None) == ARG
+    assert grad(dx=0, dw=0) == 0
+    assert lib.wf_linear_backward_workspace(4, 32, 4) >= 4 * 32 * 2 and lib.wf_linear_backward_workspace(0, 32, 4) == 0
+    assert lib.wf_linear(None, None) == ARG and lib.wf_linear_backward(None, None) == ARG
     assert lib.wf_copy_rows16(P, 4, P, 8, 3, 5, None) == ARG and lib.wf_copy_rows16(P, 8, P, 8, 0, 5, None) == 0
     assert lib.wf_linear_status(ctypes.POINTER(ctypes.c_int)()) == ARG
 
@@ -104,16 +108,37 @@ def test_c_linear_backward_refuses():
 def test_c_layer_norm_refuses():
     lib = wf("_ext").lib()
 
-    def norm(x=P, ldx=64, w=P, b=P, wt=1, y=P, ldy=64, mean=None, rstd=None, rows=4, d=64, rpg=4, eps=1e-6, type=1):
-        return lib.wf_layer_norm(x, ldx, w, b, wt, y, ldy, mean, rstd, rows, d, rpg, eps, type, None)
+    def norm(**kw):
+        return _call("wf_layer_norm", "LAYER_NORM_ARGS", dict(
+            x=P, w=P, b=P, y=P, mean=0, rstd=0, ldx=64, ldy=64, rows=4, d=64, rpg=4, eps=1e-6, type=1, wt=1, reserved=0), kw)
     assert norm(type=5) == UNSUPPORTED and norm(wt=0) == UNSUPPORTED and norm(type=2, wt=1) == UNSUPPORTED
     for bad in (dict(rows=-1), dict(d=0), dict(ldx=63), dict(ldy=63), dict(rpg=0), dict(eps=-1.0), dict(eps=float("nan")),
-                dict(mean=P), dict(x=None), dict(y=P + 1), dict(w=P + 1)):
+                dict(mean=P), dict(x=0), dict(y=P + 1), dict(w=P + 1), dict(mean=P + 2, rstd=P)):
         assert norm(**bad) == ARG, bad
     assert norm(rows=0) == 0
 
-    def back(dy=P, x=P, mean=P, rstd=P, dx=P, lddx=64, dw=None, db=None, rows=4, d=64, rpg=4, type=1, ws=None, size=0):
-        return lib.wf_layer_norm_backward(dy, 64, x, 64, P, 1, mean, rstd, dx, lddx, dw, db, rows, d, rpg, type, ws, size, None)
-    for bad in (dict(dy=None), dict(mean=None), dict(rows=0), dict(lddx=8), dict(dw=P), dict(dw=P, ws=P, size=16), dict(rpg=0)):
+    def back(**kw):
+        return _call("wf_layer_norm_backward", "LAYER_NORM_GRAD_ARGS", dict(
+            dy=P, x=P, w=P, mean=P, rstd=P, dx=P, dw=0, db=0, ws=0, lddy=64, ldx=64, lddx=64, rows=4, d=64, rpg=4, size=0,
+            type=1, wt=1), kw)
+    for bad in (dict(dy=0), dict(mean=0), dict(rows=0), dict(lddx=8), dict(dw=P), dict(dw=P, ws=P, size=16), dict(rpg=0)):
         assert back(**bad) == ARG, bad
-    assert back(dx=None) == 0
+    assert back(dx=0) == 0
+    assert lib.wf_layer_norm(None, None) == ARG and lib.wf_layer_norm_backward(None, None) == ARG
+
+
+def test_argument_structures_match_the_header(tmp_path):
+    """Each packed layout has the size that a C compiler gives the header's structure."""
+    import os
+    import subprocess
+    from conftest import REPO
+    ext = wf("_ext")
+    names = {"wf_linear_args": ext.LINEAR_ARGS, "wf_linear_grad_args": ext.LINEAR_GRAD_ARGS,
+             "wf_layer_norm_args": ext.LAYER_NORM_ARGS, "wf_layer_norm_grad_args": ext.LAYER_NORM_GRAD_ARGS}
+    src = tmp_path / "sizes.c"
+    src.write_text('#include <stdio.h>\n#include "weightferry_b200.h"\nint main(void) {'
+                   + "".join(f'printf("%zu\\n", sizeof({n}));' for n in names) + "return 0;}")
+    exe = tmp_path / "sizes"
+    subprocess.run(["gcc", "-I", os.path.join(REPO, "include"), str(src), "-o", str(exe)], check=True)
+    sizes = subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()
+    assert [int(v) for v in sizes] == [s.size for s in names.values()]

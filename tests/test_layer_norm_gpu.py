@@ -168,18 +168,17 @@ def test_empty(cuda):
 def test_neighbouring_memory_is_left_alone(cuda):
     import torch
     ext = wf("_ext")
-    lib, st = ext.lib(), ext.stream_of("cuda")
     for m, d, ld in ((5, 48, 56), (5, 45, 47), (9, 1024, 1032), (9, 1001, 1003), (3, 17000, 17002)):
         x = torch.randn((m, d), device="cuda")
         y = torch.full((m + 2, ld), -7.0, device="cuda")
         stats = torch.full((2, m + 2), -7.0, device="cuda")
-        ext.check(lib.wf_layer_norm(x.data_ptr(), d, None, None, 2, y.data_ptr(), ld, stats.data_ptr(), stats[1].data_ptr(),
-                                    m, d, m, 1e-6, 2, st), "wf_layer_norm")
+        ext.launch("wf_layer_norm", ext.LAYER_NORM_ARGS.pack(x.data_ptr(), 0, 0, y.data_ptr(), stats.data_ptr(),
+                                                             stats[1].data_ptr(), d, ld, m, d, m, 1e-6, 2, 2, 0), 0)
         assert bool((y[:m, d:] == -7).all()) and bool((y[m:] == -7).all()) and bool((stats[:, m:] == -7).all())
         dx = torch.full((m + 2, ld), -7.0, device="cuda")
-        ext.check(lib.wf_layer_norm_backward(x.data_ptr(), d, x.data_ptr(), d, None, 2, stats.data_ptr(),
-                                             stats[1].data_ptr(), dx.data_ptr(), ld, None, None, m, d, m, 2, None, 0, st),
-                  "wf_layer_norm_backward")
+        ext.launch("wf_layer_norm_backward", ext.LAYER_NORM_GRAD_ARGS.pack(
+            x.data_ptr(), x.data_ptr(), 0, stats.data_ptr(), stats[1].data_ptr(), dx.data_ptr(), 0, 0, 0, d, d, ld, m, d, m, 0,
+            2, 2), 0)
         assert bool((dx[:m, d:] == -7).all()) and bool((dx[m:] == -7).all()) and not bool((dx[:m, :d] == -7).any())
 
 

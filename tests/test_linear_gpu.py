@@ -196,26 +196,29 @@ def test_neighbouring_memory_is_left_alone(cuda):
     """The C entry points write rows of n values and nothing between or behind them."""
     import torch
     ext = wf("_ext")
-    lib, st = ext.lib(), ext.stream_of("cuda")
-    for m, n, k, ld in ((5, 72, 64, 80), (130, 70, 64, 77), (300, 264, 128, 272)):
+    for m, n, k, ld in ((5, 72, 64, 80), (130, 70, 64, 77), (300, 264, 128, 272), (2000, 1000, 64, 1008), (2000, 1001, 64, 1003)):
         x = torch.ones((m, k), device="cuda", dtype=torch.bfloat16)
         w = torch.ones((n, k), device="cuda", dtype=torch.bfloat16)
+        dy = torch.ones((m, n), device="cuda", dtype=torch.bfloat16)
         y = torch.full((m + 3, ld), -7.0, device="cuda", dtype=torch.bfloat16)
         z = torch.full((m + 3, ld), -7.0, device="cuda", dtype=torch.float16)
-        ext.check(lib.wf_linear(x.data_ptr(), k, w.data_ptr(), k, None, 1, None, 1, None, 0, y.data_ptr(), ld, z.data_ptr(),
-                                ld, 0, m, n, k, 1, st), "wf_linear")
+        ext.launch("wf_linear", ext.LINEAR_ARGS.pack(x.data_ptr(), w.data_ptr(), 0, 0, 0, y.data_ptr(), z.data_ptr(), k, k, 0,
+                                                     ld, ld, 1, m, n, k, 1, 1, 0, 0), 0)
         for t in (y, z):
             assert bool((t[:m, :n] == k).all()) and bool((t[:m, n:] == -7).all()) and bool((t[m:] == -7).all())
         dx = torch.full((m + 3, k + 8), -7.0, device="cuda", dtype=torch.bfloat16)
-        dz = torch.ones((m, -(-n // 8) * 8), device="cuda", dtype=torch.bfloat16)
-        ext.check(lib.wf_linear_backward_input(dz.data_ptr(), dz.stride(0), w.data_ptr(), k, dx.data_ptr(), k + 8, m, n, k,
-                                               1, st), "wf_linear_backward_input")
-        assert bool((dx[:m, :k] == n).all()) and bool((dx[:m, k:] == -7).all()) and bool((dx[m:] == -7).all())
         dw = torch.full((n + 3, k + 8), -7.0, device="cuda", dtype=torch.bfloat16)
-        ext.check(lib.wf_linear_backward_weight(dz.data_ptr(), dz.stride(0), x.data_ptr(), k, dw.data_ptr(), k + 8, m, n, k,
-                                                1, st), "wf_linear_backward_weight")
-        m16 = float(torch.tensor(float(m)).to(torch.bfloat16))
+        db = torch.full((n + 8,), -7.0, device="cuda", dtype=torch.bfloat16)
+        size = ext.lib().wf_linear_backward_workspace(m, n, m)
+        work = torch.full((size + 64,), 113, device="cuda", dtype=torch.uint8)
+        ext.launch("wf_linear_backward", ext.LINEAR_GRAD_ARGS.pack(
+            dy.data_ptr(), x.data_ptr(), w.data_ptr(), 0, 0, dx.data_ptr(), dw.data_ptr(), db.data_ptr(), 0, work.data_ptr(), n,
+            k, k, 0, k + 8, k + 8, m, size, m, n, k, 0, 1, 0, 0), 0)
+        assert bool((work[size:] == 113).all())
+        n16, m16 = (float(torch.tensor(float(v)).to(torch.bfloat16)) for v in (n, m))
+        assert bool((dx[:m, :k] == n16).all()) and bool((dx[:m, k:] == -7).all()) and bool((dx[m:] == -7).all())
         assert bool((dw[:n, :k] == m16).all()) and bool((dw[:n, k:] == -7).all()) and bool((dw[n:] == -7).all())
+        assert bool((db[:n] == m16).all()) and bool((db[n:] == -7).all())
 
 
 def test_streams_graphs_and_repeats(cuda):
