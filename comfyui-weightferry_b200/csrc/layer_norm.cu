@@ -9,8 +9,8 @@
 // the output's type.
 //
 // A row stays in registers: it is read once, its mean is summed, then the squares of the centred values (two sums over
-// registers, so a mean far above the spread costs no digits). A thread owns fixed columns in every row of its block, so
-// the column sums of the backward pass are plain register accumulators; a block writes them once per group as a row of
+// registers, so a mean far above the spread costs no digits). In the backward pass a thread owns fixed columns in every
+// row of its block, so the column sums are plain register accumulators; a block writes them once per group as a row of
 // partial sums, and reduce_partials adds those rows in a fixed order: the gradients are the same bits every time.
 // Bound by HBM: forward reads x and writes y, backward reads x and dy and writes dx.
 
@@ -86,6 +86,61 @@ __device__ __forceinline__ void store_chunk(const float (&v)[8], void *row, int 
             if (col < d) store1<T>(row, col, v[j]);
         }
     }
+}
+
+// eight values of a row as they lie in memory (16-byte aligned): zeros past d
+template <int T>
+struct Raw8 {
+    uint4 q[T == WF_F32 ? 2 : 1];
+    __device__ __forceinline__ void load(const void *row, int col, int d) {
+        const uint4 *p = reinterpret_cast<const uint4 *>(static_cast<const char *>(row) + static_cast<int64_t>(col) * dtype_size(T));
+#pragma unroll
+        for (int i = 0; i < (T == WF_F32 ? 2 : 1); ++i) q[i] = col < d ? p[i] : make_uint4(0u, 0u, 0u, 0u);
+    }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+        if constexpr (T == WF_F32) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                v[4 * i] = __uint_as_float(q[i].x), v[4 * i + 1] = __uint_as_float(q[i].y);
+                v[4 * i + 2] = __uint_as_float(q[i].z), v[4 * i + 3] = __uint_as_float(q[i].w);
+            }
+        } else {
+            const uint32_t w[4] = {q[0].x, q[0].y, q[0].z, q[0].w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 f = unpack2<T>(w[i]);
+                v[2 * i] = f.x;
+                v[2 * i + 1] = f.y;
+            }
+        }
+    }
+};
+
+// the sum over aligned sets of LPR lanes, in each of them
+template <int LPR>
+__device__ __forceinline__ float lanes_sum(float v) {
+#pragma unroll
+    for (int o = LPR / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+    return v;
+}
+
+// The sums of N values (a power of 2) over the warp's lanes: lane l gets sum l / (32 / N). Each exchange halves the sums
+// that a lane still carries, N + log2(32 / N) - 1 shuffles instead of 5 N.
+template <int N>
+__device__ __forceinline__ float lanes_sum_many(float (&v)[N], int lane) {
+#pragma unroll
+    for (int n = N / 2, o = 16; n > 0; n /= 2, o /= 2) {
+        const bool upper = (lane & o) != 0;
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+            const float keep = upper ? v[i + n] : v[i], give = upper ? v[i] : v[i + n];
+            v[i] = keep + __shfl_xor_sync(0xFFFFFFFFu, give, o);
+        }
+    }
+    float s = v[0];
+#pragma unroll
+    for (int o = 16 / N; o > 0; o /= 2) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+    return s;
 }
 
 struct NormArgs {
@@ -192,6 +247,152 @@ __global__ void __launch_bounds__(kMaxThreads) layer_norm_wide_kernel(const __gr
     }
 }
 
+// Narrow rows (up to 256 values) that 16-byte accesses fit: LPR lanes a row, 8 values a lane, 32 / LPR rows a warp.
+template <int T, int W, int LPR>
+__global__ void __launch_bounds__(256) layer_norm_narrow_kernel(const __grid_constant__ NormArgs a) {
+    constexpr int RPW = 32 / LPR;
+    const int lane = threadIdx.x & (LPR - 1), sub = (threadIdx.x & 31) / LPR, col = lane * 8;
+    const float inv_d = 1.0f / static_cast<float>(a.d);
+    const bool in = col < a.d;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * 8 * RPW;
+    wait_prior_grid();
+    for (int64_t first = (static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5)) * RPW; first < a.rows; first += step) {
+        const int64_t row = first + sub;
+        const bool on = row < a.rows;
+        Raw8<T> x;
+        x.load(row_of<T>(a.x, row, a.ldx), col, on ? a.d : 0);
+        float v[8], s = 0.f, q = 0.f;
+        x.get(v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s += v[j];
+        const float mean = lanes_sum<LPR>(s) * inv_d;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            v[j] -= mean;
+            if (in) q = fmaf(v[j], v[j], q);
+        }
+        const float rstd = rsqrtf(fmaf(lanes_sum<LPR>(q), inv_d, a.eps));
+        if (!on || !in) continue;
+        if (a.mean != nullptr && lane == 0) {
+            a.mean[row] = mean;
+            a.rstd[row] = rstd;
+        }
+        float p[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] *= rstd;
+        const int64_t grp = row / a.rows_per_group;
+        if (a.w != nullptr) {
+            load8<W>(p, row_of<W>(a.w, grp, a.d), col);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] *= p[j];
+        }
+        if (a.b != nullptr) {
+            load8<W>(p, row_of<W>(a.b, grp, a.d), col);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] += p[j];
+        }
+        store8<T, true>(static_cast<char *>(row_of<T>(a.y, row, a.ldy)) + static_cast<size_t>(col) * dtype_size(T), v);
+    }
+}
+
+// Many wider rows that 16-byte accesses fit: a team of WPR warps a row, NCH chunks of 8 values a lane, held as they came
+// from memory (a 5120-wide bf16 row is 80 registers of a warp) and widened anew for each of the three passes over them:
+// all of a row's loads are in flight at once and no barrier is wider than a team. A block takes a run of rows (RowSplit)
+// and keeps their group's w and b in shared memory: read from L2 for every row they cost more than x itself (16384 x
+// 5120 bf16, 16 groups: 222 us). Groups of fewer than kStageRows rows are read from L2 all the same.
+constexpr int kStageRows = 16;
+template <int T, int W, int NCH, int WPR>
+__global__ void __launch_bounds__(256) layer_norm_team_kernel(const __grid_constant__ NormArgs a, const __grid_constant__ RowSplit split,
+                                                              bool stage) {
+    extern __shared__ uint4 staged[];  // w then b of the current group
+    __shared__ float red[2][8];
+    const int warp = threadIdx.x >> 5, team = warp / WPR, lane = (threadIdx.x & 31) + 32 * (warp % WPR);
+    const int64_t bytes = static_cast<int64_t>(a.d) * dtype_size(W);
+    const float inv_d = 1.0f / static_cast<float>(a.d);
+    auto team_total = [&](float v, float *buf) {
+        v = lanes_sum<32>(v);
+        if constexpr (WPR > 1) {
+            if ((threadIdx.x & 31) == 0) buf[warp] = v;
+            asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(32 * WPR) : "memory");
+            v = 0.f;
+#pragma unroll
+            for (int i = 0; i < WPR; ++i) v += buf[team * WPR + i];
+        }
+        return v;
+    };
+    wait_prior_grid();
+    for (int64_t grp = split.first_group(blockIdx.x), end = split.last_group(blockIdx.x); grp < end; ++grp) {
+        int64_t lo, hi;
+        split.rows_of(blockIdx.x, grp, lo, hi);
+        const void *w = a.w == nullptr ? nullptr : row_of<W>(a.w, grp, a.d), *b = a.b == nullptr ? nullptr : row_of<W>(a.b, grp, a.d);
+        if (stage) {
+            __syncthreads();
+            uint4 *sw = staged, *sb = staged + bytes / 16;
+            for (int i = threadIdx.x; i < bytes / 16; i += 256) {
+                if (w != nullptr) sw[i] = static_cast<const uint4 *>(w)[i];
+                if (b != nullptr) sb[i] = static_cast<const uint4 *>(b)[i];
+            }
+            __syncthreads();
+            if (w != nullptr) w = sw;
+            if (b != nullptr) b = sb;
+        }
+        for (int64_t row = lo + team; row < hi; row += 8 / WPR) {
+            Raw8<T> x[NCH];
+            const void *xr = row_of<T>(a.x, row, a.ldx);
+#pragma unroll
+            for (int c = 0; c < NCH; ++c) x[c].load(xr, (c * 32 * WPR + lane) * 8, a.d);
+            float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+            for (int c = 0; c < NCH; ++c) {
+                float v[8];
+                x[c].get(v);
+#pragma unroll
+                for (int j = 0; j < 8; j += 2) s0 += v[j], s1 += v[j + 1];
+            }
+            const float mean = team_total(s0 + s1, red[0]) * inv_d;
+            s0 = s1 = 0.f;
+#pragma unroll
+            for (int c = 0; c < NCH; ++c) {
+                if ((c * 32 * WPR + lane) * 8 >= a.d) continue;
+                float v[8];
+                x[c].get(v);
+#pragma unroll
+                for (int j = 0; j < 8; j += 2) {
+                    const float c0 = v[j] - mean, c1 = v[j + 1] - mean;
+                    s0 = fmaf(c0, c0, s0);
+                    s1 = fmaf(c1, c1, s1);
+                }
+            }
+            const float rstd = rsqrtf(fmaf(team_total(s0 + s1, red[1]), inv_d, a.eps));
+            if (a.mean != nullptr && lane == 0) {
+                a.mean[row] = mean;
+                a.rstd[row] = rstd;
+            }
+            char *yr = static_cast<char *>(row_of<T>(a.y, row, a.ldy));
+#pragma unroll
+            for (int c = 0; c < NCH; ++c) {
+                const int col = (c * 32 * WPR + lane) * 8;
+                if (col >= a.d) continue;
+                float v[8], p[8];
+                x[c].get(v);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = (v[j] - mean) * rstd;
+                if (w != nullptr) {
+                    load8<W>(p, w, col);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[j] *= p[j];
+                }
+                if (b != nullptr) {
+                    load8<W>(p, b, col);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[j] += p[j];
+                }
+                store8<T, true>(yr + static_cast<size_t>(col) * dtype_size(T), v);
+            }
+        }
+    }
+}
+
 struct NormGradArgs {
     const void *x, *w, *dy;
     const float *mean, *rstd;
@@ -202,12 +403,168 @@ struct NormGradArgs {
     int d;
 };
 
-// Block blockIdx.x takes one share of the rows (RowSplit). WARP: each warp of the block takes every warps-th row of
-// the share and the warps' column sums are added at the end through shared memory.
-template <int T, int W, int NC, bool VEC, bool WARP>
-__global__ void __launch_bounds__(kMaxThreads) layer_norm_grad_kernel(const __grid_constant__ NormGradArgs a) {
+// The backward pass of rows that 16-byte accesses fit, up to 8 values a thread of a block: R rows at a time, whose 2 R
+// sums share one barrier (their shuffles, too: lanes_sum_many).
+template <int T, int W, int R, int THREADS, int BLOCKS>
+__global__ void __launch_bounds__(THREADS, BLOCKS) layer_norm_grad_rows_kernel(const __grid_constant__ NormGradArgs a) {
+    __shared__ float red[2][32][2 * R];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, warps = blockDim.x >> 5, col = tid * 8;
+    const bool in = col < a.d;
+    const float inv_d = 1.0f / static_cast<float>(a.d);
+    int buf = 0;
+    wait_prior_grid();
+    for (int64_t grp = a.split.first_group(blockIdx.x), end = a.split.last_group(blockIdx.x); grp < end; ++grp) {
+        int64_t lo, hi;
+        a.split.rows_of(blockIdx.x, grp, lo, hi);
+        float w[8], dw[8], db[8];
+        if (a.w != nullptr && in) load8<W>(w, row_of<W>(a.w, grp, a.d), col);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            dw[j] = db[j] = 0.f;
+            if (a.w == nullptr || !in) w[j] = 1.f;
+        }
+        for (int64_t row = lo; row < hi; row += R) {
+            Raw8<T> x[R], dy[R];
+            float scale[R], shift[R], s[2 * R];
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const bool on = row + r < hi;
+                x[r].load(row_of<T>(a.x, row + r, a.ldx), col, on ? a.d : 0);
+                dy[r].load(row_of<T>(a.dy, row + r, a.lddy), col, on ? a.d : 0);
+            }
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const bool on = row + r < hi;
+                scale[r] = on ? a.rstd[row + r] : 0.f;
+                shift[r] = on ? a.mean[row + r] : 0.f;
+            }
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                float v[8], g[8];
+                x[r].get(v);
+                dy[r].get(g);
+                s[2 * r] = s[2 * r + 1] = 0.f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float xh = (v[j] - shift[r]) * scale[r];  // dy is 0 outside
+                    db[j] += g[j];
+                    dw[j] = fmaf(g[j], xh, dw[j]);
+                    const float u = g[j] * w[j];
+                    s[2 * r] += u;
+                    s[2 * r + 1] = fmaf(u, xh, s[2 * r + 1]);
+                }
+            }
+            if (a.dx == nullptr) continue;
+            // every warp's sums to shared memory, then every warp adds all of them
+            const float mine = lanes_sum_many<2 * R>(s, lane);
+            if ((lane & (32 / (2 * R) - 1)) == 0) red[buf][warp][lane / (32 / (2 * R))] = mine;
+            __syncthreads();
+            float t = 0.f;  // sum lane % (2 R), of the warps lane / (2 R), + 32 / (2 R), ...
+            for (int i = lane / (2 * R); i < warps; i += 32 / (2 * R)) t += red[buf][i][lane % (2 * R)];
+#pragma unroll
+            for (int o = 2 * R; o < 32; o *= 2) t += __shfl_xor_sync(0xFFFFFFFFu, t, o);
+            buf ^= 1;
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const float m0 = __shfl_sync(0xFFFFFFFFu, t, 2 * r) * inv_d, m1 = __shfl_sync(0xFFFFFFFFu, t, 2 * r + 1) * inv_d;
+                if (!in || row + r >= hi) continue;
+                float v[8], g[8];
+                x[r].get(v);
+                dy[r].get(g);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) g[j] = scale[r] * (fmaf(g[j], w[j], -m0) - (v[j] - shift[r]) * scale[r] * m1);
+                store8<T, true>(static_cast<char *>(row_of<T>(a.dx, row + r, a.lddx)) + static_cast<size_t>(col) * dtype_size(T), g);
+            }
+        }
+        const int64_t part = a.split.partial_row(blockIdx.x, grp) * a.d + col;
+        if (a.part_w != nullptr && in) store8<WF_F32, true>(a.part_w + part, dw);
+        if (a.part_b != nullptr && in) store8<WF_F32, true>(a.part_b + part, db);
+    }
+}
+
+// The backward pass of narrow rows (up to 256 values) that 16-byte accesses fit: LPR lanes a row, 32 / LPR rows a warp, R
+// of them at a time. At the end of a group the lanes that own the same columns, then the warps, add their column sums.
+template <int T, int W, int LPR>
+__global__ void __launch_bounds__(256) layer_norm_grad_narrow_kernel(const __grid_constant__ NormGradArgs a) {
+    constexpr int RPW = 32 / LPR, R = 4;
+    __shared__ float col_red[8][16][LPR];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & (LPR - 1), sub = (threadIdx.x & 31) / LPR, col = lane * 8;
+    const bool in = col < a.d;
+    const float inv_d = 1.0f / static_cast<float>(a.d);
+    wait_prior_grid();
+    for (int64_t grp = a.split.first_group(blockIdx.x), end = a.split.last_group(blockIdx.x); grp < end; ++grp) {
+        int64_t lo, hi;
+        a.split.rows_of(blockIdx.x, grp, lo, hi);
+        float w[8], sums[16];  // dw, db
+        if (a.w != nullptr && in) load8<W>(w, row_of<W>(a.w, grp, a.d), col);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            sums[j] = sums[j + 8] = 0.f;
+            if (a.w == nullptr || !in) w[j] = 1.f;
+        }
+        for (int64_t first = lo + warp * RPW * R; first < hi; first += 8 * RPW * R) {
+            Raw8<T> x[R], dy[R];
+            float scale[R], shift[R];
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const int64_t row = first + r * RPW + sub;
+                const bool on = row < hi;
+                x[r].load(row_of<T>(a.x, row, a.ldx), col, on ? a.d : 0);
+                dy[r].load(row_of<T>(a.dy, row, a.lddy), col, on ? a.d : 0);
+                scale[r] = on ? a.rstd[row] : 0.f;
+                shift[r] = on ? a.mean[row] : 0.f;
+            }
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const int64_t row = first + r * RPW + sub;
+                float v[8], g[8], s0 = 0.f, s1 = 0.f;
+                x[r].get(v);
+                dy[r].get(g);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    v[j] = (v[j] - shift[r]) * scale[r];
+                    sums[j + 8] += g[j];
+                    sums[j] = fmaf(g[j], v[j], sums[j]);
+                    g[j] *= w[j];
+                    s0 += g[j];
+                    s1 = fmaf(g[j], v[j], s1);
+                }
+                if (a.dx == nullptr) continue;
+                const float m0 = lanes_sum<LPR>(s0) * inv_d, m1 = lanes_sum<LPR>(s1) * inv_d;
+                if (row >= hi || !in) continue;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) g[j] = scale[r] * (g[j] - m0 - v[j] * m1);
+                store8<T, true>(static_cast<char *>(row_of<T>(a.dx, row, a.lddx)) + static_cast<size_t>(col) * dtype_size(T), g);
+            }
+            __syncwarp();
+        }
+        if (a.part_w == nullptr && a.part_b == nullptr) continue;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+#pragma unroll
+            for (int o = LPR; o < 32; o *= 2) sums[i] += __shfl_xor_sync(0xFFFFFFFFu, sums[i], o);
+            if (sub == 0) col_red[warp][i][lane] = sums[i];
+        }
+        __syncthreads();
+        const int64_t part = a.split.partial_row(blockIdx.x, grp) * a.d;
+        for (int t = threadIdx.x; t < 16 * LPR; t += 256) {
+            const int i = t / LPR, l = t % LPR, c = l * 8 + (i & 7);
+            float s = 0.f;
+#pragma unroll
+            for (int v = 0; v < 8; ++v) s += col_red[v][i][l];
+            float *dst = i < 8 ? a.part_w : a.part_b;
+            if (dst != nullptr && c < a.d) dst[part + c] = s;
+        }
+    }
+}
+
+// The same value by value, for any width and alignment, one row at a time. WARP: a row a warp; each warp of the block takes every
+// warps-th row of the share and the warps' column sums are added at the end through shared memory.
+template <int T, int W, bool WARP>
+__global__ void __launch_bounds__(WARP ? 256 : kMaxThreads) layer_norm_grad_kernel(const __grid_constant__ NormGradArgs a) {
     __shared__ float red[2][64];
-    __shared__ float col_red[WARP ? 8 * 32 * 8 : 1];  // WARP: one chunk of every warp (blocks of at most 8 warps)
+    __shared__ float col_red[WARP ? 8 * 32 * 8 : 1];
     const int threads = WARP ? 32 : blockDim.x, tid = WARP ? (threadIdx.x & 31) : threadIdx.x;
     const int warps = WARP ? 1 : (blockDim.x >> 5);
     const int row_step = WARP ? (blockDim.x >> 5) : 1, row_first = WARP ? (threadIdx.x >> 5) : 0;
@@ -217,79 +574,67 @@ __global__ void __launch_bounds__(kMaxThreads) layer_norm_grad_kernel(const __gr
     for (int64_t grp = a.split.first_group(blockIdx.x), end = a.split.last_group(blockIdx.x); grp < end; ++grp) {
         int64_t lo, hi;
         a.split.rows_of(blockIdx.x, grp, lo, hi);
-        float w[NC][8], dw[NC][8], db[NC][8];
+        float w[8], dw[8], db[8];
+        if (a.w != nullptr) load_chunk<W, false>(w, row_of<W>(a.w, grp, a.d), 0, tid, threads, a.d);
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            if (a.w != nullptr) load_chunk<W, VEC>(w[c], row_of<W>(a.w, grp, a.d), c, tid, threads, a.d);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                dw[c][j] = db[c][j] = 0.f;
-                if (a.w == nullptr) w[c][j] = 1.f;
-            }
+        for (int j = 0; j < 8; ++j) {
+            dw[j] = db[j] = 0.f;
+            if (a.w == nullptr) w[j] = 1.f;
         }
         for (int64_t row = lo + row_first; row < hi; row += row_step) {
             const float mean = a.mean[row], rstd = a.rstd[row];
-            float xh[NC][8], dy[NC][8];
+            float xh[8], dy[8];
             float s[2] = {0.f, 0.f};
+            load_chunk<T, false>(xh, row_of<T>(a.x, row, a.ldx), 0, tid, threads, a.d);
+            load_chunk<T, false>(dy, row_of<T>(a.dy, row, a.lddy), 0, tid, threads, a.d);
 #pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                load_chunk<T, VEC>(xh[c], row_of<T>(a.x, row, a.ldx), c, tid, threads, a.d);
-                load_chunk<T, VEC>(dy[c], row_of<T>(a.dy, row, a.lddy), c, tid, threads, a.d);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    xh[c][j] = (xh[c][j] - mean) * rstd;  // dy is 0 past the row's end
-                    db[c][j] += dy[c][j];
-                    dw[c][j] = fmaf(dy[c][j], xh[c][j], dw[c][j]);
-                    dy[c][j] *= w[c][j];
-                    s[0] += dy[c][j];
-                    s[1] = fmaf(dy[c][j], xh[c][j], s[1]);
-                }
+            for (int j = 0; j < 8; ++j) {
+                xh[j] = (xh[j] - mean) * rstd;  // dy is 0 past the row's end
+                db[j] += dy[j];
+                dw[j] = fmaf(dy[j], xh[j], dw[j]);
+                dy[j] *= w[j];
+                s[0] += dy[j];
+                s[1] = fmaf(dy[j], xh[j], s[1]);
             }
             if (a.dx == nullptr) continue;
             team_sum<2>(s, red[buf], warps);
             buf ^= 1;
             const float m0 = s[0] * inv_d, m1 = s[1] * inv_d;
 #pragma unroll
-            for (int c = 0; c < NC; ++c) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) dy[c][j] = rstd * (dy[c][j] - m0 - xh[c][j] * m1);
-                store_chunk<T, VEC>(dy[c], row_of<T>(a.dx, row, a.lddx), c, tid, threads, a.d);
-            }
+            for (int j = 0; j < 8; ++j) dy[j] = rstd * (dy[j] - m0 - xh[j] * m1);
+            store_chunk<T, false>(dy, row_of<T>(a.dx, row, a.lddx), 0, tid, threads, a.d);
         }
         const int64_t part = a.split.partial_row(blockIdx.x, grp);
         for (int which = 0; which < 2; ++which) {
             float *dst = which ? a.part_b : a.part_w;
             if (dst == nullptr) continue;
             dst += part * a.d;
+            float v[8];
 #pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                float v[8];
+            for (int j = 0; j < 8; ++j) v[j] = which ? db[j] : dw[j];
+            if constexpr (WARP) {
+                __syncthreads();
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = which ? db[c][j] : dw[c][j];
-                if constexpr (WARP) {
-                    __syncthreads();
+                for (int j = 0; j < 8; ++j) col_red[(threadIdx.x >> 5) * 256 + j * 32 + tid] = v[j];
+                __syncthreads();
+                if (threadIdx.x < 32) {
+                    for (int o = 1; o < static_cast<int>(blockDim.x >> 5); ++o)
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) col_red[(threadIdx.x >> 5) * 256 + j * 32 + tid] = v[j];
-                    __syncthreads();
-                    if (threadIdx.x < 32) {
-                        for (int o = 1; o < static_cast<int>(blockDim.x >> 5); ++o)
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) v[j] += col_red[o * 256 + j * 32 + tid];
-                        store_chunk<WF_F32, VEC>(v, dst, c, tid, threads, a.d);
-                    }
-                } else {
-                    store_chunk<WF_F32, VEC>(v, dst, c, tid, threads, a.d);
+                        for (int j = 0; j < 8; ++j) v[j] += col_red[o * 256 + j * 32 + tid];
+                    store_chunk<WF_F32, false>(v, dst, 0, tid, threads, a.d);
                 }
+            } else {
+                store_chunk<WF_F32, false>(v, dst, 0, tid, threads, a.d);
             }
         }
     }
 }
 
-// The backward pass of rows wider than a block's registers hold: dx row by row with the row read twice ...
-template <int T, int W>
+// The backward pass of wider rows: dx row by row with the row read twice (the second time from L2) ...
+template <int T, int W, bool VEC>
 __global__ void __launch_bounds__(kMaxThreads) layer_norm_grad_wide_kernel(const __grid_constant__ NormGradArgs a) {
     __shared__ float red[2][64];
-    const int warps = blockDim.x >> 5;
+    const int warps = blockDim.x >> 5, chunks = (a.d + 8 * static_cast<int>(blockDim.x) - 1) / (8 * static_cast<int>(blockDim.x));
     const float inv_d = 1.0f / static_cast<float>(a.d);
     wait_prior_grid();
     int buf = 0;
@@ -297,127 +642,196 @@ __global__ void __launch_bounds__(kMaxThreads) layer_norm_grad_wide_kernel(const
         const float mean = a.mean[row], rstd = a.rstd[row];
         const void *xr = row_of<T>(a.x, row, a.ldx), *gr = row_of<T>(a.dy, row, a.lddy);
         const void *wr = a.w == nullptr ? nullptr : row_of<W>(a.w, row / a.split.rows_per_group, a.d);
-        float s[2] = {0.f, 0.f};
-        for (int col = threadIdx.x; col < a.d; col += blockDim.x) {
-            const float u = load1<T>(gr, col) * (wr != nullptr ? load1<W>(wr, col) : 1.f);
-            s[0] += u;
-            s[1] = fmaf(u, (load1<T>(xr, col) - mean) * rstd, s[1]);
+        float s[2] = {0.f, 0.f}, x[8], g[8], w[8];
+        for (int c = 0; c < chunks; ++c) {
+            load_chunk<T, VEC>(x, xr, c, threadIdx.x, blockDim.x, a.d);
+            load_chunk<T, VEC>(g, gr, c, threadIdx.x, blockDim.x, a.d);
+            if (wr != nullptr) load_chunk<W, VEC>(w, wr, c, threadIdx.x, blockDim.x, a.d);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float u = wr != nullptr ? g[j] * w[j] : g[j];
+                s[0] += u;
+                s[1] = fmaf(u, (x[j] - mean) * rstd, s[1]);
+            }
         }
         team_sum<2>(s, red[buf], warps);
         const float m0 = s[0] * inv_d, m1 = s[1] * inv_d;
-        void *dr = row_of<T>(a.dx, row, a.lddx);
-        for (int col = threadIdx.x; col < a.d; col += blockDim.x) {
-            const float u = load1<T>(gr, col) * (wr != nullptr ? load1<W>(wr, col) : 1.f);
-            store1<T>(dr, col, rstd * (u - m0 - (load1<T>(xr, col) - mean) * rstd * m1));
+        for (int c = 0; c < chunks; ++c) {
+            load_chunk<T, VEC>(x, xr, c, threadIdx.x, blockDim.x, a.d);
+            load_chunk<T, VEC>(g, gr, c, threadIdx.x, blockDim.x, a.d);
+            if (wr != nullptr) load_chunk<W, VEC>(w, wr, c, threadIdx.x, blockDim.x, a.d);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float u = wr != nullptr ? g[j] * w[j] : g[j];
+                g[j] = rstd * (u - m0 - (x[j] - mean) * rstd * m1);
+            }
+            store_chunk<T, VEC>(g, row_of<T>(a.dx, row, a.lddx), c, threadIdx.x, blockDim.x, a.d);
         }
     }
 }
 
-// ... and the column sums by themselves: block (x, y) sums columns 256 x .. 256 x + 255 over share y of the rows.
-template <int T>
+// ... and the column sums by themselves: block (x, y) sums 2048 columns from 2048 x over share y of the rows.
+template <int T, bool VEC>
 __global__ void __launch_bounds__(256) layer_norm_column_kernel(const __grid_constant__ NormGradArgs a) {
-    const int col = blockIdx.x * 256 + threadIdx.x;
     wait_prior_grid();
-    if (col >= a.d) return;
     for (int64_t grp = a.split.first_group(blockIdx.y), end = a.split.last_group(blockIdx.y); grp < end; ++grp) {
         int64_t lo, hi;
         a.split.rows_of(blockIdx.y, grp, lo, hi);
-        float dw = 0.f, db = 0.f;
-#pragma unroll 4
+        float dw[8], db[8], x[8], g[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) dw[j] = db[j] = 0.f;
+#pragma unroll 2
         for (int64_t row = lo; row < hi; ++row) {
-            const float g = load1<T>(row_of<T>(a.dy, row, a.lddy), col);
-            db += g;
-            dw = fmaf(g, (load1<T>(row_of<T>(a.x, row, a.ldx), col) - a.mean[row]) * a.rstd[row], dw);
+            load_chunk<T, VEC>(x, row_of<T>(a.x, row, a.ldx), blockIdx.x, threadIdx.x, 256, a.d);
+            load_chunk<T, VEC>(g, row_of<T>(a.dy, row, a.lddy), blockIdx.x, threadIdx.x, 256, a.d);
+            const float mean = a.mean[row], rstd = a.rstd[row];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                db[j] += g[j];
+                dw[j] = fmaf(g[j], (x[j] - mean) * rstd, dw[j]);
+            }
         }
-        const int64_t at = a.split.partial_row(blockIdx.y, grp) * a.d + col;
-        if (a.part_w != nullptr) a.part_w[at] = dw;
-        if (a.part_b != nullptr) a.part_b[at] = db;
+        const int64_t at = a.split.partial_row(blockIdx.y, grp) * a.d;
+        if (a.part_w != nullptr) store_chunk<WF_F32, VEC>(dw, a.part_w + at, blockIdx.x, threadIdx.x, 256, a.d);
+        if (a.part_b != nullptr) store_chunk<WF_F32, VEC>(db, a.part_b + at, blockIdx.x, threadIdx.x, 256, a.d);
     }
 }
 
 // ------------------------------------------------------------------------------------------------------------- host
-// Threads of a row and the way its values are dealt to them: at least 8 values a thread; a warp up to 256 values.
-struct RowShape {
-    bool warp, wide;
-    int threads, nc;
-};
-RowShape row_shape(int d) {
-    RowShape s;
-    s.warp = d <= 256;
-    const int need = (d + 7) / 8;
-    s.threads = s.warp ? 32 : std::min(kMaxThreads, (need + 31) / 32 * 32);
-    s.nc = (need + s.threads - 1) / s.threads;
-    s.wide = s.nc > 2;
-    return s;
-}
-
 bool vec_ok(const void *p, int64_t ld, int size) {
     return p == nullptr || (aligned_to(p, 16) && (ld * size) % 16 == 0);
 }
 
+// a block's threads for 8 values each, or the most there are
+int row_threads(int d) { return std::min(kMaxThreads, ((d + 7) / 8 + 31) / 32 * 32); }
+
 template <int T, int W, int NC, bool VEC, bool WARP>
-int launch_norm(const NormArgs &a, const RowShape &s, cudaStream_t stream) {
+int launch_norm(const NormArgs &a, cudaStream_t stream) {
     constexpr auto kern = layer_norm_kernel<T, W, NC, VEC, WARP>;
-    const int block = WARP ? 256 : s.threads;
+    const int block = WARP ? 256 : row_threads(a.d);
     const int64_t need = WARP ? (a.rows + 7) / 8 : a.rows;
     const int grid = static_cast<int>(std::min<int64_t>(need, wave_ctas_at<kern>(block)));
     return launch_rows(kern, dim3(grid), block, stream, a);
 }
 
-template <int T, int W>
-int dispatch_norm(const NormArgs &a, cudaStream_t stream) {
-    const RowShape s = row_shape(a.d);
-    if (s.wide) {
-        constexpr auto kern = layer_norm_wide_kernel<T, W>;
-        const int grid = static_cast<int>(std::min<int64_t>(a.rows, wave_ctas_at<kern>(kMaxThreads)));
-        return launch_rows(kern, dim3(grid), kMaxThreads, stream, a);
+template <int T, int W, bool VEC>
+int launch_norm_block(const NormArgs &a, cudaStream_t stream) {
+    if (!VEC && a.d <= 256) return launch_norm<T, W, 1, VEC, true>(a, stream);
+    switch ((a.d + 8 * kMaxThreads - 1) / (8 * kMaxThreads)) {
+        case 1: return launch_norm<T, W, 1, VEC, false>(a, stream);
+        case 2: return launch_norm<T, W, 2, VEC, false>(a, stream);
+        case 3: return launch_norm<T, W, 3, VEC, false>(a, stream);
+        default: break;
     }
-    const bool vec = a.d % 8 == 0 && vec_ok(a.x, a.ldx, dtype_size(T)) && vec_ok(a.y, a.ldy, dtype_size(T)) &&
-                     vec_ok(a.w, a.d, dtype_size(W)) && vec_ok(a.b, a.d, dtype_size(W));
-    if (s.warp) return vec ? launch_norm<T, W, 1, true, true>(a, s, stream) : launch_norm<T, W, 1, false, true>(a, s, stream);
-    if (s.nc == 1) return vec ? launch_norm<T, W, 1, true, false>(a, s, stream) : launch_norm<T, W, 1, false, false>(a, s, stream);
-    return vec ? launch_norm<T, W, 2, true, false>(a, s, stream) : launch_norm<T, W, 2, false, false>(a, s, stream);
+    constexpr auto kern = layer_norm_wide_kernel<T, W>;
+    const int grid = static_cast<int>(std::min<int64_t>(a.rows, wave_ctas_at<kern>(kMaxThreads)));
+    return launch_rows(kern, dim3(grid), kMaxThreads, stream, a);
 }
 
-template <int T, int W, int NC, bool VEC, bool WARP>
-int launch_norm_grad(const NormGradArgs &a, const RowShape &s, cudaStream_t stream) {
-    return launch_rows(layer_norm_grad_kernel<T, W, NC, VEC, WARP>, dim3(static_cast<unsigned>(a.split.blocks())),
-                       WARP ? 256 : s.threads, stream, a);
+template <int T, int W, int LPR>
+int launch_norm_narrow(const NormArgs &a, cudaStream_t stream) {
+    constexpr auto kern = layer_norm_narrow_kernel<T, W, LPR>;
+    constexpr int per_block = 8 * (32 / LPR);
+    const int grid = static_cast<int>(std::min<int64_t>((a.rows + per_block - 1) / per_block, wave_ctas_at<kern>(256)));
+    return launch_rows(kern, dim3(grid), 256, stream, a);
+}
+
+template <int T, int W, int NCH, int WPR>
+int launch_norm_team(const NormArgs &a, cudaStream_t stream) {
+    constexpr auto kern = layer_norm_team_kernel<T, W, NCH, WPR>;
+    constexpr size_t most = 2u * NCH * WPR * 256 * dtype_size(W);
+    static std::atomic<int> resident[64];  // blocks on the device at the widest row; any host thread may launch first
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64) return WF_ERR_DEVICE;
+    if (resident[dev].load(std::memory_order_acquire) == 0) {
+        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(most));
+        if (e != cudaSuccess) return static_cast<int>(e);
+        int n = 0;
+        e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, 256, most);
+        if (e != cudaSuccess) return static_cast<int>(e);
+        resident[dev].store(std::max(n, 1) * device_sm_count(), std::memory_order_release);
+    }
+    const RowSplit split = make_split(a.rows, a.rows_per_group, resident[dev].load(std::memory_order_acquire), 8 / WPR);
+    const bool stage = (a.w != nullptr || a.b != nullptr) && split.rows_per_group >= kStageRows;
+    const size_t smem = stage ? 2 * static_cast<size_t>(a.d) * dtype_size(W) : 0;
+    const cudaError_t e = launch_dependent(kern, dim3(static_cast<unsigned>(split.blocks())), 256, smem, stream, a, split, stage);
+    return static_cast<int>(e != cudaSuccess ? e : cudaGetLastError());
+}
+
+template <int T, int W>
+int dispatch_norm(const NormArgs &a, cudaStream_t stream) {
+    const bool vec = a.d % 8 == 0 && vec_ok(a.x, a.ldx, dtype_size(T)) && vec_ok(a.y, a.ldy, dtype_size(T)) &&
+                     vec_ok(a.w, a.d, dtype_size(W)) && vec_ok(a.b, a.d, dtype_size(W));
+    if (!vec) return launch_norm_block<T, W, false>(a, stream);
+    const int chunks = a.d / 8;
+    if (chunks <= 4) return launch_norm_narrow<T, W, 4>(a, stream);
+    if (chunks <= 8) return launch_norm_narrow<T, W, 8>(a, stream);
+    if (chunks <= 16) return launch_norm_narrow<T, W, 16>(a, stream);
+    if (chunks <= 32) return launch_norm_narrow<T, W, 32>(a, stream);
+    // teams of warps where there are rows for them; else a row a block
+    if (a.rows >= 4ll * device_sm_count()) {
+        constexpr int wide = T == WF_F32 ? 10 : 20;  // chunks a lane: 80 registers
+        const int need = (chunks + 31) / 32;
+        if (need <= 2) return launch_norm_team<T, W, 2, 1>(a, stream);
+        if (need <= 4) return launch_norm_team<T, W, 4, 1>(a, stream);
+        if (need <= 8) return launch_norm_team<T, W, 8, 1>(a, stream);
+        if constexpr (T != WF_F32) {
+            if (need <= 12) return launch_norm_team<T, W, 12, 1>(a, stream);
+            if (need <= 16) return launch_norm_team<T, W, 16, 1>(a, stream);
+        }
+        if (need <= wide) return launch_norm_team<T, W, wide, 1>(a, stream);
+        if (need <= 2 * wide) return launch_norm_team<T, W, wide, 2>(a, stream);
+        if (need <= 4 * wide && W != WF_F32) return launch_norm_team<T, W, wide, 4>(a, stream);
+    }
+    return launch_norm_block<T, W, true>(a, stream);
+}
+
+template <int T, int W, bool VEC>
+int launch_norm_grad_wide(const NormGradArgs &a, cudaStream_t stream) {
+    int rc = WF_OK;
+    if (a.dx != nullptr) {
+        constexpr auto kern = layer_norm_grad_wide_kernel<T, W, VEC>;
+        const int grid = static_cast<int>(std::min<int64_t>(a.rows, wave_ctas_at<kern>(kMaxThreads)));
+        rc = launch_rows(kern, dim3(grid), kMaxThreads, stream, a);
+    }
+    if (rc == WF_OK && (a.part_w != nullptr || a.part_b != nullptr))
+        rc = launch_rows(layer_norm_column_kernel<T, VEC>, dim3((a.d + 2047) / 2048, static_cast<unsigned>(a.split.blocks())),
+                         256, stream, a);
+    return rc;
 }
 
 template <int T, int W>
 int dispatch_norm_grad(const NormGradArgs &a, cudaStream_t stream) {
-    const RowShape s = row_shape(a.d);
-    if (s.wide) {
-        int rc = WF_OK;
-        if (a.dx != nullptr) {
-            constexpr auto kern = layer_norm_grad_wide_kernel<T, W>;
-            const int grid = static_cast<int>(std::min<int64_t>(a.rows, wave_ctas_at<kern>(kMaxThreads)));
-            rc = launch_rows(kern, dim3(grid), kMaxThreads, stream, a);
-        }
-        if (rc == WF_OK && (a.part_w != nullptr || a.part_b != nullptr))
-            rc = launch_rows(layer_norm_column_kernel<T>, dim3((a.d + 255) / 256, static_cast<unsigned>(a.split.blocks())),
-                             256, stream, a);
-        return rc;
-    }
     const bool vec = a.d % 8 == 0 && vec_ok(a.x, a.ldx, dtype_size(T)) && vec_ok(a.dy, a.lddy, dtype_size(T)) &&
                      vec_ok(a.dx, a.lddx, dtype_size(T)) && vec_ok(a.w, a.d, dtype_size(W)) && vec_ok(a.part_w, a.d, 4) &&
                      vec_ok(a.part_b, a.d, 4);
-    if (s.warp) return vec ? launch_norm_grad<T, W, 1, true, true>(a, s, stream) : launch_norm_grad<T, W, 1, false, true>(a, s, stream);
-    if (s.nc == 1) return vec ? launch_norm_grad<T, W, 1, true, false>(a, s, stream) : launch_norm_grad<T, W, 1, false, false>(a, s, stream);
-    return vec ? launch_norm_grad<T, W, 2, true, false>(a, s, stream) : launch_norm_grad<T, W, 2, false, false>(a, s, stream);
+    const dim3 grid(static_cast<unsigned>(a.split.blocks()));
+    if (a.d > 8 * kMaxThreads) return vec ? launch_norm_grad_wide<T, W, true>(a, stream) : launch_norm_grad_wide<T, W, false>(a, stream);
+    if (a.d <= 256) {
+        if (!vec) return launch_rows(layer_norm_grad_kernel<T, W, true>, grid, 256, stream, a);
+        if (a.d <= 32) return launch_rows(layer_norm_grad_narrow_kernel<T, W, 4>, grid, 256, stream, a);
+        if (a.d <= 64) return launch_rows(layer_norm_grad_narrow_kernel<T, W, 8>, grid, 256, stream, a);
+        if (a.d <= 128) return launch_rows(layer_norm_grad_narrow_kernel<T, W, 16>, grid, 256, stream, a);
+        return launch_rows(layer_norm_grad_narrow_kernel<T, W, 32>, grid, 256, stream, a);
+    }
+    const int threads = row_threads(a.d);
+    if (!vec) return launch_rows(layer_norm_grad_kernel<T, W, false>, grid, threads, stream, a);
+    if (threads <= 256) return launch_rows(layer_norm_grad_rows_kernel<T, W, 4, 256, 2>, grid, threads, stream, a);
+    if (threads <= 640) return launch_rows(layer_norm_grad_rows_kernel<T, W, 2, 640, 1>, grid, threads, stream, a);
+    return launch_rows(layer_norm_grad_rows_kernel<T, W, 1, 1024, 1>, grid, threads, stream, a);
 }
 
 bool norm_types_ok(int type, int w_type) {
     return (type == WF_F16 || type == WF_BF16 || type == WF_F32) && (w_type == type || w_type == WF_F32);
 }
 
-// the shares of the rows that the backward pass's blocks take
+// The shares of the rows that the backward pass's blocks take: about as many as are resident at once.
 RowSplit norm_split(int64_t rows, int64_t rows_per_group, int d) {
-    const RowShape s = row_shape(d);
-    const int64_t wanted = s.wide ? std::max<int64_t>(1, 4ll * device_sm_count() * 256 / d)
-                                  : static_cast<int64_t>(device_sm_count()) * (s.warp ? 8 : std::max(1, 2048 / s.threads));
-    return make_split(rows, rows_per_group, wanted, s.warp ? 8 : 1);
+    const int64_t sms = device_sm_count();
+    if (d > 8 * kMaxThreads) return make_split(rows, rows_per_group, std::max<int64_t>(1, 4 * sms * 2048 / d), 16);
+    if (d <= 256) return make_split(rows, rows_per_group, 4 * sms, 8);
+    return make_split(rows, rows_per_group, sms * std::max(1, std::min(8, 640 / row_threads(d))), 4);
 }
 
 }  // namespace

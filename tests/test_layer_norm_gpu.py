@@ -50,7 +50,8 @@ def test_widths(cuda, d):
         _compare(torch, *_data(torch, m, d, dtype, wdtype))
 
 
-@pytest.mark.parametrize("m,d", [(5000, 64), (3001, 520), (700, 2048), (40000, 8), (2100, 1001)])
+@pytest.mark.parametrize("m,d", [(5000, 64), (3001, 520), (700, 2048), (40000, 8), (2100, 1001), (4001, 24), (3000, 120),
+                                 (650, 1000), (650, 2816), (650, 4096), (650, 5120), (650, 6144), (650, 6152), (600, 8200)])
 def test_many_rows(cuda, m, d):
     import torch
     _compare(torch, *_data(torch, m, d, torch.bfloat16, torch.float32))
