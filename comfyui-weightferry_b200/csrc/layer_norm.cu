@@ -15,6 +15,7 @@
 // Bound by HBM: forward reads x and writes y, backward reads x and dy and writes dx.
 
 #include "wf_common.cuh"
+#include "wf_pairs.cuh"
 #include "wf_rows.cuh"
 
 #include <algorithm>
@@ -97,24 +98,32 @@ struct Raw8 {
 #pragma unroll
         for (int i = 0; i < (T == WF_F32 ? 2 : 1); ++i) q[i] = col < d ? p[i] : make_uint4(0u, 0u, 0u, 0u);
     }
-    __device__ __forceinline__ void get(float (&v)[8]) const {
+    __device__ __forceinline__ void get(uint64_t (&v)[4]) const {
         if constexpr (T == WF_F32) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                v[4 * i] = __uint_as_float(q[i].x), v[4 * i + 1] = __uint_as_float(q[i].y);
-                v[4 * i + 2] = __uint_as_float(q[i].z), v[4 * i + 3] = __uint_as_float(q[i].w);
+                v[2 * i] = pack_f2(__uint_as_float(q[i].x), __uint_as_float(q[i].y));
+                v[2 * i + 1] = pack_f2(__uint_as_float(q[i].z), __uint_as_float(q[i].w));
             }
         } else {
             const uint32_t w[4] = {q[0].x, q[0].y, q[0].z, q[0].w};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float2 f = unpack2<T>(w[i]);
-                v[2 * i] = f.x;
-                v[2 * i + 1] = f.y;
+                v[i] = pack_f2(f.x, f.y);
             }
         }
     }
 };
+
+// eight values, rounded to T, to column col of a row (16-byte aligned)
+template <int T>
+__device__ __forceinline__ void store_pairs(void *row, int col, const uint64_t (&v)[4]) {
+    float f[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) unpack_f2(v[i], f[2 * i], f[2 * i + 1]);
+    store8<T, true>(static_cast<char *>(row) + static_cast<int64_t>(col) * dtype_size(T), f);
+}
 
 // the sum over aligned sets of LPR lanes, in each of them
 template <int LPR>
@@ -247,6 +256,25 @@ __global__ void __launch_bounds__(kMaxThreads) layer_norm_wide_kernel(const __gr
     }
 }
 
+// v * w + b with eight values of w and b (either may be null) from column col
+template <int W>
+__device__ __forceinline__ void affine(uint64_t (&v)[4], const void *w, const void *b, int col) {
+    Raw8<W> raw;
+    uint64_t p[4];
+    if (w != nullptr) {
+        raw.load(w, col, col + 8);
+        raw.get(p);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = mul_f2(v[j], p[j]);
+    }
+    if (b != nullptr) {
+        raw.load(b, col, col + 8);
+        raw.get(p);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = add_f2(v[j], p[j]);
+    }
+}
+
 // Narrow rows (up to 256 values) that 16-byte accesses fit: LPR lanes a row, 8 values a lane, 32 / LPR rows a warp.
 template <int T, int W, int LPR>
 __global__ void __launch_bounds__(256) layer_norm_narrow_kernel(const __grid_constant__ NormArgs a) {
@@ -261,59 +289,92 @@ __global__ void __launch_bounds__(256) layer_norm_narrow_kernel(const __grid_con
         const bool on = row < a.rows;
         Raw8<T> x;
         x.load(row_of<T>(a.x, row, a.ldx), col, on ? a.d : 0);
-        float v[8], s = 0.f, q = 0.f;
+        uint64_t v[4], s = 0, q = 0;  // +0, +0
         x.get(v);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s += v[j];
-        const float mean = lanes_sum<LPR>(s) * inv_d;
+        for (int j = 0; j < 4; ++j) s = add_f2(s, v[j]);
+        const float mean = lanes_sum<LPR>(sum_f2(s)) * inv_d;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            v[j] -= mean;
-            if (in) q = fmaf(v[j], v[j], q);
+        for (int j = 0; j < 4; ++j) {
+            v[j] = add_f2(v[j], pack_f2(-mean, -mean));
+            if (in) q = fma_f2(v[j], v[j], q);
         }
-        const float rstd = rsqrtf(fmaf(lanes_sum<LPR>(q), inv_d, a.eps));
+        const float rstd = rsqrtf(fmaf(lanes_sum<LPR>(sum_f2(q)), inv_d, a.eps));
         if (!on || !in) continue;
         if (a.mean != nullptr && lane == 0) {
             a.mean[row] = mean;
             a.rstd[row] = rstd;
         }
-        float p[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] *= rstd;
+        for (int j = 0; j < 4; ++j) v[j] = mul_f2(v[j], pack_f2(rstd, rstd));
         const int64_t grp = row / a.rows_per_group;
-        if (a.w != nullptr) {
-            load8<W>(p, row_of<W>(a.w, grp, a.d), col);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] *= p[j];
-        }
-        if (a.b != nullptr) {
-            load8<W>(p, row_of<W>(a.b, grp, a.d), col);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] += p[j];
-        }
-        store8<T, true>(static_cast<char *>(row_of<T>(a.y, row, a.ldy)) + static_cast<size_t>(col) * dtype_size(T), v);
+        affine<W>(v, a.w == nullptr ? nullptr : row_of<W>(a.w, grp, a.d), a.b == nullptr ? nullptr : row_of<W>(a.b, grp, a.d), col);
+        store_pairs<T>(row_of<T>(a.y, row, a.ldy), col, v);
     }
 }
 
-// Many wider rows that 16-byte accesses fit: a team of WPR warps a row, NCH chunks of 8 values a lane, held as they came
-// from memory (a 5120-wide bf16 row is 80 registers of a warp) and widened anew for each of the three passes over them:
-// all of a row's loads are in flight at once and no barrier is wider than a team. A block takes a run of rows (RowSplit)
-// and keeps their group's w and b in shared memory: read from L2 for every row they cost more than x itself (16384 x
-// 5120 bf16, 16 groups: 222 us). Groups of fewer than kStageRows rows are read from L2 all the same.
+// 16 bytes from global to shared memory past the registers (zeros where `on` is false)
+__device__ __forceinline__ void copy16(void *dst, const void *src, bool on) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))),
+                 "l"(src), "r"(on ? 16 : 0)
+                 : "memory");
+}
+
+// 16 bytes of T as pairs: 8 or 4 values
+template <int T>
+__device__ __forceinline__ void widen(uint64_t (&v)[T == WF_F32 ? 2 : 4], const uint4 &q) {
+    if constexpr (T == WF_F32) {
+        v[0] = pack_f2(__uint_as_float(q.x), __uint_as_float(q.y));
+        v[1] = pack_f2(__uint_as_float(q.z), __uint_as_float(q.w));
+    } else {
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = unpack2<T>(w[i]);
+            v[i] = pack_f2(f.x, f.y);
+        }
+    }
+}
+
+// The values of w (or b) that belong to 16-byte piece `piece` of a row of T. Staged, a float32 row beside 16-bit values
+// lies in two planes (a piece's first and second four values), so that neighbouring lanes read neighbouring 16 bytes.
+template <int T, int W>
+__device__ __forceinline__ void param_piece(uint64_t (&p)[T == WF_F32 ? 2 : 4], const uint4 *row, int piece, int pieces, bool staged) {
+    if constexpr (T == W) {
+        widen<T>(p, row[piece]);
+    } else {
+        uint64_t h[2];
+        widen<WF_F32>(h, row[staged ? piece : 2 * piece]);
+        p[0] = h[0], p[1] = h[1];
+        widen<WF_F32>(h, row[staged ? pieces + piece : 2 * piece + 1]);
+        p[2] = h[0], p[3] = h[1];
+    }
+}
+
+// Many wider rows that 16-byte accesses fit: a team of WPR warps a row. Each thread copies its own 16-byte pieces of the
+// team's next rows into a ring in shared memory (cp.async) and reads nobody else's, so that rows stream in without a
+// barrier and without registers (a row held in registers, widened three times, needed 234 of them for 5120 values and
+// left 8 warps an SM: 84 us where this takes 66). A block takes a run of rows (RowSplit) and keeps their group's w and b
+// in shared memory: read from L2 for every row they cost more than x itself (16384 x 5120 bf16 in 16 groups: 222 us).
+// Groups of fewer than kStageRows rows are read from L2 all the same.
 constexpr int kStageRows = 16;
-template <int T, int W, int NCH, int WPR>
-__global__ void __launch_bounds__(256) layer_norm_team_kernel(const __grid_constant__ NormArgs a, const __grid_constant__ RowSplit split,
-                                                              bool stage) {
-    extern __shared__ uint4 staged[];  // w then b of the current group
+template <int T, int W, int WPR>
+__global__ void __launch_bounds__(256) layer_norm_stream_kernel(const __grid_constant__ NormArgs a,
+                                                                const __grid_constant__ RowSplit split, int bufs, bool stage) {
+    constexpr int NP = T == WF_F32 ? 2 : 4;           // pairs of a piece
+    constexpr int TEAMS = 8 / WPR, LANES = 32 * WPR;
+    extern __shared__ uint4 smem[];                   // w and b of the group (where staged), then a ring a team
     __shared__ float red[2][8];
-    const int warp = threadIdx.x >> 5, team = warp / WPR, lane = (threadIdx.x & 31) + 32 * (warp % WPR);
-    const int64_t bytes = static_cast<int64_t>(a.d) * dtype_size(W);
+    const int warp = threadIdx.x >> 5, team = warp / WPR, lane = threadIdx.x & (LANES - 1);
+    const int pieces = a.d / (2 * NP), w_pieces = a.d * dtype_size(W) / 16;
+    uint4 *sw = smem, *sb = smem + w_pieces;
+    uint4 *ring = smem + (stage ? 2 * w_pieces : 0) + team * bufs * pieces;
     const float inv_d = 1.0f / static_cast<float>(a.d);
     auto team_total = [&](float v, float *buf) {
         v = lanes_sum<32>(v);
         if constexpr (WPR > 1) {
             if ((threadIdx.x & 31) == 0) buf[warp] = v;
-            asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(32 * WPR) : "memory");
+            asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(LANES) : "memory");
             v = 0.f;
 #pragma unroll
             for (int i = 0; i < WPR; ++i) v += buf[team * WPR + i];
@@ -324,72 +385,91 @@ __global__ void __launch_bounds__(256) layer_norm_team_kernel(const __grid_const
     for (int64_t grp = split.first_group(blockIdx.x), end = split.last_group(blockIdx.x); grp < end; ++grp) {
         int64_t lo, hi;
         split.rows_of(blockIdx.x, grp, lo, hi);
-        const void *w = a.w == nullptr ? nullptr : row_of<W>(a.w, grp, a.d), *b = a.b == nullptr ? nullptr : row_of<W>(a.b, grp, a.d);
+        auto fetch = [&](int64_t row, int buf) {  // one copy group a row, empty past the last
+            if (row < hi) {
+                const char *src = static_cast<const char *>(row_of<T>(a.x, row, a.ldx));
+                for (int i = lane; i < pieces; i += LANES) copy16(ring + buf * pieces + i, src + 16 * i, true);
+            }
+            cp_async_commit();
+        };
+        int64_t ahead = lo + team;
+        for (int i = 0; i < bufs - 1; ++i, ahead += TEAMS) fetch(ahead, i);
+        const uint4 *w = a.w == nullptr ? nullptr : static_cast<const uint4 *>(row_of<W>(a.w, grp, a.d));
+        const uint4 *b = a.b == nullptr ? nullptr : static_cast<const uint4 *>(row_of<W>(a.b, grp, a.d));
         if (stage) {
             __syncthreads();
-            uint4 *sw = staged, *sb = staged + bytes / 16;
-            for (int i = threadIdx.x; i < bytes / 16; i += 256) {
-                if (w != nullptr) sw[i] = static_cast<const uint4 *>(w)[i];
-                if (b != nullptr) sb[i] = static_cast<const uint4 *>(b)[i];
+            for (int i = threadIdx.x; i < w_pieces; i += 256) {
+                const int at = T == W ? i : (i & 1) * pieces + (i >> 1);
+                if (w != nullptr) sw[at] = w[i];
+                if (b != nullptr) sb[at] = b[i];
             }
             __syncthreads();
             if (w != nullptr) w = sw;
             if (b != nullptr) b = sb;
         }
-        for (int64_t row = lo + team; row < hi; row += 8 / WPR) {
-            Raw8<T> x[NCH];
-            const void *xr = row_of<T>(a.x, row, a.ldx);
+        int buf = 0, next = bufs - 1;
+        for (int64_t row = lo + team; row < hi; row += TEAMS, ahead += TEAMS) {
+            fetch(ahead, next);
+            if (++next == bufs) next = 0;
+            if (bufs == 2) cp_async_wait<1>();
+            else if (bufs == 3) cp_async_wait<2>();
+            else cp_async_wait<3>();
+            const uint4 *x = ring + buf * pieces;
+            if (++buf == bufs) buf = 0;
+            uint64_t v[NP], s = 0, s1 = 0;  // +0, +0
+#pragma unroll 4
+            for (int i = lane; i < pieces; i += LANES) {
+                widen<T>(v, x[i]);
 #pragma unroll
-            for (int c = 0; c < NCH; ++c) x[c].load(xr, (c * 32 * WPR + lane) * 8, a.d);
-            float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-            for (int c = 0; c < NCH; ++c) {
-                float v[8];
-                x[c].get(v);
-#pragma unroll
-                for (int j = 0; j < 8; j += 2) s0 += v[j], s1 += v[j + 1];
+                for (int j = 0; j < NP; j += 2) s = add_f2(s, v[j]), s1 = add_f2(s1, v[j + 1]);
             }
-            const float mean = team_total(s0 + s1, red[0]) * inv_d;
-            s0 = s1 = 0.f;
+            const float mean = team_total(sum_f2(s) + sum_f2(s1), red[0]) * inv_d;
+            const uint64_t shift = pack_f2(-mean, -mean);
+            s = s1 = 0;
+#pragma unroll 4
+            for (int i = lane; i < pieces; i += LANES) {
+                widen<T>(v, x[i]);
 #pragma unroll
-            for (int c = 0; c < NCH; ++c) {
-                if ((c * 32 * WPR + lane) * 8 >= a.d) continue;
-                float v[8];
-                x[c].get(v);
-#pragma unroll
-                for (int j = 0; j < 8; j += 2) {
-                    const float c0 = v[j] - mean, c1 = v[j + 1] - mean;
-                    s0 = fmaf(c0, c0, s0);
-                    s1 = fmaf(c1, c1, s1);
+                for (int j = 0; j < NP; j += 2) {
+                    const uint64_t c0 = add_f2(v[j], shift), c1 = add_f2(v[j + 1], shift);
+                    s = fma_f2(c0, c0, s);
+                    s1 = fma_f2(c1, c1, s1);
                 }
             }
-            const float rstd = rsqrtf(fmaf(team_total(s0 + s1, red[1]), inv_d, a.eps));
+            const float rstd = rsqrtf(fmaf(team_total(sum_f2(s) + sum_f2(s1), red[1]), inv_d, a.eps));
             if (a.mean != nullptr && lane == 0) {
                 a.mean[row] = mean;
                 a.rstd[row] = rstd;
             }
-            char *yr = static_cast<char *>(row_of<T>(a.y, row, a.ldy));
+            const uint64_t rs = pack_f2(rstd, rstd);
+            uint4 *y = static_cast<uint4 *>(row_of<T>(a.y, row, a.ldy));
+#pragma unroll 4
+            for (int i = lane; i < pieces; i += LANES) {
+                uint64_t p[NP];
+                widen<T>(v, x[i]);
 #pragma unroll
-            for (int c = 0; c < NCH; ++c) {
-                const int col = (c * 32 * WPR + lane) * 8;
-                if (col >= a.d) continue;
-                float v[8], p[8];
-                x[c].get(v);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = (v[j] - mean) * rstd;
+                for (int j = 0; j < NP; ++j) v[j] = mul_f2(add_f2(v[j], shift), rs);
                 if (w != nullptr) {
-                    load8<W>(p, w, col);
+                    param_piece<T, W>(p, w, i, pieces, stage);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) v[j] *= p[j];
+                    for (int j = 0; j < NP; ++j) v[j] = mul_f2(v[j], p[j]);
                 }
                 if (b != nullptr) {
-                    load8<W>(p, b, col);
+                    param_piece<T, W>(p, b, i, pieces, stage);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) v[j] += p[j];
+                    for (int j = 0; j < NP; ++j) v[j] = add_f2(v[j], p[j]);
                 }
-                store8<T, true>(yr + static_cast<size_t>(col) * dtype_size(T), v);
+                float f[2 * NP];
+#pragma unroll
+                for (int j = 0; j < NP; ++j) unpack_f2(v[j], f[2 * j], f[2 * j + 1]);
+                if constexpr (T == WF_F32) {
+                    y[i] = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+                } else {
+                    store8<T, true>(y + i, f);
+                }
             }
         }
+        cp_async_wait<0>();
     }
 }
 
@@ -403,82 +483,128 @@ struct NormGradArgs {
     int d;
 };
 
-// The backward pass of rows that 16-byte accesses fit, up to 8 values a thread of a block: R rows at a time, whose 2 R
-// sums share one barrier (their shuffles, too: lanes_sum_many).
+// The backward pass of rows that 16-byte accesses fit, 8 values a thread of a block: R rows at a time, whose 2 R sums
+// share one barrier (and their shuffles: lanes_sum_many). Each thread copies its own values of the next rows into a ring
+// of kRing stages in shared memory (cp.async) and reads nobody else's: the loads run on behind the barrier.
+constexpr int kRing = 3;
 template <int T, int W, int R, int THREADS, int BLOCKS>
 __global__ void __launch_bounds__(THREADS, BLOCKS) layer_norm_grad_rows_kernel(const __grid_constant__ NormGradArgs a) {
+    constexpr int H = T == WF_F32 ? 2 : 1;            // 16-byte pieces of 8 values
+    extern __shared__ uint4 smem[];                   // [kRing][R][x, dy][H][threads]
     __shared__ float red[2][32][2 * R];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, warps = blockDim.x >> 5, col = tid * 8;
+    const int tid = threadIdx.x, threads = blockDim.x, warp = tid >> 5, lane = tid & 31, warps = threads >> 5, col = tid * 8;
     const bool in = col < a.d;
     const float inv_d = 1.0f / static_cast<float>(a.d);
+    auto piece = [&](int stage, int r, int which, int h) { return smem + (((stage * R + r) * 2 + which) * H + h) * threads + tid; };
+    auto get = [&](uint64_t (&v)[4], int stage, int r, int which) {
+        Raw8<T> raw;
+#pragma unroll
+        for (int h = 0; h < H; ++h) raw.q[h] = *piece(stage, r, which, h);
+        raw.get(v);
+    };
     int buf = 0;
     wait_prior_grid();
     for (int64_t grp = a.split.first_group(blockIdx.x), end = a.split.last_group(blockIdx.x); grp < end; ++grp) {
         int64_t lo, hi;
         a.split.rows_of(blockIdx.x, grp, lo, hi);
-        float w[8], dw[8], db[8];
-        if (a.w != nullptr && in) load8<W>(w, row_of<W>(a.w, grp, a.d), col);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            dw[j] = db[j] = 0.f;
-            if (a.w == nullptr || !in) w[j] = 1.f;
-        }
-        for (int64_t row = lo; row < hi; row += R) {
-            Raw8<T> x[R], dy[R];
-            float scale[R], shift[R], s[2 * R];
+        auto fetch = [&](int64_t row, int stage) {  // one copy group for R rows, zeros past the last
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                const bool on = row + r < hi;
-                x[r].load(row_of<T>(a.x, row + r, a.ldx), col, on ? a.d : 0);
-                dy[r].load(row_of<T>(a.dy, row + r, a.lddy), col, on ? a.d : 0);
-            }
+                const bool on = in && row + r < hi;
+                const int64_t at = on ? row + r : 0;
+                const int c = on ? col : 0;
+                const char *x = static_cast<const char *>(row_of<T>(a.x, at, a.ldx)) + c * dtype_size(T);
+                const char *g = static_cast<const char *>(row_of<T>(a.dy, at, a.lddy)) + c * dtype_size(T);
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
-                const bool on = row + r < hi;
-                scale[r] = on ? a.rstd[row + r] : 0.f;
-                shift[r] = on ? a.mean[row + r] : 0.f;
-            }
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-                float v[8], g[8];
-                x[r].get(v);
-                dy[r].get(g);
-                s[2 * r] = s[2 * r + 1] = 0.f;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float xh = (v[j] - shift[r]) * scale[r];  // dy is 0 outside
-                    db[j] += g[j];
-                    dw[j] = fmaf(g[j], xh, dw[j]);
-                    const float u = g[j] * w[j];
-                    s[2 * r] += u;
-                    s[2 * r + 1] = fmaf(u, xh, s[2 * r + 1]);
+                for (int h = 0; h < H; ++h) {
+                    copy16(piece(stage, r, 0, h), x + 16 * h, on);
+                    copy16(piece(stage, r, 1, h), g + 16 * h, on);
                 }
             }
-            if (a.dx == nullptr) continue;
-            // every warp's sums to shared memory, then every warp adds all of them
-            const float mine = lanes_sum_many<2 * R>(s, lane);
-            if ((lane & (32 / (2 * R) - 1)) == 0) red[buf][warp][lane / (32 / (2 * R))] = mine;
-            __syncthreads();
-            float t = 0.f;  // sum lane % (2 R), of the warps lane / (2 R), + 32 / (2 R), ...
-            for (int i = lane / (2 * R); i < warps; i += 32 / (2 * R)) t += red[buf][i][lane % (2 * R)];
+            cp_async_commit();
+        };
+        for (int i = 0; i < kRing - 1; ++i) fetch(lo + i * R, i);
+        uint64_t w[4], dw[4], db[4];
+        if (a.w != nullptr && in) {
+            Raw8<W> raw;
+            raw.load(row_of<W>(a.w, grp, a.d), col, a.d);
+            raw.get(w);
+        }
 #pragma unroll
-            for (int o = 2 * R; o < 32; o *= 2) t += __shfl_xor_sync(0xFFFFFFFFu, t, o);
-            buf ^= 1;
+        for (int j = 0; j < 4; ++j) {
+            dw[j] = db[j] = 0;  // +0, +0
+            if (a.w == nullptr || !in) w[j] = pack_f2(1.f, 1.f);
+        }
+        int stage = 0, next = kRing - 1;
+        float scale[R], shift[R];  // of the rows at hand; the next ones are loaded a tile ahead
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            scale[r] = lo + r < hi ? a.rstd[lo + r] : 0.f;
+            shift[r] = lo + r < hi ? a.mean[lo + r] : 0.f;
+        }
+        for (int64_t row = lo; row < hi; row += R) {
+            fetch(row + (kRing - 1) * R, next);
+            if (++next == kRing) next = 0;
+            float scale1[R], shift1[R], s[2 * R];
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                const float m0 = __shfl_sync(0xFFFFFFFFu, t, 2 * r) * inv_d, m1 = __shfl_sync(0xFFFFFFFFu, t, 2 * r + 1) * inv_d;
-                if (!in || row + r >= hi) continue;
-                float v[8], g[8];
-                x[r].get(v);
-                dy[r].get(g);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) g[j] = scale[r] * (fmaf(g[j], w[j], -m0) - (v[j] - shift[r]) * scale[r] * m1);
-                store8<T, true>(static_cast<char *>(row_of<T>(a.dx, row + r, a.lddx)) + static_cast<size_t>(col) * dtype_size(T), g);
+                scale1[r] = row + R + r < hi ? a.rstd[row + R + r] : 0.f;
+                shift1[r] = row + R + r < hi ? a.mean[row + R + r] : 0.f;
             }
+            cp_async_wait<kRing - 1>();
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                uint64_t v[4], g[4], s0 = 0, s1 = 0;
+                get(v, stage, r, 0);
+                get(g, stage, r, 1);
+                const uint64_t rs = pack_f2(scale[r], scale[r]), mu = pack_f2(-shift[r], -shift[r]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint64_t xh = mul_f2(add_f2(v[j], mu), rs);  // dy is 0 outside
+                    db[j] = add_f2(db[j], g[j]);
+                    dw[j] = fma_f2(g[j], xh, dw[j]);
+                    const uint64_t u = mul_f2(g[j], w[j]);
+                    s0 = add_f2(s0, u);
+                    s1 = fma_f2(u, xh, s1);
+                }
+                s[2 * r] = sum_f2(s0);
+                s[2 * r + 1] = sum_f2(s1);
+            }
+            if (a.dx != nullptr) {
+                // every warp's sums to shared memory, then every warp adds all of them
+                const float mine = lanes_sum_many<2 * R>(s, lane);
+                if ((lane & (32 / (2 * R) - 1)) == 0) red[buf][warp][lane / (32 / (2 * R))] = mine;
+                __syncthreads();
+                float t = 0.f;  // sum lane % (2 R), of the warps lane / (2 R), + 32 / (2 R), ...
+                for (int i = lane / (2 * R); i < warps; i += 32 / (2 * R)) t += red[buf][i][lane % (2 * R)];
+#pragma unroll
+                for (int o = 2 * R; o < 32; o *= 2) t += __shfl_xor_sync(0xFFFFFFFFu, t, o);
+                buf ^= 1;
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    const float m0 = __shfl_sync(0xFFFFFFFFu, t, 2 * r) * inv_d, m1 = __shfl_sync(0xFFFFFFFFu, t, 2 * r + 1) * inv_d;
+                    if (!in || row + r >= hi) continue;
+                    uint64_t v[4], g[4];
+                    get(v, stage, r, 0);
+                    get(g, stage, r, 1);
+                    const uint64_t rs = pack_f2(scale[r], scale[r]), mu = pack_f2(-shift[r], -shift[r]);
+                    const uint64_t a0 = pack_f2(-m0, -m0), a1 = pack_f2(-m1, -m1);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint64_t xh = mul_f2(add_f2(v[j], mu), rs);
+                        g[j] = mul_f2(rs, fma_f2(xh, a1, fma_f2(g[j], w[j], a0)));
+                    }
+                    store_pairs<T>(row_of<T>(a.dx, row + r, a.lddx), col, g);
+                }
+            }
+            if (++stage == kRing) stage = 0;
+#pragma unroll
+            for (int r = 0; r < R; ++r) scale[r] = scale1[r], shift[r] = shift1[r];
         }
-        const int64_t part = a.split.partial_row(blockIdx.x, grp) * a.d + col;
-        if (a.part_w != nullptr && in) store8<WF_F32, true>(a.part_w + part, dw);
-        if (a.part_b != nullptr && in) store8<WF_F32, true>(a.part_b + part, db);
+        cp_async_wait<0>();
+        const int64_t part = a.split.partial_row(blockIdx.x, grp) * a.d;
+        if (a.part_w != nullptr && in) store_pairs<WF_F32>(a.part_w + part, col, dw);
+        if (a.part_b != nullptr && in) store_pairs<WF_F32>(a.part_b + part, col, db);
     }
 }
 
@@ -495,12 +621,16 @@ __global__ void __launch_bounds__(256) layer_norm_grad_narrow_kernel(const __gri
     for (int64_t grp = a.split.first_group(blockIdx.x), end = a.split.last_group(blockIdx.x); grp < end; ++grp) {
         int64_t lo, hi;
         a.split.rows_of(blockIdx.x, grp, lo, hi);
-        float w[8], sums[16];  // dw, db
-        if (a.w != nullptr && in) load8<W>(w, row_of<W>(a.w, grp, a.d), col);
+        uint64_t w[4], dw[4], db[4];
+        if (a.w != nullptr && in) {
+            Raw8<W> raw;
+            raw.load(row_of<W>(a.w, grp, a.d), col, a.d);
+            raw.get(w);
+        }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            sums[j] = sums[j + 8] = 0.f;
-            if (a.w == nullptr || !in) w[j] = 1.f;
+        for (int j = 0; j < 4; ++j) {
+            dw[j] = db[j] = 0;  // +0, +0
+            if (a.w == nullptr || !in) w[j] = pack_f2(1.f, 1.f);
         }
         for (int64_t first = lo + warp * RPW * R; first < hi; first += 8 * RPW * R) {
             Raw8<T> x[R], dy[R];
@@ -517,28 +647,35 @@ __global__ void __launch_bounds__(256) layer_norm_grad_narrow_kernel(const __gri
 #pragma unroll
             for (int r = 0; r < R; ++r) {
                 const int64_t row = first + r * RPW + sub;
-                float v[8], g[8], s0 = 0.f, s1 = 0.f;
+                uint64_t v[4], g[4], s0 = 0, s1 = 0;
                 x[r].get(v);
                 dy[r].get(g);
+                const uint64_t rs = pack_f2(scale[r], scale[r]), mu = pack_f2(-shift[r], -shift[r]);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    v[j] = (v[j] - shift[r]) * scale[r];
-                    sums[j + 8] += g[j];
-                    sums[j] = fmaf(g[j], v[j], sums[j]);
-                    g[j] *= w[j];
-                    s0 += g[j];
-                    s1 = fmaf(g[j], v[j], s1);
+                for (int j = 0; j < 4; ++j) {
+                    v[j] = mul_f2(add_f2(v[j], mu), rs);
+                    db[j] = add_f2(db[j], g[j]);
+                    dw[j] = fma_f2(g[j], v[j], dw[j]);
+                    g[j] = mul_f2(g[j], w[j]);
+                    s0 = add_f2(s0, g[j]);
+                    s1 = fma_f2(g[j], v[j], s1);
                 }
                 if (a.dx == nullptr) continue;
-                const float m0 = lanes_sum<LPR>(s0) * inv_d, m1 = lanes_sum<LPR>(s1) * inv_d;
+                const float m0 = lanes_sum<LPR>(sum_f2(s0)) * inv_d, m1 = lanes_sum<LPR>(sum_f2(s1)) * inv_d;
                 if (row >= hi || !in) continue;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) g[j] = scale[r] * (g[j] - m0 - v[j] * m1);
-                store8<T, true>(static_cast<char *>(row_of<T>(a.dx, row, a.lddx)) + static_cast<size_t>(col) * dtype_size(T), g);
+                for (int j = 0; j < 4; ++j) g[j] = mul_f2(rs, fma_f2(v[j], pack_f2(-m1, -m1), add_f2(g[j], pack_f2(-m0, -m0))));
+                store_pairs<T>(row_of<T>(a.dx, row, a.lddx), col, g);
             }
             __syncwarp();
         }
         if (a.part_w == nullptr && a.part_b == nullptr) continue;
+        float sums[16];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            unpack_f2(dw[j], sums[2 * j], sums[2 * j + 1]);
+            unpack_f2(db[j], sums[8 + 2 * j], sums[9 + 2 * j]);
+        }
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -736,26 +873,28 @@ int launch_norm_narrow(const NormArgs &a, cudaStream_t stream) {
     return launch_rows(kern, dim3(grid), 256, stream, a);
 }
 
-template <int T, int W, int NCH, int WPR>
-int launch_norm_team(const NormArgs &a, cudaStream_t stream) {
-    constexpr auto kern = layer_norm_team_kernel<T, W, NCH, WPR>;
-    constexpr size_t most = 2u * NCH * WPR * 256 * dtype_size(W);
-    static std::atomic<int> resident[64];  // blocks on the device at the widest row; any host thread may launch first
+// rings for a block of at most 96 KB (two blocks an SM), of at most 4 rows a team; 0: not even two rows fit 200 KB
+template <int T, int W, int WPR>
+int launch_norm_stream(const NormArgs &a, cudaStream_t stream) {
+    constexpr auto kern = layer_norm_stream_kernel<T, W, WPR>;
+    constexpr int most = 200 * 1024;
+    const int64_t row = static_cast<int64_t>(a.d) * dtype_size(T) * (8 / WPR), params = 2ll * a.d * dtype_size(W);
+    const bool params_fit = params + 2 * row <= most;
+    const int bufs = static_cast<int>(std::max<int64_t>(2, std::min<int64_t>(4, (96 * 1024 - (params_fit ? params : 0)) / row)));
+    static std::atomic<bool> ready[64];  // any host thread may launch first
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64) return WF_ERR_DEVICE;
-    if (resident[dev].load(std::memory_order_acquire) == 0) {
-        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(most));
+    if (!ready[dev].load(std::memory_order_acquire)) {
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
         if (e != cudaSuccess) return static_cast<int>(e);
-        int n = 0;
-        e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, 256, most);
-        if (e != cudaSuccess) return static_cast<int>(e);
-        resident[dev].store(std::max(n, 1) * device_sm_count(), std::memory_order_release);
+        ready[dev].store(true, std::memory_order_release);
     }
-    const RowSplit split = make_split(a.rows, a.rows_per_group, resident[dev].load(std::memory_order_acquire), 8 / WPR);
-    const bool stage = (a.w != nullptr || a.b != nullptr) && split.rows_per_group >= kStageRows;
-    const size_t smem = stage ? 2 * static_cast<size_t>(a.d) * dtype_size(W) : 0;
-    const cudaError_t e = launch_dependent(kern, dim3(static_cast<unsigned>(split.blocks())), 256, smem, stream, a, split, stage);
+    const bool stage = (a.w != nullptr || a.b != nullptr) && params_fit && std::min(a.rows_per_group, a.rows) >= kStageRows;
+    const int64_t smem = bufs * row + (stage ? params : 0);
+    const int64_t resident = std::max<int64_t>(1, std::min<int64_t>(6, 220 * 1024 / (smem + 1024))) * device_sm_count();
+    const RowSplit split = make_split(a.rows, a.rows_per_group, resident, 8 / WPR);
+    const cudaError_t e = launch_dependent(kern, dim3(static_cast<unsigned>(split.blocks())), 256, smem, stream, a, split, bufs, stage);
     return static_cast<int>(e != cudaSuccess ? e : cudaGetLastError());
 }
 
@@ -769,20 +908,13 @@ int dispatch_norm(const NormArgs &a, cudaStream_t stream) {
     if (chunks <= 8) return launch_norm_narrow<T, W, 8>(a, stream);
     if (chunks <= 16) return launch_norm_narrow<T, W, 16>(a, stream);
     if (chunks <= 32) return launch_norm_narrow<T, W, 32>(a, stream);
-    // teams of warps where there are rows for them; else a row a block
+    // teams of warps where there are rows for them, up to 10 KB of a row a warp; else a row a block
+    const int kb = (a.d * dtype_size(T) + 1023) / 1024;
     if (a.rows >= 4ll * device_sm_count()) {
-        constexpr int wide = T == WF_F32 ? 10 : 20;  // chunks a lane: 80 registers
-        const int need = (chunks + 31) / 32;
-        if (need <= 2) return launch_norm_team<T, W, 2, 1>(a, stream);
-        if (need <= 4) return launch_norm_team<T, W, 4, 1>(a, stream);
-        if (need <= 8) return launch_norm_team<T, W, 8, 1>(a, stream);
-        if constexpr (T != WF_F32) {
-            if (need <= 12) return launch_norm_team<T, W, 12, 1>(a, stream);
-            if (need <= 16) return launch_norm_team<T, W, 16, 1>(a, stream);
-        }
-        if (need <= wide) return launch_norm_team<T, W, wide, 1>(a, stream);
-        if (need <= 2 * wide) return launch_norm_team<T, W, wide, 2>(a, stream);
-        if (need <= 4 * wide && W != WF_F32) return launch_norm_team<T, W, wide, 4>(a, stream);
+        if (kb <= 10) return launch_norm_stream<T, W, 1>(a, stream);
+        if (kb <= 20) return launch_norm_stream<T, W, 2>(a, stream);
+        if (kb <= 40) return launch_norm_stream<T, W, 4>(a, stream);
+        if (kb <= 80) return launch_norm_stream<T, W, 8>(a, stream);
     }
     return launch_norm_block<T, W, true>(a, stream);
 }
@@ -801,6 +933,24 @@ int launch_norm_grad_wide(const NormGradArgs &a, cudaStream_t stream) {
     return rc;
 }
 
+template <int T, int W, int R, int THREADS, int BLOCKS>
+int launch_norm_grad_rows(const NormGradArgs &a, int threads, cudaStream_t stream) {
+    constexpr auto kern = layer_norm_grad_rows_kernel<T, W, R, THREADS, BLOCKS>;
+    constexpr int per_thread = kRing * R * 2 * (T == WF_F32 ? 32 : 16);
+    static std::atomic<bool> ready[64];  // any host thread may launch first
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64) return WF_ERR_DEVICE;
+    if (!ready[dev].load(std::memory_order_acquire)) {
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, THREADS * per_thread);
+        if (e != cudaSuccess) return static_cast<int>(e);
+        ready[dev].store(true, std::memory_order_release);
+    }
+    const cudaError_t e = launch_dependent(kern, dim3(static_cast<unsigned>(a.split.blocks())), threads,
+                                           static_cast<size_t>(threads) * per_thread, stream, a);
+    return static_cast<int>(e != cudaSuccess ? e : cudaGetLastError());
+}
+
 template <int T, int W>
 int dispatch_norm_grad(const NormGradArgs &a, cudaStream_t stream) {
     const bool vec = a.d % 8 == 0 && vec_ok(a.x, a.ldx, dtype_size(T)) && vec_ok(a.dy, a.lddy, dtype_size(T)) &&
@@ -817,9 +967,10 @@ int dispatch_norm_grad(const NormGradArgs &a, cudaStream_t stream) {
     }
     const int threads = row_threads(a.d);
     if (!vec) return launch_rows(layer_norm_grad_kernel<T, W, false>, grid, threads, stream, a);
-    if (threads <= 256) return launch_rows(layer_norm_grad_rows_kernel<T, W, 4, 256, 2>, grid, threads, stream, a);
-    if (threads <= 640) return launch_rows(layer_norm_grad_rows_kernel<T, W, 2, 640, 1>, grid, threads, stream, a);
-    return launch_rows(layer_norm_grad_rows_kernel<T, W, 1, 1024, 1>, grid, threads, stream, a);
+    constexpr int half = T == WF_F32 ? 2 : 1;  // rows of half as many: as many bytes, 96 to 192 KB a block
+    if (threads <= 256) return launch_norm_grad_rows<T, W, 4 / half, 256, 2>(a, threads, stream);
+    if (threads <= 640) return launch_norm_grad_rows<T, W, 2 / half, 640, 1>(a, threads, stream);
+    return launch_norm_grad_rows<T, W, 1, 1024, 1>(a, threads, stream);
 }
 
 bool norm_types_ok(int type, int w_type) {

@@ -2,6 +2,7 @@
 #pragma once
 
 #include "wf_common.cuh"
+#include "wf_pairs.cuh"
 
 namespace wf {
 namespace {
@@ -25,26 +26,6 @@ __device__ __forceinline__ float fast_exp(float x) {
 
 // 1 / (1 + exp(-v))
 __device__ __forceinline__ float sigmoid(float v) { return fast_rcp(1.0f + fast_exp(-v)); }
-
-// Two float32 lanes in one 64-bit register: one packed instruction rounds each lane as the scalar one does.
-__device__ __forceinline__ uint64_t pack_f2(float lo, float hi) {
-    uint64_t v;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
-    return v;
-}
-__device__ __forceinline__ void unpack_f2(uint64_t v, float &lo, float &hi) {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
-}
-__device__ __forceinline__ uint64_t fma_f2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
-}
-__device__ __forceinline__ uint64_t mul_f2(uint64_t a, uint64_t b) {
-    uint64_t d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
 
 // The normal distribution function of two values: 0.5 + v g(v^2), g the minimax polynomial (weighted by v) of degree 14
 // in s = 2 (v / 5.25)^2 - 1, fitted on |v| <= 5.25. Off by at most 1.1e-7, evaluated in float32, over all v: past 5.25
