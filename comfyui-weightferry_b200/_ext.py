@@ -82,7 +82,7 @@ SIGNATURES = {
     "wf_copy_rows16": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p] + [ctypes.c_int64] * 3
                        + [ctypes.c_void_p]),
     "wf_layer_norm": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]),
-    "wf_layer_norm_backward_workspace": (ctypes.c_int64, [ctypes.c_int64] * 3),
+    "wf_layer_norm_backward_workspace": (ctypes.c_int64, [ctypes.c_int64] * 3 + [ctypes.c_int]),
     "wf_layer_norm_backward": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]),
 }
 

@@ -25,13 +25,6 @@ namespace {
 
 constexpr int kMaxThreads = 1024;
 
-// the sum of v over the 32 lanes, in every lane
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
-    return v;
-}
-
 // The sums of N values over the block's threads, in every thread (one warp: shuffles alone). `red` has room for
 // 32 * N floats; two calls in a row take different buffers, so that one barrier a call is enough.
 template <int N>
@@ -116,13 +109,18 @@ struct Raw8 {
     }
 };
 
-// eight values, rounded to T, to column col of a row (16-byte aligned)
-template <int T>
-__device__ __forceinline__ void store_pairs(void *row, int col, const uint64_t (&v)[4]) {
-    float f[8];
+// eight values, or four of float32, rounded to T, to column col of a row (16-byte aligned)
+template <int T, int NP>
+__device__ __forceinline__ void store_pairs(void *row, int col, const uint64_t (&v)[NP]) {
+    static_assert(NP == 4 || (NP == 2 && T == WF_F32), "16 or 32 bytes");
+    float f[2 * NP];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) unpack_f2(v[i], f[2 * i], f[2 * i + 1]);
-    store8<T, true>(static_cast<char *>(row) + static_cast<int64_t>(col) * dtype_size(T), f);
+    for (int i = 0; i < NP; ++i) unpack_f2(v[i], f[2 * i], f[2 * i + 1]);
+    if constexpr (NP == 4) {
+        store8<T, true>(static_cast<char *>(row) + static_cast<int64_t>(col) * dtype_size(T), f);
+    } else {
+        *reinterpret_cast<float4 *>(static_cast<float *>(row) + col) = make_float4(f[0], f[1], f[2], f[3]);
+    }
 }
 
 // the sum over aligned sets of LPR lanes, in each of them
@@ -313,13 +311,6 @@ __global__ void __launch_bounds__(256) layer_norm_narrow_kernel(const __grid_con
     }
 }
 
-// 16 bytes from global to shared memory past the registers (zeros where `on` is false)
-__device__ __forceinline__ void copy16(void *dst, const void *src, bool on) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))),
-                 "l"(src), "r"(on ? 16 : 0)
-                 : "memory");
-}
-
 // 16 bytes of T as pairs: 8 or 4 values
 template <int T>
 __device__ __forceinline__ void widen(uint64_t (&v)[T == WF_F32 ? 2 : 4], const uint4 &q) {
@@ -483,24 +474,27 @@ struct NormGradArgs {
     int d;
 };
 
-// The backward pass of rows that 16-byte accesses fit, 8 values a thread of a block: R rows at a time, whose 2 R sums
+// The backward pass of rows that 16-byte accesses fit, V (8 or 4) values a thread of a block: R rows at a time, whose 2 R sums
 // share one barrier (and their shuffles: lanes_sum_many). Each thread copies its own values of the next rows into a ring
 // of kRing stages in shared memory (cp.async) and reads nobody else's: the loads run on behind the barrier.
 constexpr int kRing = 3;
-template <int T, int W, int R, int THREADS, int BLOCKS>
+template <int T, int W, int V, int R, int THREADS, int BLOCKS>
 __global__ void __launch_bounds__(THREADS, BLOCKS) layer_norm_grad_rows_kernel(const __grid_constant__ NormGradArgs a) {
-    constexpr int H = T == WF_F32 ? 2 : 1;            // 16-byte pieces of 8 values
+    constexpr int H = V * dtype_size(T) / 16, NP = V / 2;  // 16-byte pieces and pairs of V values
     extern __shared__ uint4 smem[];                   // [kRing][R][x, dy][H][threads]
     __shared__ float red[2][32][2 * R];
-    const int tid = threadIdx.x, threads = blockDim.x, warp = tid >> 5, lane = tid & 31, warps = threads >> 5, col = tid * 8;
+    const int tid = threadIdx.x, threads = blockDim.x, warp = tid >> 5, lane = tid & 31, warps = threads >> 5, col = tid * V;
     const bool in = col < a.d;
     const float inv_d = 1.0f / static_cast<float>(a.d);
     auto piece = [&](int stage, int r, int which, int h) { return smem + (((stage * R + r) * 2 + which) * H + h) * threads + tid; };
-    auto get = [&](uint64_t (&v)[4], int stage, int r, int which) {
-        Raw8<T> raw;
+    auto get = [&](uint64_t (&v)[NP], int stage, int r, int which) {
 #pragma unroll
-        for (int h = 0; h < H; ++h) raw.q[h] = *piece(stage, r, which, h);
-        raw.get(v);
+        for (int h = 0; h < H; ++h) {
+            uint64_t p[NP / H];
+            widen<T>(p, *piece(stage, r, which, h));
+#pragma unroll
+            for (int j = 0; j < NP / H; ++j) v[h * (NP / H) + j] = p[j];
+        }
     };
     int buf = 0;
     wait_prior_grid();
@@ -524,16 +518,12 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) layer_norm_grad_rows_kernel(c
             cp_async_commit();
         };
         for (int i = 0; i < kRing - 1; ++i) fetch(lo + i * R, i);
-        uint64_t w[4], dw[4], db[4];
-        if (a.w != nullptr && in) {
-            Raw8<W> raw;
-            raw.load(row_of<W>(a.w, grp, a.d), col, a.d);
-            raw.get(w);
-        }
+        uint64_t w[NP], dw[NP], db[NP];
+        const void *wr = row_of<W>(a.w, grp, a.d);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < NP; ++j) {
             dw[j] = db[j] = 0;  // +0, +0
-            if (a.w == nullptr || !in) w[j] = pack_f2(1.f, 1.f);
+            w[j] = a.w != nullptr && in ? pack_f2(load1<W>(wr, col + 2 * j), load1<W>(wr, col + 2 * j + 1)) : pack_f2(1.f, 1.f);
         }
         int stage = 0, next = kRing - 1;
         float scale[R], shift[R];  // of the rows at hand; the next ones are loaded a tile ahead
@@ -554,12 +544,12 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) layer_norm_grad_rows_kernel(c
             cp_async_wait<kRing - 1>();
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                uint64_t v[4], g[4], s0 = 0, s1 = 0;
+                uint64_t v[NP], g[NP], s0 = 0, s1 = 0;
                 get(v, stage, r, 0);
                 get(g, stage, r, 1);
                 const uint64_t rs = pack_f2(scale[r], scale[r]), mu = pack_f2(-shift[r], -shift[r]);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
+                for (int j = 0; j < NP; ++j) {
                     const uint64_t xh = mul_f2(add_f2(v[j], mu), rs);  // dy is 0 outside
                     db[j] = add_f2(db[j], g[j]);
                     dw[j] = fma_f2(g[j], xh, dw[j]);
@@ -584,13 +574,13 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) layer_norm_grad_rows_kernel(c
                 for (int r = 0; r < R; ++r) {
                     const float m0 = __shfl_sync(0xFFFFFFFFu, t, 2 * r) * inv_d, m1 = __shfl_sync(0xFFFFFFFFu, t, 2 * r + 1) * inv_d;
                     if (!in || row + r >= hi) continue;
-                    uint64_t v[4], g[4];
+                    uint64_t v[NP], g[NP];
                     get(v, stage, r, 0);
                     get(g, stage, r, 1);
                     const uint64_t rs = pack_f2(scale[r], scale[r]), mu = pack_f2(-shift[r], -shift[r]);
                     const uint64_t a0 = pack_f2(-m0, -m0), a1 = pack_f2(-m1, -m1);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
+                    for (int j = 0; j < NP; ++j) {
                         const uint64_t xh = mul_f2(add_f2(v[j], mu), rs);
                         g[j] = mul_f2(rs, fma_f2(xh, a1, fma_f2(g[j], w[j], a0)));
                     }
@@ -611,8 +601,8 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) layer_norm_grad_rows_kernel(c
 // The backward pass of narrow rows (up to 256 values) that 16-byte accesses fit: LPR lanes a row, 32 / LPR rows a warp, R
 // of them at a time. At the end of a group the lanes that own the same columns, then the warps, add their column sums.
 template <int T, int W, int LPR>
-__global__ void __launch_bounds__(256) layer_norm_grad_narrow_kernel(const __grid_constant__ NormGradArgs a) {
-    constexpr int RPW = 32 / LPR, R = 4;
+__global__ void __launch_bounds__(256, 3) layer_norm_grad_narrow_kernel(const __grid_constant__ NormGradArgs a) {
+    constexpr int RPW = 32 / LPR, R = 2;
     __shared__ float col_red[8][16][LPR];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & (LPR - 1), sub = (threadIdx.x & 31) / LPR, col = lane * 8;
     const bool in = col < a.d;
@@ -839,6 +829,12 @@ bool vec_ok(const void *p, int64_t ld, int size) {
     return p == nullptr || (aligned_to(p, 16) && (ld * size) % 16 == 0);
 }
 
+// threads of the backward pass's block: 16 bytes of a row each, or (float32 past 4096 values) 32
+int grad_threads(int d, int type) {
+    const int v = type == WF_F32 && d <= 4 * kMaxThreads ? 4 : 8;
+    return ((d + v - 1) / v + 31) / 32 * 32;
+}
+
 // a block's threads for 8 values each, or the most there are
 int row_threads(int d) { return std::min(kMaxThreads, ((d + 7) / 8 + 31) / 32 * 32); }
 
@@ -873,14 +869,14 @@ int launch_norm_narrow(const NormArgs &a, cudaStream_t stream) {
     return launch_rows(kern, dim3(grid), 256, stream, a);
 }
 
-// rings for a block of at most 96 KB (two blocks an SM), of at most 4 rows a team; 0: not even two rows fit 200 KB
+// rings of 2 to 4 rows a team, for blocks of about 64 KB where a row is short enough
 template <int T, int W, int WPR>
 int launch_norm_stream(const NormArgs &a, cudaStream_t stream) {
     constexpr auto kern = layer_norm_stream_kernel<T, W, WPR>;
     constexpr int most = 200 * 1024;
     const int64_t row = static_cast<int64_t>(a.d) * dtype_size(T) * (8 / WPR), params = 2ll * a.d * dtype_size(W);
     const bool params_fit = params + 2 * row <= most;
-    const int bufs = static_cast<int>(std::max<int64_t>(2, std::min<int64_t>(4, (96 * 1024 - (params_fit ? params : 0)) / row)));
+    const int bufs = static_cast<int>(std::max<int64_t>(2, std::min<int64_t>(4, (64 * 1024 - (params_fit ? params : 0)) / row)));
     static std::atomic<bool> ready[64];  // any host thread may launch first
     int dev = 0;
     cudaGetDevice(&dev);
@@ -933,10 +929,10 @@ int launch_norm_grad_wide(const NormGradArgs &a, cudaStream_t stream) {
     return rc;
 }
 
-template <int T, int W, int R, int THREADS, int BLOCKS>
+template <int T, int W, int V, int R, int THREADS, int BLOCKS>
 int launch_norm_grad_rows(const NormGradArgs &a, int threads, cudaStream_t stream) {
-    constexpr auto kern = layer_norm_grad_rows_kernel<T, W, R, THREADS, BLOCKS>;
-    constexpr int per_thread = kRing * R * 2 * (T == WF_F32 ? 32 : 16);
+    constexpr auto kern = layer_norm_grad_rows_kernel<T, W, V, R, THREADS, BLOCKS>;
+    constexpr int per_thread = kRing * R * 2 * V * dtype_size(T);
     static std::atomic<bool> ready[64];  // any host thread may launch first
     int dev = 0;
     cudaGetDevice(&dev);
@@ -965,12 +961,13 @@ int dispatch_norm_grad(const NormGradArgs &a, cudaStream_t stream) {
         if (a.d <= 128) return launch_rows(layer_norm_grad_narrow_kernel<T, W, 16>, grid, 256, stream, a);
         return launch_rows(layer_norm_grad_narrow_kernel<T, W, 32>, grid, 256, stream, a);
     }
-    const int threads = row_threads(a.d);
-    if (!vec) return launch_rows(layer_norm_grad_kernel<T, W, false>, grid, threads, stream, a);
-    constexpr int half = T == WF_F32 ? 2 : 1;  // rows of half as many: as many bytes, 96 to 192 KB a block
-    if (threads <= 256) return launch_norm_grad_rows<T, W, 4 / half, 256, 2>(a, threads, stream);
-    if (threads <= 640) return launch_norm_grad_rows<T, W, 2 / half, 640, 1>(a, threads, stream);
-    return launch_norm_grad_rows<T, W, 1, 1024, 1>(a, threads, stream);
+    if (!vec) return launch_rows(layer_norm_grad_kernel<T, W, false>, grid, row_threads(a.d), stream, a);
+    constexpr int V = T == WF_F32 ? 4 : 8;  // 16 bytes a thread; float32 rows past 4096 values take 32
+    const int threads = grad_threads(a.d, T);
+    if (T == WF_F32 && a.d > V * kMaxThreads) return launch_norm_grad_rows<T, W, 8, 1, kMaxThreads, 1>(a, threads, stream);
+    if (threads <= 256) return launch_norm_grad_rows<T, W, V, 4, 256, 2>(a, threads, stream);
+    if (threads <= 640) return launch_norm_grad_rows<T, W, V, 2, 640, 1>(a, threads, stream);
+    return launch_norm_grad_rows<T, W, V, 1, kMaxThreads, 1>(a, threads, stream);
 }
 
 bool norm_types_ok(int type, int w_type) {
@@ -978,11 +975,11 @@ bool norm_types_ok(int type, int w_type) {
 }
 
 // The shares of the rows that the backward pass's blocks take: about as many as are resident at once.
-RowSplit norm_split(int64_t rows, int64_t rows_per_group, int d) {
+RowSplit norm_split(int64_t rows, int64_t rows_per_group, int d, int type) {
     const int64_t sms = device_sm_count();
     if (d > 8 * kMaxThreads) return make_split(rows, rows_per_group, std::max<int64_t>(1, 4 * sms * 2048 / d), 16);
-    if (d <= 256) return make_split(rows, rows_per_group, 4 * sms, 8);
-    return make_split(rows, rows_per_group, sms * std::max(1, std::min(8, 640 / row_threads(d))), 4);
+    if (d <= 256) return make_split(rows, rows_per_group, 3 * sms, 16);
+    return make_split(rows, rows_per_group, sms * std::max(1, std::min(8, 640 / (d % 8 == 0 ? grad_threads(d, type) : row_threads(d)))), 4);
 }
 
 }  // namespace
@@ -1010,10 +1007,10 @@ extern "C" WF_API int wf_layer_norm(const wf_layer_norm_args *args, wf_stream_t 
     return g.w_type == WF_F32 ? dispatch_norm<WF_F16, WF_F32>(a, st) : dispatch_norm<WF_F16, WF_F16>(a, st);
 }
 
-extern "C" WF_API int64_t wf_layer_norm_backward_workspace(int64_t rows, int64_t d, int64_t rows_per_group) {
+extern "C" WF_API int64_t wf_layer_norm_backward_workspace(int64_t rows, int64_t d, int64_t rows_per_group, int type) {
     using namespace wf;
     if (rows < 1 || d < 1 || d > (1 << 30) || rows_per_group < 1) return 0;
-    return 2 * norm_split(rows, rows_per_group, static_cast<int>(d)).partial_rows() * d * static_cast<int64_t>(sizeof(float));
+    return 2 * norm_split(rows, rows_per_group, static_cast<int>(d), type).partial_rows() * d * static_cast<int64_t>(sizeof(float));
 }
 
 extern "C" WF_API int wf_layer_norm_backward(const wf_layer_norm_grad_args *args, wf_stream_t stream) {
@@ -1030,7 +1027,7 @@ extern "C" WF_API int wf_layer_norm_backward(const wf_layer_norm_grad_args *args
         !aligned_to(g.rstd, 4))
         return WF_ERR_ARG;
     if (!g.dx && !g.dw && !g.db) return WF_OK;
-    const RowSplit split = norm_split(g.rows, g.rows_per_group, static_cast<int>(g.d));
+    const RowSplit split = norm_split(g.rows, g.rows_per_group, static_cast<int>(g.d), g.type);
     const int64_t half = split.partial_rows() * g.d;
     if ((g.dw || g.db) && (!g.workspace || !aligned_to(g.workspace, 16) ||
                            g.workspace_bytes < 2 * half * static_cast<int64_t>(sizeof(float))))

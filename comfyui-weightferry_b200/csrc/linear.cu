@@ -16,6 +16,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 namespace wf {
 namespace {
@@ -141,16 +142,6 @@ __device__ __forceinline__ void load4(float (&v)[4], const void *row, int col, i
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = col + i < n ? load1<T>(row, col + i) : 0.f;
-    }
-}
-template <int T>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-    if constexpr (T == WF_BF16) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-        return *reinterpret_cast<const uint32_t *>(&h);
-    } else {
-        const __half2 h = __floats2half2_rn(a, b);
-        return *reinterpret_cast<const uint32_t *>(&h);
     }
 }
 template <int T>
@@ -332,17 +323,27 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_const
     if (warp == 5)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::tmem_cols) : "memory");
     // this CTA finishes rows t_lo .. t_hi of the tile, a row a warp, four columns a lane
-    const int t_lo = NT * rank / split, t_hi = min(NT * (rank + 1) / split, m - i0);
-    for (int t = t_lo + warp; t < t_hi; t += TILE_THREADS / 32) {
-        const uint32_t at = ring0 + static_cast<uint32_t>(t * TILE_J + lane * 4) * 4u;
-        float v[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int r = 0; r < split; ++r) {
-            const float4 p = ld_cluster4(split > 1 ? map_to_rank(at, r) : at);
-            v[0] += p.x, v[1] += p.y, v[2] += p.z, v[3] += p.w;
+    const int t_lo = NT * rank / split, t_hi = min(NT * (rank + 1) / split, m - i0), col = j0 + lane * 4;
+    auto finish = [&](auto parts) {  // all of a row's parts are read before the first is added
+        constexpr int S = decltype(parts)::value;
+        uint32_t base[S];
+#pragma unroll
+        for (int r = 0; r < S; ++r) base[r] = S > 1 ? map_to_rank(ring0, r) : ring0;
+#pragma unroll 2
+        for (int t = t_lo + warp; t < t_hi; t += TILE_THREADS / 32) {
+            float4 p[S];
+#pragma unroll
+            for (int r = 0; r < S; ++r) p[r] = ld_cluster4(base[r] + static_cast<uint32_t>(t * TILE_J + lane * 4) * 4u);
+            float v[4] = {p[0].x, p[0].y, p[0].z, p[0].w};
+#pragma unroll
+            for (int r = 1; r < S; ++r) v[0] += p[r].x, v[1] += p[r].y, v[2] += p[r].z, v[3] += p[r].w;
+            if (col < n) finish4<T>(epi, v, i0 + t, col, n);
         }
-        const int col = j0 + lane * 4;
-        if (col < n) finish4<T>(epi, v, i0 + t, col, n);
-    }
+    };
+    if (split == 1) finish(std::integral_constant<int, 1>{});
+    else if (split == 2) finish(std::integral_constant<int, 2>{});
+    else if (split == 4) finish(std::integral_constant<int, 4>{});
+    else finish(std::integral_constant<int, 8>{});
     if (split > 1) cluster_sync();  // no CTA leaves while another reads its part
 }
 

@@ -10,12 +10,13 @@ struct ReduceArgs {
     int64_t d;
 };
 
-// Block (x, y, z): columns 32 x .. 32 x + 31 of groups y, y + gridDim.y, ... of sum z. Eight warps take every eighth
-// part, then their sums are added in warp order: a fixed order for a given shape. A few MB at most; bound by latency.
+// Block (x, y, z): columns 32 x .. 32 x + 31 of groups y, y + gridDim.y, ... of sum z. Warp w takes parts w,
+// w + warps, ..., then a tree adds the warps' sums: a fixed order for a given shape. A few MB at most; bound by latency:
+// 8 to 32 warps by the number of parts.
 template <int T>
-__global__ void __launch_bounds__(256) reduce_partials_kernel(const __grid_constant__ ReduceArgs a) {
-    __shared__ float red[8][33];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+__global__ void __launch_bounds__(1024) reduce_partials_kernel(const __grid_constant__ ReduceArgs a) {
+    __shared__ float red[32][33];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     const int64_t col = static_cast<int64_t>(blockIdx.x) * 32 + lane;
     const PartialSum &sum = a.sum[blockIdx.z];
     wait_prior_grid();
@@ -23,13 +24,12 @@ __global__ void __launch_bounds__(256) reduce_partials_kernel(const __grid_const
         float s = 0.f;
         if (col < a.d)
 #pragma unroll 8
-            for (int64_t p = warp; p < sum.parts; p += 8) s += sum.part[(g * sum.parts + p) * a.d + col];
+            for (int64_t p = warp; p < sum.parts; p += warps) s += sum.part[(g * sum.parts + p) * a.d + col];
         red[warp][lane] = s;
         __syncthreads();
-        if (warp == 0 && col < a.d) {
-#pragma unroll
-            for (int w = 1; w < 8; ++w) s += red[w][lane];
-            store1<T>(row_of<T>(sum.out, g, a.d), col, s);
+        for (int c = warp; c < 32; c += warps) {  // a warp adds the sums of a column
+            const float t = warp_sum(lane < warps ? red[lane][c] : 0.f);
+            if (lane == 0 && blockIdx.x * 32ll + c < a.d) store1<T>(row_of<T>(sum.out, g, a.d), blockIdx.x * 32ll + c, t);
         }
         __syncthreads();
     }
@@ -43,9 +43,11 @@ int reduce_partials(const PartialSum &s0, const PartialSum &s1, int64_t d, int t
     const bool both = s0.out != nullptr && s1.out != nullptr;
     const int64_t groups = both ? std::max(s0.groups, s1.groups) : a.sum[0].groups;
     const dim3 grid(static_cast<unsigned>((d + 31) / 32), static_cast<unsigned>(std::min<int64_t>(groups, 32768)), both ? 2 : 1);
-    if (type == WF_F32) return launch_rows(reduce_partials_kernel<WF_F32>, grid, 256, stream, a);
-    if (type == WF_BF16) return launch_rows(reduce_partials_kernel<WF_BF16>, grid, 256, stream, a);
-    return launch_rows(reduce_partials_kernel<WF_F16>, grid, 256, stream, a);
+    const int64_t parts = both ? std::max(s0.parts, s1.parts) : a.sum[0].parts;
+    const int threads = parts >= 512 ? 1024 : parts >= 200 ? 512 : 256;
+    if (type == WF_F32) return launch_rows(reduce_partials_kernel<WF_F32>, grid, threads, stream, a);
+    if (type == WF_BF16) return launch_rows(reduce_partials_kernel<WF_BF16>, grid, threads, stream, a);
+    return launch_rows(reduce_partials_kernel<WF_F16>, grid, threads, stream, a);
 }
 
 namespace {

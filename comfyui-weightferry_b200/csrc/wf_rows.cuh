@@ -81,6 +81,13 @@ __device__ __forceinline__ void store1(void *row, int64_t col, float v) {
     else static_cast<__half *>(row)[col] = __float2half_rn(v);
 }
 
+// the sum of v over the 32 lanes, in every lane
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+    return v;
+}
+
 // two 16-bit values of a word as float32
 template <int T>
 __device__ __forceinline__ float2 unpack2(uint32_t w) {
@@ -88,6 +95,24 @@ __device__ __forceinline__ float2 unpack2(uint32_t w) {
     else return __half22float2(*reinterpret_cast<const __half2 *>(&w));
 }
 
+// 16 bytes from global to shared memory past the registers (cp.async; zeros where `on` is false)
+__device__ __forceinline__ void copy16(void *dst, const void *src, bool on = true) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))),
+                 "l"(src), "r"(on ? 16 : 0)
+                 : "memory");
+}
+
+// ... and the pair of float32 values rounded to the type
+template <int T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if constexpr (T == WF_BF16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    } else {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+}
 // eight values from column col of a row (16-byte aligned)
 template <int T>
 __device__ __forceinline__ void load8(float (&v)[8], const void *row, int64_t col) {

@@ -95,7 +95,7 @@ class _LayerNorm(torch.autograd.Function):
             dy2, lddy = _rows(dy if dy.dim() == 2 else dy.reshape(m, d))
             size, work = 0, None
             if need_w or need_b:
-                size = _ext.lib().wf_layer_norm_backward_workspace(m, d, rpg)
+                size = _ext.lib().wf_layer_norm_backward_workspace(m, d, rpg, _CODES[dtype])
                 work = torch.empty(size, dtype=torch.uint8, device=device)
             if weight is not None:
                 weight = weight.contiguous()

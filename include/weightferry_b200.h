@@ -260,7 +260,7 @@ typedef struct wf_layer_norm_grad_args {
     int64_t lddy, ldx, lddx, rows, d, rows_per_group, workspace_bytes;
     int32_t type, w_type;
 } wf_layer_norm_grad_args;
-WF_API int64_t wf_layer_norm_backward_workspace(int64_t rows, int64_t d, int64_t rows_per_group);
+WF_API int64_t wf_layer_norm_backward_workspace(int64_t rows, int64_t d, int64_t rows_per_group, int type);
 WF_API int wf_layer_norm_backward(const wf_layer_norm_grad_args *args, wf_stream_t stream);
 
 #ifdef __cplusplus
