@@ -16,6 +16,9 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
+#include <cstdio>
+#include <cstdlib>
 #include <type_traits>
 
 namespace wf {
@@ -117,12 +120,16 @@ __device__ __forceinline__ uint32_t pack2_sat(float a, float b) {
     return w;
 }
 
-template <int ACT>
-__device__ __forceinline__ void act4(float (&v)[4]) {
-    act2<ACT>(v[0], v[1]);
-    act2<ACT>(v[2], v[3]);
+template <int ACT, int R>
+__device__ __forceinline__ void act4(float (&v)[R][4]) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        act2<ACT>(v[r][0], v[r][1]);
+        act2<ACT>(v[r][2], v[r][3]);
+    }
 }
-__device__ __forceinline__ void apply_act4(int kind, float (&v)[4]) {
+template <int R>
+__device__ __forceinline__ void apply_act4(int kind, float (&v)[R][4]) {
     switch (kind) {
         case WF_ACT_RELU: act4<WF_ACT_RELU>(v); break;
         case WF_ACT_SILU: act4<WF_ACT_SILU>(v); break;
@@ -132,10 +139,10 @@ __device__ __forceinline__ void apply_act4(int kind, float (&v)[4]) {
     }
 }
 
-// four neighbouring values of a row, those at and past n as 0
-template <int T>
-__device__ __forceinline__ void load4(float (&v)[4], const void *row, int col, int n, bool vec) {
-    if (vec && col + 4 <= n) {
+// four neighbouring values of a row: one 8-byte access, or (VEC false) value by value, those at and past n as 0
+template <int T, bool VEC>
+__device__ __forceinline__ void load4(float (&v)[4], const void *row, int col, int n) {
+    if constexpr (VEC) {
         const uint2 q = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(row) + col);
         const float2 a = unpack2<T>(q.x), b = unpack2<T>(q.y);
         v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
@@ -144,9 +151,9 @@ __device__ __forceinline__ void load4(float (&v)[4], const void *row, int col, i
         for (int i = 0; i < 4; ++i) v[i] = col + i < n ? load1<T>(row, col + i) : 0.f;
     }
 }
-template <int T>
-__device__ __forceinline__ void store4(void *row, int col, int n, bool vec, const float (&v)[4]) {
-    if (vec && col + 4 <= n) {
+template <int T, bool VEC>
+__device__ __forceinline__ void store4(void *row, int col, int n, const float (&v)[4]) {
+    if constexpr (VEC) {
         *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(row) + col) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
     } else {
 #pragma unroll
@@ -155,44 +162,67 @@ __device__ __forceinline__ void store4(void *row, int col, int n, bool vec, cons
     }
 }
 
-// the epilogue of four neighbouring outputs of one row
-template <int T>
-__device__ __forceinline__ void finish4(const Epilogue &e, float (&v)[4], int row, int col, int n) {
+// The epilogue of four neighbouring outputs in each of R rows (row, row + step, ...; those from row_end on are left out).
+// Several rows share each of its branches, and their chains of loads and arithmetic overlap.
+template <int T, bool VEC, int R>
+__device__ __forceinline__ void finish4(const Epilogue &e, float (&v)[R][4], int row, int step, int row_end, int col, int n) {
+    float o[R][4];
     if (e.bias != nullptr) {
-        float b[4];
-        load4<T>(b, e.bias, col, n, e.vec);
+        load4<T, VEC>(o[0], e.bias, col, n);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] += b[i];
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[r][i] += o[0][i];
     }
     if (e.keep != KEEP_NONE) {
-        if (e.keep == KEEP_F16) {
-            const uint32_t w[2] = {pack2_sat(v[0], v[1]), pack2_sat(v[2], v[3])};
-            uint16_t *dst = static_cast<uint16_t *>(e.kept) + row * e.ld_kept + col;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (col + i < n) dst[i] = static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1)));
-        } else if (e.keep == KEEP_F32) {
+        for (int r = 0; r < R; ++r) {
+            const int at = row + r * step;
+            if (at >= row_end) continue;
+            if (e.keep == KEEP_F16) {
+                const uint32_t w[2] = {pack2_sat(v[r][0], v[r][1]), pack2_sat(v[r][2], v[r][3])};
+                uint16_t *dst = static_cast<uint16_t *>(e.kept) + at * e.ld_kept + col;
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (col + i < n) static_cast<float *>(e.kept)[row * e.ld_kept + col + i] = v[i];
-        } else {
-            store4<T>(row_of<T>(e.kept, row, e.ld_kept), col, n, e.vec, v);
+                for (int i = 0; i < 4; ++i)
+                    if (col + i < n) dst[i] = static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1)));
+            } else if (e.keep == KEEP_F32) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (col + i < n) static_cast<float *>(e.kept)[at * e.ld_kept + col + i] = v[r][i];
+            } else {
+                store4<T, false>(row_of<T>(e.kept, at, e.ld_kept), col, n, v[r]);
+            }
         }
     }
-    apply_act4(e.act, v);
+    if (e.act != WF_ACT_NONE) apply_act4(e.act, v);
     if (e.gate != nullptr) {
-        float g[4];
-        load4<T>(g, row_of<T>(e.gate, row / e.rows_per_group, n), col, n, e.vec);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] *= g[i];
+        for (int r = 0; r < R; ++r)
+            if (row + r * step < row_end) load4<T, VEC>(o[r], row_of<T>(e.gate, (row + r * step) / e.rows_per_group, n), col, n);
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[r][i] *= o[r][i];
     }
     if (e.resid != nullptr) {
-        float r[4];
-        load4<T>(r, row_of<T>(e.resid, row, e.ld_resid), col, n, e.vec);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] += r[i];
+        for (int r = 0; r < R; ++r)
+            if (row + r * step < row_end) load4<T, VEC>(o[r], row_of<T>(e.resid, row + r * step, e.ld_resid), col, n);
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[r][i] += o[r][i];
     }
-    store4<T>(row_of<T>(e.out, row, e.ld_out), col, n, e.vec, v);
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+        if (row + r * step < row_end) store4<T, VEC>(row_of<T>(e.out, row + r * step, e.ld_out), col, n, v[r]);
+}
+
+// Value by value, out of line: the loop around the epilogue has to stay small (see linear_tile_kernel).
+template <int T>
+__device__ __noinline__ void finish4_any(const Epilogue &e, float4 sum, int row, int col, int n) {
+    float v[1][4] = {{sum.x, sum.y, sum.z, sum.w}};
+    finish4<T, false, 1>(e, v, row, 1, row + 1, col, n);
 }
 
 // ------------------------------------------------------------------------------------------------ few-rows kernel
@@ -201,31 +231,33 @@ __device__ __forceinline__ void finish4(const Epilogue &e, float (&v)[4], int ro
 // no more than NT - m rows. The CTAs of a cluster share the contraction, and their float32 parts are added through
 // distributed shared memory in rank order (the same bits every time): with few tiles every SM still reads weights. Warp
 // 4 loads tiles by TMA into a ring, warp 5 issues the MMAs, warps 0-3 move the accumulator to shared memory, and all
-// threads finish the CTA's share of the rows.
+// eight warps finish the CTA's share of the rows.
 constexpr int TILE_J = 128;
-constexpr int TILE_THREADS = 192;
+constexpr int TILE_THREADS = 256;
 template <int NT>
 struct TileShape {
     static constexpr int p_bytes = TILE_J * BC * 2, q_bytes = NT * BC * 2, stage = p_bytes + q_bytes;
-    static constexpr int stages = NT <= 32 ? 5 : NT <= 64 ? 4 : 3;  // about 100 KB: two CTAs an SM
-    static constexpr int smem = stages * stage + 1024 + 128;
+    static constexpr int shallow = NT <= 32 ? 5 : NT <= 64 ? 4 : 3;  // stages: about 100 KB, two CTAs an SM ...
+    static constexpr int deep = 2 * shallow;                         // ... or all of it
+    static constexpr int smem(int stages) { return stages * stage + 1024 + 16 * deep + 16; }
     static constexpr int tmem_cols = NT < 32 ? 32 : NT;
-    static_assert(NT * TILE_J * 4 <= stages * stage, "the float32 tile reuses the ring");
+    static_assert(NT * TILE_J * 4 <= shallow * stage, "the float32 tile reuses the ring");
 };
 
 template <bool P_ROWS, bool Q_ROWS, int NT, int T>
 __global__ void __launch_bounds__(TILE_THREADS)
 linear_tile_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
-                   const __grid_constant__ Epilogue epi, int m, int n, int c, int tiles_q, int split) {
+                   const __grid_constant__ Epilogue epi, int m, int n, int c, int tiles_q, int split,
+                   int stages) {
     using S = TileShape<NT>;
     constexpr uint32_t idesc = f16_idesc(T == WF_BF16, P_ROWS, Q_ROWS, TILE_J, NT);
     extern __shared__ uint8_t smem_raw[];
     uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t *bars = reinterpret_cast<uint64_t *>(ring + S::stages * S::stage);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(ring + stages * S::stage);
     __shared__ uint32_t s_tmem_base;
     __shared__ int s_abort;
-    const uint32_t ring0 = smem_u32(ring), full0 = smem_u32(bars), empty0 = full0 + 8 * S::stages,
-                   done = empty0 + 8 * S::stages;
+    const uint32_t ring0 = smem_u32(ring), full0 = smem_u32(bars), empty0 = full0 + 8 * stages,
+                   done = empty0 + 8 * stages;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = split > 1 ? static_cast<int>(cluster_rank()) : 0;
     const int tile = blockIdx.x / split;
@@ -236,7 +268,7 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_const
 
     if (threadIdx.x == 0) {
         s_abort = 0;
-        for (int s = 0; s < S::stages; ++s) {
+        for (int s = 0; s < stages; ++s) {
             mbar_init(full0 + 8 * s, 1);
             mbar_init(empty0 + 8 * s, 1);
         }
@@ -275,12 +307,12 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_const
                 } else {
                     tma_load_2d(q, &map_q, s * BC, i0, bar);
                 }
-                if (++stage == S::stages) stage = 0, phase ^= 1u;
+                if (++stage == stages) stage = 0, phase ^= 1u;
             }
             // every load has landed before the CTA leaves or reuses the ring: only the last use of a stage can be
             // outstanding, and only after an abort
-            for (int s = 0; s < S::stages && s < issued; ++s)
-                mbar_drain_wait(full0 + 8 * s, static_cast<uint32_t>((issued - 1 - s) / S::stages) & 1u);
+            for (int s = 0; s < stages && s < issued; ++s)
+                mbar_drain_wait(full0 + 8 * s, static_cast<uint32_t>((issued - 1 - s) / stages) & 1u);
         }
         __syncwarp();
     } else if (warp == 5) {
@@ -295,24 +327,30 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_const
                 for (int k = 0; k < BC / 16; ++k)
                     mma_f16(tmem, operand_desc<P_ROWS>(p, k), operand_desc<Q_ROWS>(q, k), idesc, s > c_lo || k > 0);
                 mma_commit(empty0 + 8 * stage);
-                if (++stage == S::stages) stage = 0, phase ^= 1u;
+                if (++stage == stages) stage = 0, phase ^= 1u;
             }
             mma_commit(done);  // the accumulator is complete
             mbar_drain_wait(done, 0);
         }
         __syncwarp();
-    } else {
-        // lane w * 32 + l of tensor memory is column j0 + 32 w + l; its NT rows go to part[row][column]
+    } else if (warp < 4) {
+        // lane w * 32 + l of tensor memory is column j0 + 32 w + l
         const bool ok = __all_sync(0xFFFFFFFFu, pipe_wait(done, 0, abort_flag, 3) && !*abort_flag);
         fence_after();
-        if (ok) {
-            float *part = reinterpret_cast<float *>(ring);
+        if (ok) {  // the NT rows to part[row][column]
+            float *part = reinterpret_cast<float *>(ring) + warp * 32 + lane;
+            constexpr int STEP = NT < 32 ? 16 : 32;
 #pragma unroll
-            for (int t = 0; t < NT; t += 16) {
-                uint32_t r[16];
-                tmem_ld16(tmem + (static_cast<uint32_t>(warp * 32) << 16) + t, r);
+            for (int t = 0; t < NT; t += STEP) {
+                uint32_t r[STEP];
+                if constexpr (STEP == 16) {
+                    tmem_ld16(tmem + (static_cast<uint32_t>(warp * 32) << 16), r);
+                } else {
+                    tmem_ld32(tmem + (static_cast<uint32_t>(warp * 32) << 16) + t, r);
+                    tmem_wait32(r);
+                }
 #pragma unroll
-                for (int u = 0; u < 16; ++u) part[(t + u) * TILE_J + warp * 32 + lane] = __uint_as_float(r[u]);
+                for (int u = 0; u < STEP; ++u) part[(t + u) * TILE_J] = __uint_as_float(r[u]);
             }
         }
     }
@@ -322,47 +360,83 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_const
     fence_after();
     if (warp == 5)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::tmem_cols) : "memory");
-    // this CTA finishes rows t_lo .. t_hi of the tile, a row a warp, four columns a lane
+    // This CTA finishes rows t_lo .. t_hi of the tile, a row a warp, four columns a lane: it adds their parts, in rank
+    // order, to its own copy, then runs the epilogue over them. The sums are unrolled (distributed shared memory is far
+    // away); the epilogue is one copy of its code, four rows through each of its branches: with one row at a time, or
+    // unrolled into the sums, 128 rows took 6.5 to 7.6 us.
     const int t_lo = NT * rank / split, t_hi = min(NT * (rank + 1) / split, m - i0), col = j0 + lane * 4;
-    auto finish = [&](auto parts) {  // all of a row's parts are read before the first is added
-        constexpr int S = decltype(parts)::value;
+    constexpr int WARPS = TILE_THREADS / 32;
+    auto add_parts = [&](auto parts) {
+        constexpr int S = decltype(parts)::value, R = S == 8 ? 2 : 4;
         uint32_t base[S];
 #pragma unroll
-        for (int r = 0; r < S; ++r) base[r] = S > 1 ? map_to_rank(ring0, r) : ring0;
-#pragma unroll 2
-        for (int t = t_lo + warp; t < t_hi; t += TILE_THREADS / 32) {
-            float4 p[S];
+        for (int r = 0; r < S; ++r) base[r] = map_to_rank(ring0, r);
+        for (int t = t_lo + warp; t < t_hi; t += R * WARPS) {
+            float4 p[R][S];
 #pragma unroll
-            for (int r = 0; r < S; ++r) p[r] = ld_cluster4(base[r] + static_cast<uint32_t>(t * TILE_J + lane * 4) * 4u);
-            float v[4] = {p[0].x, p[0].y, p[0].z, p[0].w};
+            for (int i = 0; i < R; ++i)
 #pragma unroll
-            for (int r = 1; r < S; ++r) v[0] += p[r].x, v[1] += p[r].y, v[2] += p[r].z, v[3] += p[r].w;
-            if (col < n) finish4<T>(epi, v, i0 + t, col, n);
+                for (int r = 0; r < S; ++r) {
+                    p[i][r] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (t + i * WARPS < t_hi)
+                        p[i][r] = ld_cluster4(base[r] + static_cast<uint32_t>((t + i * WARPS) * TILE_J + lane * 4) * 4u);
+                }
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                if (t + i * WARPS >= t_hi) continue;
+#pragma unroll
+                for (int r = 1; r < S; ++r)
+                    p[i][0].x += p[i][r].x, p[i][0].y += p[i][r].y, p[i][0].z += p[i][r].z, p[i][0].w += p[i][r].w;
+                reinterpret_cast<float4 *>(ring)[(t + i * WARPS) * (TILE_J / 4) + lane] = p[i][0];
+            }
         }
     };
-    if (split == 1) finish(std::integral_constant<int, 1>{});
-    else if (split == 2) finish(std::integral_constant<int, 2>{});
-    else if (split == 4) finish(std::integral_constant<int, 4>{});
-    else finish(std::integral_constant<int, 8>{});
-    if (split > 1) cluster_sync();  // no CTA leaves while another reads its part
+    if (split == 2) add_parts(std::integral_constant<int, 2>{});
+    else if (split == 4) add_parts(std::integral_constant<int, 4>{});
+    else if (split == 8) add_parts(std::integral_constant<int, 8>{});
+    // No CTA leaves while another reads its part. Every read above has been waited for here, because its value has been
+    // stored: a read that nobody waits for (of a row past t_hi, say) could still be under way when the CTA that it reads
+    // has left, an illegal access.
+    if (split > 1) cluster_sync();
+    const float4 *sums = reinterpret_cast<const float4 *>(ring);
+    if (epi.vec && col + 4 <= n) {
+        constexpr int R = 4;
+#pragma unroll 1
+        for (int t = t_lo + warp; t < t_hi; t += R * WARPS) {
+            float v[R][4];
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const float4 q = sums[min(t + r * WARPS, NT - 1) * (TILE_J / 4) + lane];
+                v[r][0] = q.x, v[r][1] = q.y, v[r][2] = q.z, v[r][3] = q.w;
+            }
+            finish4<T, true, R>(epi, v, i0 + t, WARPS, i0 + t_hi, col, n);
+        }
+    } else if (col < n) {
+#pragma unroll 1
+        for (int t = t_lo + warp; t < t_hi; t += WARPS) finish4_any<T>(epi, sums[t * (TILE_J / 4) + lane], i0 + t, col, n);
+    }
 }
 
 // ------------------------------------------------------------------------------------------------- many-rows kernel
 // One 256 x 256 tile of D for each pair of CTAs (a cluster of 2 on neighbouring SMs), persistent. tcgen05.mma
 // cta_group::2 (M = 256, N = 256, K = 16), issued by one thread of the even CTA, reads rows 0..127 of the A tile and
 // columns 0..127 of the B tile from the even CTA's shared memory and the other halves from the odd CTA's; each CTA's
-// tensor memory holds its 128 rows x 256 columns, twice, so that the next tile's MMAs run while this one is written
-// out. Warp 8 loads (six 32 KB stages), warp 9 of the even CTA issues, warps 0..7 are the epilogue: a warp takes 32
-// rows and 128 columns of the accumulator in chunks of 32 x 32, which leave through a swizzled 2 KB buffer and one TMA
-// store each (plain stores where the output's pitch or base is not a multiple of 16 bytes).
-constexpr int PAIR_STAGES = 6;
+// tensor memory holds its 128 rows x 256 columns, twice, so that the next tile's MMAs run while this one is written out.
+// Warp 8 loads (six 32 KB stages), warp 9 of the even CTA issues, warps 0..7 are the epilogue: a warp takes 32 rows and
+// 128 columns of the accumulator in chunks of 32 x 32, which leave through a swizzled 2 KB buffer and one TMA store each
+// (plain stores where the output's pitch or base is not a multiple of 16 bytes).
+// What bounds it: a stage is 512 cycles of MMAs and 32 KB an SM, 64 bytes a cycle -- what an SM takes in from L2 (56 to
+// 60 measured) -- and in long runs the board's power. A 256 x 128 tile (24 KB for 256 cycles) was no faster anywhere:
+// 2048^3 30.5 against 20.6 us, 8192 x 256 x 2048 24.4 against 20.8.
+constexpr int BN = 256;
 constexpr int PAIR_THREADS = 320;
 constexpr int PAIR_EPI_THREADS = 256;
+constexpr int PAIR_STAGES = 6;
 constexpr int PAIR_HALF = 128 * BC * 2;            // 16 KB: this CTA's 128 rows of A or columns of B
 constexpr int PAIR_STAGE = 2 * PAIR_HALF;
 constexpr int PAIR_OUT = 8 * 2 * 2048;             // two chunks an epilogue warp
-constexpr int kBand = 8;                           // tile rows of a band of the tile order
 constexpr int PAIR_SMEM = PAIR_STAGES * PAIR_STAGE + PAIR_OUT + 1024 + 256;
+constexpr int kBand = 8;                           // tile rows of a band of the tile order
 
 __device__ __forceinline__ void mma_f16_pair(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
@@ -373,23 +447,29 @@ __device__ __forceinline__ void mma_f16_pair(uint32_t d_tmem, uint64_t a, uint64
         : "memory");
 }
 
+// Value by value and out of line, for rows that 16-byte accesses do not fit.
+__device__ __noinline__ void load32_any(uint32_t (&w)[16], const uint16_t *row, int col, int n) {
+    for (int i = 0; i < 16; ++i) {
+        const int c = col + 2 * i;
+        const uint32_t lo = c < n ? row[c] : 0u, hi = c + 1 < n ? row[c + 1] : 0u;
+        w[i] = lo | (hi << 16);
+    }
+}
+
 // 32 neighbouring 16-bit values of a row in 16 registers, those at and past n as 0; vec: 16-byte aligned, n % 8 == 0
 __device__ __forceinline__ void load32(uint32_t (&w)[16], const void *row, int col, int n, bool vec) {
+    if (vec) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        const int c = col + 8 * q;
-        if (vec) {
+        for (int q = 0; q < 4; ++q) {
             uint4 v = make_uint4(0u, 0u, 0u, 0u);
-            if (c < n) v = __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(row) + c));
+            if (col + 8 * q < n) v = __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(row) + col + 8 * q));
             w[4 * q] = v.x, w[4 * q + 1] = v.y, w[4 * q + 2] = v.z, w[4 * q + 3] = v.w;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint16_t *p = static_cast<const uint16_t *>(row) + c + 2 * i;
-                const uint32_t lo = c + 2 * i < n ? p[0] : 0u, hi = c + 2 * i + 1 < n ? p[1] : 0u;
-                w[4 * q + i] = lo | (hi << 16);
-            }
         }
+    } else {
+        uint32_t any[16];
+        load32_any(any, static_cast<const uint16_t *>(row), col, n);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) w[i] = any[i];
     }
 }
 
@@ -433,7 +513,7 @@ __device__ __forceinline__ void emit32(const uint32_t (&p)[16], uint32_t buf, in
     }
 }
 
-// what one epilogue warp knows of its 32 rows x 128 columns
+// what one epilogue warp knows of its 32 rows
 struct Warp32 {
     uint32_t buf;             // its two chunk buffers
     uint32_t chunks;          // chunks written so far: which buffer is next
@@ -509,12 +589,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
 linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                    const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_kept,
                    const __grid_constant__ Epilogue epi, int m, int n, int c, int band, bool tma_out, bool tma_kept) {
-    constexpr uint32_t idesc = f16_idesc(T == WF_BF16, A_ROWS, B_ROWS, 256, 256);
+    constexpr uint32_t idesc = f16_idesc(T == WF_BF16, A_ROWS, B_ROWS, 256, BN);
     extern __shared__ uint8_t smem_raw[];
     uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t *out_chunks = ring + PAIR_STAGES * PAIR_STAGE;
     uint64_t *bars = reinterpret_cast<uint64_t *>(out_chunks + PAIR_OUT);
-    // full[0..5] (used in the even CTA), empty[0..5], tmem_full[0..1], tmem_empty[0..1] (even CTA), drain
+    // full (used in the even CTA) and empty of each stage, tmem_full[0..1], tmem_empty[0..1] (even CTA), drain
     __shared__ uint32_t s_tmem_base;
     __shared__ int s_abort;
     __shared__ int s_issued[2];  // stage loads issued by this CTA's producer; [1] in the even CTA: the odd CTA's
@@ -522,7 +602,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
                    tfull0 = empty0 + 8 * PAIR_STAGES, tempty0 = tfull0 + 16, drain = tempty0 + 16;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank(), peer = rank ^ 1u;
-    const int tiles_m = (m + 255) / 256, tiles_n = (n + 255) / 256, n_tiles = tiles_m * tiles_n;
+    const int tiles_m = (m + 255) / 256, tiles_n = (n + BN - 1) / BN, n_tiles = tiles_m * tiles_n;
     const int steps = (c + BC - 1) / BC;
     const int cluster_id = blockIdx.x >> 1, n_clusters = gridDim.x >> 1;
 
@@ -543,7 +623,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     }
     if (warp == 9) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
-                     ::"r"(smem_u32(&s_tmem_base)), "r"(512) : "memory");
+                     ::"r"(smem_u32(&s_tmem_base)), "r"(2 * BN) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
     fence_before();
@@ -563,7 +643,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
             for (int tile = cluster_id; tile < n_tiles && ok; tile += n_clusters) {
                 int mi, ni;
                 tile_coords(tile, tiles_m, tiles_n, band, mi, ni);
-                const int i0 = mi * 256 + static_cast<int>(rank) * 128, j0 = ni * 256 + static_cast<int>(rank) * 128;
+                const int i0 = mi * 256 + static_cast<int>(rank) * 128, j0 = ni * BN + static_cast<int>(rank) * (BN / 2);
                 for (int s = 0; s < steps; ++s) {
                     if (!pipe_wait(empty0 + 8 * stage, phase ^ 1u, abort_flag, 1)) { ok = false; break; }
                     const uint32_t bar = (full0 + 8 * stage) & kPeerBitMask;  // the even CTA's
@@ -576,8 +656,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
                         tma_load_2d_pair(a, &map_a, s * BC, i0, bar);
                     }
                     if constexpr (B_ROWS) {
-                        tma_load_2d_pair(b, &map_b, j0, s * BC, bar);
-                        tma_load_2d_pair(b + BC * 128, &map_b, j0 + 64, s * BC, bar);
+                        for (int h = 0; h < BN / 128; ++h) tma_load_2d_pair(b + h * BC * 128, &map_b, j0 + 64 * h, s * BC, bar);
                     } else {
                         tma_load_2d_pair(b, &map_b, s * BC, j0, bar);
                     }
@@ -603,7 +682,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
             for (int tile = cluster_id; tile < n_tiles && ok; tile += n_clusters) {
                 if (!pipe_wait(tempty0 + 8 * acc, acc_phase ^ 1u, abort_flag, 2)) break;
                 fence_after();
-                const uint32_t d = tmem + static_cast<uint32_t>(acc * 256);
+                const uint32_t d = tmem + static_cast<uint32_t>(acc * BN);
                 for (int s = 0; s < steps; ++s) {
                     if (!pipe_wait(full0 + 8 * stage, phase, abort_flag, 2)) { ok = false; break; }
                     fence_after();
@@ -638,23 +717,23 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
             int mi, ni;
             tile_coords(tile, tiles_m, tiles_n, band, mi, ni);
             w.row0 = mi * 256 + static_cast<int>(rank) * 128 + quarter * 32;
-            const int col0 = ni * 256 + half * 128, row = w.row0 + lane;
+            const int col0 = ni * BN + half * (BN / 2), row = w.row0 + lane;
             const bool in = row < m;
             w.gate = FULL && epi.gate != nullptr && in ? row_of<T>(epi.gate, row / epi.rows_per_group, n) : nullptr;
             w.resid = FULL && epi.resid != nullptr && in ? row_of<T>(epi.resid, row, epi.ld_resid) : nullptr;
             if (FULL && w.resid != nullptr && epi.vec && col0 < n)  // the row's span to L2 while the MMAs run
                 asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;"
-                             ::"l"(static_cast<const uint16_t *>(w.resid) + col0), "r"(static_cast<uint32_t>(min(128, n - col0)) * 2u)
+                             ::"l"(static_cast<const uint16_t *>(w.resid) + col0), "r"(static_cast<uint32_t>(min(BN / 2, n - col0)) * 2u)
                              : "memory");
             if (!__all_sync(0xFFFFFFFFu, pipe_wait(tfull0 + 8 * acc, acc_phase, abort_flag, 3))) break;
             fence_after();
-            const uint32_t taddr = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * 256 + half * 128);
+            const uint32_t taddr = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * BN + half * (BN / 2));
             uint32_t r[32], res[16];
             tmem_ld32(taddr, r);
             // one copy of the chunk's code (unrolled four times, with every activation inside, it outgrew the
             // instruction cache: 266 against 137 us for a gelu layer of 8192 x 512 x 8192)
 #pragma unroll 1
-            for (int q = 0; q < 4; ++q) {
+            for (int q = 0; q < BN / 64; ++q) {
                 if (FULL && epi.resid != nullptr) {
                     if (w.resid != nullptr) {
                         load32(res, w.resid, col0 + 32 * q, n, epi.vec);
@@ -667,7 +746,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
                 float v[32];
 #pragma unroll
                 for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-                if (q < 3) {
+                if (q < BN / 64 - 1) {
                     tmem_ld32(taddr + 32 * (q + 1), r);  // in flight while this chunk is finished
                 } else {  // the accumulator is in registers: it may be overwritten
                     fence_before();
@@ -700,7 +779,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     cluster_sync();  // no CTA leaves (or frees tensor memory) while loads into it or the pair's MMAs may still run
     fence_after();
     if (warp == 9)
-        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * BN) : "memory");
 }
 
 // ------------------------------------------------------------------------------------------------------------- host
@@ -726,12 +805,12 @@ struct Product {
 };
 
 template <bool A_ROWS, bool B_ROWS, int NT, int T>
-int launch_tile(const Product &p, const Epilogue &e, int split, int dev, cudaStream_t stream) {
+int launch_tile(const Product &p, const Epilogue &e, int split, bool deep, int dev, cudaStream_t stream) {
     using S = TileShape<NT>;
     constexpr auto kern = linear_tile_kernel<B_ROWS, A_ROWS, NT, T>;
     static std::atomic<bool> ready[64];  // any host thread may launch first
     if (!ready[dev].load(std::memory_order_acquire)) {
-        const cudaError_t e0 = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::smem);
+        const cudaError_t e0 = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::smem(S::deep));
         if (e0 != cudaSuccess) return static_cast<int>(e0);
         ready[dev].store(true, std::memory_order_release);
     }
@@ -741,9 +820,10 @@ int launch_tile(const Product &p, const Epilogue &e, int split, int dev, cudaStr
     if (rc != WF_OK) return rc;
     const int64_t tiles_q = (p.m + NT - 1) / NT, tiles = (p.n + TILE_J - 1) / TILE_J * tiles_q;
     if (tiles * split > (1ll << 31) - 1) return WF_ERR_ARG;
+    const int stages = deep ? S::deep : S::shallow;
     const cudaError_t err = launch_dependent_clusters(
-        kern, dim3(static_cast<unsigned>(tiles * split)), split > 1 ? split : 0, TILE_THREADS, S::smem, stream, mp, mq, e,
-        static_cast<int>(p.m), static_cast<int>(p.n), static_cast<int>(p.c), static_cast<int>(tiles_q), split);
+        kern, dim3(static_cast<unsigned>(tiles * split)), split > 1 ? split : 0, TILE_THREADS, S::smem(stages), stream, mp, mq, e,
+        static_cast<int>(p.m), static_cast<int>(p.n), static_cast<int>(p.c), static_cast<int>(tiles_q), split, stages);
     return static_cast<int>(err != cudaSuccess ? err : cudaGetLastError());
 }
 
@@ -766,14 +846,15 @@ template <bool A_ROWS, bool B_ROWS, int T>
 int launch_pair(const Product &p, const Epilogue &e0, int dev, cudaStream_t stream) {
     constexpr bool full = !A_ROWS && !B_ROWS;
     constexpr auto kern = linear_pair_kernel<A_ROWS, B_ROWS, T, full>;
+    constexpr int smem = PAIR_SMEM;
     static std::atomic<int> clusters[64];  // resident pairs; any host thread may launch first
     if (clusters[dev].load(std::memory_order_acquire) == 0) {
-        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, PAIR_SMEM);
+        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e != cudaSuccess) return static_cast<int>(e);
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(2 * device_sm_count());
         cfg.blockDim = dim3(PAIR_THREADS);
-        cfg.dynamicSmemBytes = PAIR_SMEM;
+        cfg.dynamicSmemBytes = smem;
         cudaLaunchAttribute attr;
         attr.id = cudaLaunchAttributeClusterDimension;
         attr.val.clusterDim.x = 2;
@@ -792,23 +873,67 @@ int launch_pair(const Product &p, const Epilogue &e0, int dev, cudaStream_t stre
     const bool tma_kept = (e.keep == KEEP_F16 || e.keep == KEEP_SAME) && vec8_ok(e.kept, e.ld_kept);
     CUtensorMap ma, mb, mo = {}, mk = {};
     int rc = A_ROWS ? operand_map(&ma, p.a, p.c, p.m, p.lda, BC) : operand_map(&ma, p.a, p.m, p.c, p.lda, 128);
-    if (rc == WF_OK) rc = B_ROWS ? operand_map(&mb, p.b, p.c, p.n, p.ldb, BC) : operand_map(&mb, p.b, p.n, p.c, p.ldb, 128);
+    if (rc == WF_OK) rc = B_ROWS ? operand_map(&mb, p.b, p.c, p.n, p.ldb, BC) : operand_map(&mb, p.b, p.n, p.c, p.ldb, BN / 2);
     if (rc == WF_OK && tma_out) rc = output_map(&mo, e.out, p.m, p.n, e.ld_out);
     if (rc == WF_OK && tma_kept) rc = output_map(&mk, e.kept, p.m, p.n, e.ld_kept);
     if (rc != WF_OK) return rc;
-    const int64_t tiles = ((p.m + 255) / 256) * ((p.n + 255) / 256);
+    const int64_t tiles = ((p.m + 255) / 256) * ((p.n + BN - 1) / BN);
     if (tiles > (1ll << 30)) return WF_ERR_ARG;
     const int grid = 2 * static_cast<int>(std::min<int64_t>(tiles, clusters[dev].load(std::memory_order_acquire)));
-    const cudaError_t err = launch_dependent(kern, dim3(grid), PAIR_THREADS, PAIR_SMEM, stream, ma, mb, mo, mk, e,
+    const cudaError_t err = launch_dependent(kern, dim3(grid), PAIR_THREADS, smem, stream, ma, mb, mo, mk, e,
                                              static_cast<int>(p.m), static_cast<int>(p.n), static_cast<int>(p.c),
                                              kBand, tma_out, tma_kept);
     return static_cast<int>(err != cudaSuccess ? err : cudaGetLastError());
 }
 
-bool use_pair(const Product &p) {
-    static const int forced = env_digit("WEIGHTFERRY_LINEAR_PAIR", 2);
-    if (forced < 2) return forced == 1;
-    return ((p.m + 255) / 256) * ((p.n + 255) / 256) >= device_sm_count() / 4;
+// Which kernel and shape take a product: the one of the least estimated time, from what one B200 measured (graphs of
+// calls over operands that do not stay in L2).
+//   tile kernel (NT rows, S CTAs to a tile): a CTA lasts 4 us and its contraction steps; a step takes its bytes at 58 a
+//     cycle (NT = 128: 0.30 us, 64: 0.22, 16: 0.17) or the ring's share of a 1.2 us round trip; one or two CTAs share an
+//     SM. The epilogue takes 13 ns a row; sharing a tile costs 1.2 us of cluster barriers and the parts' way through
+//     distributed shared memory at 3.3 TB/s. Nothing is faster than the operands' bytes at 6 TB/s.
+//   pair kernel: 8.5 us, and for each round of 74 tiles 0.38 us a step, or 3.3 us where the epilogue is longer.
+// Measured either side of the choice (us): 333 x 1024 x 5120 tile 10.7, pair 14.5; 512 x 5120 x 5120 tile 38.4, pair
+// 36.3; 2048 x 2048 x 2048 tile 26.5, pair 20.6; 128 x 2048 x 2048 NT = 64 and S = 4 9.0, NT = 128 and S = 1 14.7.
+struct Plan {
+    int nt, split;  // nt 0: the pair kernel
+    bool deep;
+    double us;
+};
+
+Plan tile_plan(const Product &p, int nt, int split, int sms) {
+    const double stage_kb = 16 + nt / 8.0, steps = static_cast<double>((p.c + BC * split - 1) / (BC * split));
+    const double ctas = static_cast<double>((p.n + TILE_J - 1) / TILE_J * ((p.m + nt - 1) / nt)) * split;
+    const bool deep = split == 1 && ctas <= sms;
+    const int stages = (nt <= 32 ? 5 : nt <= 64 ? 4 : 3) * (deep ? 2 : 1);
+    const double load = std::min(2.0, std::max(1.0, ctas / sms));  // CTAs that share an SM
+    const double step = std::max(stage_kb * 0.0093 * load, 1.2 / stages);
+    const double rows = std::min<double>(nt, static_cast<double>(p.m)) / split;
+    double cta = 4.0 + steps * step + 0.013 * rows;
+    if (split > 1) cta += 1.2 + nt * 512.0 * (split - 1) / split * std::min(ctas, 2.0 * sms) / 3.3e6;
+    const double bytes = 2.0 * (static_cast<double>(p.m) * p.c + static_cast<double>(p.n) * p.c + static_cast<double>(p.m) * p.n);
+    return {nt, split, deep, std::max(cta * std::max(1.0, ctas / (2.0 * sms)), bytes / 6.0e6 + 4.0)};
+}
+
+Plan make_plan(const Product &p, int least_nt) {
+    static const int forced = env_digit("WEIGHTFERRY_LINEAR_PAIR", 2);  // 0 / 1: the tile / the pair kernel only
+    const int sms = device_sm_count();
+    const double tiles = static_cast<double>((p.m + 255) / 256) * ((p.n + BN - 1) / BN), steps = static_cast<double>((p.c + BC - 1) / BC);
+    const Plan pair{0, 1, false, 8.5 + std::ceil(tiles / (sms / 2)) * std::max(0.38 * steps, 3.3)};
+    if (forced == 1) return pair;
+    static const int fnt = getenv("WF_NT") ? atoi(getenv("WF_NT")) : 0, fsp = getenv("WF_SPLIT") ? atoi(getenv("WF_SPLIT")) : 0;
+    if (fnt) return tile_plan(p, std::max(least_nt, fnt), fsp, sms);
+    Plan best = pair;
+    best.us = forced == 0 ? 1e30 : pair.us;
+    for (int nt = least_nt; nt <= 128; nt *= 2) {
+        for (int split = 1; split <= 8 && (split == 1 || split <= steps); split *= 2) {
+            const Plan t = tile_plan(p, nt, split, sms);
+            if (t.us < best.us) best = t;
+        }
+        if (p.m <= nt) break;  // wider tiles would hold nothing more
+    }
+    if (getenv("WF_PLAN")) printf("plan m%ld n%ld k%ld: nt %d split %d deep %d us %.1f pair %.1f\n", (long)p.m, (long)p.n, (long)p.c, best.nt, best.split, best.deep, best.us, pair.us);
+    return best;
 }
 
 template <bool A_ROWS, bool B_ROWS, int T>
@@ -816,17 +941,18 @@ int dispatch(const Product &p, const Epilogue &e, cudaStream_t stream) {
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64) return WF_ERR_DEVICE;
-    const int nt = A_ROWS ? (p.m <= 64 ? 64 : 128) : p.m <= 16 ? 16 : p.m <= 32 ? 32 : p.m <= 64 ? 64 : 128;
-    const int64_t tiles = (p.n + TILE_J - 1) / TILE_J * ((p.m + nt - 1) / nt), steps = (p.c + BC - 1) / BC;
-    if (use_pair(p)) return launch_pair<A_ROWS, B_ROWS, T>(p, e, dev, stream);
-    int split = 1;
-    while (split < 8 && tiles * split * 2 <= 2 * device_sm_count() && steps >= split * 4) split *= 2;
-    if constexpr (!A_ROWS) {
-        if (nt == 16) return launch_tile<A_ROWS, B_ROWS, 16, T>(p, e, split, dev, stream);
-        if (nt == 32) return launch_tile<A_ROWS, B_ROWS, 32, T>(p, e, split, dev, stream);
+    const Plan plan = make_plan(p, A_ROWS ? 64 : 16);  // a row-major operand comes in swizzle rows of 64
+    switch (plan.nt) {
+        case 0: return launch_pair<A_ROWS, B_ROWS, T>(p, e, dev, stream);
+        case 64: return launch_tile<A_ROWS, B_ROWS, 64, T>(p, e, plan.split, plan.deep, dev, stream);
+        case 128: return launch_tile<A_ROWS, B_ROWS, 128, T>(p, e, plan.split, plan.deep, dev, stream);
+        default: break;
     }
-    if (nt == 64) return launch_tile<A_ROWS, B_ROWS, 64, T>(p, e, split, dev, stream);
-    return launch_tile<A_ROWS, B_ROWS, 128, T>(p, e, split, dev, stream);
+    if constexpr (!A_ROWS) {
+        if (plan.nt == 16) return launch_tile<A_ROWS, B_ROWS, 16, T>(p, e, plan.split, plan.deep, dev, stream);
+        if (plan.nt == 32) return launch_tile<A_ROWS, B_ROWS, 32, T>(p, e, plan.split, plan.deep, dev, stream);
+    }
+    return WF_ERR_ARG;
 }
 
 // what TMA asks of an operand: a 16-byte aligned base and row pitch
