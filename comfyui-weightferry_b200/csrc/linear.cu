@@ -45,23 +45,20 @@ __device__ __forceinline__ bool pipe_wait(uint32_t a, uint32_t parity, volatile 
     }
 }
 
-// Shared-memory matrix descriptor of a row-major operand: 64 rows (128 bytes) of one contraction index side by side,
-// 128-byte swizzle; 8 contraction indexes 1024 B apart, blocks of 64 rows `block` B apart.
-__device__ __forceinline__ uint64_t smem_desc_rows(uint32_t addr, uint32_t block) {
-    uint64_t d = 0;
-    d |= static_cast<uint64_t>((addr >> 4) & 0x3FFFu);
-    d |= static_cast<uint64_t>(block >> 4) << 16;   // leading byte offset: from 64 rows to the next 64
-    d |= static_cast<uint64_t>(1024u >> 4) << 32;   // stride byte offset: from 8 contraction indexes to the next 8
-    d |= static_cast<uint64_t>(1u) << 46;
-    d |= static_cast<uint64_t>(2u) << 61;
-    return d;
-}
-
-// descriptor of the operand at addr for contraction indexes 16 step .. 16 step + 15 of a stage
+// Shared-memory matrix descriptors, 128-byte swizzle, as two words: the high one is constant, the low one holds the
+// address in 16 bytes, to which a stage or a step within it is a plain addition. One thread issues every MMA of a tile, so
+// its instructions count: with descriptors put together from scratch (some 100 instructions a stage) a stage took 0.30 us
+// however small its tile was.
+//   c-major operand: rows 128 B apart, 8 rows 1024 B apart; 16 contraction indexes are the next 32 B
+//   row-major operand: 64 rows (128 B) of one contraction index side by side, 8 contraction indexes 1024 B apart (stride
+//     byte offset), the next 64 rows BC * 128 B on (leading byte offset); 16 contraction indexes are 2048 B
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);  // stride offset, version, 128-byte swizzle
 template <bool ROWS>
-__device__ __forceinline__ uint64_t operand_desc(uint32_t addr, int step) {
-    return ROWS ? smem_desc_rows(addr + 2048u * step, BC * 128u) : smem_desc(addr + 32u * step);
+__device__ __forceinline__ uint32_t desc_low(uint32_t addr) {  // the mask drops the CTA's rank in its cluster
+    return ((addr >> 4) & 0x3FFFu) | ((ROWS ? BC * 128u >> 4 : 1u) << 16);
 }
+template <bool ROWS>
+constexpr uint32_t kDescStep = ROWS ? 2048u >> 4 : 32u >> 4;
 
 // instruction descriptor of kind::f16: D float32 (bits 4-5 = 1), A and B f16 (0) or bf16 (1) at bits 7-9 and 10-12,
 // row-major A / B at bits 15 / 16, N >> 3 at bits 17-22, M >> 4 at bits 24-28
@@ -71,13 +68,17 @@ constexpr uint32_t f16_idesc(bool bf16, bool a_rows, bool b_rows, int m, int n) 
            (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
 
-__device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(d_tmem), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-        : "memory");
+template <bool PAIR>
+__device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+#define WF_MMA_F16(GROUP)                                                             \
+    asm volatile(                                                                     \
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"                               \
+        "mov.b64 da, {%1, %3};\n\tmov.b64 db, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t" \
+        "tcgen05.mma.cta_group::" GROUP ".kind::f16 [%0], da, db, %4, p;\n\t}"          \
+        ::"r"(d_tmem), "r"(a), "r"(b), "r"(kDescHigh), "r"(idesc), "r"(accumulate) : "memory")
+    if constexpr (PAIR) WF_MMA_F16("2");
+    else WF_MMA_F16("1");
+#undef WF_MMA_F16
 }
 
 // tcgen05.ld of 16 consecutive columns of this thread's lane
@@ -317,15 +318,16 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_const
         __syncwarp();
     } else if (warp == 5) {
         if (lane == 0) {
+            const uint32_t p0 = desc_low<P_ROWS>(ring0), q0 = desc_low<Q_ROWS>(ring0 + S::p_bytes);
             int stage = 0;
             uint32_t phase = 0;
             for (int s = c_lo; s < c_hi; ++s) {
                 if (!pipe_wait(full0 + 8 * stage, phase, abort_flag, 2)) break;
                 fence_after();
-                const uint32_t p = ring0 + stage * S::stage, q = p + S::p_bytes;
+                const uint32_t p = p0 + stage * (S::stage >> 4), q = q0 + stage * (S::stage >> 4);
 #pragma unroll
                 for (int k = 0; k < BC / 16; ++k)
-                    mma_f16(tmem, operand_desc<P_ROWS>(p, k), operand_desc<Q_ROWS>(q, k), idesc, s > c_lo || k > 0);
+                    mma_f16<false>(tmem, p + k * kDescStep<P_ROWS>, q + k * kDescStep<Q_ROWS>, idesc, s > c_lo || k > 0);
                 mma_commit(empty0 + 8 * stage);
                 if (++stage == stages) stage = 0, phase ^= 1u;
             }
@@ -437,15 +439,6 @@ constexpr int PAIR_STAGE = 2 * PAIR_HALF;
 constexpr int PAIR_OUT = 8 * 2 * 2048;             // two chunks an epilogue warp
 constexpr int PAIR_SMEM = PAIR_STAGES * PAIR_STAGE + PAIR_OUT + 1024 + 256;
 constexpr int kBand = 8;                           // tile rows of a band of the tile order
-
-__device__ __forceinline__ void mma_f16_pair(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(d_tmem), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
 
 // Value by value and out of line, for rows that 16-byte accesses do not fit.
 __device__ __noinline__ void load32_any(uint32_t (&w)[16], const uint16_t *row, int col, int n) {
@@ -676,6 +669,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     } else if (warp == 9) {
         if (lane == 0 && rank == 0) {
             const uint32_t empty_peer = map_to_rank(empty0, peer), tfull_peer = map_to_rank(tfull0, peer);
+            const uint32_t a0 = desc_low<A_ROWS>(ring0), b0 = desc_low<B_ROWS>(ring0 + PAIR_HALF);
             int stage = 0, acc = 0;
             uint32_t phase = 0, acc_phase = 0;
             bool ok = true;
@@ -686,10 +680,10 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
                 for (int s = 0; s < steps; ++s) {
                     if (!pipe_wait(full0 + 8 * stage, phase, abort_flag, 2)) { ok = false; break; }
                     fence_after();
-                    const uint32_t a = ring0 + stage * PAIR_STAGE, b = a + PAIR_HALF;
+                    const uint32_t a = a0 + stage * (PAIR_STAGE >> 4), b = b0 + stage * (PAIR_STAGE >> 4);
 #pragma unroll
                     for (int k = 0; k < BC / 16; ++k)
-                        mma_f16_pair(d, operand_desc<A_ROWS>(a, k), operand_desc<B_ROWS>(b, k), idesc, s > 0 || k > 0);
+                        mma_f16<true>(d, a + k * kDescStep<A_ROWS>, b + k * kDescStep<B_ROWS>, idesc, s > 0 || k > 0);
                     mma_commit_pair(empty0 + 8 * stage);
                     mma_commit_pair(empty_peer + 8 * stage);
                     if (++stage == PAIR_STAGES) stage = 0, phase ^= 1u;
