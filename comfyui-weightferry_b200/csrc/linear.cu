@@ -81,6 +81,18 @@ __device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint32_t a, uint32_t b,
 #undef WF_MMA_F16
 }
 
+// True in one lane of a converged warp. The roles that issue loads and MMAs run their loops in all lanes and only the
+// issue itself in one: the compiler then knows loop counters, addresses and descriptors to be the same in every lane and
+// keeps them in uniform registers, where those instructions want them. With the whole loop in lane 0, each MMA waited some
+// 50 cycles for its operands to get there and each stage 340 more (547 cycles a stage, more than its MMAs take).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+    return p != 0;
+}
+// this thread's warp in its block, known to be the same in every lane
+__device__ __forceinline__ int uniform_warp() { return __shfl_sync(0xFFFFFFFFu, static_cast<int>(threadIdx.x >> 5), 0); }
+
 // tcgen05.ld of 16 consecutive columns of this thread's lane
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
     asm volatile(
@@ -259,7 +271,7 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_const
     __shared__ int s_abort;
     const uint32_t ring0 = smem_u32(ring), full0 = smem_u32(bars), empty0 = full0 + 8 * stages,
                    done = empty0 + 8 * stages;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = uniform_warp(), lane = threadIdx.x & 31;
     const int rank = split > 1 ? static_cast<int>(cluster_rank()) : 0;
     const int tile = blockIdx.x / split;
     const int j0 = tile / tiles_q * TILE_J, i0 = tile % tiles_q * NT;
@@ -290,13 +302,13 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_const
     volatile int *abort_flag = &s_abort;
 
     if (warp == 4) {
-        if (lane == 0) {
-            int stage = 0;
-            uint32_t phase = 0;
-            int issued = 0;
-            for (int s = c_lo; s < c_hi; ++s, ++issued) {
-                if (!pipe_wait(empty0 + 8 * stage, phase ^ 1u, abort_flag, 1)) break;
-                const uint32_t bar = full0 + 8 * stage, p = ring0 + stage * S::stage, q = p + S::p_bytes;
+        int stage = 0;
+        uint32_t phase = 0;
+        int issued = 0;
+        for (int s = c_lo; s < c_hi; ++s, ++issued) {
+            if (!__all_sync(0xFFFFFFFFu, pipe_wait(empty0 + 8 * stage, phase ^ 1u, abort_flag, 1))) break;
+            const uint32_t bar = full0 + 8 * stage, p = ring0 + stage * S::stage, q = p + S::p_bytes;
+            if (elect_one()) {
                 mbar_expect_tx(bar, S::stage);
                 if constexpr (P_ROWS) {
                     for (int h = 0; h < TILE_J / 64; ++h) tma_load_2d(p + h * BC * 128, &map_p, j0 + 64 * h, s * BC, bar);
@@ -308,32 +320,34 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_const
                 } else {
                     tma_load_2d(q, &map_q, s * BC, i0, bar);
                 }
-                if (++stage == stages) stage = 0, phase ^= 1u;
             }
-            // every load has landed before the CTA leaves or reuses the ring: only the last use of a stage can be
-            // outstanding, and only after an abort
-            for (int s = 0; s < stages && s < issued; ++s)
-                mbar_drain_wait(full0 + 8 * s, static_cast<uint32_t>((issued - 1 - s) / stages) & 1u);
+            __syncwarp();
+            if (++stage == stages) stage = 0, phase ^= 1u;
         }
+        // every load has landed before the CTA leaves or reuses the ring: only the last use of a stage can be
+        // outstanding, and only after an abort
+        for (int s = 0; s < stages && s < issued; ++s)
+            mbar_drain_wait(full0 + 8 * s, static_cast<uint32_t>((issued - 1 - s) / stages) & 1u);
         __syncwarp();
     } else if (warp == 5) {
-        if (lane == 0) {
-            const uint32_t p0 = desc_low<P_ROWS>(ring0), q0 = desc_low<Q_ROWS>(ring0 + S::p_bytes);
-            int stage = 0;
-            uint32_t phase = 0;
-            for (int s = c_lo; s < c_hi; ++s) {
-                if (!pipe_wait(full0 + 8 * stage, phase, abort_flag, 2)) break;
-                fence_after();
-                const uint32_t p = p0 + stage * (S::stage >> 4), q = q0 + stage * (S::stage >> 4);
+        const uint32_t p0 = desc_low<P_ROWS>(ring0), q0 = desc_low<Q_ROWS>(ring0 + S::p_bytes);
+        int stage = 0;
+        uint32_t phase = 0;
+        for (int s = c_lo; s < c_hi; ++s) {
+            if (!__all_sync(0xFFFFFFFFu, pipe_wait(full0 + 8 * stage, phase, abort_flag, 2))) break;
+            const uint32_t p = p0 + stage * (S::stage >> 4), q = q0 + stage * (S::stage >> 4);
+            if (elect_one()) {
 #pragma unroll
                 for (int k = 0; k < BC / 16; ++k)
                     mma_f16<false>(tmem, p + k * kDescStep<P_ROWS>, q + k * kDescStep<Q_ROWS>, idesc, s > c_lo || k > 0);
                 mma_commit(empty0 + 8 * stage);
-                if (++stage == stages) stage = 0, phase ^= 1u;
             }
-            mma_commit(done);  // the accumulator is complete
-            mbar_drain_wait(done, 0);
+            __syncwarp();
+            if (++stage == stages) stage = 0, phase ^= 1u;
         }
+        if (elect_one()) mma_commit(done);  // the accumulator is complete
+        __syncwarp();
+        mbar_drain_wait(done, 0);
         __syncwarp();
     } else if (warp < 4) {
         // lane w * 32 + l of tensor memory is column j0 + 32 w + l
@@ -593,7 +607,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     __shared__ int s_issued[2];  // stage loads issued by this CTA's producer; [1] in the even CTA: the odd CTA's
     const uint32_t ring0 = smem_u32(ring), full0 = smem_u32(bars), empty0 = full0 + 8 * PAIR_STAGES,
                    tfull0 = empty0 + 8 * PAIR_STAGES, tempty0 = tfull0 + 16, drain = tempty0 + 16;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = uniform_warp(), lane = threadIdx.x & 31;
     const uint32_t rank = cluster_rank(), peer = rank ^ 1u;
     const int tiles_m = (m + 255) / 256, tiles_n = (n + BN - 1) / BN, n_tiles = tiles_m * tiles_n;
     const int steps = (c + BC - 1) / BC;
@@ -627,21 +641,24 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     volatile int *abort_flag = &s_abort;
 
     if (warp == 8) {
-        if (lane == 0) {
+        if (elect_one()) {
             asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_a)) : "memory");
             asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_b)) : "memory");
-            int stage = 0, issued = 0;
-            uint32_t phase = 0;
-            bool ok = true;
-            for (int tile = cluster_id; tile < n_tiles && ok; tile += n_clusters) {
-                int mi, ni;
-                tile_coords(tile, tiles_m, tiles_n, band, mi, ni);
-                const int i0 = mi * 256 + static_cast<int>(rank) * 128, j0 = ni * BN + static_cast<int>(rank) * (BN / 2);
-                for (int s = 0; s < steps; ++s) {
-                    if (!pipe_wait(empty0 + 8 * stage, phase ^ 1u, abort_flag, 1)) { ok = false; break; }
-                    const uint32_t bar = (full0 + 8 * stage) & kPeerBitMask;  // the even CTA's
+        }
+        __syncwarp();
+        int stage = 0, issued = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int tile = cluster_id; tile < n_tiles && ok; tile += n_clusters) {
+            int mi, ni;
+            tile_coords(tile, tiles_m, tiles_n, band, mi, ni);
+            const int i0 = mi * 256 + static_cast<int>(rank) * 128, j0 = ni * BN + static_cast<int>(rank) * (BN / 2);
+            for (int s = 0; s < steps; ++s) {
+                if (!__all_sync(0xFFFFFFFFu, pipe_wait(empty0 + 8 * stage, phase ^ 1u, abort_flag, 1))) { ok = false; break; }
+                const uint32_t bar = (full0 + 8 * stage) & kPeerBitMask;  // the even CTA's
+                const uint32_t a = ring0 + stage * PAIR_STAGE, b = a + PAIR_HALF;
+                if (elect_one()) {
                     if (rank == 0) mbar_expect_tx(full0 + 8 * stage, 2 * PAIR_STAGE);
-                    const uint32_t a = ring0 + stage * PAIR_STAGE, b = a + PAIR_HALF;
                     if constexpr (A_ROWS) {
                         tma_load_2d_pair(a, &map_a, i0, s * BC, bar);
                         tma_load_2d_pair(a + BC * 128, &map_a, i0 + 64, s * BC, bar);
@@ -649,15 +666,19 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
                         tma_load_2d_pair(a, &map_a, s * BC, i0, bar);
                     }
                     if constexpr (B_ROWS) {
-                        for (int h = 0; h < BN / 128; ++h) tma_load_2d_pair(b + h * BC * 128, &map_b, j0 + 64 * h, s * BC, bar);
+                        tma_load_2d_pair(b, &map_b, j0, s * BC, bar);
+                        tma_load_2d_pair(b + BC * 128, &map_b, j0 + 64, s * BC, bar);
                     } else {
                         tma_load_2d_pair(b, &map_b, s * BC, j0, bar);
                     }
-                    ++issued;
-                    if (++stage == PAIR_STAGES) stage = 0, phase ^= 1u;
                 }
+                __syncwarp();
+                ++issued;
+                if (++stage == PAIR_STAGES) stage = 0, phase ^= 1u;
             }
-            // the count goes to the even CTA, whose full barriers count both CTAs' bytes: it drains (below)
+        }
+        // the count goes to the even CTA, whose full barriers count both CTAs' bytes: it drains (below)
+        if (lane == 0) {
             if (rank == 0) {
                 s_issued[0] = issued;
             } else {
@@ -667,33 +688,39 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
         }
         __syncwarp();
     } else if (warp == 9) {
-        if (lane == 0 && rank == 0) {
+        if (rank == 0) {
             const uint32_t empty_peer = map_to_rank(empty0, peer), tfull_peer = map_to_rank(tfull0, peer);
             const uint32_t a0 = desc_low<A_ROWS>(ring0), b0 = desc_low<B_ROWS>(ring0 + PAIR_HALF);
             int stage = 0, acc = 0;
             uint32_t phase = 0, acc_phase = 0;
             bool ok = true;
             for (int tile = cluster_id; tile < n_tiles && ok; tile += n_clusters) {
-                if (!pipe_wait(tempty0 + 8 * acc, acc_phase ^ 1u, abort_flag, 2)) break;
+                if (!__all_sync(0xFFFFFFFFu, pipe_wait(tempty0 + 8 * acc, acc_phase ^ 1u, abort_flag, 2))) break;
                 fence_after();
                 const uint32_t d = tmem + static_cast<uint32_t>(acc * BN);
                 for (int s = 0; s < steps; ++s) {
-                    if (!pipe_wait(full0 + 8 * stage, phase, abort_flag, 2)) { ok = false; break; }
-                    fence_after();
+                    if (!__all_sync(0xFFFFFFFFu, pipe_wait(full0 + 8 * stage, phase, abort_flag, 2))) { ok = false; break; }
                     const uint32_t a = a0 + stage * (PAIR_STAGE >> 4), b = b0 + stage * (PAIR_STAGE >> 4);
+                    if (elect_one()) {
 #pragma unroll
-                    for (int k = 0; k < BC / 16; ++k)
-                        mma_f16<true>(d, a + k * kDescStep<A_ROWS>, b + k * kDescStep<B_ROWS>, idesc, s > 0 || k > 0);
-                    mma_commit_pair(empty0 + 8 * stage);
-                    mma_commit_pair(empty_peer + 8 * stage);
+                        for (int k = 0; k < BC / 16; ++k)
+                            mma_f16<true>(d, a + k * kDescStep<A_ROWS>, b + k * kDescStep<B_ROWS>, idesc, s > 0 || k > 0);
+                        mma_commit_pair(empty0 + 8 * stage);
+                        mma_commit_pair(empty_peer + 8 * stage);
+                    }
+                    __syncwarp();
                     if (++stage == PAIR_STAGES) stage = 0, phase ^= 1u;
                 }
                 if (!ok) break;
-                mma_commit_pair(tfull0 + 8 * acc);
-                mma_commit_pair(tfull_peer + 8 * acc);
+                if (elect_one()) {
+                    mma_commit_pair(tfull0 + 8 * acc);
+                    mma_commit_pair(tfull_peer + 8 * acc);
+                }
+                __syncwarp();
                 if (++acc == 2) acc = 0, acc_phase ^= 1u;
             }
-            mma_commit_pair(drain);
+            if (elect_one()) mma_commit_pair(drain);
+            __syncwarp();
             mbar_drain_wait(drain, 0);
         }
         __syncwarp();
