@@ -17,8 +17,6 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
-#include <cstdio>
-#include <cstdlib>
 #include <type_traits>
 
 namespace wf {
@@ -908,14 +906,16 @@ int launch_pair(const Product &p, const Epilogue &e0, int dev, cudaStream_t stre
 }
 
 // Which kernel and shape take a product: the one of the least estimated time, from what one B200 measured (graphs of
-// calls over operands that do not stay in L2).
-//   tile kernel (NT rows, S CTAs to a tile): a CTA lasts 4 us and its contraction steps; a step takes its bytes at 58 a
-//     cycle (NT = 128: 0.30 us, 64: 0.22, 16: 0.17) or the ring's share of a 1.2 us round trip; one or two CTAs share an
-//     SM. The epilogue takes 13 ns a row; sharing a tile costs 1.2 us of cluster barriers and the parts' way through
-//     distributed shared memory at 3.3 TB/s. Nothing is faster than the operands' bytes at 6 TB/s.
-//   pair kernel: 8.5 us, and for each round of 74 tiles 0.38 us a step, or 3.3 us where the epilogue is longer.
-// Measured either side of the choice (us): 333 x 1024 x 5120 tile 10.7, pair 14.5; 512 x 5120 x 5120 tile 38.4, pair
-// 36.3; 2048 x 2048 x 2048 tile 26.5, pair 20.6; 128 x 2048 x 2048 NT = 64 and S = 4 9.0, NT = 128 and S = 1 14.7.
+// calls over operands that do not stay in L2; the estimates are within some 15 %).
+//   tile kernel (NT rows, S CTAs to a tile): a CTA takes 3.8 us, 13 ns a row of its epilogue, and its contraction steps. A
+//     step takes 0.19 us, 7.2 ns a KB of its operands, or the ring's share of a 1.2 us round trip; CTAs that share an SM
+//     share that rate. More than two CTAs an SM come in rounds. Sharing a tile costs 1.2 us of cluster barriers and the
+//     parts' way through distributed shared memory at 3.3 TB/s. Nothing is faster than the operands' bytes at 6 TB/s.
+//   pair kernel: 8.9 us and 0.275 us a step for the first 74 tiles (somewhat less for a step or two), and for each further
+//     74 0.3 us a step, or 4.2 us where the epilogue is longer.
+// Measured on both sides of the choice, in us (tile NT, S / pair): 333 x 1024 x 5120 128, 1 9.6 / 13.8; 1024 x 2048 x 2048
+// 128, 1 13.0 / 18.2; 512 x 5120 x 5120 128, 1 35.1 / 33.2; 5000 x 72 x 2048 128, 1 18.3 / 16.5; 8192 x 256 x 2048 128, 1 26.5 /
+// 20.5. Among tiles: 128 x 2048 x 2048 64, 4 8.5, 128, 1 12.3, 16, 8 23; 8192 rows to a 256 x 256 gradient 64, 8 10.2, 64, 1 29.
 struct Plan {
     int nt, split;  // nt 0: the pair kernel
     bool deep;
@@ -923,29 +923,26 @@ struct Plan {
 };
 
 Plan tile_plan(const Product &p, int nt, int split, int sms) {
-    const double stage_kb = 16 + nt / 8.0, steps = static_cast<double>((p.c + BC * split - 1) / (BC * split));
+    const double steps = static_cast<double>((p.c + BC * split - 1) / (BC * split));
     const double ctas = static_cast<double>((p.n + TILE_J - 1) / TILE_J * ((p.m + nt - 1) / nt)) * split;
     const bool deep = split == 1 && ctas <= sms;
     const int stages = (nt <= 32 ? 5 : nt <= 64 ? 4 : 3) * (deep ? 2 : 1);
-    const double load = std::min(2.0, std::max(1.0, ctas / sms));  // CTAs that share an SM
-    const double step = std::max(stage_kb * 0.0093 * load, 1.2 / stages);
-    const double rows = std::min<double>(nt, static_cast<double>(p.m)) / split;
-    double cta = 4.0 + steps * step + 0.013 * rows;
+    const double shared = ctas > sms ? std::min(2.0, 1.0 + 1.5 * std::sqrt(ctas / sms - 1.0)) : 1.0;
+    const double step = std::max(std::max(0.19, (16 + nt / 8.0) * 0.0072) * shared, 1.2 / stages);
+    double cta = 3.8 + steps * step + 0.013 * std::min<double>(nt, static_cast<double>(p.m)) / split;
     if (split > 1) cta += 1.2 + nt * 512.0 * (split - 1) / split * std::min(ctas, 2.0 * sms) / 3.3e6;
     const double bytes = 2.0 * (static_cast<double>(p.m) * p.c + static_cast<double>(p.n) * p.c + static_cast<double>(p.m) * p.n);
-    return {nt, split, deep, std::max(cta * std::max(1.0, ctas / (2.0 * sms)), bytes / 6.0e6 + 4.0)};
+    return {nt, split, deep, std::max(cta * std::ceil(ctas / (2.0 * sms)), bytes / 6.0e6 + 4.0)};
 }
 
 Plan make_plan(const Product &p, int least_nt) {
     static const int forced = env_digit("WEIGHTFERRY_LINEAR_PAIR", 2);  // 0 / 1: the tile / the pair kernel only
     const int sms = device_sm_count();
     const double tiles = static_cast<double>((p.m + 255) / 256) * ((p.n + BN - 1) / BN), steps = static_cast<double>((p.c + BC - 1) / BC);
-    const Plan pair{0, 1, false, 8.5 + std::ceil(tiles / (sms / 2)) * std::max(0.38 * steps, 3.3)};
-    if (forced == 1) return pair;
-    static const int fnt = getenv("WF_NT") ? atoi(getenv("WF_NT")) : 0, fsp = getenv("WF_SPLIT") ? atoi(getenv("WF_SPLIT")) : 0;
-    if (fnt) return tile_plan(p, std::max(least_nt, fnt), fsp, sms);
-    Plan best = pair;
-    best.us = forced == 0 ? 1e30 : pair.us;
+    Plan best{0, 1, false, 8.9 + 0.275 * steps - 0.2 * std::max(0.0, 8.0 - steps) +
+                               (std::ceil(tiles / (sms / 2)) - 1.0) * std::max(0.3 * steps, 4.2)};
+    if (forced == 1) return best;
+    if (forced == 0) best.us = 1e30;
     for (int nt = least_nt; nt <= 128; nt *= 2) {
         for (int split = 1; split <= 8 && (split == 1 || split <= steps); split *= 2) {
             const Plan t = tile_plan(p, nt, split, sms);
@@ -953,7 +950,6 @@ Plan make_plan(const Product &p, int least_nt) {
         }
         if (p.m <= nt) break;  // wider tiles would hold nothing more
     }
-    if (getenv("WF_PLAN")) printf("plan m%ld n%ld k%ld: nt %d split %d deep %d us %.1f pair %.1f\n", (long)p.m, (long)p.n, (long)p.c, best.nt, best.split, best.deep, best.us, pair.us);
     return best;
 }
 
