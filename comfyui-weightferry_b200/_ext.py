@@ -5,17 +5,19 @@ library's status string. Every launch takes the caller's current CUDA stream, as
 (enhancers/fused_int8.py:151 passes torch.cuda.current_stream(dev).cuda_stream)."""
 
 import ctypes
+import importlib.util
 import os
-import struct
 import threading
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "_lib", "libweightferry_b200.so")
+OPS_PATH = os.path.join(HERE, "_lib", "wf_torch.so")
 
 WF_F16, WF_BF16, WF_F32 = 0, 1, 2
 
 _lock = threading.Lock()
 _lib = None
+_ops = None
 
 
 class ExtensionMissing(RuntimeError):
@@ -31,14 +33,6 @@ class WFError(RuntimeError):
 class DequantTask(ctypes.Structure):
     _fields_ = [("src", ctypes.c_void_p), ("dst", ctypes.c_void_p), ("n_values", ctypes.c_int64)]
 
-
-# The argument structures of the dense linear layer and layer norm, packed as bytes: one conversion for some twenty
-# arguments (ctypes takes 3 us for as many one by one, more than a small launch). Pointers, 64-bit sizes, then 32-bit
-# fields, in the header's order.
-LINEAR_ARGS = struct.Struct("=7Q9q4i")
-LINEAR_GRAD_ARGS = struct.Struct("=10Q11q4i")
-LAYER_NORM_ARGS = struct.Struct("=6Q5qf3i")
-LAYER_NORM_GRAD_ARGS = struct.Struct("=9Q7q2i")
 
 # (name, restype, argtypes) of every exported function; the CPU test checks the header declares exactly these
 SIGNATURES = {
@@ -75,15 +69,15 @@ SIGNATURES = {
     "wf_gated_residual": (ctypes.c_int, [ctypes.c_void_p] * 4 + [ctypes.c_int64] * 3 + [ctypes.c_void_p]),
     "wf_hbm_probe": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]),
     "wf_w8a8_linear_noalloc": (ctypes.c_int, [ctypes.c_void_p] * 4 + [ctypes.c_int64] * 3 + [ctypes.c_void_p]),
-    "wf_linear": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]),
+    "wf_linear": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
     "wf_linear_backward_workspace": (ctypes.c_int64, [ctypes.c_int64] * 3),
-    "wf_linear_backward": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]),
+    "wf_linear_backward": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
     "wf_linear_status": (ctypes.c_int, [ctypes.POINTER(ctypes.c_int)]),
     "wf_copy_rows16": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p] + [ctypes.c_int64] * 3
                        + [ctypes.c_void_p]),
-    "wf_layer_norm": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]),
+    "wf_layer_norm": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
     "wf_layer_norm_backward_workspace": (ctypes.c_int64, [ctypes.c_int64] * 3 + [ctypes.c_int]),
-    "wf_layer_norm_backward": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_void_p]),
+    "wf_layer_norm_backward": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
 }
 
 
@@ -108,6 +102,24 @@ def _load():
             fn.argtypes = args
         _lib = lib
     return _lib
+
+
+def ops():
+    """The module of the differentiable operations (csrc/torch_ops.cpp; raises ExtensionMissing when it is not built)."""
+    global _ops
+    if _ops is not None:
+        return _ops
+    _load()  # the library that the module links
+    with _lock:
+        if _ops is None:
+            if not os.path.exists(OPS_PATH):
+                raise ExtensionMissing(f"weightferry_b200 operations not built: {OPS_PATH} is missing "
+                                       "(run __graft_entry__.build())")
+            spec = importlib.util.spec_from_file_location("wf_torch", OPS_PATH)
+            mod = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(mod)
+            _ops = mod
+    return _ops
 
 
 def lib():
@@ -171,20 +183,6 @@ def on_device(device):
     if idx is None or idx == torch.cuda.current_device():
         return _SAME
     return torch.cuda.device(idx)
-
-
-def launch(name, packed, index):
-    """Call entry point `name` with its packed argument structure on device `index` (made current for the launch) and
-    PyTorch's current stream there; raises WFError when it refuses."""
-    import torch
-    fn = getattr(_lib or _load(), name)
-    if index == torch._C._cuda_getDevice():
-        rc = fn(packed, torch._C._cuda_getCurrentRawStream(index))
-    else:
-        with torch.cuda.device(index):
-            rc = fn(packed, torch._C._cuda_getCurrentRawStream(index))
-    if rc != 0:
-        raise WFError(rc, name)
 
 
 def dtype_code(dtype):

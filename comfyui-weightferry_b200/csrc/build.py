@@ -3,7 +3,8 @@
 Every .cu file of this folder is compiled for sm_100a only (``-gencode arch=compute_100a,code=sm_100a``) and linked
 into one shared library with the CUDA runtime linked dynamically, so that the process shares one runtime (and one
 stream namespace) with PyTorch. Objects go to ``csrc/_build/``, the library to ``<package>/_lib/``. A file is
-recompiled only when it, or a header, is newer than its object.
+recompiled only when it, or a header, is newer than its object. torch_ops.cpp (the operations with autograd nodes) becomes
+a Python module of its own beside the library, which it links; it is host code against PyTorch's headers.
 
     python comfyui-weightferry_b200/csrc/build.py [--force] [-j N]
 """
@@ -12,8 +13,10 @@ import argparse
 import glob
 import os
 import shutil
+import importlib.util
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -23,6 +26,7 @@ INCLUDE = os.path.join(REPO, "include")
 OBJ_DIR = os.path.join(HERE, "_build")
 LIB_DIR = os.path.join(PKG, "_lib")
 LIB_NAME = "libweightferry_b200.so"
+OPS_NAME = "wf_torch.so"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -40,6 +44,24 @@ def _cuda_home(nvcc):
 def _cflags():
     return ARCH + ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
                    "-I", INCLUDE, "-I", HERE, "--expt-relaxed-constexpr", "-Xptxas", "-warn-spills"]
+
+
+def _torch_dir():
+    spec = importlib.util.find_spec("torch")
+    if spec is None:
+        raise RuntimeError("PyTorch not found: the operations of torch_ops.cpp are built against its headers")
+    return os.path.dirname(spec.origin)
+
+
+def _cxx_cmd(nvcc, src, obj):
+    torch = _torch_dir()
+    inc = [os.path.join(torch, "include"), os.path.join(torch, "include", "torch", "csrc", "api", "include"),
+           sysconfig.get_paths()["include"], os.path.join(_cuda_home(nvcc), "include")]
+    cmd = ["g++", "-c", src, "-o", obj, "-fPIC", "-O2", "-std=c++17", "-fvisibility=hidden", "-D_GLIBCXX_USE_CXX11_ABI=1",
+           "-I", INCLUDE]
+    for d in inc:
+        cmd += ["-isystem", d]
+    return cmd
 
 
 def _headers():
@@ -68,14 +90,19 @@ def build(force=False, jobs=None, verbose=False):
         if force or _stale(src, obj, newest_header):
             todo.append((src, obj))
 
+    ops_src, ops_obj = os.path.join(HERE, "torch_ops.cpp"), os.path.join(OBJ_DIR, "torch_ops.o")
+    api_header = os.path.getmtime(os.path.join(INCLUDE, "weightferry_b200.h"))
+    if force or _stale(ops_src, ops_obj, api_header):
+        todo.insert(0, (ops_src, ops_obj))
+
     def compile_one(pair):
         src, obj = pair
-        cmd = [nvcc, "-c", src, "-o", obj] + _cflags()
+        cmd = _cxx_cmd(nvcc, src, obj) if src == ops_src else [nvcc, "-c", src, "-o", obj] + _cflags()
         if verbose:
             print(" ".join(cmd), flush=True)
         res = subprocess.run(cmd, capture_output=True, text=True)
         if res.returncode != 0:
-            raise RuntimeError(f"nvcc failed on {os.path.basename(src)}:\n{res.stdout}\n{res.stderr}")
+            raise RuntimeError(f"{os.path.basename(cmd[0])} failed on {os.path.basename(src)}:\n{res.stdout}\n{res.stderr}")
         return res.stderr
 
     if todo:
@@ -92,6 +119,15 @@ def build(force=False, jobs=None, verbose=False):
         if res.returncode != 0:
             raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
         os.replace(lib + ".tmp", lib)
+    ops = os.path.join(LIB_DIR, OPS_NAME)
+    if not os.path.exists(ops) or os.path.getmtime(ops_obj) > os.path.getmtime(ops):
+        torch_lib = os.path.join(_torch_dir(), "lib")
+        cmd = ["g++", "-shared", "-o", ops + ".tmp", ops_obj, "-L" + LIB_DIR, "-l:" + LIB_NAME, "-L" + torch_lib, "-ltorch",
+               "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"]
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError(f"link of {OPS_NAME} failed:\n{res.stdout}\n{res.stderr}")
+        os.replace(ops + ".tmp", ops)
     return lib
 
 

@@ -6,6 +6,7 @@ import ctypes
 
 import pytest
 
+import dense_cabi
 from conftest import wf
 
 BF = "bfloat16"
@@ -66,8 +67,7 @@ P = 4096  # an aligned address that no refused call reads
 
 def _call(name, layout, fields, kw):
     assert set(kw) <= set(fields), kw
-    ext = wf("_ext")
-    return getattr(ext.lib(), name)(getattr(ext, layout).pack(*{**fields, **kw}.values()), None)
+    return getattr(wf("_ext").lib(), name)(getattr(dense_cabi, layout).pack(*{**fields, **kw}.values()), None)
 
 
 def _linear(**kw):
@@ -132,9 +132,8 @@ def test_argument_structures_match_the_header(tmp_path):
     import os
     import subprocess
     from conftest import REPO
-    ext = wf("_ext")
-    names = {"wf_linear_args": ext.LINEAR_ARGS, "wf_linear_grad_args": ext.LINEAR_GRAD_ARGS,
-             "wf_layer_norm_args": ext.LAYER_NORM_ARGS, "wf_layer_norm_grad_args": ext.LAYER_NORM_GRAD_ARGS}
+    names = {"wf_linear_args": dense_cabi.LINEAR_ARGS, "wf_linear_grad_args": dense_cabi.LINEAR_GRAD_ARGS,
+             "wf_layer_norm_args": dense_cabi.LAYER_NORM_ARGS, "wf_layer_norm_grad_args": dense_cabi.LAYER_NORM_GRAD_ARGS}
     src = tmp_path / "sizes.c"
     src.write_text('#include <stdio.h>\n#include "weightferry_b200.h"\nint main(void) {'
                    + "".join(f'printf("%zu\\n", sizeof({n}));' for n in names) + "return 0;}")

@@ -3,6 +3,7 @@ groups and layouts."""
 
 import pytest
 
+import dense_cabi
 from conftest import wf
 from dense_reference import assert_within, norm_reference
 
@@ -173,13 +174,13 @@ def test_neighbouring_memory_is_left_alone(cuda):
         x = torch.randn((m, d), device="cuda")
         y = torch.full((m + 2, ld), -7.0, device="cuda")
         stats = torch.full((2, m + 2), -7.0, device="cuda")
-        ext.launch("wf_layer_norm", ext.LAYER_NORM_ARGS.pack(x.data_ptr(), 0, 0, y.data_ptr(), stats.data_ptr(),
-                                                             stats[1].data_ptr(), d, ld, m, d, m, 1e-6, 2, 2, 0), 0)
+        dense_cabi.launch("wf_layer_norm", dense_cabi.LAYER_NORM_ARGS.pack(x.data_ptr(), 0, 0, y.data_ptr(), stats.data_ptr(),
+                                                             stats[1].data_ptr(), d, ld, m, d, m, 1e-6, 2, 2, 0))
         assert bool((y[:m, d:] == -7).all()) and bool((y[m:] == -7).all()) and bool((stats[:, m:] == -7).all())
         dx = torch.full((m + 2, ld), -7.0, device="cuda")
-        ext.launch("wf_layer_norm_backward", ext.LAYER_NORM_GRAD_ARGS.pack(
+        dense_cabi.launch("wf_layer_norm_backward", dense_cabi.LAYER_NORM_GRAD_ARGS.pack(
             x.data_ptr(), x.data_ptr(), 0, stats.data_ptr(), stats[1].data_ptr(), dx.data_ptr(), 0, 0, 0, d, d, ld, m, d, m, 0,
-            2, 2), 0)
+            2, 2))
         assert bool((dx[:m, d:] == -7).all()) and bool((dx[m:] == -7).all()) and not bool((dx[:m, :d] == -7).any())
 
 

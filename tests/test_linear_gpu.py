@@ -5,6 +5,7 @@ import math
 
 import pytest
 
+import dense_cabi
 from conftest import wf
 from dense_reference import ACTS, act, assert_within, linear_reference
 
@@ -202,8 +203,8 @@ def test_neighbouring_memory_is_left_alone(cuda):
         dy = torch.ones((m, n), device="cuda", dtype=torch.bfloat16)
         y = torch.full((m + 3, ld), -7.0, device="cuda", dtype=torch.bfloat16)
         z = torch.full((m + 3, ld), -7.0, device="cuda", dtype=torch.float16)
-        ext.launch("wf_linear", ext.LINEAR_ARGS.pack(x.data_ptr(), w.data_ptr(), 0, 0, 0, y.data_ptr(), z.data_ptr(), k, k, 0,
-                                                     ld, ld, 1, m, n, k, 1, 1, 0, 0), 0)
+        dense_cabi.launch("wf_linear", dense_cabi.LINEAR_ARGS.pack(x.data_ptr(), w.data_ptr(), 0, 0, 0, y.data_ptr(), z.data_ptr(), k, k, 0,
+                                                     ld, ld, 1, m, n, k, 1, 1, 0, 0))
         for t in (y, z):
             assert bool((t[:m, :n] == k).all()) and bool((t[:m, n:] == -7).all()) and bool((t[m:] == -7).all())
         dx = torch.full((m + 3, k + 8), -7.0, device="cuda", dtype=torch.bfloat16)
@@ -211,9 +212,9 @@ def test_neighbouring_memory_is_left_alone(cuda):
         db = torch.full((n + 8,), -7.0, device="cuda", dtype=torch.bfloat16)
         size = ext.lib().wf_linear_backward_workspace(m, n, m)
         work = torch.full((size + 64,), 113, device="cuda", dtype=torch.uint8)
-        ext.launch("wf_linear_backward", ext.LINEAR_GRAD_ARGS.pack(
+        dense_cabi.launch("wf_linear_backward", dense_cabi.LINEAR_GRAD_ARGS.pack(
             dy.data_ptr(), x.data_ptr(), w.data_ptr(), 0, 0, dx.data_ptr(), dw.data_ptr(), db.data_ptr(), 0, work.data_ptr(), n,
-            k, k, 0, k + 8, k + 8, m, size, m, n, k, 0, 1, 0, 0), 0)
+            k, k, 0, k + 8, k + 8, m, size, m, n, k, 0, 1, 0, 0))
         assert bool((work[size:] == 113).all())
         n16, m16 = (float(torch.tensor(float(v)).to(torch.bfloat16)) for v in (n, m))
         assert bool((dx[:m, :k] == n16).all()) and bool((dx[:m, k:] == -7).all()) and bool((dx[m:] == -7).all())
