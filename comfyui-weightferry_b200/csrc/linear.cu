@@ -437,19 +437,23 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_const
 // columns 0..127 of the B tile from the even CTA's shared memory and the other halves from the odd CTA's; each CTA's
 // tensor memory holds its 128 rows x 256 columns, twice, so that the next tile's MMAs run while this one is written out.
 // Warp 8 loads (six 32 KB stages), warp 9 of the even CTA issues, warps 0..7 are the epilogue: a warp takes 32 rows and
-// 128 columns of the accumulator in chunks of 32 x 32, which leave through a swizzled 2 KB buffer and one TMA store each
-// (plain stores where the output's pitch or base is not a multiple of 16 bytes).
+// 128 columns of the accumulator in chunks of 32 x 64 (32 x 32 where z is kept, too), which leave through a swizzled buffer
+// and one TMA store each (plain stores where the output's pitch or base is not a multiple of 16 bytes). Chunks of 32 x 32
+// for y alone: 8192 x 512 x 8192 63.9 against 58.9 us; a stage given up for a second wide buffer: 8192 x 2048 x 8192 with
+// silu and z 214 against 197.
 // What bounds it: a stage is 512 cycles of MMAs and 32 KB an SM, 64 bytes a cycle -- what an SM takes in from L2 (56 to
 // 60 measured) -- and in long runs the board's power. A 256 x 128 tile (24 KB for 256 cycles) was no faster anywhere:
 // 2048^3 30.5 against 20.6 us, 8192 x 256 x 2048 24.4 against 20.8.
 constexpr int BN = 256;
 constexpr int PAIR_THREADS = 320;
 constexpr int PAIR_EPI_THREADS = 256;
-constexpr int PAIR_STAGES = 6;
 constexpr int PAIR_HALF = 128 * BC * 2;            // 16 KB: this CTA's 128 rows of A or columns of B
 constexpr int PAIR_STAGE = 2 * PAIR_HALF;
-constexpr int PAIR_OUT = 8 * 2 * 2048;             // two chunks an epilogue warp
-constexpr int PAIR_SMEM = PAIR_STAGES * PAIR_STAGE + PAIR_OUT + 1024 + 256;
+constexpr int PAIR_STAGES = 6;
+constexpr int WARP_OUT = 4096;                     // output chunks of an epilogue warp: 32 rows of 64 columns of y, or of 32 of y
+                                                   // and 32 of the kept z
+constexpr int PAIR_SMEM = PAIR_STAGES * PAIR_STAGE + 8 * WARP_OUT + 1024 + 256;
+constexpr int chunk_cols(bool keep) { return keep ? 32 : 64; }
 constexpr int kBand = 8;                           // tile rows of a band of the tile order
 
 // Value by value and out of line, for rows that 16-byte accesses do not fit.
@@ -484,52 +488,69 @@ __device__ __forceinline__ void act32(float (&v)[32]) {
     for (int i = 0; i < 32; i += 2) act2<ACT>(v[i], v[i + 1]);
 }
 
-// 32 x 32 values (this lane's row in p) to the warp's chunk buffer and out: 16-byte piece j of row r sits at piece
-// j ^ ((r >> 1) & 3). The buffer is used every second time: lane 0 first waits until its last store has been read.
-__device__ __forceinline__ void emit32(const uint32_t (&p)[16], uint32_t buf, int lane, bool tma, const CUtensorMap *map,
-                                       void *out, int64_t ld, int row0, int col0, int m, int n) {
-    if (lane == 0) bulk_wait_read1();
-    __syncwarp();
-    const uint32_t row_addr = buf + 64u * static_cast<uint32_t>(lane), sw = (static_cast<uint32_t>(lane) >> 1) & 3u;
+// An output chunk of a warp in shared memory: 32 rows of CW columns, sent off with one TMA store (which clips what lies
+// outside), or row by row. 16-byte piece j of row r lies at piece j ^ (r & 7) (CW = 64: 128-byte swizzle) or
+// j ^ ((r >> 1) & 3) (CW = 32: 64-byte swizzle).
+struct ChunkOut {
+    const CUtensorMap *map;
+    void *out;
+    int64_t ld;
+    uint32_t buf;
+    bool tma;
+};
+
+template <int CW>
+__device__ __forceinline__ uint32_t piece_at(uint32_t buf, uint32_t row, uint32_t piece) {
+    return buf + 2u * CW * row + 16u * (piece ^ (CW == 64 ? row & 7u : (row >> 1) & 3u));
+}
+
+// 32 columns (this lane's row in p), half h of the chunk; the buffer's last store has been read
+template <int CW>
+__device__ __forceinline__ void put32(const ChunkOut &o, const uint32_t (&p)[16], int h, int lane) {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row_addr + 16u * (static_cast<uint32_t>(j) ^ sw)),
-                     "r"(p[4 * j]), "r"(p[4 * j + 1]), "r"(p[4 * j + 2]), "r"(p[4 * j + 3])
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(piece_at<CW>(o.buf, lane, 4 * h + j)), "r"(p[4 * j]),
+                     "r"(p[4 * j + 1]), "r"(p[4 * j + 2]), "r"(p[4 * j + 3])
                      : "memory");
-    if (tma) {
+}
+
+// the chunk's values one by one, a row at a time: rows and columns past the output's are left alone
+template <int CW>
+__device__ __noinline__ void send_any(uint16_t *out, int64_t ld, uint32_t buf, int lane, int rows, int cols) {
+    for (int r = 0; r < rows; ++r)
+        for (int c = lane; c < cols; c += 32) {
+            uint16_t v;
+            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(piece_at<CW>(buf, r, c >> 3) + 2u * (c & 7)) : "memory");
+            out[r * ld + c] = v;
+        }
+}
+
+template <int CW>
+__device__ __forceinline__ void send_chunk(const ChunkOut &o, int lane, int row0, int col0, int m, int n) {
+    if (o.tma) {
         fence_async_smem();
         __syncwarp();
         if (lane == 0) {
-            tma_store_2d(map, buf, col0, row0);
+            tma_store_2d(o.map, o.buf, col0, row0);
             bulk_commit();
         }
-        return;
-    }
-    __syncwarp();
-    if (col0 + lane < n) {
-        const int rows = min(32, m - row0);
-        uint16_t *dst = static_cast<uint16_t *>(out) + row0 * ld + col0 + lane;
-        for (int r = 0; r < rows; ++r) {
-            uint16_t v;
-            const uint32_t piece = (static_cast<uint32_t>(lane) >> 3) ^ ((static_cast<uint32_t>(r) >> 1) & 3u);
-            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(buf + 64u * r + 16u * piece + 2u * (lane & 7)) : "memory");
-            dst[r * ld] = v;
-        }
+    } else {
+        __syncwarp();
+        send_any<CW>(static_cast<uint16_t *>(o.out) + row0 * o.ld + col0, o.ld, o.buf, lane, min(32, m - row0), min(CW, n - col0));
+        __syncwarp();
     }
 }
 
 // what one epilogue warp knows of its 32 rows
 struct Warp32 {
-    uint32_t buf;             // its two chunk buffers
-    uint32_t chunks;          // chunks written so far: which buffer is next
     int lane, row0, m, n;
     const void *gate, *resid; // this lane's rows (null: none, or a row past m)
-    bool tma_out, tma_kept;
+    ChunkOut y, z;
 };
 
-template <int T, bool FULL>
-__device__ __forceinline__ void finish_chunk(float (&v)[32], Warp32 &w, const Epilogue &e, const CUtensorMap *map_out,
-                                             const CUtensorMap *map_kept, const uint32_t (&res)[16], int col0) {
+// 32 columns of the warp's rows, half h of a chunk of 64 (KEEP: a chunk of their own)
+template <int T, bool FULL, bool KEEP>
+__device__ __forceinline__ void finish_half(float (&v)[32], Warp32 &w, const Epilogue &e, const uint32_t (&res)[16], int col0, int h) {
     uint32_t p[16];
     if constexpr (FULL) {
         if (e.bias != nullptr) {
@@ -542,20 +563,24 @@ __device__ __forceinline__ void finish_chunk(float (&v)[32], Warp32 &w, const Ep
                 v[2 * i + 1] += f.y;
             }
         }
-        if (e.keep == KEEP_F32) {
-            const int row = w.row0 + w.lane;
-            if (row < w.m) {
-                float *dst = static_cast<float *>(e.kept) + row * e.ld_kept + col0;
+        if constexpr (KEEP) {
+            if (e.keep == KEEP_F32) {
+                const int row = w.row0 + w.lane;
+                if (row < w.m) {
+                    float *dst = static_cast<float *>(e.kept) + row * e.ld_kept + col0;
 #pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    if (col0 + i < w.n) dst[i] = v[i];
-            }
-        } else if (e.keep != KEEP_NONE) {
+                    for (int i = 0; i < 32; ++i)
+                        if (col0 + i < w.n) dst[i] = v[i];
+                }
+            } else {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                p[i] = e.keep == KEEP_F16 ? pack2_sat(v[2 * i], v[2 * i + 1]) : pack2<T>(v[2 * i], v[2 * i + 1]);
+                for (int i = 0; i < 16; ++i)
+                    p[i] = e.keep == KEEP_F16 ? pack2_sat(v[2 * i], v[2 * i + 1]) : pack2<T>(v[2 * i], v[2 * i + 1]);
+                if (w.lane == 0) bulk_wait_read1();  // all but y's last store have been read
+                __syncwarp();
+                put32<32>(w.z, p, 0, w.lane);
+                send_chunk<32>(w.z, w.lane, w.row0, col0, w.m, w.n);
             }
-            emit32(p, w.buf + 2048u * (w.chunks++ & 1u), w.lane, w.tma_kept, map_kept, e.kept, e.ld_kept, w.row0, col0, w.m, w.n);
         }
         switch (e.act) {
             case WF_ACT_RELU: act32<WF_ACT_RELU>(v); break;
@@ -585,11 +610,23 @@ __device__ __forceinline__ void finish_chunk(float (&v)[32], Warp32 &w, const Ep
     }
 #pragma unroll
     for (int i = 0; i < 16; ++i) p[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
-    emit32(p, w.buf + 2048u * (w.chunks++ & 1u), w.lane, w.tma_out, map_out, e.out, e.ld_out, w.row0, col0, w.m, w.n);
+    if constexpr (KEEP) {
+        if (w.lane == 0) e.keep == KEEP_F32 ? bulk_wait_read_all() : bulk_wait_read1();  // all but z's last store
+        __syncwarp();
+        put32<32>(w.y, p, 0, w.lane);
+        send_chunk<32>(w.y, w.lane, w.row0, col0, w.m, w.n);
+    } else {
+        if (h == 0) {
+            if (w.lane == 0) bulk_wait_read_all();
+            __syncwarp();
+        }
+        put32<64>(w.y, p, h, w.lane);
+        if (h == 1) send_chunk<64>(w.y, w.lane, w.row0, col0 - 32, w.m, w.n);
+    }
 }
 
-// FULL: the forward pass's epilogue; else D is rounded and stored
-template <bool A_ROWS, bool B_ROWS, int T, bool FULL>
+// FULL: the forward pass's epilogue; else D is rounded and stored. KEEP: z is kept
+template <bool A_ROWS, bool B_ROWS, int T, bool FULL, bool KEEP>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
 linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                    const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_kept,
@@ -598,7 +635,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     extern __shared__ uint8_t smem_raw[];
     uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t *out_chunks = ring + PAIR_STAGES * PAIR_STAGE;
-    uint64_t *bars = reinterpret_cast<uint64_t *>(out_chunks + PAIR_OUT);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(out_chunks + 8 * WARP_OUT);
     // full (used in the even CTA) and empty of each stage, tmem_full[0..1], tmem_empty[0..1] (even CTA), drain
     __shared__ uint32_t s_tmem_base;
     __shared__ int s_abort;
@@ -726,10 +763,9 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
         const int quarter = warp & 3, half = warp >> 2;
         const uint32_t tempty_leader = map_to_rank(tempty0, 0);
         Warp32 w;
-        w.buf = smem_u32(out_chunks + warp * 4096);
-        w.chunks = 0;
         w.lane = lane, w.m = m, w.n = n;
-        w.tma_out = tma_out, w.tma_kept = tma_kept;
+        w.y = ChunkOut{&map_out, epi.out, epi.ld_out, smem_u32(out_chunks + warp * WARP_OUT), tma_out};
+        w.z = ChunkOut{&map_kept, epi.kept, epi.ld_kept, w.y.buf + WARP_OUT / 2, tma_kept};
         int acc = 0;
         uint32_t acc_phase = 0;
         for (int tile = cluster_id; tile < n_tiles; tile += n_clusters) {
@@ -766,12 +802,12 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
 #pragma unroll
                 for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
                 if (q < BN / 64 - 1) {
-                    tmem_ld32(taddr + 32 * (q + 1), r);  // in flight while this chunk is finished
+                    tmem_ld32(taddr + 32 * (q + 1), r);  // in flight while this half is finished
                 } else {  // the accumulator is in registers: it may be overwritten
                     fence_before();
                     mbar_arrive_cluster(tempty_leader + 8 * acc);
                 }
-                finish_chunk<T, FULL>(v, w, epi, &map_out, &map_kept, res, col0 + 32 * q);
+                finish_half<T, FULL, KEEP>(v, w, epi, res, col0 + 32 * q, q & 1);
             }
             if (++acc == 2) acc = 0, acc_phase ^= 1u;
         }
@@ -846,25 +882,25 @@ int launch_tile(const Product &p, const Epilogue &e, int split, bool deep, int d
     return static_cast<int>(err != cudaSuccess ? err : cudaGetLastError());
 }
 
-// a 16-bit [rows, cols] output as boxes of 32 x 32 values with 64-byte swizzle
-int output_map(CUtensorMap *map, void *base, int64_t rows, int64_t cols, int64_t ld) {
+// a 16-bit [rows, cols] output as boxes of 32 rows x 64 or 32 values, swizzled over a box's row
+int output_map(CUtensorMap *map, void *base, int64_t rows, int64_t cols, int64_t ld, int box_cols) {
     EncodeTiled enc = encoder();
     if (enc == nullptr) return WF_ERR_DEVICE;
     cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
     cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld) * 2};
-    cuuint32_t box[2] = {32, 32};
+    cuuint32_t box[2] = {static_cast<cuuint32_t>(box_cols), 32};
     cuuint32_t estr[2] = {1, 1};
     CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                     CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                     box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? WF_OK : WF_ERR_ARG;
 }
 
 bool vec8_ok(const void *p, int64_t ld) { return p == nullptr || (aligned_to(p, 16) && ld % 8 == 0); }
 
-template <bool A_ROWS, bool B_ROWS, int T>
+template <bool A_ROWS, bool B_ROWS, int T, bool KEEP>
 int launch_pair(const Product &p, const Epilogue &e0, int dev, cudaStream_t stream) {
     constexpr bool full = !A_ROWS && !B_ROWS;
-    constexpr auto kern = linear_pair_kernel<A_ROWS, B_ROWS, T, full>;
+    constexpr auto kern = linear_pair_kernel<A_ROWS, B_ROWS, T, full, KEEP>;
     constexpr int smem = PAIR_SMEM;
     static std::atomic<int> clusters[64];  // resident pairs; any host thread may launch first
     if (clusters[dev].load(std::memory_order_acquire) == 0) {
@@ -893,8 +929,8 @@ int launch_pair(const Product &p, const Epilogue &e0, int dev, cudaStream_t stre
     CUtensorMap ma, mb, mo = {}, mk = {};
     int rc = A_ROWS ? operand_map(&ma, p.a, p.c, p.m, p.lda, BC) : operand_map(&ma, p.a, p.m, p.c, p.lda, 128);
     if (rc == WF_OK) rc = B_ROWS ? operand_map(&mb, p.b, p.c, p.n, p.ldb, BC) : operand_map(&mb, p.b, p.n, p.c, p.ldb, BN / 2);
-    if (rc == WF_OK && tma_out) rc = output_map(&mo, e.out, p.m, p.n, e.ld_out);
-    if (rc == WF_OK && tma_kept) rc = output_map(&mk, e.kept, p.m, p.n, e.ld_kept);
+    if (rc == WF_OK && tma_out) rc = output_map(&mo, e.out, p.m, p.n, e.ld_out, chunk_cols(KEEP));
+    if (rc == WF_OK && tma_kept) rc = output_map(&mk, e.kept, p.m, p.n, e.ld_kept, chunk_cols(KEEP));
     if (rc != WF_OK) return rc;
     const int64_t tiles = ((p.m + 255) / 256) * ((p.n + BN - 1) / BN);
     if (tiles > (1ll << 30)) return WF_ERR_ARG;
@@ -960,7 +996,10 @@ int dispatch(const Product &p, const Epilogue &e, cudaStream_t stream) {
     if (dev < 0 || dev >= 64) return WF_ERR_DEVICE;
     const Plan plan = make_plan(p, A_ROWS ? 64 : 16);  // a row-major operand comes in swizzle rows of 64
     switch (plan.nt) {
-        case 0: return launch_pair<A_ROWS, B_ROWS, T>(p, e, dev, stream);
+        case 0:
+            if constexpr (!A_ROWS && !B_ROWS)
+                if (e.keep != KEEP_NONE) return launch_pair<A_ROWS, B_ROWS, T, true>(p, e, dev, stream);
+            return launch_pair<A_ROWS, B_ROWS, T, false>(p, e, dev, stream);
         case 64: return launch_tile<A_ROWS, B_ROWS, 64, T>(p, e, plan.split, plan.deep, dev, stream);
         case 128: return launch_tile<A_ROWS, B_ROWS, 128, T>(p, e, plan.split, plan.deep, dev, stream);
         default: break;
