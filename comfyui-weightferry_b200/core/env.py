@@ -27,6 +27,7 @@ DEFAULTS = {
     "WEIGHTFERRY_DISK_THREADS": None,      # SSD reader threads (None: the probe's fastest count)
     "WEIGHTFERRY_SSD_LAYOUT": "interleave",  # which streamed blocks go to the SSD: interleave / tail
     "WEIGHTFERRY_TP_CHUNKS": "1",          # row chunks of the tensor-parallel stack's overlapped sub-layers (1: off)
+    "WEIGHTFERRY_FUSED_LINEAR": None,      # 1: the streamed stack's MLP and output projections as the fused dense linear layer
     "WEIGHTFERRY_SETTINGS_FILE": None,
 }
 

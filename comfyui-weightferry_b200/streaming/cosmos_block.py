@@ -11,7 +11,9 @@ then three sub-layers, each ``x = x + gate * sublayer(LayerNorm(x) * (1 + scale)
 * MLP: layer1, GELU, layer2.
 
 LayerNorm + modulate is kernel A (one pass), the projections are cuBLAS bf16 GEMMs on the weights the streaming
-state dequantised on arrival.
+state dequantised on arrival. With WEIGHTFERRY_FUSED_LINEAR=1 the MLP's input projection with its GELU, and the three
+output projections with their gated residuals, run as the fused dense linear layer instead (one launch each, one rounding;
+whole weights on the rank, that is one GPU or the sequence-parallel stack).
 
 Tensor parallel over N GPUs (one process per GPU, NCCL over NVLink): the residual stream is sharded by token rows
 (each rank holds rows [r * R, (r + 1) * R) of the B * L rows); before each sub-layer the modulated rows are
@@ -27,6 +29,7 @@ import torch.nn.functional as F
 from ..core import env as _env
 
 from ..enhancers import fused_block as _fb
+from ..enhancers import fused_linear as _fl
 from ..enhancers import sage_fused as _sf
 from .state import ParamSpec
 
@@ -306,6 +309,26 @@ def _residual(x_rows, gate_b, o, row0, rows_per_batch):
     return _fb.gated_residual(x_rows, gate_b[b0:b0 + 1].contiguous(), o.contiguous(), n)
 
 
+def _fused_linear(x_rows):
+    """The fused dense linear layer is asked for and covers these rows."""
+    return _env.get("WEIGHTFERRY_FUSED_LINEAR") == "1" and x_rows.is_cuda and x_rows.dtype in (torch.bfloat16, torch.float16)
+
+
+def _mlp_hidden(normed, w):
+    """GELU(normed w^T)."""
+    if _fused_linear(normed):
+        return _fl.linear(normed, w, activation="gelu")
+    return F.gelu(F.linear(normed, w))
+
+
+def _project_residual(x_rows, gate_b, a, w, row0, rows_per_batch):
+    """x + gate * (a w^T) on the shard's rows: an output projection with whole weights and its block residual."""
+    if not _fused_linear(x_rows):
+        return _residual(x_rows, gate_b, F.linear(a, w), row0, rows_per_batch)
+    b0, nb = row0 // rows_per_batch, max(1, x_rows.shape[0] // rows_per_batch)
+    return _fl.linear(a, w, residual=x_rows, gate=gate_b[b0:b0 + nb])
+
+
 def _attention(q, k, v):
     """softmax(q k^T / sqrt(d)) v for (B, L, H, d) tensors -> (B, L, H * d)."""
     o = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2))
@@ -321,6 +344,13 @@ def adaln(W, sub, emb, lora_term, tp=None):
     if tp is not None and tp.world > 1:
         m = tp.all_gather_rows(m.t().contiguous()).t()
     return (m + lora_term).chunk(3, dim=-1)
+
+
+def _output(tp, x_rows, gate, a, w, row0, rows_per_batch):
+    """x + gate * (the row-parallel output projection of a)."""
+    if tp.world == 1:
+        return _project_residual(x_rows, gate, a, w, row0, rows_per_batch)
+    return _residual(x_rows, gate, tp.row_parallel_rows(a, w), row0, rows_per_batch)
 
 
 def block_forward(x_rows, emb, ctx, rope, W, cfg, tp, batch, tokens, lora_term=None):
@@ -343,8 +373,7 @@ def block_forward(x_rows, emb, ctx, rope, W, cfg, tp, batch, tokens, lora_term=N
     v = F.linear(normed, W["self_attn.v_proj.weight"]).view(batch, tokens, Hw, hd)
     q, k = _sf.rms_rope_pair(q, k, rope, W["self_attn.q_norm.weight"], W["self_attn.k_norm.weight"], eps)
     a = _attention(q, k, v).view(batch * tokens, Hw * hd)
-    o = tp.row_parallel_rows(a, W["self_attn.output_proj.weight"])                          # (n, D)
-    x_rows = _residual(x_rows, gate, o, row0, tokens)
+    x_rows = _output(tp, x_rows, gate, a, W["self_attn.output_proj.weight"], row0, tokens)   # (n, D)
 
     # --- cross-attention
     shift, scale, gate = adaln(W, "cross_attn", emb, lora_term, tp)
@@ -356,13 +385,15 @@ def block_forward(x_rows, emb, ctx, rope, W, cfg, tp, batch, tokens, lora_term=N
     kc = _fb.rms_norm_128(kc.contiguous(), W["cross_attn.k_norm.weight"], eps)
     vc = F.linear(ctx, W["cross_attn.v_proj.weight"]).view(batch, S, Hw, hd)
     a = _attention(q, kc, vc).view(batch * tokens, Hw * hd)
-    o = tp.row_parallel_rows(a, W["cross_attn.output_proj.weight"])
-    x_rows = _residual(x_rows, gate, o, row0, tokens)
+    x_rows = _output(tp, x_rows, gate, a, W["cross_attn.output_proj.weight"], row0, tokens)
 
     # --- MLP
     shift, scale, gate = adaln(W, "mlp", emb, lora_term, tp)
-    o = tp.mlp_rows(_ln_mod_rows(x_rows, scale, shift, row0, tokens, eps), W["mlp.layer1.weight"],
-                    W["mlp.layer2.weight"])
+    normed = _ln_mod_rows(x_rows, scale, shift, row0, tokens, eps)
+    if tp.world == 1:
+        h = _mlp_hidden(normed, W["mlp.layer1.weight"])
+        return _project_residual(x_rows, gate, h, W["mlp.layer2.weight"], row0, tokens)
+    o = tp.mlp_rows(normed, W["mlp.layer1.weight"], W["mlp.layer2.weight"])
     return _residual(x_rows, gate, o, row0, tokens)
 
 
@@ -446,7 +477,7 @@ def block_forward_sp(x_rows, emb, ctx, rope, W, cfg, sp, batch, tokens, lora_ter
     q, k = _sf.rms_rope_pair(q, k, rope_b, W["self_attn.q_norm.weight"], W["self_attn.k_norm.weight"], eps)
     k, v = sp.gather_kv(k, v)
     a = _attention(q, k, v).view(n, D)
-    x_rows = _residual(x_rows, gate, F.linear(a, W["self_attn.output_proj.weight"]), 0, L)
+    x_rows = _project_residual(x_rows, gate, a, W["self_attn.output_proj.weight"], 0, L)
 
     # --- cross-attention
     shift, scale, gate = adaln(W, "cross_attn", emb_b, lora_b)
@@ -458,12 +489,12 @@ def block_forward_sp(x_rows, emb, ctx, rope, W, cfg, sp, batch, tokens, lora_ter
                           W["cross_attn.k_norm.weight"], eps)
     vc = F.linear(ctx_b, W["cross_attn.v_proj.weight"]).view(nb, S, H, hd)
     a = _attention(q, kc, vc).view(n, D)
-    x_rows = _residual(x_rows, gate, F.linear(a, W["cross_attn.output_proj.weight"]), 0, L)
+    x_rows = _project_residual(x_rows, gate, a, W["cross_attn.output_proj.weight"], 0, L)
 
     # --- MLP
     shift, scale, gate = adaln(W, "mlp", emb_b, lora_b)
-    h = F.gelu(F.linear(_ln_mod_rows(x_rows, scale, shift, 0, L, eps), W["mlp.layer1.weight"]))
-    return _residual(x_rows, gate, F.linear(h, W["mlp.layer2.weight"]), 0, L)
+    h = _mlp_hidden(_ln_mod_rows(x_rows, scale, shift, 0, L, eps), W["mlp.layer1.weight"])
+    return _project_residual(x_rows, gate, h, W["mlp.layer2.weight"], 0, L)
 
 
 def flops_per_block(cfg, batch, tokens, ctx_tokens):

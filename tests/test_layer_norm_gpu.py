@@ -55,8 +55,8 @@ def test_widths(cuda, d):
                                  (650, 1000), (650, 2816), (650, 4096), (650, 5120), (650, 6144), (650, 6152), (600, 8200)])
 def test_many_rows(cuda, m, d):
     import torch
-    _compare(torch, *_data(torch, m, d, torch.bfloat16, torch.float32))
-    _compare(torch, *_data(torch, m, d, torch.float32, torch.float32))
+    for dtype, wdtype in ((torch.bfloat16, torch.float32), (torch.float32, torch.float32), (torch.float16, torch.float16)):
+        _compare(torch, *_data(torch, m, d, dtype, wdtype))
 
 
 @pytest.mark.parametrize("m,rpg", [(12, 1), (100, 10), (100, 33), (4096, 2), (1000, 999), (257, 256), (50, 70)])
