@@ -52,16 +52,20 @@ int reduce_partials(const PartialSum &s0, const PartialSum &s1, int64_t d, int t
 
 namespace {
 
-struct CopyRowsArgs {
+struct CopyRows {
     const uint16_t *src;
     uint16_t *dst;
     int64_t rows, cols, lds, ldd;
 };
+struct CopyRowsArgs {
+    CopyRows job[2];
+};
 
-// Rows of 16-bit values to another row pitch: a warp a row, neighbouring values in neighbouring lanes (the source may
-// have any 2-byte alignment).
-__global__ void __launch_bounds__(256) copy_rows_kernel(const __grid_constant__ CopyRowsArgs a) {
-    const int64_t per = (a.cols + 255) / 256;  // pieces of 256 values a row
+// Rows of 16-bit values to another row pitch (job blockIdx.y): a warp a piece of 256 values, neighbouring values in
+// neighbouring lanes (the source may have any 2-byte alignment).
+__global__ void __launch_bounds__(256) copy_rows_kernel(const __grid_constant__ CopyRowsArgs args) {
+    const CopyRows &a = args.job[blockIdx.y];
+    const int64_t per = (a.cols + 255) / 256;  // pieces of a row
     const int64_t step = static_cast<int64_t>(gridDim.x) * 8;
     wait_prior_grid();
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); i < a.rows * per; i += step) {
@@ -78,19 +82,30 @@ __global__ void __launch_bounds__(256) copy_rows_kernel(const __grid_constant__ 
     }
 }
 
+int copy_job(CopyRows &job, const wf_copy_rows &c) {
+    if (c.rows < 0 || c.cols < 0 || c.ld_src < c.cols || c.ld_dst < c.cols) return WF_ERR_ARG;
+    if (c.rows > 0 && c.cols > 0 && (!c.src || !c.dst || !aligned_to(c.src, 2) || !aligned_to(c.dst, 2))) return WF_ERR_ARG;
+    job = CopyRows{static_cast<const uint16_t *>(c.src), static_cast<uint16_t *>(c.dst), c.cols > 0 ? c.rows : 0, c.cols, c.ld_src,
+                   c.ld_dst};
+    return WF_OK;
+}
+
 }  // namespace
 }  // namespace wf
 
-extern "C" WF_API int wf_copy_rows16(const void *src, int64_t ld_src, void *dst, int64_t ld_dst, int64_t rows,
-                                     int64_t cols, wf_stream_t stream) {
+extern "C" WF_API int wf_copy_rows16(const wf_copy_rows *copies, int n_copies, wf_stream_t stream) {
     using namespace wf;
-    if (rows < 0 || cols < 0 || ld_src < cols || ld_dst < cols) return WF_ERR_ARG;
-    if (rows == 0 || cols == 0) return WF_OK;
-    if (!src || !dst || !aligned_to(src, 2) || !aligned_to(dst, 2)) return WF_ERR_ARG;
+    if (copies == nullptr || n_copies < 1 || n_copies > 2) return WF_ERR_ARG;
+    CopyRowsArgs a = {};
+    int64_t pieces = 0;
+    for (int i = 0; i < n_copies; ++i) {
+        const int rc = copy_job(a.job[i], copies[i]);
+        if (rc != WF_OK) return rc;
+        pieces = std::max(pieces, a.job[i].rows * ((a.job[i].cols + 255) / 256));
+    }
+    if (pieces == 0) return WF_OK;
     const int rc = check_device();
     if (rc != WF_OK) return rc;
-    CopyRowsArgs a{static_cast<const uint16_t *>(src), static_cast<uint16_t *>(dst), rows, cols, ld_src, ld_dst};
-    const int64_t need = (rows * ((cols + 255) / 256) + 7) / 8;
-    const int grid = static_cast<int>(std::min<int64_t>(need, wave_ctas_at<copy_rows_kernel>(256)));
-    return launch_rows(copy_rows_kernel, dim3(grid), 256, reinterpret_cast<cudaStream_t>(stream), a);
+    const int grid = static_cast<int>(std::min<int64_t>((pieces + 7) / 8, wave_ctas_at<copy_rows_kernel>(256)));
+    return launch_rows(copy_rows_kernel, dim3(grid, n_copies), 256, reinterpret_cast<cudaStream_t>(stream), a);
 }

@@ -58,15 +58,34 @@ std::pair<Tensor, int64_t> as_rows(const Tensor &t) {
     return {t, s0};
 }
 
-// ... as TMA reads it: 16-byte aligned, a pitch of a multiple of 8 values. Other layouts (odd widths, slices) are copied.
-std::pair<Tensor, int64_t> as_operand(const Tensor &t) {
+// An operand of a product as TMA reads it: 16-byte aligned, a pitch of a multiple of 8 values. Other layouts (odd widths,
+// slices) are to be copied.
+struct Operand {
+    Tensor t;
+    int64_t ld;
+    wf_copy_rows copy = {};
+};
+
+Operand as_operand(const Tensor &t) {
     const int64_t rows = t.size(0), cols = t.size(1), s0 = rows == 1 ? up8(cols) : t.stride(0);
     if ((t.stride(1) == 1 || cols == 1) && s0 % 8 == 0 && s0 >= cols && reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0)
         return {t, s0};
-    const auto [src, ld] = as_rows(t);
-    Tensor out = at::empty({rows, up8(cols)}, t.options());
-    check(wf_copy_rows16(src.const_data_ptr(), ld, out.mutable_data_ptr(), up8(cols), rows, cols, stream_of(t)), "wf_copy_rows16");
-    return {out, up8(cols)};
+    Operand o{at::empty({rows, up8(cols)}, t.options()), up8(cols)};
+    o.copy = {t.const_data_ptr(), o.t.mutable_data_ptr(), t.stride(0), o.ld, rows, cols};
+    return o;
+}
+
+// x's and w's operands, their copies in one launch
+std::pair<Operand, Operand> as_operands(const Tensor &x, const Tensor &w) {
+    const auto [x2, ldx] = as_rows(x);  // x2 and w2 live until the copies are launched
+    const auto [w2, ldw] = as_rows(w);
+    Operand xo = as_operand(x2), wo = as_operand(w2);
+    wf_copy_rows copies[2];
+    int n = 0;
+    if (xo.copy.dst != nullptr) copies[n] = xo.copy, copies[n++].ld_src = ldx;
+    if (wo.copy.dst != nullptr) copies[n] = wo.copy, copies[n++].ld_src = ldw;
+    if (n > 0) check(wf_copy_rows16(copies, n, stream_of(x)), "wf_copy_rows16");
+    return {xo, wo};
 }
 
 // rows of x for each row of p ([n] or [groups, n]): as given, or all m rows divided evenly
@@ -111,8 +130,7 @@ Tensor linear_forward(const Tensor &x, const Tensor &w, const MaybeTensor &bias,
     shape.back() = c.n;
     Tensor y = at::empty(shape, x.options());
     if (c.m == 0 || c.n == 0) return y;
-    const auto [xo, ldx] = as_operand(x.dim() == 2 ? x : x.reshape({c.m, c.k}));
-    const auto [wo, ldw] = as_operand(w);
+    const auto [xo, wo] = as_operands(x.dim() == 2 ? x : x.reshape({c.m, c.k}), w);
     wf_linear_args a = {};
     Tensor b, g, r, z;
     if (bias) b = bias->contiguous();
@@ -124,12 +142,12 @@ Tensor linear_forward(const Tensor &x, const Tensor &w, const MaybeTensor &bias,
         a.ldz = up8(c.n);
         a.z_type = code_of(*z_type);
     }
-    a.x = xo.const_data_ptr(), a.w = wo.const_data_ptr(), a.bias = ptr(b), a.gate = ptr(g), a.resid = ptr(r);
+    a.x = xo.t.const_data_ptr(), a.w = wo.t.const_data_ptr(), a.bias = ptr(b), a.gate = ptr(g), a.resid = ptr(r);
     a.y = y.mutable_data_ptr();
-    a.ldx = ldx, a.ldw = ldw, a.ldy = c.n, a.rows_per_group = c.rpg, a.m = c.m, a.n = c.n, a.k = c.k;
+    a.ldx = xo.ld, a.ldw = wo.ld, a.ldy = c.n, a.rows_per_group = c.rpg, a.m = c.m, a.n = c.n, a.k = c.k;
     a.act = static_cast<int32_t>(c.act), a.type = code_of(x.scalar_type());
     check(wf_linear(&a, stream_of(x)), "wf_linear");
-    if (kept != nullptr) *kept = Kept{xo, wo, z, ldx, ldw};
+    if (kept != nullptr) *kept = Kept{xo.t, wo.t, z, xo.ld, wo.ld};
     return y;
 }
 

@@ -229,9 +229,13 @@ WF_API int wf_linear_backward(const wf_linear_grad_args *args, wf_stream_t strea
 /* Status word of the dense linear layer's kernels, as wf_w8a8_gemm_status. Reading it synchronises and clears it. */
 WF_API int wf_linear_status(int *status);
 
-/* rows x cols 16-bit values to another row pitch (any 2-byte alignment). */
-WF_API int wf_copy_rows16(const void *src, int64_t ld_src, void *dst, int64_t ld_dst, int64_t rows, int64_t cols,
-                          wf_stream_t stream);
+/* One or two copies of rows x cols 16-bit values to another row pitch (any 2-byte alignment) in one launch. */
+typedef struct wf_copy_rows {
+    const void *src;
+    void *dst;
+    int64_t ld_src, ld_dst, rows, cols;
+} wf_copy_rows;
+WF_API int wf_copy_rows16(const wf_copy_rows *copies, int n_copies, wf_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------- layer norm
  * Rows of d values of `type` (f16, bf16 or f32) with a row pitch in values; w and b of `type` or f32 (w_type), one

@@ -7,6 +7,7 @@ from conftest import wf
 # pointers, 64-bit sizes, then 32-bit fields, in the header's order
 LINEAR_ARGS = struct.Struct("=7Q9q4i")
 LINEAR_GRAD_ARGS = struct.Struct("=10Q11q4i")
+COPY_ROWS = struct.Struct("=2Q4q")
 LAYER_NORM_ARGS = struct.Struct("=6Q5qf3i")
 LAYER_NORM_GRAD_ARGS = struct.Struct("=9Q7q2i")
 

@@ -101,7 +101,9 @@ def test_c_linear_backward_refuses():
     assert grad(dx=0, dw=0) == 0
     assert lib.wf_linear_backward_workspace(4, 32, 4) >= 4 * 32 * 2 and lib.wf_linear_backward_workspace(0, 32, 4) == 0
     assert lib.wf_linear(None, None) == ARG and lib.wf_linear_backward(None, None) == ARG
-    assert lib.wf_copy_rows16(P, 4, P, 8, 3, 5, None) == ARG and lib.wf_copy_rows16(P, 8, P, 8, 0, 5, None) == 0
+    copy = dense_cabi.COPY_ROWS.pack
+    assert lib.wf_copy_rows16(copy(P, P, 4, 8, 3, 5), 1, None) == ARG and lib.wf_copy_rows16(copy(P, P, 8, 8, 0, 5), 1, None) == 0
+    assert lib.wf_copy_rows16(copy(P, P, 8, 8, 3, 5), 3, None) == ARG and lib.wf_copy_rows16(None, 1, None) == ARG
     assert lib.wf_linear_status(ctypes.POINTER(ctypes.c_int)()) == ARG
 
 
@@ -133,7 +135,8 @@ def test_argument_structures_match_the_header(tmp_path):
     import subprocess
     from conftest import REPO
     names = {"wf_linear_args": dense_cabi.LINEAR_ARGS, "wf_linear_grad_args": dense_cabi.LINEAR_GRAD_ARGS,
-             "wf_layer_norm_args": dense_cabi.LAYER_NORM_ARGS, "wf_layer_norm_grad_args": dense_cabi.LAYER_NORM_GRAD_ARGS}
+             "wf_copy_rows": dense_cabi.COPY_ROWS, "wf_layer_norm_args": dense_cabi.LAYER_NORM_ARGS,
+             "wf_layer_norm_grad_args": dense_cabi.LAYER_NORM_GRAD_ARGS}
     src = tmp_path / "sizes.c"
     src.write_text('#include <stdio.h>\n#include "weightferry_b200.h"\nint main(void) {'
                    + "".join(f'printf("%zu\\n", sizeof({n}));' for n in names) + "return 0;}")
