@@ -345,7 +345,7 @@ __device__ __forceinline__ void param_piece(uint64_t (&p)[T == WF_F32 ? 2 : 4], 
 // Many wider rows that 16-byte accesses fit: a team of WPR warps a row. Each thread copies its own 16-byte pieces of the
 // team's next rows into a ring in shared memory (cp.async) and reads nobody else's, so that rows stream in without a
 // barrier and without registers (a row held in registers, widened three times, needed 234 of them for 5120 values and
-// left 8 warps an SM: 84 us where this takes 66). A block takes a run of rows (RowSplit) and keeps their group's w and b
+// left 8 warps an SM: 16384 x 5120 took 84 us where this takes 62). A block takes a run of rows (RowSplit) and keeps their group's w and b
 // in shared memory: read from L2 for every row they cost more than x itself (16384 x 5120 bf16 in 16 groups: 222 us).
 // Groups of fewer than kStageRows rows are read from L2 all the same.
 constexpr int kStageRows = 16;
@@ -904,12 +904,14 @@ int dispatch_norm(const NormArgs &a, cudaStream_t stream) {
     if (chunks <= 8) return launch_norm_narrow<T, W, 8>(a, stream);
     if (chunks <= 16) return launch_norm_narrow<T, W, 16>(a, stream);
     if (chunks <= 32) return launch_norm_narrow<T, W, 32>(a, stream);
-    // teams of warps where there are rows for them, up to 10 KB of a row a warp; else a row a block
+    // Teams of warps where there are rows for them, else a row a block. Larger teams leave room for more rows in flight, at
+    // a barrier a sum: 16384 x 2048 with teams of 1 / 2 / 4 27.4 / 31.1 / 43.7 us, 16384 x 5120 63.5 / 61.7 / 67.0, 8192 x 8192
+    // with 2 / 4 / 8 55.4 / 50.8 / 55.3, 4096 x 12288 with 4 / 8 46.1 / 44.0.
     const int kb = (a.d * dtype_size(T) + 1023) / 1024;
     if (a.rows >= 4ll * device_sm_count()) {
-        if (kb <= 10) return launch_norm_stream<T, W, 1>(a, stream);
-        if (kb <= 20) return launch_norm_stream<T, W, 2>(a, stream);
-        if (kb <= 40) return launch_norm_stream<T, W, 4>(a, stream);
+        if (kb <= 8) return launch_norm_stream<T, W, 1>(a, stream);
+        if (kb <= 12) return launch_norm_stream<T, W, 2>(a, stream);
+        if (kb <= 20) return launch_norm_stream<T, W, 4>(a, stream);
         if (kb <= 80) return launch_norm_stream<T, W, 8>(a, stream);
     }
     return launch_norm_block<T, W, true>(a, stream);
