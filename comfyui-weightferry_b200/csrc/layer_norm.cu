@@ -17,6 +17,7 @@
 #include "wf_common.cuh"
 #include "wf_pairs.cuh"
 #include "wf_rows.cuh"
+#include "wf_tcgen05.cuh"
 
 #include <algorithm>
 
@@ -24,6 +25,7 @@ namespace wf {
 namespace {
 
 constexpr int kMaxThreads = 1024;
+constexpr int kTeam = 8;  // CTAs of a team
 
 // The sums of N values over the block's threads, in every thread (one warp: shuffles alone). `red` has room for
 // 32 * N floats; two calls in a row take different buffers, so that one barrier a call is enough.
@@ -464,6 +466,111 @@ __global__ void __launch_bounds__(256) layer_norm_stream_kernel(const __grid_con
     }
 }
 
+// The sums of N values (a power of 2) over the block's threads: sum k in the lanes k, k + N, ... of every warp. One barrier;
+// two calls in a row take different buffers.
+template <int N>
+__device__ __forceinline__ float block_sums(float (&v)[N], float (*red)[N], int warp, int lane, int warps) {
+    constexpr int L = 32 / N;  // lanes that hold the same sum
+    const float mine = lanes_sum_many<N>(v, lane);
+    if ((lane & (L - 1)) == 0) red[warp][lane / L] = mine;
+    __syncthreads();
+    float t = 0.f;
+    for (int i = lane / N; i < warps; i += L) t += red[i][lane % N];
+#pragma unroll
+    for (int o = N; o < 32; o *= 2) t += __shfl_xor_sync(0xFFFFFFFFu, t, o);
+    return t;
+}
+
+// A row that 16-byte accesses do not fit, in shared memory: the aligned 16-byte pieces that it lies in are copied (cp.async),
+// and values are read one by one from where its first byte falls in them. What a piece holds before the row is copied with
+// it and never read (the piece holds a byte of the row, so it lies in its allocation); nothing past the row is read.
+// Single values copied straight from HBM keep too few bytes in flight (16384 x 5119
+// bf16: forward 186 us and backward 346, where these take 134 and 182).
+__host__ __device__ inline int cover_bytes(int d, int type) { return (d * dtype_size(type) + 15) / 16 * 16 + 16; }
+__device__ __forceinline__ int skew(const void *row) { return static_cast<int>(reinterpret_cast<uintptr_t>(row) & 15); }
+__device__ __forceinline__ void copy_cover(char *dst, const void *row, int bytes, int tid, int threads) {
+    const int s = skew(row), n = s + bytes;
+    const char *src = static_cast<const char *>(row) - s;
+    for (int i = 16 * tid; i < n; i += 16 * threads)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst + i)), "l"(src + i), "r"(min(16, n - i))
+                     : "memory");
+}
+
+// The forward pass of rows of 257 to 8192 values that 16-byte accesses do not fit: eight values a thread, with their w and b
+// in registers, R rows at a time through a ring of such copies; one barrier a sum.
+constexpr int kRing = 3;
+template <int T, int W, int R, int THREADS, int BLOCKS>
+__global__ void __launch_bounds__(THREADS, BLOCKS) layer_norm_unaligned_kernel(const __grid_constant__ NormArgs a,
+                                                                               const __grid_constant__ RowSplit split) {
+    extern __shared__ uint4 smem[];
+    __shared__ float red[2][32][R];
+    const int tid = threadIdx.x, threads = blockDim.x, warp = tid >> 5, lane = tid & 31, warps = threads >> 5;
+    const int cover = cover_bytes(a.d, T), bytes = a.d * dtype_size(T);
+    char *ring = reinterpret_cast<char *>(smem);
+    const float inv_d = 1.0f / static_cast<float>(a.d);
+    wait_prior_grid();
+    for (int64_t grp = split.first_group(blockIdx.x), end = split.last_group(blockIdx.x); grp < end; ++grp) {
+        int64_t lo, hi;
+        split.rows_of(blockIdx.x, grp, lo, hi);
+        auto fetch = [&](int64_t row, int slot) {
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+                if (row + r < hi) copy_cover(ring + (slot * R + r) * cover, row_of<T>(a.x, row + r, a.ldx), bytes, tid, threads);
+            cp_async_commit();
+        };
+        for (int i = 0; i < kRing; ++i) fetch(lo + i * R, i);
+        float w[8], b[8];
+        if (a.w != nullptr) load_chunk<W, false>(w, row_of<W>(a.w, grp, a.d), 0, tid, threads, a.d);
+        if (a.b != nullptr) load_chunk<W, false>(b, row_of<W>(a.b, grp, a.d), 0, tid, threads, a.d);
+        cp_async_wait<kRing - 1>();
+        __syncthreads();
+        int slot = 0;
+        for (int64_t row = lo; row < hi; row += R) {
+            float v[R][8], s[R];
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const char *x = ring + (slot * R + r) * cover + skew(row_of<T>(a.x, row + r, a.ldx));
+                load_chunk<T, false>(v[r], x, 0, tid, threads, a.d);
+                s[r] = 0.f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) s[r] += v[r][j];
+            }
+            cp_async_wait<kRing - 2>();  // the next rows are here for this thread, and behind the barrier for all
+            const float mean = block_sums<R>(s, red[0], warp, lane, warps) * inv_d;
+            fetch(row + kRing * R, slot);  // every thread has read this slot
+            if (++slot == kRing) slot = 0;
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const float mu = __shfl_sync(0xFFFFFFFFu, mean, r);
+                s[r] = 0.f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    v[r][j] -= mu;
+                    if (column<false>(0, j, tid, threads) < a.d) s[r] = fmaf(v[r][j], v[r][j], s[r]);
+                }
+            }
+            const float rstd = rsqrtf(fmaf(block_sums<R>(s, red[1], warp, lane, warps), inv_d, a.eps));
+            if (a.mean != nullptr && tid < R && row + tid < hi) {
+                a.mean[row + tid] = mean;
+                a.rstd[row + tid] = rstd;
+            }
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const float rs = __shfl_sync(0xFFFFFFFFu, rstd, r);
+                if (row + r >= hi) continue;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    v[r][j] *= rs;
+                    if (a.w != nullptr) v[r][j] *= w[j];
+                    if (a.b != nullptr) v[r][j] += b[j];
+                }
+                store_chunk<T, false>(v[r], row_of<T>(a.y, row + r, a.ldy), 0, tid, threads, a.d);
+            }
+        }
+    }
+    cp_async_wait<0>();
+}
+
 struct NormGradArgs {
     const void *x, *w, *dy;
     const float *mean, *rstd;
@@ -471,20 +578,24 @@ struct NormGradArgs {
     float *part_w, *part_b;   // [groups * chunks, d] partial sums, or null
     int64_t rows, ldx, lddy, lddx;
     RowSplit split;
-    int d;
+    int d, block_cols;        // block_cols: d, or a team's columns of each CTA (a multiple of 8)
 };
 
 // The backward pass of rows that 16-byte accesses fit, V (8 or 4) values a thread of a block: R rows at a time, whose 2 R sums
 // share one barrier (and their shuffles: lanes_sum_many). Each thread copies its own values of the next rows into a ring
 // of kRing stages in shared memory (cp.async) and reads nobody else's: the loads run on behind the barrier.
-constexpr int kRing = 3;
-template <int T, int W, int V, int R, int THREADS, int BLOCKS>
+// TEAM: a cluster of kTeam CTAs shares the rows, each CTA a run of a.block_cols columns; every warp writes its sums to all of
+// them (distributed shared memory) and the cluster's barrier takes the block's place: 4096 x 12288 bf16 109 us where the wide
+// kernels, which read x and dy once more, take 157; 4096 x 16384 151 us against 190.
+template <int T, int W, int V, int R, int THREADS, int BLOCKS, bool TEAM>
 __global__ void __launch_bounds__(THREADS, BLOCKS) layer_norm_grad_rows_kernel(const __grid_constant__ NormGradArgs a) {
     constexpr int H = V * dtype_size(T) / 16, NP = V / 2;  // 16-byte pieces and pairs of V values
     extern __shared__ uint4 smem[];                   // [kRing][R][x, dy][H][threads]
-    __shared__ float red[2][32][2 * R];
-    const int tid = threadIdx.x, threads = blockDim.x, warp = tid >> 5, lane = tid & 31, warps = threads >> 5, col = tid * V;
-    const bool in = col < a.d;
+    __shared__ float red[2][TEAM ? kTeam * THREADS / 32 : 32][2 * R];
+    const int tid = threadIdx.x, threads = blockDim.x, warp = tid >> 5, lane = tid & 31, warps = threads >> 5;
+    const int rank = TEAM ? static_cast<int>(cluster_rank()) : 0, col = rank * a.block_cols + tid * V;
+    const int64_t share = TEAM ? blockIdx.x / kTeam : blockIdx.x;
+    const bool in = tid * V < a.block_cols && col < a.d;
     const float inv_d = 1.0f / static_cast<float>(a.d);
     auto piece = [&](int stage, int r, int which, int h) { return smem + (((stage * R + r) * 2 + which) * H + h) * threads + tid; };
     auto get = [&](uint64_t (&v)[NP], int stage, int r, int which) {
@@ -497,10 +608,11 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) layer_norm_grad_rows_kernel(c
         }
     };
     int buf = 0;
+    if constexpr (TEAM) cluster_sync();  // every CTA of the team runs before another writes to its shared memory
     wait_prior_grid();
-    for (int64_t grp = a.split.first_group(blockIdx.x), end = a.split.last_group(blockIdx.x); grp < end; ++grp) {
+    for (int64_t grp = a.split.first_group(share), end = a.split.last_group(share); grp < end; ++grp) {
         int64_t lo, hi;
-        a.split.rows_of(blockIdx.x, grp, lo, hi);
+        a.split.rows_of(share, grp, lo, hi);
         auto fetch = [&](int64_t row, int stage) {  // one copy group for R rows, zeros past the last
 #pragma unroll
             for (int r = 0; r < R; ++r) {
@@ -562,11 +674,22 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) layer_norm_grad_rows_kernel(c
             }
             if (a.dx != nullptr) {
                 // every warp's sums to shared memory, then every warp adds all of them
+                constexpr int L = 32 / (2 * R);  // lanes that hold the same sum
                 const float mine = lanes_sum_many<2 * R>(s, lane);
-                if ((lane & (32 / (2 * R) - 1)) == 0) red[buf][warp][lane / (32 / (2 * R))] = mine;
-                __syncthreads();
+                if constexpr (TEAM) {
+                    // no CTA leaves before the last barrier, and nothing is written after it
+                    const uint32_t at = smem_u32(&red[buf][rank * warps + warp][lane / L]);
+                    for (int to = lane & (L - 1); to < kTeam; to += L)
+                        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(map_to_rank(at, to)), "f"(mine) : "memory");
+                    __syncwarp();
+                    cluster_sync();
+                } else {
+                    if ((lane & (L - 1)) == 0) red[buf][warp][lane / L] = mine;
+                    __syncthreads();
+                }
                 float t = 0.f;  // sum lane % (2 R), of the warps lane / (2 R), + 32 / (2 R), ...
-                for (int i = lane / (2 * R); i < warps; i += 32 / (2 * R)) t += red[buf][i][lane % (2 * R)];
+                const int all = TEAM ? warps * kTeam : warps;
+                for (int i = lane / (2 * R); i < all; i += L) t += red[buf][i][lane % (2 * R)];
 #pragma unroll
                 for (int o = 2 * R; o < 32; o *= 2) t += __shfl_xor_sync(0xFFFFFFFFu, t, o);
                 buf ^= 1;
@@ -592,7 +715,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) layer_norm_grad_rows_kernel(c
             for (int r = 0; r < R; ++r) scale[r] = scale1[r], shift[r] = shift1[r];
         }
         cp_async_wait<0>();
-        const int64_t part = a.split.partial_row(blockIdx.x, grp) * a.d;
+        const int64_t part = a.split.partial_row(share, grp) * a.d;
         if (a.part_w != nullptr && in) store_pairs<WF_F32>(a.part_w + part, col, dw);
         if (a.part_b != nullptr && in) store_pairs<WF_F32>(a.part_b + part, col, db);
     }
@@ -686,21 +809,89 @@ __global__ void __launch_bounds__(256, 3) layer_norm_grad_narrow_kernel(const __
     }
 }
 
-// The same value by value, for any width and alignment, one row at a time. WARP: a row a warp; each warp of the block takes every
-// warps-th row of the share and the warps' column sums are added at the end through shared memory.
-template <int T, int W, bool WARP>
-__global__ void __launch_bounds__(WARP ? 256 : kMaxThreads) layer_norm_grad_kernel(const __grid_constant__ NormGradArgs a) {
-    __shared__ float red[2][64];
-    __shared__ float col_red[WARP ? 8 * 32 * 8 : 1];
-    const int threads = WARP ? 32 : blockDim.x, tid = WARP ? (threadIdx.x & 31) : threadIdx.x;
-    const int warps = WARP ? 1 : (blockDim.x >> 5);
-    const int row_step = WARP ? (blockDim.x >> 5) : 1, row_first = WARP ? (threadIdx.x >> 5) : 0;
+// The same for narrow rows that 16-byte accesses do not fit, value by value: a row a warp. Each warp of the block takes every
+// eighth row of the share, and the warps' column sums are added at the end through shared memory.
+template <int T, int W>
+__global__ void __launch_bounds__(256) layer_norm_grad_warp_kernel(const __grid_constant__ NormGradArgs a) {
+    __shared__ float col_red[8][8][32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const float inv_d = 1.0f / static_cast<float>(a.d);
     wait_prior_grid();
-    int buf = 0;
     for (int64_t grp = a.split.first_group(blockIdx.x), end = a.split.last_group(blockIdx.x); grp < end; ++grp) {
         int64_t lo, hi;
         a.split.rows_of(blockIdx.x, grp, lo, hi);
+        float w[8], dw[8], db[8];
+        if (a.w != nullptr) load_chunk<W, false>(w, row_of<W>(a.w, grp, a.d), 0, lane, 32, a.d);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            dw[j] = db[j] = 0.f;
+            if (a.w == nullptr) w[j] = 1.f;
+        }
+        for (int64_t row = lo + warp; row < hi; row += 8) {
+            const float mean = a.mean[row], rstd = a.rstd[row];
+            float xh[8], dy[8], s0 = 0.f, s1 = 0.f;
+            load_chunk<T, false>(xh, row_of<T>(a.x, row, a.ldx), 0, lane, 32, a.d);
+            load_chunk<T, false>(dy, row_of<T>(a.dy, row, a.lddy), 0, lane, 32, a.d);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                xh[j] = (xh[j] - mean) * rstd;  // dy is 0 past the row's end
+                db[j] += dy[j];
+                dw[j] = fmaf(dy[j], xh[j], dw[j]);
+                dy[j] *= w[j];
+                s0 += dy[j];
+                s1 = fmaf(dy[j], xh[j], s1);
+            }
+            if (a.dx == nullptr) continue;
+            const float m0 = warp_sum(s0) * inv_d, m1 = warp_sum(s1) * inv_d;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) dy[j] = rstd * (dy[j] - m0 - xh[j] * m1);
+            store_chunk<T, false>(dy, row_of<T>(a.dx, row, a.lddx), 0, lane, 32, a.d);
+        }
+        const int64_t part = a.split.partial_row(blockIdx.x, grp) * a.d;
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+            float *dst = which ? a.part_b : a.part_w;
+            if (dst == nullptr) continue;
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < 8; ++j) col_red[warp][j][lane] = which ? db[j] : dw[j];
+            __syncthreads();
+            if (static_cast<int>(threadIdx.x) < a.d) {  // column 32 j + lane
+                float v = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v += col_red[i][warp][lane];
+                dst[part + threadIdx.x] = v;
+            }
+        }
+    }
+}
+
+// ... and for 257 to 8192 values: eight values a thread, R rows at a time through a ring of unaligned copies, one barrier for
+// the rows' 2 R sums.
+template <int T, int W, int R, int THREADS, int BLOCKS>
+__global__ void __launch_bounds__(THREADS, BLOCKS) layer_norm_grad_unaligned_kernel(const __grid_constant__ NormGradArgs a) {
+    extern __shared__ uint4 smem[];  // [kRing][R][x, dy][cover]
+    __shared__ float red[2][32][2 * R];
+    const int tid = threadIdx.x, threads = blockDim.x, warp = tid >> 5, lane = tid & 31, warps = threads >> 5;
+    const int cover = cover_bytes(a.d, T), bytes = a.d * dtype_size(T);
+    char *ring = reinterpret_cast<char *>(smem);
+    const float inv_d = 1.0f / static_cast<float>(a.d);
+    int buf = 0;
+    wait_prior_grid();
+    for (int64_t grp = a.split.first_group(blockIdx.x), end = a.split.last_group(blockIdx.x); grp < end; ++grp) {
+        int64_t lo, hi;
+        a.split.rows_of(blockIdx.x, grp, lo, hi);
+        auto fetch = [&](int64_t row, int slot) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                if (row + r >= hi) break;
+                char *dst = ring + (slot * R + r) * 2 * cover;
+                copy_cover(dst, row_of<T>(a.x, row + r, a.ldx), bytes, tid, threads);
+                copy_cover(dst + cover, row_of<T>(a.dy, row + r, a.lddy), bytes, tid, threads);
+            }
+            cp_async_commit();
+        };
+        for (int i = 0; i < kRing; ++i) fetch(lo + i * R, i);
         float w[8], dw[8], db[8];
         if (a.w != nullptr) load_chunk<W, false>(w, row_of<W>(a.w, grp, a.d), 0, tid, threads, a.d);
 #pragma unroll
@@ -708,53 +899,50 @@ __global__ void __launch_bounds__(WARP ? 256 : kMaxThreads) layer_norm_grad_kern
             dw[j] = db[j] = 0.f;
             if (a.w == nullptr) w[j] = 1.f;
         }
-        for (int64_t row = lo + row_first; row < hi; row += row_step) {
-            const float mean = a.mean[row], rstd = a.rstd[row];
-            float xh[8], dy[8];
-            float s[2] = {0.f, 0.f};
-            load_chunk<T, false>(xh, row_of<T>(a.x, row, a.ldx), 0, tid, threads, a.d);
-            load_chunk<T, false>(dy, row_of<T>(a.dy, row, a.lddy), 0, tid, threads, a.d);
+        cp_async_wait<kRing - 1>();
+        __syncthreads();
+        int slot = 0;
+        for (int64_t row = lo; row < hi; row += R) {
+            float xh[R][8], u[R][8], s[2 * R], rstd[R];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                xh[j] = (xh[j] - mean) * rstd;  // dy is 0 past the row's end
-                db[j] += dy[j];
-                dw[j] = fmaf(dy[j], xh[j], dw[j]);
-                dy[j] *= w[j];
-                s[0] += dy[j];
-                s[1] = fmaf(dy[j], xh[j], s[1]);
-            }
-            if (a.dx == nullptr) continue;
-            team_sum<2>(s, red[buf], warps);
-            buf ^= 1;
-            const float m0 = s[0] * inv_d, m1 = s[1] * inv_d;
+            for (int r = 0; r < R; ++r) {
+                const bool on = row + r < hi;  // else the slot holds older rows: count nothing
+                const float mean = on ? a.mean[row + r] : 0.f;
+                const char *x = ring + (slot * R + r) * 2 * cover;
+                rstd[r] = on ? a.rstd[row + r] : 0.f;
+                load_chunk<T, false>(xh[r], x + skew(row_of<T>(a.x, row + r, a.ldx)), 0, tid, threads, on ? a.d : 0);
+                load_chunk<T, false>(u[r], x + cover + skew(row_of<T>(a.dy, row + r, a.lddy)), 0, tid, threads, on ? a.d : 0);
+                s[2 * r] = s[2 * r + 1] = 0.f;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) dy[j] = rstd * (dy[j] - m0 - xh[j] * m1);
-            store_chunk<T, false>(dy, row_of<T>(a.dx, row, a.lddx), 0, tid, threads, a.d);
-        }
-        const int64_t part = a.split.partial_row(blockIdx.x, grp);
-        for (int which = 0; which < 2; ++which) {
-            float *dst = which ? a.part_b : a.part_w;
-            if (dst == nullptr) continue;
-            dst += part * a.d;
-            float v[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = which ? db[j] : dw[j];
-            if constexpr (WARP) {
-                __syncthreads();
-#pragma unroll
-                for (int j = 0; j < 8; ++j) col_red[(threadIdx.x >> 5) * 256 + j * 32 + tid] = v[j];
-                __syncthreads();
-                if (threadIdx.x < 32) {
-                    for (int o = 1; o < static_cast<int>(blockDim.x >> 5); ++o)
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) v[j] += col_red[o * 256 + j * 32 + tid];
-                    store_chunk<WF_F32, false>(v, dst, 0, tid, threads, a.d);
+                for (int j = 0; j < 8; ++j) {
+                    xh[r][j] = (xh[r][j] - mean) * rstd[r];  // dy is 0 past the row's end
+                    db[j] += u[r][j];
+                    dw[j] = fmaf(u[r][j], xh[r][j], dw[j]);
+                    u[r][j] *= w[j];
+                    s[2 * r] += u[r][j];
+                    s[2 * r + 1] = fmaf(u[r][j], xh[r][j], s[2 * r + 1]);
                 }
-            } else {
-                store_chunk<WF_F32, false>(v, dst, 0, tid, threads, a.d);
+            }
+            cp_async_wait<kRing - 2>();  // the next rows are here for this thread, and behind the barrier for all
+            const float mean_u = block_sums<2 * R>(s, red[buf], warp, lane, warps) * inv_d;
+            buf ^= 1;
+            fetch(row + kRing * R, slot);  // every thread has read this slot
+            if (++slot == kRing) slot = 0;
+            if (a.dx == nullptr) continue;
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const float m0 = __shfl_sync(0xFFFFFFFFu, mean_u, 2 * r), m1 = __shfl_sync(0xFFFFFFFFu, mean_u, 2 * r + 1);
+                if (row + r >= hi) continue;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) u[r][j] = rstd[r] * (u[r][j] - m0 - xh[r][j] * m1);
+                store_chunk<T, false>(u[r], row_of<T>(a.dx, row + r, a.lddx), 0, tid, threads, a.d);
             }
         }
+        const int64_t part = a.split.partial_row(blockIdx.x, grp) * a.d;
+        if (a.part_w != nullptr) store_chunk<WF_F32, false>(dw, a.part_w + part, 0, tid, threads, a.d);
+        if (a.part_b != nullptr) store_chunk<WF_F32, false>(db, a.part_b + part, 0, tid, threads, a.d);
     }
+    cp_async_wait<0>();
 }
 
 // The backward pass of wider rows: dx row by row with the row read twice (the second time from L2) ...
@@ -835,8 +1023,17 @@ int grad_threads(int d, int type) {
     return ((d + v - 1) / v + 31) / 32 * 32;
 }
 
+// Whether a team shares the rows in the backward pass: 16-bit rows too wide for one block, up to kTeam x 2048 columns. Past
+// that a CTA has the SM to itself and the exchange stands in the open (4096 x 20480 229 us against 242 for the wide
+// kernels; float32, 2048 x 20480, 250 against 192); below it one block is faster (8192 x 8192 96 us against 117).
+bool grad_team(int d, int type) { return type != WF_F32 && d % 8 == 0 && d > 8 * kMaxThreads && d <= kTeam * 2048; }
+int team_columns(int d) { return (d / 8 + kTeam - 1) / kTeam * 8; }
+
 // a block's threads for 8 values each, or the most there are
 int row_threads(int d) { return std::min(kMaxThreads, ((d + 7) / 8 + 31) / 32 * 32); }
+
+template <int T, int W>
+int dispatch_norm_unaligned(const NormArgs &a, cudaStream_t stream);
 
 template <int T, int W, int NC, bool VEC, bool WARP>
 int launch_norm(const NormArgs &a, cudaStream_t stream) {
@@ -849,9 +1046,13 @@ int launch_norm(const NormArgs &a, cudaStream_t stream) {
 
 template <int T, int W, bool VEC>
 int launch_norm_block(const NormArgs &a, cudaStream_t stream) {
-    if (!VEC && a.d <= 256) return launch_norm<T, W, 1, VEC, true>(a, stream);
+    if constexpr (!VEC) {
+        if (a.d <= 256) return launch_norm<T, W, 1, VEC, true>(a, stream);
+    }
     switch ((a.d + 8 * kMaxThreads - 1) / (8 * kMaxThreads)) {
-        case 1: return launch_norm<T, W, 1, VEC, false>(a, stream);
+        case 1:
+            if constexpr (VEC) return launch_norm<T, W, 1, VEC, false>(a, stream);
+            else return dispatch_norm_unaligned<T, W>(a, stream);
         case 2: return launch_norm<T, W, 2, VEC, false>(a, stream);
         case 3: return launch_norm<T, W, 3, VEC, false>(a, stream);
         default: break;
@@ -859,6 +1060,45 @@ int launch_norm_block(const NormArgs &a, cudaStream_t stream) {
     constexpr auto kern = layer_norm_wide_kernel<T, W>;
     const int grid = static_cast<int>(std::min<int64_t>(a.rows, wave_ctas_at<kern>(kMaxThreads)));
     return launch_rows(kern, dim3(grid), kMaxThreads, stream, a);
+}
+
+// blocks an SM of a kernel whose block's threads hold some 100 registers each
+int blocks_by_threads(int threads) { return std::max(1, std::min(8, 640 / threads)); }
+
+template <auto KERN>
+cudaError_t allow_smem(int bytes) {
+    static std::atomic<bool> ready[64];  // any host thread may launch first
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    if (ready[dev].load(std::memory_order_acquire)) return cudaSuccess;
+    e = cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) ready[dev].store(true, std::memory_order_release);
+    return e;
+}
+constexpr int kMostSmem = 200 * 1024;  // beside the kernels' static shared memory
+
+template <int T, int W, int R, int THREADS, int BLOCKS>
+int launch_norm_unaligned(const NormArgs &a, cudaStream_t stream) {
+    constexpr auto kern = layer_norm_unaligned_kernel<T, W, R, THREADS, BLOCKS>;
+    cudaError_t e = allow_smem<kern>(kMostSmem);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    const int threads = row_threads(a.d), smem = kRing * R * cover_bytes(a.d, T);
+    const int per_sm = std::max(1, std::min(blocks_by_threads(threads), 220 * 1024 / (smem + 2048)));
+    const RowSplit split = make_split(a.rows, a.rows_per_group, per_sm * device_sm_count(), R);
+    e = launch_dependent(kern, dim3(static_cast<unsigned>(split.blocks())), threads, smem, stream, a, split);
+    return static_cast<int>(e != cudaSuccess ? e : cudaGetLastError());
+}
+
+// R rows at a time: as many as the registers of so many threads hold, half as many of float32 (the ring's room)
+template <int T, int W>
+int dispatch_norm_unaligned(const NormArgs &a, cudaStream_t stream) {
+    constexpr int R = T == WF_F32 ? 2 : 4;
+    const int threads = row_threads(a.d);
+    if (threads <= 256) return launch_norm_unaligned<T, W, R, 256, 2>(a, stream);
+    if (threads <= 640) return launch_norm_unaligned<T, W, R / 2, 640, 1>(a, stream);
+    return launch_norm_unaligned<T, W, 1, kMaxThreads, 1>(a, stream);
 }
 
 template <int T, int W, int LPR>
@@ -873,24 +1113,17 @@ int launch_norm_narrow(const NormArgs &a, cudaStream_t stream) {
 template <int T, int W, int WPR>
 int launch_norm_stream(const NormArgs &a, cudaStream_t stream) {
     constexpr auto kern = layer_norm_stream_kernel<T, W, WPR>;
-    constexpr int most = 200 * 1024;
+    constexpr int most = kMostSmem;
     const int64_t row = static_cast<int64_t>(a.d) * dtype_size(T) * (8 / WPR), params = 2ll * a.d * dtype_size(W);
     const bool params_fit = params + 2 * row <= most;
     const int bufs = static_cast<int>(std::max<int64_t>(2, std::min<int64_t>(4, (64 * 1024 - (params_fit ? params : 0)) / row)));
-    static std::atomic<bool> ready[64];  // any host thread may launch first
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (dev < 0 || dev >= 64) return WF_ERR_DEVICE;
-    if (!ready[dev].load(std::memory_order_acquire)) {
-        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
-        if (e != cudaSuccess) return static_cast<int>(e);
-        ready[dev].store(true, std::memory_order_release);
-    }
+    cudaError_t e = allow_smem<kern>(most);
+    if (e != cudaSuccess) return static_cast<int>(e);
     const bool stage = (a.w != nullptr || a.b != nullptr) && params_fit && std::min(a.rows_per_group, a.rows) >= kStageRows;
     const int64_t smem = bufs * row + (stage ? params : 0);
     const int64_t resident = std::max<int64_t>(1, std::min<int64_t>(6, 220 * 1024 / (smem + 1024))) * device_sm_count();
     const RowSplit split = make_split(a.rows, a.rows_per_group, resident, 8 / WPR);
-    const cudaError_t e = launch_dependent(kern, dim3(static_cast<unsigned>(split.blocks())), 256, smem, stream, a, split, bufs, stage);
+    e = launch_dependent(kern, dim3(static_cast<unsigned>(split.blocks())), 256, smem, stream, a, split, bufs, stage);
     return static_cast<int>(e != cudaSuccess ? e : cudaGetLastError());
 }
 
@@ -931,21 +1164,23 @@ int launch_norm_grad_wide(const NormGradArgs &a, cudaStream_t stream) {
     return rc;
 }
 
-template <int T, int W, int V, int R, int THREADS, int BLOCKS>
+template <int T, int W, int V, int R, int THREADS, int BLOCKS, bool TEAM>
 int launch_norm_grad_rows(const NormGradArgs &a, int threads, cudaStream_t stream) {
-    constexpr auto kern = layer_norm_grad_rows_kernel<T, W, V, R, THREADS, BLOCKS>;
+    constexpr auto kern = layer_norm_grad_rows_kernel<T, W, V, R, THREADS, BLOCKS, TEAM>;
     constexpr int per_thread = kRing * R * 2 * V * dtype_size(T);
-    static std::atomic<bool> ready[64];  // any host thread may launch first
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (dev < 0 || dev >= 64) return WF_ERR_DEVICE;
-    if (!ready[dev].load(std::memory_order_acquire)) {
-        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, THREADS * per_thread);
-        if (e != cudaSuccess) return static_cast<int>(e);
-        ready[dev].store(true, std::memory_order_release);
-    }
-    const cudaError_t e = launch_dependent(kern, dim3(static_cast<unsigned>(a.split.blocks())), threads,
-                                           static_cast<size_t>(threads) * per_thread, stream, a);
+    cudaError_t e = allow_smem<kern>(THREADS * per_thread);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    e = launch_dependent_clusters(kern, dim3(static_cast<unsigned>(a.split.blocks() * (TEAM ? kTeam : 1))), TEAM ? kTeam : 0,
+                                  threads, static_cast<size_t>(threads) * per_thread, stream, a);
+    return static_cast<int>(e != cudaSuccess ? e : cudaGetLastError());
+}
+
+template <int T, int W, int R, int THREADS, int BLOCKS>
+int launch_norm_grad_unaligned(const NormGradArgs &a, cudaStream_t stream) {
+    constexpr auto kern = layer_norm_grad_unaligned_kernel<T, W, R, THREADS, BLOCKS>;
+    cudaError_t e = allow_smem<kern>(kMostSmem);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    e = launch_dependent(kern, dim3(static_cast<unsigned>(a.split.blocks())), row_threads(a.d), kRing * R * 2 * cover_bytes(a.d, T), stream, a);
     return static_cast<int>(e != cudaSuccess ? e : cudaGetLastError());
 }
 
@@ -955,21 +1190,32 @@ int dispatch_norm_grad(const NormGradArgs &a, cudaStream_t stream) {
                      vec_ok(a.dx, a.lddx, dtype_size(T)) && vec_ok(a.w, a.d, dtype_size(W)) && vec_ok(a.part_w, a.d, 4) &&
                      vec_ok(a.part_b, a.d, 4);
     const dim3 grid(static_cast<unsigned>(a.split.blocks()));
+    if constexpr (T != WF_F32) {
+        if (vec && grad_team(a.d, T))
+            return launch_norm_grad_rows<T, W, 8, 4, 256, 2, true>(a, grad_threads(a.block_cols, T), stream);
+    }
     if (a.d > 8 * kMaxThreads) return vec ? launch_norm_grad_wide<T, W, true>(a, stream) : launch_norm_grad_wide<T, W, false>(a, stream);
     if (a.d <= 256) {
-        if (!vec) return launch_rows(layer_norm_grad_kernel<T, W, true>, grid, 256, stream, a);
+        if (!vec) return launch_rows(layer_norm_grad_warp_kernel<T, W>, grid, 256, stream, a);
         if (a.d <= 32) return launch_rows(layer_norm_grad_narrow_kernel<T, W, 4>, grid, 256, stream, a);
         if (a.d <= 64) return launch_rows(layer_norm_grad_narrow_kernel<T, W, 8>, grid, 256, stream, a);
         if (a.d <= 128) return launch_rows(layer_norm_grad_narrow_kernel<T, W, 16>, grid, 256, stream, a);
         return launch_rows(layer_norm_grad_narrow_kernel<T, W, 32>, grid, 256, stream, a);
     }
-    if (!vec) return launch_rows(layer_norm_grad_kernel<T, W, false>, grid, row_threads(a.d), stream, a);
+    if (!vec) {  // R as in the forward pass
+        constexpr int R = T == WF_F32 ? 2 : 4;
+        if (row_threads(a.d) <= 256) return launch_norm_grad_unaligned<T, W, R, 256, 2>(a, stream);
+        if (row_threads(a.d) <= 640) return launch_norm_grad_unaligned<T, W, R / 2, 640, 1>(a, stream);
+        return launch_norm_grad_unaligned<T, W, 1, kMaxThreads, 1>(a, stream);
+    }
     constexpr int V = T == WF_F32 ? 4 : 8;  // 16 bytes a thread; float32 rows past 4096 values take 32
     const int threads = grad_threads(a.d, T);
-    if (T == WF_F32 && a.d > V * kMaxThreads) return launch_norm_grad_rows<T, W, 8, 1, kMaxThreads, 1>(a, threads, stream);
-    if (threads <= 256) return launch_norm_grad_rows<T, W, V, 4, 256, 2>(a, threads, stream);
-    if (threads <= 640) return launch_norm_grad_rows<T, W, V, 2, 640, 1>(a, threads, stream);
-    return launch_norm_grad_rows<T, W, V, 1, kMaxThreads, 1>(a, threads, stream);
+    if constexpr (T == WF_F32) {
+        if (a.d > V * kMaxThreads) return launch_norm_grad_rows<T, W, 8, 1, kMaxThreads, 1, false>(a, threads, stream);
+    }
+    if (threads <= 256) return launch_norm_grad_rows<T, W, V, 4, 256, 2, false>(a, threads, stream);
+    if (threads <= 640) return launch_norm_grad_rows<T, W, V, 2, 640, 1, false>(a, threads, stream);
+    return launch_norm_grad_rows<T, W, V, 1, kMaxThreads, 1, false>(a, threads, stream);
 }
 
 bool norm_types_ok(int type, int w_type) {
@@ -979,9 +1225,10 @@ bool norm_types_ok(int type, int w_type) {
 // The shares of the rows that the backward pass's blocks take: about as many as are resident at once.
 RowSplit norm_split(int64_t rows, int64_t rows_per_group, int d, int type) {
     const int64_t sms = device_sm_count();
+    if (grad_team(d, type)) return make_split(rows, rows_per_group, std::max<int64_t>(1, blocks_by_threads(grad_threads(team_columns(d), type)) * sms / kTeam), 4);
     if (d > 8 * kMaxThreads) return make_split(rows, rows_per_group, std::max<int64_t>(1, 4 * sms * 2048 / d), 16);
     if (d <= 256) return make_split(rows, rows_per_group, 3 * sms, 16);
-    return make_split(rows, rows_per_group, sms * std::max(1, std::min(8, 640 / (d % 8 == 0 ? grad_threads(d, type) : row_threads(d)))), 4);
+    return make_split(rows, rows_per_group, sms * blocks_by_threads(d % 8 == 0 ? grad_threads(d, type) : row_threads(d)), 4);
 }
 
 }  // namespace
@@ -1031,6 +1278,7 @@ extern "C" WF_API int wf_layer_norm_backward(const wf_layer_norm_grad_args *args
     if (!g.dx && !g.dw && !g.db) return WF_OK;
     const RowSplit split = norm_split(g.rows, g.rows_per_group, static_cast<int>(g.d), g.type);
     const int64_t half = split.partial_rows() * g.d;
+    const int d = static_cast<int>(g.d);
     if ((g.dw || g.db) && (!g.workspace || !aligned_to(g.workspace, 16) ||
                            g.workspace_bytes < 2 * half * static_cast<int64_t>(sizeof(float))))
         return WF_ERR_ARG;
@@ -1038,7 +1286,7 @@ extern "C" WF_API int wf_layer_norm_backward(const wf_layer_norm_grad_args *args
     if (rc != WF_OK) return rc;
     float *part = static_cast<float *>(g.workspace);
     const NormGradArgs a{g.x, g.w, g.dy, g.mean, g.rstd, g.dx, g.dw ? part : nullptr, g.db ? part + half : nullptr, g.rows,
-                         g.ldx, g.lddy, g.lddx, split, static_cast<int>(g.d)};
+                         g.ldx, g.lddy, g.lddx, split, d, grad_team(d, g.type) ? team_columns(d) : d};
     const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     if (g.type == WF_F32) rc = dispatch_norm_grad<WF_F32, WF_F32>(a, st);
     else if (g.type == WF_BF16) rc = g.w_type == WF_F32 ? dispatch_norm_grad<WF_BF16, WF_F32>(a, st) : dispatch_norm_grad<WF_BF16, WF_BF16>(a, st);

@@ -67,6 +67,20 @@ def test_groups(cuda, m, rpg, d):
     _compare(torch, data, dy, rpg=rpg)
 
 
+@pytest.mark.parametrize("m,rpg", [(1, 1), (300, 75), (301, 300), (64, 3)])
+@pytest.mark.parametrize("d", [8200, 12288, 12296, 16384, 16392])
+def test_rows_shared_by_clusters(cuda, m, rpg, d):
+    import torch
+    for wdtype in (torch.float16, torch.float32):
+        data, dy = _data(torch, m, d, torch.float16, wdtype, groups=-(-m // rpg))
+        _compare(torch, data, dy, rpg=rpg)
+    # the gradients of w and b alone take no exchange
+    fn, want = wf("enhancers.fused_norm"), norm_reference(data["x"], data["weight"], data["bias"], 1e-6, rpg, dy)
+    y = fn.layer_norm(data["x"].detach(), data["weight"], data["bias"], 1e-6, rpg)
+    for nm, got in zip(("weight", "bias"), torch.autograd.grad(y, (data["weight"], data["bias"]), dy)):
+        assert_within(got, want[nm], nm)
+
+
 def test_without_weight_or_bias(cuda):
     import torch
     for d in (40, 1001, 2048):
