@@ -364,6 +364,7 @@ Tensor layer_norm(const Tensor &x, const MaybeTensor &weight, const MaybeTensor 
 }  // namespace
 
 PYBIND11_MODULE(wf_torch, m) {
-    m.def("linear", &linear);
-    m.def("layer_norm", &layer_norm);
+    // wrapped: PyTorch's own errors keep their types, an allocation that fails is a torch.OutOfMemoryError
+    m.def("linear", torch::wrap_pybind_function(&linear));
+    m.def("layer_norm", torch::wrap_pybind_function(&layer_norm));
 }

@@ -79,25 +79,25 @@ __device__ __forceinline__ void act_slope2(const float (&v)[2], float (&h)[2], f
             h[i] = v[i] * c[i];
             slope[i] = fmaf(v[i] * kInvSqrt2Pi, fast_exp(-0.5f * v[i] * v[i]), c[i]);
         }
-        return;
-    }
+    } else {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        if constexpr (ACT == WF_ACT_RELU) {
-            h[i] = v[i] < 0.f ? 0.f : v[i];
-            slope[i] = v[i] > 0.f ? 1.f : 0.f;
-        } else if constexpr (ACT == WF_ACT_SILU) {
-            const float p = sigmoid(v[i]);
-            h[i] = v[i] * p;
-            slope[i] = fmaf(h[i], 1.f - p, p);
-        } else if constexpr (ACT == WF_ACT_GELU_TANH) {
-            const float v2 = v[i] * v[i], p = sigmoid(2.0f * kSqrt2OverPi * fmaf(kGeluCubic * v2, v[i], v[i]));
-            h[i] = v[i] * p;
-            // past |v| = 1e4 the slope is p alone; the square must not overflow to 0 * infinity
-            slope[i] = fmaf(h[i] * (1.f - p), 2.0f * kSqrt2OverPi * fmaf(3.0f * kGeluCubic, fminf(v2, 1e8f), 1.f), p);
-        } else {
-            h[i] = v[i];
-            slope[i] = 1.f;
+        for (int i = 0; i < 2; ++i) {
+            if constexpr (ACT == WF_ACT_RELU) {
+                h[i] = v[i] < 0.f ? 0.f : v[i];
+                slope[i] = v[i] > 0.f ? 1.f : 0.f;
+            } else if constexpr (ACT == WF_ACT_SILU) {
+                const float p = sigmoid(v[i]);
+                h[i] = v[i] * p;
+                slope[i] = fmaf(h[i], 1.f - p, p);
+            } else if constexpr (ACT == WF_ACT_GELU_TANH) {
+                const float v2 = v[i] * v[i], p = sigmoid(2.0f * kSqrt2OverPi * fmaf(kGeluCubic * v2, v[i], v[i]));
+                h[i] = v[i] * p;
+                // past |v| = 1e4 the slope is p alone; the square must not overflow to 0 * infinity
+                slope[i] = fmaf(h[i] * (1.f - p), 2.0f * kSqrt2OverPi * fmaf(3.0f * kGeluCubic, fminf(v2, 1e8f), 1.f), p);
+            } else {
+                h[i] = v[i];
+                slope[i] = 1.f;
+            }
         }
     }
 }
