@@ -152,6 +152,13 @@ __device__ __forceinline__ float lanes_sum_many(float (&v)[N], int lane) {
     return s;
 }
 
+// NV values a lane, 32 columns apart
+template <int T, int NV>
+__device__ __forceinline__ void load_lanes(float (&v)[NV], const void *row, int lane, int d) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) v[j] = j * 32 + lane < d ? load1<T>(row, j * 32 + lane) : 0.f;
+}
+
 struct NormArgs {
     const void *x, *w, *b;
     void *y;
@@ -161,18 +168,14 @@ struct NormArgs {
     float eps;
 };
 
-// One row a block (threads = the block), or one row a warp (blocks of several warps, threads = 32). NC chunks of 8
-// values a thread.
-template <int T, int W, int NC, bool VEC, bool WARP>
+// One row a block, NC chunks of 8 values a thread.
+template <int T, int W, int NC, bool VEC>
 __global__ void __launch_bounds__(kMaxThreads) layer_norm_kernel(const __grid_constant__ NormArgs a) {
     __shared__ float red[2][32];
-    const int threads = WARP ? 32 : blockDim.x, tid = WARP ? (threadIdx.x & 31) : threadIdx.x;
-    const int warps = WARP ? 1 : (blockDim.x >> 5);
-    const int64_t step = WARP ? static_cast<int64_t>(gridDim.x) * (blockDim.x >> 5) : gridDim.x;
+    const int threads = blockDim.x, tid = threadIdx.x, warps = blockDim.x >> 5;
     const float inv_d = 1.0f / static_cast<float>(a.d);
     wait_prior_grid();
-    for (int64_t row = WARP ? static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
-         row < a.rows; row += step) {
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const void *xr = row_of<T>(a.x, row, a.ldx);
         float x[NC][8];
         float s[1] = {0.f};
@@ -252,6 +255,59 @@ __global__ void __launch_bounds__(kMaxThreads) layer_norm_wide_kernel(const __gr
             if (a.w != nullptr) v *= load1<W>(row_of<W>(a.w, grp, a.d), col);
             if (a.b != nullptr) v += load1<W>(row_of<W>(a.b, grp, a.d), col);
             store1<T>(yr, col, v);
+        }
+    }
+}
+
+// Narrow rows (up to 32 NV values) that 16-byte accesses do not fit, value by value: 8 / NV rows a warp at a time.
+template <int T, int W, int NV>
+__global__ void __launch_bounds__(256) layer_norm_warp_kernel(const __grid_constant__ NormArgs a) {
+    constexpr int R = 8 / NV, L = 32 / R;  // lanes that hold the same sum
+    const int lane = threadIdx.x & 31;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * 8 * R;
+    const float inv_d = 1.0f / static_cast<float>(a.d);
+    wait_prior_grid();
+    for (int64_t row = (static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5)) * R; row < a.rows; row += step) {
+        float v[R][NV], s[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            load_lanes<T, NV>(v[r], row_of<T>(a.x, row + r, a.ldx), lane, row + r < a.rows ? a.d : 0);
+            s[r] = 0.f;
+#pragma unroll
+            for (int j = 0; j < NV; ++j) s[r] += v[r][j];
+        }
+        const float mean = lanes_sum_many<R>(s, lane) * inv_d;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const float mu = __shfl_sync(0xFFFFFFFFu, mean, r * L);
+            s[r] = 0.f;
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                v[r][j] -= mu;
+                if (j * 32 + lane < a.d) s[r] = fmaf(v[r][j], v[r][j], s[r]);
+            }
+        }
+        const float rstd = rsqrtf(fmaf(lanes_sum_many<R>(s, lane), inv_d, a.eps));
+        if (a.mean != nullptr && (lane & (L - 1)) == 0 && row + lane / L < a.rows) {
+            a.mean[row + lane / L] = mean;
+            a.rstd[row + lane / L] = rstd;
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const float rs = __shfl_sync(0xFFFFFFFFu, rstd, r * L);
+            if (row + r >= a.rows) continue;
+            const int64_t grp = a.w != nullptr || a.b != nullptr ? (row + r) / a.rows_per_group : 0;
+            const void *w = row_of<W>(a.w, grp, a.d), *b = row_of<W>(a.b, grp, a.d);
+            void *y = row_of<T>(a.y, row + r, a.ldy);
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int col = j * 32 + lane;
+                if (col >= a.d) continue;
+                float f = v[r][j] * rs;
+                if (a.w != nullptr) f *= load1<W>(w, col);
+                if (a.b != nullptr) f += load1<W>(b, col);
+                store1<T>(y, col, f);
+            }
         }
     }
 }
@@ -347,9 +403,9 @@ __device__ __forceinline__ void param_piece(uint64_t (&p)[T == WF_F32 ? 2 : 4], 
 // Many wider rows that 16-byte accesses fit: a team of WPR warps a row. Each thread copies its own 16-byte pieces of the
 // team's next rows into a ring in shared memory (cp.async) and reads nobody else's, so that rows stream in without a
 // barrier and without registers (a row held in registers, widened three times, needed 234 of them for 5120 values and
-// left 8 warps an SM: 16384 x 5120 took 84 us where this takes 62). A block takes a run of rows (RowSplit) and keeps their group's w and b
-// in shared memory: read from L2 for every row they cost more than x itself (16384 x 5120 bf16 in 16 groups: 222 us).
-// Groups of fewer than kStageRows rows are read from L2 all the same.
+// left 8 warps an SM: 16384 x 5120 took 84 us where this takes 62). A block takes a run of rows (RowSplit) and keeps their
+// group's w and b in shared memory: read from L2 for every row they cost more than x itself (16384 x 5120 bf16 in 16
+// groups: 222 us). Groups of fewer than kStageRows rows are read from L2 all the same.
 constexpr int kStageRows = 16;
 template <int T, int W, int WPR>
 __global__ void __launch_bounds__(256) layer_norm_stream_kernel(const __grid_constant__ NormArgs a,
@@ -466,16 +522,27 @@ __global__ void __launch_bounds__(256) layer_norm_stream_kernel(const __grid_con
     }
 }
 
-// The sums of N values (a power of 2) over the block's threads: sum k in the lanes k, k + N, ... of every warp. One barrier;
-// two calls in a row take different buffers.
-template <int N>
+// The sums of N values (a power of 2) over the block's threads, or (TEAM) over those of a cluster of kTeam CTAs: sum k in the
+// lanes k, k + N, ... of every warp. One barrier; two calls in a row take different buffers. In a cluster every warp writes
+// its sums to all CTAs (distributed shared memory): nothing is written after a barrier that a CTA leaves behind.
+template <int N, bool TEAM>
 __device__ __forceinline__ float block_sums(float (&v)[N], float (*red)[N], int warp, int lane, int warps) {
     constexpr int L = 32 / N;  // lanes that hold the same sum
     const float mine = lanes_sum_many<N>(v, lane);
-    if ((lane & (L - 1)) == 0) red[warp][lane / L] = mine;
-    __syncthreads();
+    int all = warps;
+    if constexpr (TEAM) {
+        all = warps * kTeam;
+        const uint32_t at = smem_u32(&red[cluster_rank() * warps + warp][lane / L]);
+        for (int to = lane & (L - 1); to < kTeam; to += L)
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(map_to_rank(at, to)), "f"(mine) : "memory");
+        __syncwarp();
+        cluster_sync();
+    } else {
+        if ((lane & (L - 1)) == 0) red[warp][lane / L] = mine;
+        __syncthreads();
+    }
     float t = 0.f;
-    for (int i = lane / N; i < warps; i += L) t += red[i][lane % N];
+    for (int i = lane / N; i < all; i += L) t += red[i][lane % N];
 #pragma unroll
     for (int o = N; o < 32; o *= 2) t += __shfl_xor_sync(0xFFFFFFFFu, t, o);
     return t;
@@ -485,7 +552,7 @@ __device__ __forceinline__ float block_sums(float (&v)[N], float (*red)[N], int 
 // and values are read one by one from where its first byte falls in them. What a piece holds before the row is copied with
 // it and never read (the piece holds a byte of the row, so it lies in its allocation); nothing past the row is read.
 // Single values copied straight from HBM keep too few bytes in flight (16384 x 5119
-// bf16: forward 186 us and backward 346, where these take 134 and 182).
+// bf16: forward 186 us and backward 346, where these take 133 and 176).
 __host__ __device__ inline int cover_bytes(int d, int type) { return (d * dtype_size(type) + 15) / 16 * 16 + 16; }
 __device__ __forceinline__ int skew(const void *row) { return static_cast<int>(reinterpret_cast<uintptr_t>(row) & 15); }
 __device__ __forceinline__ void copy_cover(char *dst, const void *row, int bytes, int tid, int threads) {
@@ -496,32 +563,37 @@ __device__ __forceinline__ void copy_cover(char *dst, const void *row, int bytes
                      : "memory");
 }
 
-// The forward pass of rows of 257 to 8192 values that 16-byte accesses do not fit: eight values a thread, with their w and b
-// in registers, R rows at a time through a ring of such copies; one barrier a sum.
+// The forward pass of rows of 257 to 16384 values that 16-byte accesses do not fit: eight values a thread, with their w and b
+// in registers, R rows at a time through a ring of such copies; one barrier a sum. TEAM: a cluster of kTeam CTAs shares
+// the rows, each CTA a run of columns.
 constexpr int kRing = 3;
-template <int T, int W, int R, int THREADS, int BLOCKS>
+template <int T, int W, int R, int THREADS, int BLOCKS, bool TEAM>
 __global__ void __launch_bounds__(THREADS, BLOCKS) layer_norm_unaligned_kernel(const __grid_constant__ NormArgs a,
-                                                                               const __grid_constant__ RowSplit split) {
+                                                                               const __grid_constant__ RowSplit split, int block_cols) {
     extern __shared__ uint4 smem[];
-    __shared__ float red[2][32][R];
+    __shared__ float red[2][TEAM ? kTeam * THREADS / 32 : 32][R];
     const int tid = threadIdx.x, threads = blockDim.x, warp = tid >> 5, lane = tid & 31, warps = threads >> 5;
-    const int cover = cover_bytes(a.d, T), bytes = a.d * dtype_size(T);
+    const int64_t col0 = TEAM ? cluster_rank() * block_cols : 0, share = TEAM ? blockIdx.x / kTeam : blockIdx.x;
+    const int d = TEAM ? min(block_cols, a.d - static_cast<int>(col0)) : a.d;  // this CTA's columns, from col0
+    const int cover = cover_bytes(block_cols, T), bytes = d * dtype_size(T);
     char *ring = reinterpret_cast<char *>(smem);
     const float inv_d = 1.0f / static_cast<float>(a.d);
+    auto x_row = [&](int64_t row) { return row_of<T>(a.x, row, a.ldx, col0); };
+    if constexpr (TEAM) cluster_sync();  // every CTA of the team runs before another writes to its shared memory
     wait_prior_grid();
-    for (int64_t grp = split.first_group(blockIdx.x), end = split.last_group(blockIdx.x); grp < end; ++grp) {
+    for (int64_t grp = split.first_group(share), end = split.last_group(share); grp < end; ++grp) {
         int64_t lo, hi;
-        split.rows_of(blockIdx.x, grp, lo, hi);
+        split.rows_of(share, grp, lo, hi);
         auto fetch = [&](int64_t row, int slot) {
 #pragma unroll
             for (int r = 0; r < R; ++r)
-                if (row + r < hi) copy_cover(ring + (slot * R + r) * cover, row_of<T>(a.x, row + r, a.ldx), bytes, tid, threads);
+                if (row + r < hi) copy_cover(ring + (slot * R + r) * cover, x_row(row + r), bytes, tid, threads);
             cp_async_commit();
         };
         for (int i = 0; i < kRing; ++i) fetch(lo + i * R, i);
         float w[8], b[8];
-        if (a.w != nullptr) load_chunk<W, false>(w, row_of<W>(a.w, grp, a.d), 0, tid, threads, a.d);
-        if (a.b != nullptr) load_chunk<W, false>(b, row_of<W>(a.b, grp, a.d), 0, tid, threads, a.d);
+        if (a.w != nullptr) load_chunk<W, false>(w, row_of<W>(a.w, grp, a.d, col0), 0, tid, threads, d);
+        if (a.b != nullptr) load_chunk<W, false>(b, row_of<W>(a.b, grp, a.d, col0), 0, tid, threads, d);
         cp_async_wait<kRing - 1>();
         __syncthreads();
         int slot = 0;
@@ -529,14 +601,13 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) layer_norm_unaligned_kernel(c
             float v[R][8], s[R];
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                const char *x = ring + (slot * R + r) * cover + skew(row_of<T>(a.x, row + r, a.ldx));
-                load_chunk<T, false>(v[r], x, 0, tid, threads, a.d);
+                load_chunk<T, false>(v[r], ring + (slot * R + r) * cover + skew(x_row(row + r)), 0, tid, threads, d);
                 s[r] = 0.f;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) s[r] += v[r][j];
             }
             cp_async_wait<kRing - 2>();  // the next rows are here for this thread, and behind the barrier for all
-            const float mean = block_sums<R>(s, red[0], warp, lane, warps) * inv_d;
+            const float mean = block_sums<R, TEAM>(s, red[0], warp, lane, warps) * inv_d;
             fetch(row + kRing * R, slot);  // every thread has read this slot
             if (++slot == kRing) slot = 0;
 #pragma unroll
@@ -546,11 +617,11 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) layer_norm_unaligned_kernel(c
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     v[r][j] -= mu;
-                    if (column<false>(0, j, tid, threads) < a.d) s[r] = fmaf(v[r][j], v[r][j], s[r]);
+                    if (column<false>(0, j, tid, threads) < d) s[r] = fmaf(v[r][j], v[r][j], s[r]);
                 }
             }
-            const float rstd = rsqrtf(fmaf(block_sums<R>(s, red[1], warp, lane, warps), inv_d, a.eps));
-            if (a.mean != nullptr && tid < R && row + tid < hi) {
+            const float rstd = rsqrtf(fmaf(block_sums<R, TEAM>(s, red[1], warp, lane, warps), inv_d, a.eps));
+            if (a.mean != nullptr && col0 == 0 && tid < R && row + tid < hi) {
                 a.mean[row + tid] = mean;
                 a.rstd[row + tid] = rstd;
             }
@@ -564,7 +635,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) layer_norm_unaligned_kernel(c
                     if (a.w != nullptr) v[r][j] *= w[j];
                     if (a.b != nullptr) v[r][j] += b[j];
                 }
-                store_chunk<T, false>(v[r], row_of<T>(a.y, row + r, a.ldy), 0, tid, threads, a.d);
+                store_chunk<T, false>(v[r], row_of<T>(a.y, row + r, a.ldy, col0), 0, tid, threads, d);
             }
         }
     }
@@ -584,9 +655,8 @@ struct NormGradArgs {
 // The backward pass of rows that 16-byte accesses fit, V (8 or 4) values a thread of a block: R rows at a time, whose 2 R sums
 // share one barrier (and their shuffles: lanes_sum_many). Each thread copies its own values of the next rows into a ring
 // of kRing stages in shared memory (cp.async) and reads nobody else's: the loads run on behind the barrier.
-// TEAM: a cluster of kTeam CTAs shares the rows, each CTA a run of a.block_cols columns; every warp writes its sums to all of
-// them (distributed shared memory) and the cluster's barrier takes the block's place: 4096 x 12288 bf16 109 us where the wide
-// kernels, which read x and dy once more, take 157; 4096 x 16384 151 us against 190.
+// TEAM: a cluster of kTeam CTAs shares the rows, each CTA a run of a.block_cols columns: the wide kernels
+// read x and dy once more.
 template <int T, int W, int V, int R, int THREADS, int BLOCKS, bool TEAM>
 __global__ void __launch_bounds__(THREADS, BLOCKS) layer_norm_grad_rows_kernel(const __grid_constant__ NormGradArgs a) {
     constexpr int H = V * dtype_size(T) / 16, NP = V / 2;  // 16-byte pieces and pairs of V values
@@ -673,25 +743,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) layer_norm_grad_rows_kernel(c
                 s[2 * r + 1] = sum_f2(s1);
             }
             if (a.dx != nullptr) {
-                // every warp's sums to shared memory, then every warp adds all of them
-                constexpr int L = 32 / (2 * R);  // lanes that hold the same sum
-                const float mine = lanes_sum_many<2 * R>(s, lane);
-                if constexpr (TEAM) {
-                    // no CTA leaves before the last barrier, and nothing is written after it
-                    const uint32_t at = smem_u32(&red[buf][rank * warps + warp][lane / L]);
-                    for (int to = lane & (L - 1); to < kTeam; to += L)
-                        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(map_to_rank(at, to)), "f"(mine) : "memory");
-                    __syncwarp();
-                    cluster_sync();
-                } else {
-                    if ((lane & (L - 1)) == 0) red[buf][warp][lane / L] = mine;
-                    __syncthreads();
-                }
-                float t = 0.f;  // sum lane % (2 R), of the warps lane / (2 R), + 32 / (2 R), ...
-                const int all = TEAM ? warps * kTeam : warps;
-                for (int i = lane / (2 * R); i < all; i += L) t += red[buf][i][lane % (2 * R)];
-#pragma unroll
-                for (int o = 2 * R; o < 32; o *= 2) t += __shfl_xor_sync(0xFFFFFFFFu, t, o);
+                const float t = block_sums<2 * R, TEAM>(s, red[buf], warp, lane, warps);
                 buf ^= 1;
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
@@ -809,43 +861,57 @@ __global__ void __launch_bounds__(256, 3) layer_norm_grad_narrow_kernel(const __
     }
 }
 
-// The same for narrow rows that 16-byte accesses do not fit, value by value: a row a warp. Each warp of the block takes every
-// eighth row of the share, and the warps' column sums are added at the end through shared memory.
-template <int T, int W>
+// The same for narrow rows (up to 32 NV values) that 16-byte accesses do not fit, value by value: 8 / NV rows a warp at a time,
+// and the warps' column sums are added at the end through shared memory.
+template <int T, int W, int NV>
 __global__ void __launch_bounds__(256) layer_norm_grad_warp_kernel(const __grid_constant__ NormGradArgs a) {
-    __shared__ float col_red[8][8][32];
+    constexpr int R = 8 / NV;
+    __shared__ float col_red[8][NV][32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const float inv_d = 1.0f / static_cast<float>(a.d);
     wait_prior_grid();
     for (int64_t grp = a.split.first_group(blockIdx.x), end = a.split.last_group(blockIdx.x); grp < end; ++grp) {
         int64_t lo, hi;
         a.split.rows_of(blockIdx.x, grp, lo, hi);
-        float w[8], dw[8], db[8];
-        if (a.w != nullptr) load_chunk<W, false>(w, row_of<W>(a.w, grp, a.d), 0, lane, 32, a.d);
+        float w[NV], dw[NV], db[NV];
+        if (a.w != nullptr) load_lanes<W, NV>(w, row_of<W>(a.w, grp, a.d), lane, a.d);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < NV; ++j) {
             dw[j] = db[j] = 0.f;
             if (a.w == nullptr) w[j] = 1.f;
         }
-        for (int64_t row = lo + warp; row < hi; row += 8) {
-            const float mean = a.mean[row], rstd = a.rstd[row];
-            float xh[8], dy[8], s0 = 0.f, s1 = 0.f;
-            load_chunk<T, false>(xh, row_of<T>(a.x, row, a.ldx), 0, lane, 32, a.d);
-            load_chunk<T, false>(dy, row_of<T>(a.dy, row, a.lddy), 0, lane, 32, a.d);
+        for (int64_t row = lo + warp * R; row < hi; row += 8 * R) {
+            float xh[R][NV], u[R][NV], s[2 * R], rstd[R];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                xh[j] = (xh[j] - mean) * rstd;  // dy is 0 past the row's end
-                db[j] += dy[j];
-                dw[j] = fmaf(dy[j], xh[j], dw[j]);
-                dy[j] *= w[j];
-                s0 += dy[j];
-                s1 = fmaf(dy[j], xh[j], s1);
+            for (int r = 0; r < R; ++r) {
+                const int d = row + r < hi ? a.d : 0;
+                const float mean = d ? a.mean[row + r] : 0.f;
+                rstd[r] = d ? a.rstd[row + r] : 0.f;
+                load_lanes<T, NV>(xh[r], row_of<T>(a.x, row + r, a.ldx), lane, d);
+                load_lanes<T, NV>(u[r], row_of<T>(a.dy, row + r, a.lddy), lane, d);
+                s[2 * r] = s[2 * r + 1] = 0.f;
+#pragma unroll
+                for (int j = 0; j < NV; ++j) {
+                    xh[r][j] = (xh[r][j] - mean) * rstd[r];  // dy is 0 past the row's end
+                    db[j] += u[r][j];
+                    dw[j] = fmaf(u[r][j], xh[r][j], dw[j]);
+                    u[r][j] *= w[j];
+                    s[2 * r] += u[r][j];
+                    s[2 * r + 1] = fmaf(u[r][j], xh[r][j], s[2 * r + 1]);
+                }
             }
             if (a.dx == nullptr) continue;
-            const float m0 = warp_sum(s0) * inv_d, m1 = warp_sum(s1) * inv_d;
+            constexpr int L = 32 / (2 * R);
+            const float mean_u = lanes_sum_many<2 * R>(s, lane) * inv_d;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) dy[j] = rstd * (dy[j] - m0 - xh[j] * m1);
-            store_chunk<T, false>(dy, row_of<T>(a.dx, row, a.lddx), 0, lane, 32, a.d);
+            for (int r = 0; r < R; ++r) {
+                const float m0 = __shfl_sync(0xFFFFFFFFu, mean_u, 2 * r * L), m1 = __shfl_sync(0xFFFFFFFFu, mean_u, (2 * r + 1) * L);
+                if (row + r >= hi) continue;
+                void *dx = row_of<T>(a.dx, row + r, a.lddx);
+#pragma unroll
+                for (int j = 0; j < NV; ++j)
+                    if (j * 32 + lane < a.d) store1<T>(dx, j * 32 + lane, rstd[r] * (u[r][j] - m0 - xh[r][j] * m1));
+            }
         }
         const int64_t part = a.split.partial_row(blockIdx.x, grp) * a.d;
 #pragma unroll
@@ -854,7 +920,7 @@ __global__ void __launch_bounds__(256) layer_norm_grad_warp_kernel(const __grid_
             if (dst == nullptr) continue;
             __syncthreads();
 #pragma unroll
-            for (int j = 0; j < 8; ++j) col_red[warp][j][lane] = which ? db[j] : dw[j];
+            for (int j = 0; j < NV; ++j) col_red[warp][j][lane] = which ? db[j] : dw[j];
             __syncthreads();
             if (static_cast<int>(threadIdx.x) < a.d) {  // column 32 j + lane
                 float v = 0.f;
@@ -867,33 +933,38 @@ __global__ void __launch_bounds__(256) layer_norm_grad_warp_kernel(const __grid_
 }
 
 // ... and for 257 to 8192 values: eight values a thread, R rows at a time through a ring of unaligned copies, one barrier for
-// the rows' 2 R sums.
-template <int T, int W, int R, int THREADS, int BLOCKS>
+// the rows' 2 R sums. TEAM: a cluster shares the rows.
+template <int T, int W, int R, int THREADS, int BLOCKS, bool TEAM>
 __global__ void __launch_bounds__(THREADS, BLOCKS) layer_norm_grad_unaligned_kernel(const __grid_constant__ NormGradArgs a) {
     extern __shared__ uint4 smem[];  // [kRing][R][x, dy][cover]
-    __shared__ float red[2][32][2 * R];
+    __shared__ float red[2][TEAM ? kTeam * THREADS / 32 : 32][2 * R];
     const int tid = threadIdx.x, threads = blockDim.x, warp = tid >> 5, lane = tid & 31, warps = threads >> 5;
-    const int cover = cover_bytes(a.d, T), bytes = a.d * dtype_size(T);
+    const int64_t col0 = TEAM ? cluster_rank() * a.block_cols : 0, share = TEAM ? blockIdx.x / kTeam : blockIdx.x;
+    const int d = TEAM ? min(a.block_cols, a.d - static_cast<int>(col0)) : a.d;  // this CTA's columns, from col0
+    const int cover = cover_bytes(a.block_cols, T), bytes = d * dtype_size(T);
+    auto x_row = [&](int64_t row) { return row_of<T>(a.x, row, a.ldx, col0); };
+    auto dy_row = [&](int64_t row) { return row_of<T>(a.dy, row, a.lddy, col0); };
     char *ring = reinterpret_cast<char *>(smem);
     const float inv_d = 1.0f / static_cast<float>(a.d);
     int buf = 0;
+    if constexpr (TEAM) cluster_sync();  // every CTA of the team runs before another writes to its shared memory
     wait_prior_grid();
-    for (int64_t grp = a.split.first_group(blockIdx.x), end = a.split.last_group(blockIdx.x); grp < end; ++grp) {
+    for (int64_t grp = a.split.first_group(share), end = a.split.last_group(share); grp < end; ++grp) {
         int64_t lo, hi;
-        a.split.rows_of(blockIdx.x, grp, lo, hi);
+        a.split.rows_of(share, grp, lo, hi);
         auto fetch = [&](int64_t row, int slot) {
 #pragma unroll
             for (int r = 0; r < R; ++r) {
                 if (row + r >= hi) break;
                 char *dst = ring + (slot * R + r) * 2 * cover;
-                copy_cover(dst, row_of<T>(a.x, row + r, a.ldx), bytes, tid, threads);
-                copy_cover(dst + cover, row_of<T>(a.dy, row + r, a.lddy), bytes, tid, threads);
+                copy_cover(dst, x_row(row + r), bytes, tid, threads);
+                copy_cover(dst + cover, dy_row(row + r), bytes, tid, threads);
             }
             cp_async_commit();
         };
         for (int i = 0; i < kRing; ++i) fetch(lo + i * R, i);
         float w[8], dw[8], db[8];
-        if (a.w != nullptr) load_chunk<W, false>(w, row_of<W>(a.w, grp, a.d), 0, tid, threads, a.d);
+        if (a.w != nullptr) load_chunk<W, false>(w, row_of<W>(a.w, grp, a.d, col0), 0, tid, threads, d);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             dw[j] = db[j] = 0.f;
@@ -910,8 +981,8 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) layer_norm_grad_unaligned_ker
                 const float mean = on ? a.mean[row + r] : 0.f;
                 const char *x = ring + (slot * R + r) * 2 * cover;
                 rstd[r] = on ? a.rstd[row + r] : 0.f;
-                load_chunk<T, false>(xh[r], x + skew(row_of<T>(a.x, row + r, a.ldx)), 0, tid, threads, on ? a.d : 0);
-                load_chunk<T, false>(u[r], x + cover + skew(row_of<T>(a.dy, row + r, a.lddy)), 0, tid, threads, on ? a.d : 0);
+                load_chunk<T, false>(xh[r], x + skew(x_row(row + r)), 0, tid, threads, on ? d : 0);
+                load_chunk<T, false>(u[r], x + cover + skew(dy_row(row + r)), 0, tid, threads, on ? d : 0);
                 s[2 * r] = s[2 * r + 1] = 0.f;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
@@ -924,7 +995,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) layer_norm_grad_unaligned_ker
                 }
             }
             cp_async_wait<kRing - 2>();  // the next rows are here for this thread, and behind the barrier for all
-            const float mean_u = block_sums<2 * R>(s, red[buf], warp, lane, warps) * inv_d;
+            const float mean_u = block_sums<2 * R, TEAM>(s, red[buf], warp, lane, warps) * inv_d;
             buf ^= 1;
             fetch(row + kRing * R, slot);  // every thread has read this slot
             if (++slot == kRing) slot = 0;
@@ -935,12 +1006,12 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) layer_norm_grad_unaligned_ker
                 if (row + r >= hi) continue;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) u[r][j] = rstd[r] * (u[r][j] - m0 - xh[r][j] * m1);
-                store_chunk<T, false>(u[r], row_of<T>(a.dx, row + r, a.lddx), 0, tid, threads, a.d);
+                store_chunk<T, false>(u[r], row_of<T>(a.dx, row + r, a.lddx, col0), 0, tid, threads, d);
             }
         }
-        const int64_t part = a.split.partial_row(blockIdx.x, grp) * a.d;
-        if (a.part_w != nullptr) store_chunk<WF_F32, false>(dw, a.part_w + part, 0, tid, threads, a.d);
-        if (a.part_b != nullptr) store_chunk<WF_F32, false>(db, a.part_b + part, 0, tid, threads, a.d);
+        const int64_t part = a.split.partial_row(share, grp) * a.d + col0;
+        if (a.part_w != nullptr) store_chunk<WF_F32, false>(dw, a.part_w + part, 0, tid, threads, d);
+        if (a.part_b != nullptr) store_chunk<WF_F32, false>(db, a.part_b + part, 0, tid, threads, d);
     }
     cp_async_wait<0>();
 }
@@ -1023,43 +1094,37 @@ int grad_threads(int d, int type) {
     return ((d + v - 1) / v + 31) / 32 * 32;
 }
 
-// Whether a team shares the rows in the backward pass: 16-bit rows too wide for one block, up to kTeam x 2048 columns. Past
-// that a CTA has the SM to itself and the exchange stands in the open (4096 x 20480 229 us against 242 for the wide
-// kernels; float32, 2048 x 20480, 250 against 192); below it one block is faster (8192 x 8192 96 us against 117).
-bool grad_team(int d, int type) { return type != WF_F32 && d % 8 == 0 && d > 8 * kMaxThreads && d <= kTeam * 2048; }
-int team_columns(int d) { return (d / 8 + kTeam - 1) / kTeam * 8; }
+// Whether a cluster shares the rows in the backward pass (and in the forward pass of rows that 16-byte accesses do not fit):
+// rows too wide for one block, up to 2048 columns a CTA, in us against the wide kernels: 4096 x 12288 bf16 109 / 157 and
+// float32 205 / 236, 4096 x 16384 152 / 190 and 302 / 286, 8192 x 9999 bf16 279 / 519. Past that a CTA has the SM to itself and the
+// exchange stands in the open (4096 x 20480 bf16 332 / 230, 2000 x 17777 float32 249 / 188); below it one block is faster
+// (8192 x 8192 bf16 117 / 96).
+bool is_team(int d) { return d > 8 * kMaxThreads && d <= kTeam * 8 * 256; }
+int team_columns(int d) { return (d + 8 * kTeam - 1) / (8 * kTeam) * 8; }
 
 // a block's threads for 8 values each, or the most there are
 int row_threads(int d) { return std::min(kMaxThreads, ((d + 7) / 8 + 31) / 32 * 32); }
 
-template <int T, int W>
-int dispatch_norm_unaligned(const NormArgs &a, cudaStream_t stream);
-
-template <int T, int W, int NC, bool VEC, bool WARP>
-int launch_norm(const NormArgs &a, cudaStream_t stream) {
-    constexpr auto kern = layer_norm_kernel<T, W, NC, VEC, WARP>;
-    const int block = WARP ? 256 : row_threads(a.d);
-    const int64_t need = WARP ? (a.rows + 7) / 8 : a.rows;
-    const int grid = static_cast<int>(std::min<int64_t>(need, wave_ctas_at<kern>(block)));
+template <int T, int W, int NC, bool VEC>
+int launch_norm_block(const NormArgs &a, cudaStream_t stream) {
+    constexpr auto kern = layer_norm_kernel<T, W, NC, VEC>;
+    const int block = row_threads(a.d), grid = static_cast<int>(std::min<int64_t>(a.rows, wave_ctas_at<kern>(block)));
     return launch_rows(kern, dim3(grid), block, stream, a);
 }
 
-template <int T, int W, bool VEC>
-int launch_norm_block(const NormArgs &a, cudaStream_t stream) {
-    if constexpr (!VEC) {
-        if (a.d <= 256) return launch_norm<T, W, 1, VEC, true>(a, stream);
-    }
-    switch ((a.d + 8 * kMaxThreads - 1) / (8 * kMaxThreads)) {
-        case 1:
-            if constexpr (VEC) return launch_norm<T, W, 1, VEC, false>(a, stream);
-            else return dispatch_norm_unaligned<T, W>(a, stream);
-        case 2: return launch_norm<T, W, 2, VEC, false>(a, stream);
-        case 3: return launch_norm<T, W, 3, VEC, false>(a, stream);
-        default: break;
-    }
+template <int T, int W>
+int launch_norm_wide(const NormArgs &a, cudaStream_t stream) {
     constexpr auto kern = layer_norm_wide_kernel<T, W>;
     const int grid = static_cast<int>(std::min<int64_t>(a.rows, wave_ctas_at<kern>(kMaxThreads)));
     return launch_rows(kern, dim3(grid), kMaxThreads, stream, a);
+}
+
+template <int T, int W, int NV>
+int launch_norm_warp(const NormArgs &a, cudaStream_t stream) {
+    constexpr auto kern = layer_norm_warp_kernel<T, W, NV>;
+    constexpr int per_block = 8 * (8 / NV);
+    const int grid = static_cast<int>(std::min<int64_t>((a.rows + per_block - 1) / per_block, wave_ctas_at<kern>(256)));
+    return launch_rows(kern, dim3(grid), 256, stream, a);
 }
 
 // blocks an SM of a kernel whose block's threads hold some 100 registers each
@@ -1079,26 +1144,34 @@ cudaError_t allow_smem(int bytes) {
 }
 constexpr int kMostSmem = 200 * 1024;  // beside the kernels' static shared memory
 
-template <int T, int W, int R, int THREADS, int BLOCKS>
+template <int T, int W, int R, int THREADS, int BLOCKS, bool TEAM>
 int launch_norm_unaligned(const NormArgs &a, cudaStream_t stream) {
-    constexpr auto kern = layer_norm_unaligned_kernel<T, W, R, THREADS, BLOCKS>;
+    constexpr auto kern = layer_norm_unaligned_kernel<T, W, R, THREADS, BLOCKS, TEAM>;
     cudaError_t e = allow_smem<kern>(kMostSmem);
     if (e != cudaSuccess) return static_cast<int>(e);
-    const int threads = row_threads(a.d), smem = kRing * R * cover_bytes(a.d, T);
+    const int cols = TEAM ? team_columns(a.d) : a.d, threads = row_threads(cols), smem = kRing * R * cover_bytes(cols, T);
     const int per_sm = std::max(1, std::min(blocks_by_threads(threads), 220 * 1024 / (smem + 2048)));
-    const RowSplit split = make_split(a.rows, a.rows_per_group, per_sm * device_sm_count(), R);
-    e = launch_dependent(kern, dim3(static_cast<unsigned>(split.blocks())), threads, smem, stream, a, split);
+    const RowSplit split = make_split(a.rows, a.rows_per_group, std::max(1, per_sm * device_sm_count() / (TEAM ? kTeam : 1)), R);
+    e = launch_dependent_clusters(kern, dim3(static_cast<unsigned>(split.blocks() * (TEAM ? kTeam : 1))), TEAM ? kTeam : 0,
+                                  threads, smem, stream, a, split, cols);
     return static_cast<int>(e != cudaSuccess ? e : cudaGetLastError());
 }
 
-// R rows at a time: as many as the registers of so many threads hold, half as many of float32 (the ring's room)
+// Rows that 16-byte accesses do not fit. R rows at a time: as many as the registers of so many threads hold, half as many of
+// float32 (the ring's room).
 template <int T, int W>
 int dispatch_norm_unaligned(const NormArgs &a, cudaStream_t stream) {
+    if (a.d <= 32) return launch_norm_warp<T, W, 1>(a, stream);
+    if (a.d <= 64) return launch_norm_warp<T, W, 2>(a, stream);
+    if (a.d <= 128) return launch_norm_warp<T, W, 4>(a, stream);
+    if (a.d <= 256) return launch_norm_warp<T, W, 8>(a, stream);
     constexpr int R = T == WF_F32 ? 2 : 4;
-    const int threads = row_threads(a.d);
-    if (threads <= 256) return launch_norm_unaligned<T, W, R, 256, 2>(a, stream);
-    if (threads <= 640) return launch_norm_unaligned<T, W, R / 2, 640, 1>(a, stream);
-    return launch_norm_unaligned<T, W, 1, kMaxThreads, 1>(a, stream);
+    if (a.d <= 8 * 256) return launch_norm_unaligned<T, W, R, 256, 2, false>(a, stream);
+    if (a.d <= 8 * 640) return launch_norm_unaligned<T, W, R / 2, 640, 1, false>(a, stream);
+    if (a.d <= 8 * kMaxThreads) return launch_norm_unaligned<T, W, 1, kMaxThreads, 1, false>(a, stream);
+    if (is_team(a.d)) return launch_norm_unaligned<T, W, R, 256, 2, true>(a, stream);
+    if (a.d <= 24 * kMaxThreads) return launch_norm_block<T, W, 3, false>(a, stream);
+    return launch_norm_wide<T, W>(a, stream);
 }
 
 template <int T, int W, int LPR>
@@ -1131,7 +1204,7 @@ template <int T, int W>
 int dispatch_norm(const NormArgs &a, cudaStream_t stream) {
     const bool vec = a.d % 8 == 0 && vec_ok(a.x, a.ldx, dtype_size(T)) && vec_ok(a.y, a.ldy, dtype_size(T)) &&
                      vec_ok(a.w, a.d, dtype_size(W)) && vec_ok(a.b, a.d, dtype_size(W));
-    if (!vec) return launch_norm_block<T, W, false>(a, stream);
+    if (!vec) return dispatch_norm_unaligned<T, W>(a, stream);
     const int chunks = a.d / 8;
     if (chunks <= 4) return launch_norm_narrow<T, W, 4>(a, stream);
     if (chunks <= 8) return launch_norm_narrow<T, W, 8>(a, stream);
@@ -1147,7 +1220,10 @@ int dispatch_norm(const NormArgs &a, cudaStream_t stream) {
         if (kb <= 20) return launch_norm_stream<T, W, 4>(a, stream);
         if (kb <= 80) return launch_norm_stream<T, W, 8>(a, stream);
     }
-    return launch_norm_block<T, W, true>(a, stream);
+    if (a.d <= 8 * kMaxThreads) return launch_norm_block<T, W, 1, true>(a, stream);
+    if (a.d <= 16 * kMaxThreads) return launch_norm_block<T, W, 2, true>(a, stream);
+    if (a.d <= 24 * kMaxThreads) return launch_norm_block<T, W, 3, true>(a, stream);
+    return launch_norm_wide<T, W>(a, stream);
 }
 
 template <int T, int W, bool VEC>
@@ -1175,13 +1251,30 @@ int launch_norm_grad_rows(const NormGradArgs &a, int threads, cudaStream_t strea
     return static_cast<int>(e != cudaSuccess ? e : cudaGetLastError());
 }
 
-template <int T, int W, int R, int THREADS, int BLOCKS>
+template <int T, int W, int R, int THREADS, int BLOCKS, bool TEAM>
 int launch_norm_grad_unaligned(const NormGradArgs &a, cudaStream_t stream) {
-    constexpr auto kern = layer_norm_grad_unaligned_kernel<T, W, R, THREADS, BLOCKS>;
+    constexpr auto kern = layer_norm_grad_unaligned_kernel<T, W, R, THREADS, BLOCKS, TEAM>;
     cudaError_t e = allow_smem<kern>(kMostSmem);
     if (e != cudaSuccess) return static_cast<int>(e);
-    e = launch_dependent(kern, dim3(static_cast<unsigned>(a.split.blocks())), row_threads(a.d), kRing * R * 2 * cover_bytes(a.d, T), stream, a);
+    e = launch_dependent_clusters(kern, dim3(static_cast<unsigned>(a.split.blocks() * (TEAM ? kTeam : 1))), TEAM ? kTeam : 0,
+                                  row_threads(a.block_cols), kRing * R * 2 * cover_bytes(a.block_cols, T), stream, a);
     return static_cast<int>(e != cudaSuccess ? e : cudaGetLastError());
+}
+
+// R as in the forward pass
+template <int T, int W>
+int dispatch_norm_grad_unaligned(const NormGradArgs &a, cudaStream_t stream) {
+    const dim3 grid(static_cast<unsigned>(a.split.blocks()));
+    if (a.d <= 32) return launch_rows(layer_norm_grad_warp_kernel<T, W, 1>, grid, 256, stream, a);
+    if (a.d <= 64) return launch_rows(layer_norm_grad_warp_kernel<T, W, 2>, grid, 256, stream, a);
+    if (a.d <= 128) return launch_rows(layer_norm_grad_warp_kernel<T, W, 4>, grid, 256, stream, a);
+    if (a.d <= 256) return launch_rows(layer_norm_grad_warp_kernel<T, W, 8>, grid, 256, stream, a);
+    constexpr int R = T == WF_F32 ? 2 : 4;
+    if (a.d <= 8 * 256) return launch_norm_grad_unaligned<T, W, R, 256, 2, false>(a, stream);
+    if (a.d <= 8 * 640) return launch_norm_grad_unaligned<T, W, R / 2, 640, 1, false>(a, stream);
+    if (a.d <= 8 * kMaxThreads) return launch_norm_grad_unaligned<T, W, 1, kMaxThreads, 1, false>(a, stream);
+    if (is_team(a.d)) return launch_norm_grad_unaligned<T, W, R, 256, 2, true>(a, stream);
+    return launch_norm_grad_wide<T, W, false>(a, stream);
 }
 
 template <int T, int W>
@@ -1189,25 +1282,16 @@ int dispatch_norm_grad(const NormGradArgs &a, cudaStream_t stream) {
     const bool vec = a.d % 8 == 0 && vec_ok(a.x, a.ldx, dtype_size(T)) && vec_ok(a.dy, a.lddy, dtype_size(T)) &&
                      vec_ok(a.dx, a.lddx, dtype_size(T)) && vec_ok(a.w, a.d, dtype_size(W)) && vec_ok(a.part_w, a.d, 4) &&
                      vec_ok(a.part_b, a.d, 4);
-    const dim3 grid(static_cast<unsigned>(a.split.blocks()));
+    if (!vec || (T == WF_F32 && is_team(a.d))) return dispatch_norm_grad_unaligned<T, W>(a, stream);
     if constexpr (T != WF_F32) {
-        if (vec && grad_team(a.d, T))
-            return launch_norm_grad_rows<T, W, 8, 4, 256, 2, true>(a, grad_threads(a.block_cols, T), stream);
+        if (is_team(a.d)) return launch_norm_grad_rows<T, W, 8, 4, 256, 2, true>(a, grad_threads(a.block_cols, T), stream);
     }
-    if (a.d > 8 * kMaxThreads) return vec ? launch_norm_grad_wide<T, W, true>(a, stream) : launch_norm_grad_wide<T, W, false>(a, stream);
-    if (a.d <= 256) {
-        if (!vec) return launch_rows(layer_norm_grad_warp_kernel<T, W>, grid, 256, stream, a);
-        if (a.d <= 32) return launch_rows(layer_norm_grad_narrow_kernel<T, W, 4>, grid, 256, stream, a);
-        if (a.d <= 64) return launch_rows(layer_norm_grad_narrow_kernel<T, W, 8>, grid, 256, stream, a);
-        if (a.d <= 128) return launch_rows(layer_norm_grad_narrow_kernel<T, W, 16>, grid, 256, stream, a);
-        return launch_rows(layer_norm_grad_narrow_kernel<T, W, 32>, grid, 256, stream, a);
-    }
-    if (!vec) {  // R as in the forward pass
-        constexpr int R = T == WF_F32 ? 2 : 4;
-        if (row_threads(a.d) <= 256) return launch_norm_grad_unaligned<T, W, R, 256, 2>(a, stream);
-        if (row_threads(a.d) <= 640) return launch_norm_grad_unaligned<T, W, R / 2, 640, 1>(a, stream);
-        return launch_norm_grad_unaligned<T, W, 1, kMaxThreads, 1>(a, stream);
-    }
+    if (a.d > 8 * kMaxThreads) return launch_norm_grad_wide<T, W, true>(a, stream);
+    const dim3 grid(static_cast<unsigned>(a.split.blocks()));
+    if (a.d <= 32) return launch_rows(layer_norm_grad_narrow_kernel<T, W, 4>, grid, 256, stream, a);
+    if (a.d <= 64) return launch_rows(layer_norm_grad_narrow_kernel<T, W, 8>, grid, 256, stream, a);
+    if (a.d <= 128) return launch_rows(layer_norm_grad_narrow_kernel<T, W, 16>, grid, 256, stream, a);
+    if (a.d <= 256) return launch_rows(layer_norm_grad_narrow_kernel<T, W, 32>, grid, 256, stream, a);
     constexpr int V = T == WF_F32 ? 4 : 8;  // 16 bytes a thread; float32 rows past 4096 values take 32
     const int threads = grad_threads(a.d, T);
     if constexpr (T == WF_F32) {
@@ -1225,7 +1309,7 @@ bool norm_types_ok(int type, int w_type) {
 // The shares of the rows that the backward pass's blocks take: about as many as are resident at once.
 RowSplit norm_split(int64_t rows, int64_t rows_per_group, int d, int type) {
     const int64_t sms = device_sm_count();
-    if (grad_team(d, type)) return make_split(rows, rows_per_group, std::max<int64_t>(1, blocks_by_threads(grad_threads(team_columns(d), type)) * sms / kTeam), 4);
+    if (is_team(d)) return make_split(rows, rows_per_group, std::max<int64_t>(1, blocks_by_threads(row_threads(team_columns(d))) * sms / kTeam), 4);
     if (d > 8 * kMaxThreads) return make_split(rows, rows_per_group, std::max<int64_t>(1, 4 * sms * 2048 / d), 16);
     if (d <= 256) return make_split(rows, rows_per_group, 3 * sms, 16);
     return make_split(rows, rows_per_group, sms * blocks_by_threads(d % 8 == 0 ? grad_threads(d, type) : row_threads(d)), 4);
@@ -1286,7 +1370,7 @@ extern "C" WF_API int wf_layer_norm_backward(const wf_layer_norm_grad_args *args
     if (rc != WF_OK) return rc;
     float *part = static_cast<float *>(g.workspace);
     const NormGradArgs a{g.x, g.w, g.dy, g.mean, g.rstd, g.dx, g.dw ? part : nullptr, g.db ? part + half : nullptr, g.rows,
-                         g.ldx, g.lddy, g.lddx, split, d, grad_team(d, g.type) ? team_columns(d) : d};
+                         g.ldx, g.lddy, g.lddx, split, d, is_team(d) ? team_columns(d) : d};
     const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     if (g.type == WF_F32) rc = dispatch_norm_grad<WF_F32, WF_F32>(a, st);
     else if (g.type == WF_BF16) rc = g.w_type == WF_F32 ? dispatch_norm_grad<WF_BF16, WF_F32>(a, st) : dispatch_norm_grad<WF_BF16, WF_BF16>(a, st);

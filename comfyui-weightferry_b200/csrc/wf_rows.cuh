@@ -59,13 +59,14 @@ namespace {
 
 inline bool aligned_to(const void *p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 
+// a row of a matrix, from column col0 on
 template <int T>
-__device__ __forceinline__ const void *row_of(const void *base, int64_t row, int64_t ld) {
-    return static_cast<const char *>(base) + row * ld * dtype_size(T);
+__device__ __forceinline__ const void *row_of(const void *base, int64_t row, int64_t ld, int64_t col0 = 0) {
+    return static_cast<const char *>(base) + (row * ld + col0) * dtype_size(T);
 }
 template <int T>
-__device__ __forceinline__ void *row_of(void *base, int64_t row, int64_t ld) {
-    return static_cast<char *>(base) + row * ld * dtype_size(T);
+__device__ __forceinline__ void *row_of(void *base, int64_t row, int64_t ld, int64_t col0 = 0) {
+    return static_cast<char *>(base) + (row * ld + col0) * dtype_size(T);
 }
 
 template <int T>

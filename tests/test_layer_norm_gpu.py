@@ -68,17 +68,28 @@ def test_groups(cuda, m, rpg, d):
 
 
 @pytest.mark.parametrize("m,rpg", [(1, 1), (300, 75), (301, 300), (64, 3)])
-@pytest.mark.parametrize("d", [8200, 12288, 12296, 16384, 16392])
+@pytest.mark.parametrize("d", [8193, 8200, 9999, 12288, 12296, 16383, 16384, 16391, 16392])
 def test_rows_shared_by_clusters(cuda, m, rpg, d):
     import torch
     for wdtype in (torch.float16, torch.float32):
         data, dy = _data(torch, m, d, torch.float16, wdtype, groups=-(-m // rpg))
         _compare(torch, data, dy, rpg=rpg)
+    _compare(torch, *_data(torch, m, d, torch.float32, torch.float32, groups=-(-m // rpg)), rpg=rpg)
     # the gradients of w and b alone take no exchange
     fn, want = wf("enhancers.fused_norm"), norm_reference(data["x"], data["weight"], data["bias"], 1e-6, rpg, dy)
     y = fn.layer_norm(data["x"].detach(), data["weight"], data["bias"], 1e-6, rpg)
     for nm, got in zip(("weight", "bias"), torch.autograd.grad(y, (data["weight"], data["bias"]), dy)):
         assert_within(got, want[nm], nm)
+
+
+@pytest.mark.parametrize("d", [3, 31, 33, 63, 65, 127, 129, 250, 300, 2045, 2049, 5119, 5121, 8191, 16389, 24575, 24577])
+def test_odd_widths(cuda, d):
+    import torch
+    for m, dtype, wdtype in ((1, torch.float32, torch.float32), (95, torch.bfloat16, torch.float32), (701, torch.float16, torch.float16),
+                             (700, torch.float32, torch.float32)):
+        _compare(torch, *_data(torch, m, d, dtype, wdtype))
+    data, dy = _data(torch, 75, d, torch.bfloat16, torch.bfloat16, groups=8)
+    _compare(torch, data, dy, rpg=10)
 
 
 def test_without_weight_or_bias(cuda):
