@@ -550,12 +550,11 @@ struct Warp32 {
 
 // 32 columns of the warp's rows, half h of a chunk of 64 (KEEP: a chunk of their own)
 template <int T, bool FULL, bool KEEP>
-__device__ __forceinline__ void finish_half(float (&v)[32], Warp32 &w, const Epilogue &e, const uint32_t (&res)[16], int col0, int h) {
+__device__ __forceinline__ void finish_half(float (&v)[32], Warp32 &w, const Epilogue &e, const uint32_t (&b)[16],
+                                            const uint32_t (&g)[16], const uint32_t (&res)[16], int col0, int h) {
     uint32_t p[16];
     if constexpr (FULL) {
         if (e.bias != nullptr) {
-            uint32_t b[16];
-            load32(b, e.bias, col0, w.n, e.vec);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const float2 f = unpack2<T>(b[i]);
@@ -590,8 +589,6 @@ __device__ __forceinline__ void finish_half(float (&v)[32], Warp32 &w, const Epi
             default: break;
         }
         if (w.gate != nullptr) {
-            uint32_t g[16];
-            load32(g, w.gate, col0, w.n, e.vec);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const float2 f = unpack2<T>(g[i]);
@@ -783,12 +780,15 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
             if (!__all_sync(0xFFFFFFFFu, pipe_wait(tfull0 + 8 * acc, acc_phase, abort_flag, 3))) break;
             fence_after();
             const uint32_t taddr = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * BN + half * (BN / 2));
-            uint32_t r[32], res[16];
+            uint32_t r[32], b[16], g[16], res[16];
             tmem_ld32(taddr, r);
             // one copy of the chunk's code (unrolled four times, with every activation inside, it outgrew the
             // instruction cache: 266 against 137 us for a gelu layer of 8192 x 512 x 8192)
 #pragma unroll 1
             for (int q = 0; q < BN / 64; ++q) {
+                // in flight together with the accumulator's columns
+                if (FULL && epi.bias != nullptr) load32(b, epi.bias, col0 + 32 * q, n, epi.vec);
+                if (FULL && w.gate != nullptr) load32(g, w.gate, col0 + 32 * q, n, epi.vec);
                 if (FULL && epi.resid != nullptr) {
                     if (w.resid != nullptr) {
                         load32(res, w.resid, col0 + 32 * q, n, epi.vec);
@@ -807,7 +807,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
                     fence_before();
                     mbar_arrive_cluster(tempty_leader + 8 * acc);
                 }
-                finish_half<T, FULL, KEEP>(v, w, epi, res, col0 + 32 * q, q & 1);
+                finish_half<T, FULL, KEEP>(v, w, epi, b, g, res, col0 + 32 * q, q & 1);
             }
             if (++acc == 2) acc = 0, acc_phase ^= 1u;
         }
