@@ -243,7 +243,9 @@ WF_API int wf_copy_rows16(const wf_copy_rows *copies, int n_copies, wf_stream_t 
  * counterpart (the reference's LayerNorm + modulate is wf_ln_modulate). */
 
 /* y = (x - mean) * rstd * w + b, rstd = 1 / sqrt(var + eps); w and b may be NULL. mean and rstd [rows] float32 (both or
- * neither NULL) are kept for the backward pass. y may be x. rows >= 0, d >= 1. */
+ * neither NULL) are kept for the backward pass. y may be x. rows >= 0, d >= 1. Here and below a row whose width, pitch or
+ * start no 16-byte access fits is read in the aligned 16-byte pieces that hold it: up to 15 bytes in front of the matrix
+ * may be read (and are not used), nothing behind it. */
 typedef struct wf_layer_norm_args {
     const void *x, *w, *b;
     void *y;

@@ -125,6 +125,25 @@ def test_nonfinite_rows_stay_in_their_rows(cuda):
         assert torch.equal(y[keep].view(torch.int16), clean[keep].view(torch.int16))
 
 
+@pytest.mark.parametrize("d", [5, 77, 1001, 4097, 8193, 9999, 12288, 17777])
+def test_nonfinite_rows_leave_their_neighbours(cuda, d):
+    """A row shares its first and last 16 bytes with its neighbours where the width is odd: y and dx of other rows keep their bits."""
+    import torch
+    for dtype in (torch.bfloat16, torch.float32):
+        data, dy = _data(torch, 23, d, dtype, dtype)
+        y, grads = _train(torch, {nm: t.clone() for nm, t in data.items()}, dy)
+        bad = {nm: t.clone() for nm, t in data.items()}
+        bad["x"][4] = float("nan")
+        bad["x"][10, -1] = float("inf")
+        bad_dy = dy.clone()
+        bad_dy[17, 0] = float("nan")
+        y1, grads1 = _train(torch, bad, bad_dy)
+        keep = [i for i in range(23) if i not in (4, 10, 17)]
+        assert torch.equal(y1[keep], y[keep]) and torch.equal(y1[17], y[17])
+        assert torch.equal(grads1["x"][keep], grads["x"][keep])
+        assert bool(torch.isnan(y1[[4, 10]]).all()) and bool(torch.isnan(grads1["x"][[4, 17]]).all())
+
+
 def test_gradients_against_differences(cuda):
     """Central differences of the definition in float64 against the gradients' inner products with a direction."""
     import torch
@@ -207,6 +226,20 @@ def test_neighbouring_memory_is_left_alone(cuda):
             x.data_ptr(), x.data_ptr(), 0, stats.data_ptr(), stats[1].data_ptr(), dx.data_ptr(), 0, 0, 0, d, d, ld, m, d, m, 0,
             2, 2))
         assert bool((dx[:m, d:] == -7).all()) and bool((dx[m:] == -7).all()) and not bool((dx[:m, :d] == -7).any())
+
+
+@pytest.mark.parametrize("d", [5, 64, 77, 250, 1001, 2048, 5119, 5120, 8191, 8192, 9999, 12288, 17777, 33000])
+def test_output_over_input(cuda, d):
+    """y may be x: the bits of a call with an output of its own."""
+    import torch
+    for dtype, code in ((torch.float16, 0), (torch.float32, 2)):
+        for m in (3, 900):
+            data, _ = _data(torch, m, d, dtype, dtype)
+            want = wf("enhancers.fused_norm").layer_norm(**data)
+            x, w, b = data["x"], data["weight"], data["bias"]
+            dense_cabi.launch("wf_layer_norm", dense_cabi.LAYER_NORM_ARGS.pack(
+                x.data_ptr(), w.data_ptr(), b.data_ptr(), x.data_ptr(), 0, 0, d, d, m, d, m, 1e-6, code, code, 0))
+            assert torch.equal(x, want), (dtype, m)
 
 
 def test_streams_graphs_and_repeats(cuda):
