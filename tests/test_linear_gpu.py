@@ -222,6 +222,19 @@ def test_neighbouring_memory_is_left_alone(cuda):
         assert bool((db[:n] == m16).all()) and bool((db[n:] == -7).all())
 
 
+@pytest.mark.parametrize("m,k,n", [(1, 512, 2048), (5, 72, 61), (300, 1024, 520), (700, 64, 1001), (3000, 256, 1280), (5001, 72, 2048)])
+def test_output_over_residual(cuda, m, k, n):
+    """y may be resid: the bits of a call with an output of its own."""
+    import torch
+    d, _ = _data(torch, m, k, n, torch.bfloat16, groups=1)
+    want = _call(d, "gelu")
+    y = d["residual"].clone()
+    dense_cabi.launch("wf_linear", dense_cabi.LINEAR_ARGS.pack(
+        d["x"].data_ptr(), d["weight"].data_ptr(), d["bias"].data_ptr(), d["gate"].data_ptr(), y.data_ptr(), y.data_ptr(), 0, k, k, n,
+        n, n, m, m, n, k, 3, 1, 0, 0))
+    assert torch.equal(y, want)
+
+
 def test_streams_graphs_and_repeats(cuda):
     """A side stream, a captured training step replayed on new values, and a second run give the same bits."""
     import torch
