@@ -121,6 +121,7 @@ struct Epilogue {
     int64_t ld_resid, ld_out, ld_kept, rows_per_group;
     int act, keep;
     bool vec;  // every pointer 8-byte aligned and every row pitch (n too, where it is one) a multiple of 4 values
+    bool vec_bias;  // the pair kernel's: 16-byte accesses to the bias, whatever n is
 };
 
 // float32 -> f16, clamped to f16's range: the kept z is read by the slopes alone, which are constant out there, and
@@ -150,7 +151,8 @@ __device__ __forceinline__ void apply_act4(int kind, float (&v)[R][4]) {
     }
 }
 
-// four neighbouring values of a row: one 8-byte access, or (VEC false) value by value, those at and past n as 0
+// Four values of a row: neighbours in one 8-byte access, or (VEC false) 32 columns apart, so that a warp's single-value
+// accesses share their sectors; those at and past n as 0
 template <int T, bool VEC>
 __device__ __forceinline__ void load4(float (&v)[4], const void *row, int col, int n) {
     if constexpr (VEC) {
@@ -159,7 +161,7 @@ __device__ __forceinline__ void load4(float (&v)[4], const void *row, int col, i
         v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = col + i < n ? load1<T>(row, col + i) : 0.f;
+        for (int i = 0; i < 4; ++i) v[i] = col + 32 * i < n ? load1<T>(row, col + 32 * i) : 0.f;
     }
 }
 template <int T, bool VEC>
@@ -169,14 +171,15 @@ __device__ __forceinline__ void store4(void *row, int col, int n, const float (&
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (col + i < n) store1<T>(row, col + i, v[i]);
+            if (col + 32 * i < n) store1<T>(row, col + 32 * i, v[i]);
     }
 }
 
-// The epilogue of four neighbouring outputs in each of R rows (row, row + step, ...; those from row_end on are left out).
+// The epilogue of four outputs (load4's columns) in each of R rows (row, row + step, ...; those from row_end on are left out).
 // Several rows share each of its branches, and their chains of loads and arithmetic overlap.
 template <int T, bool VEC, int R>
 __device__ __forceinline__ void finish4(const Epilogue &e, float (&v)[R][4], int row, int step, int row_end, int col, int n) {
+    constexpr int C = VEC ? 1 : 32;
     float o[R][4];
     if (e.bias != nullptr) {
         load4<T, VEC>(o[0], e.bias, col, n);
@@ -195,13 +198,15 @@ __device__ __forceinline__ void finish4(const Epilogue &e, float (&v)[R][4], int
                 uint16_t *dst = static_cast<uint16_t *>(e.kept) + at * e.ld_kept + col;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (col + i < n) dst[i] = static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1)));
+                    if (col + C * i < n) dst[C * i] = static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1)));
             } else if (e.keep == KEEP_F32) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (col + i < n) static_cast<float *>(e.kept)[at * e.ld_kept + col + i] = v[r][i];
+                    if (col + C * i < n) static_cast<float *>(e.kept)[at * e.ld_kept + col + C * i] = v[r][i];
             } else {
-                store4<T, false>(row_of<T>(e.kept, at, e.ld_kept), col, n, v[r]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (col + C * i < n) store1<T>(row_of<T>(e.kept, at, e.ld_kept), col + C * i, v[r][i]);
             }
         }
     }
@@ -229,11 +234,17 @@ __device__ __forceinline__ void finish4(const Epilogue &e, float (&v)[R][4], int
         if (row + r * step < row_end) store4<T, VEC>(row_of<T>(e.out, row + r * step, e.ld_out), col, n, v[r]);
 }
 
-// Value by value, out of line: the loop around the epilogue has to stay small (see linear_tile_kernel).
-template <int T>
-__device__ __noinline__ void finish4_any(const Epilogue &e, float4 sum, int row, int col, int n) {
-    float v[1][4] = {{sum.x, sum.y, sum.z, sum.w}};
-    finish4<T, false, 1>(e, v, row, 1, row + 1, col, n);
+// Value by value, out of line: the loop around the epilogue has to stay small (see linear_tile_kernel). Rows t, t + step, ...
+// of the tile's sums, whose row 0 and column 0 are row0 and j0 of D.
+template <int T, int R, int COLS>
+__device__ __noinline__ void finish4_any(const Epilogue &e, const float *sums, int t, int step, int t_end, int row0, int j0, int n) {
+    const int lane = threadIdx.x & 31;
+    float v[R][4];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[r][i] = t + r * step < t_end ? sums[(t + r * step) * COLS + lane + 32 * i] : 0.f;
+    finish4<T, false, R>(e, v, row0 + t, step, row0 + t_end, j0 + lane, n);
 }
 
 // ------------------------------------------------------------------------------------------------ few-rows kernel
@@ -413,8 +424,9 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_const
     // has left, an illegal access.
     if (split > 1) cluster_sync();
     const float4 *sums = reinterpret_cast<const float4 *>(ring);
-    if (epi.vec && col + 4 <= n) {
-        constexpr int R = 4;
+    constexpr int R = 4;
+    if (epi.vec && (n % 4 == 0 || j0 + TILE_J <= n)) {  // the whole warp, or none of it
+        if (col >= n) return;
 #pragma unroll 1
         for (int t = t_lo + warp; t < t_hi; t += R * WARPS) {
             float v[R][4];
@@ -425,9 +437,10 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_const
             }
             finish4<T, true, R>(epi, v, i0 + t, WARPS, i0 + t_hi, col, n);
         }
-    } else if (col < n) {
+    } else {
 #pragma unroll 1
-        for (int t = t_lo + warp; t < t_hi; t += WARPS) finish4_any<T>(epi, sums[t * (TILE_J / 4) + lane], i0 + t, col, n);
+        for (int t = t_lo + warp; t < t_hi; t += R * WARPS)
+            finish4_any<T, R, TILE_J>(epi, reinterpret_cast<const float *>(ring), t, WARPS, t_hi, i0, j0, n);
     }
 }
 
@@ -517,11 +530,15 @@ __device__ __forceinline__ void put32(const ChunkOut &o, const uint32_t (&p)[16]
 // the chunk's values one by one, a row at a time: rows and columns past the output's are left alone
 template <int CW>
 __device__ __noinline__ void send_any(uint16_t *out, int64_t ld, uint32_t buf, int lane, int rows, int cols) {
-    for (int r = 0; r < rows; ++r)
-        for (int c = lane; c < cols; c += 32) {
-            uint16_t v;
-            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(piece_at<CW>(buf, r, c >> 3) + 2u * (c & 7)) : "memory");
-            out[r * ld + c] = v;
+    for (int c = lane; c < cols; c += 32)
+        for (int r0 = 0; r0 < rows; r0 += 8) {  // eight rows in flight
+            uint16_t v[8];
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v[r]) : "r"(piece_at<CW>(buf, r0 + r, c >> 3) + 2u * (c & 7)) : "memory");
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+                if (r0 + r < rows) out[(r0 + r) * ld + c] = v[r];
         }
 }
 
@@ -787,7 +804,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
 #pragma unroll 1
             for (int q = 0; q < BN / 64; ++q) {
                 // in flight together with the accumulator's columns
-                if (FULL && epi.bias != nullptr) load32(b, epi.bias, col0 + 32 * q, n, epi.vec);
+                if (FULL && epi.bias != nullptr) load32(b, epi.bias, col0 + 32 * q, n, epi.vec || (epi.vec_bias && col0 + 32 * (q + 1) <= n));
                 if (FULL && w.gate != nullptr) load32(g, w.gate, col0 + 32 * q, n, epi.vec);
                 if (FULL && epi.resid != nullptr) {
                     if (w.resid != nullptr) {
@@ -923,6 +940,7 @@ int launch_pair(const Product &p, const Epilogue &e0, int dev, cudaStream_t stre
     }
     Epilogue e = e0;
     // 16-byte accesses to the bias, the gate and the residual
+    e.vec_bias = vec8_ok(e.bias, 0);
     e.vec = p.n % 8 == 0 && vec8_ok(e.bias, 0) && vec8_ok(e.gate, p.n) && vec8_ok(e.resid, e.ld_resid);
     const bool tma_out = vec8_ok(e.out, e.ld_out);
     const bool tma_kept = (e.keep == KEEP_F16 || e.keep == KEEP_SAME) && vec8_ok(e.kept, e.ld_kept);

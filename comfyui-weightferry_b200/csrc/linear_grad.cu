@@ -103,7 +103,7 @@ __global__ void __launch_bounds__(256) linear_grad_kernel(const __grid_constant_
 // The same for eight columns that 16-byte accesses fit, without a gate of its own row group and its gradient where GATE is
 // false. Each thread copies its own values of the next rows into a ring of kRing rows in shared memory (cp.async) and
 // reads nobody else's: with the loads in registers instead, two rows ahead, the pass took 138 us on 8192 x 8192 where it
-// now takes 83. ZN: no z (no activation and no gradient of the gate).
+// now takes 77. ZN: no z (no activation and no gradient of the gate).
 constexpr int kRing = 4;
 template <int T, int Z, int ACT, bool ZN, bool GATE>
 __global__ void __launch_bounds__(256, 3) linear_grad_vec_kernel(const __grid_constant__ LinearGradArgs a) {
