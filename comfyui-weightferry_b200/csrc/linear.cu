@@ -592,7 +592,8 @@ __device__ __forceinline__ void finish_half(float (&v)[32], Warp32 &w, const Epi
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
                     p[i] = e.keep == KEEP_F16 ? pack2_sat(v[2 * i], v[2 * i + 1]) : pack2<T>(v[2 * i], v[2 * i + 1]);
-                if (w.lane == 0) bulk_wait_read1();  // all but y's last store have been read
+                // z's last store has been read; y's may go on, and is the last one where y leaves by TMA at all
+                if (w.lane == 0) w.y.tma ? bulk_wait_read1() : bulk_wait_read_all();
                 __syncwarp();
                 put32<32>(w.z, p, 0, w.lane);
                 send_chunk<32>(w.z, w.lane, w.row0, col0, w.m, w.n);
@@ -625,7 +626,7 @@ __device__ __forceinline__ void finish_half(float (&v)[32], Warp32 &w, const Epi
 #pragma unroll
     for (int i = 0; i < 16; ++i) p[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
     if constexpr (KEEP) {
-        if (w.lane == 0) e.keep == KEEP_F32 ? bulk_wait_read_all() : bulk_wait_read1();  // all but z's last store
+        if (w.lane == 0) w.z.tma ? bulk_wait_read1() : bulk_wait_read_all();  // the same for y
         __syncwarp();
         put32<32>(w.y, p, 0, w.lane);
         send_chunk<32>(w.y, w.lane, w.row0, col0, w.m, w.n);

@@ -1,0 +1,59 @@
+"""What the dense linear layer keeps for its backward pass (the pre-activation z), through the C entry points: every way
+in which y and z leave the kernels."""
+
+import math
+
+import pytest
+
+import dense_cabi
+from conftest import wf
+from dense_reference import U, act, assert_within, half_step
+
+pytestmark = pytest.mark.gpu
+
+ACT = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
+CODE = {"float16": 0, "bfloat16": 1, "float32": 2}
+
+
+def _forward(torch, x, w, kind, z_type, ldy, ldz):
+    """(y, z) of x w^T with row pitches ldy and ldz."""
+    m, k = x.shape
+    n = w.shape[0]
+    y = torch.full((m, ldy), -7.0, device="cuda", dtype=x.dtype)
+    z = torch.full((m, ldz), -7.0, device="cuda", dtype=z_type)
+    code = CODE[str(x.dtype).rsplit(".", 1)[1]]
+    dense_cabi.launch("wf_linear", dense_cabi.LINEAR_ARGS.pack(
+        x.data_ptr(), w.data_ptr(), 0, 0, 0, y.data_ptr(), z.data_ptr(), k, k, 0, ldy, ldz, 1, m, n, k, ACT[kind], code,
+        CODE[str(z_type).rsplit(".", 1)[1]], 0))
+    return y, z
+
+
+@pytest.mark.parametrize("m,n,k", [(5001, 2041, 72), (5001, 2048, 72), (300, 1001, 520), (3, 61, 64)])
+@pytest.mark.parametrize("kind,z_name", [("gelu", "float16"), ("gelu", "float32"), ("none", "bfloat16")])
+def test_kept_values_in_every_layout(cuda, m, n, k, kind, z_name):
+    """y and z each at a pitch of 16-byte pieces and at an odd one: z within a rounding of its definition, y within the
+    float32 sums' error and a rounding, and the same bits in every repeat (several tiles a block, so that each buffer of an
+    epilogue warp is used again)."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(m + n + k)
+    x = torch.randn((m, k), device="cuda", generator=g).to(torch.bfloat16)
+    w = (torch.randn((n, k), device="cuda", generator=g) / math.sqrt(k)).to(torch.bfloat16)
+    z_type = getattr(torch, z_name)
+    want = x.double() @ w.double().t()
+    e = 2 * U * k * (x.double().abs() @ w.double().abs().t())
+    h, _ = act(want, kind)
+    # 1.13 is the steepest slope of gelu; 8e-6 and 2e-7 its own float32 evaluation
+    ey = 1.13 * e + 8e-6 * h.abs() + 2e-7 * want.abs() + half_step(h, x.dtype) * (1 + 1e-3)
+    ez = e + half_step(want, z_type) * (1 + 1e-3)
+    up = (n + 7) // 8 * 8
+    for ldy, ldz in ((up, up), (up, up + 3), (up + 3, up), (up + 3, up + 3)):
+        first = None
+        for _ in range(4):
+            y, z = _forward(torch, x, w, kind, z_type, ldy, ldz)
+            if first is None:
+                first = y, z
+                assert_within(y[:, :n], (h, ey), f"y {ldy} {ldz}")
+                assert_within(z[:, :n], (want, ez), f"z {ldy} {ldz}")
+            else:
+                assert torch.equal(y[:, :n], first[0][:, :n]) and torch.equal(z[:, :n], first[1][:, :n]), (ldy, ldz)
+    assert wf("enhancers.fused_linear").status() == 0
