@@ -62,7 +62,7 @@ std::pair<Tensor, int64_t> as_rows(const Tensor &t) {
 // slices) are to be copied.
 struct Operand {
     Tensor t;
-    int64_t ld;
+    int64_t ld = 0;
     wf_copy_rows copy = {};
 };
 
@@ -75,17 +75,30 @@ Operand as_operand(const Tensor &t) {
     return o;
 }
 
-// x's and w's operands, their copies in one launch
+// x's and w's operands (either may be undefined), their copies in one launch
 std::pair<Operand, Operand> as_operands(const Tensor &x, const Tensor &w) {
-    const auto [x2, ldx] = as_rows(x);  // x2 and w2 live until the copies are launched
-    const auto [w2, ldw] = as_rows(w);
-    Operand xo = as_operand(x2), wo = as_operand(w2);
+    const Tensor *given[2] = {&x, &w};
+    Operand out[2];
+    Tensor rows[2];  // live until the copies are launched
     wf_copy_rows copies[2];
     int n = 0;
-    if (xo.copy.dst != nullptr) copies[n] = xo.copy, copies[n++].ld_src = ldx;
-    if (wo.copy.dst != nullptr) copies[n] = wo.copy, copies[n++].ld_src = ldw;
-    if (n > 0) check(wf_copy_rows16(copies, n, stream_of(x)), "wf_copy_rows16");
-    return {xo, wo};
+    for (int i = 0; i < 2; ++i) {
+        if (!given[i]->defined()) continue;
+        int64_t ld;
+        std::tie(rows[i], ld) = as_rows(*given[i]);
+        out[i] = as_operand(rows[i]);
+        if (out[i].copy.dst != nullptr) copies[n] = out[i].copy, copies[n++].ld_src = ld;
+    }
+    if (n > 0) check(wf_copy_rows16(copies, n, stream_of(x.defined() ? x : w)), "wf_copy_rows16");
+    return {out[0], out[1]};
+}
+
+// A saved tensor as the graph gives it back. Hooks (save_on_cpu, checkpoints, a user's own) return a tensor of their own:
+// its strides and address are its own too, so a pitch is taken from it and never kept beside it. Its shape, type and device
+// must be what was saved.
+void check_saved(const char *what, const Tensor &t, at::IntArrayRef shape, at::ScalarType type, const at::Device &device) {
+    TORCH_CHECK(t.sizes() == shape && t.scalar_type() == type && t.device() == device, what, ": a saved tensor of shape ", shape,
+                ", ", type, " on ", device, " came back as ", t.sizes(), ", ", t.scalar_type(), " on ", t.device());
 }
 
 // rows of x for each row of p ([n] or [groups, n]): as given, or all m rows divided evenly
@@ -119,9 +132,8 @@ struct LinearCall {
     int64_t act, rpg, m, n, k;
 };
 
-struct Kept {  // what the backward pass may need
+struct Kept {  // what the backward pass may need: x and w as the products read them, z [m, up8(n)]
     Tensor x, w, z;
-    int64_t ldx = 0, ldw = 0;
 };
 
 Tensor linear_forward(const Tensor &x, const Tensor &w, const MaybeTensor &bias, const MaybeTensor &resid,
@@ -147,7 +159,7 @@ Tensor linear_forward(const Tensor &x, const Tensor &w, const MaybeTensor &bias,
     a.ldx = xo.ld, a.ldw = wo.ld, a.ldy = c.n, a.rows_per_group = c.rpg, a.m = c.m, a.n = c.n, a.k = c.k;
     a.act = static_cast<int32_t>(c.act), a.type = code_of(x.scalar_type());
     check(wf_linear(&a, stream_of(x)), "wf_linear");
-    if (kept != nullptr) *kept = Kept{xo.t, wo.t, z, xo.ld, wo.ld};
+    if (kept != nullptr) *kept = Kept{xo.t, wo.t, z};
     return y;
 }
 
@@ -165,8 +177,9 @@ struct LinearNode : public torch::autograd::Function<LinearNode> {
         Tensor y = linear_forward(x, w, bias, resid, gate, c, z_type, &kept);
         ctx->save_for_backward({need_w ? kept.x : Tensor(), need_x ? kept.w : Tensor(),
                                 gate && (need_x || need_w || need_b) ? *gate : Tensor(), kept.z});
-        std::vector<int64_t> d{c.act, c.rpg, c.m, c.n, c.k, kept.ldx, kept.ldw, need_x, need_w, need_b, wants_grad(resid), need_g,
-                               gate ? gate->dim() : 0, gate ? gate->size(0) : 0};
+        std::vector<int64_t> d{c.act, c.rpg, c.m, c.n, c.k, c.m && c.n ? kept.x.size(1) : 0, c.m && c.n ? kept.w.size(1) : 0, need_x, need_w, need_b, wants_grad(resid), need_g,
+                               gate ? gate->dim() : 0, gate ? gate->size(0) : 0,
+                               z_type ? static_cast<int64_t>(*z_type) : 0};
         d.insert(d.end(), x.sizes().begin(), x.sizes().end());
         ctx->saved_data["call"] = std::move(d);
         return y;
@@ -184,7 +197,7 @@ struct LinearNode : public torch::autograd::Function<LinearNode> {
             return !need ? Tensor() : m && n ? at::empty(shape, opt) : at::zeros(shape, opt);
         };
         const std::vector<int64_t> gate_shape = d[12] == 2 ? std::vector<int64_t>{d[13], n} : std::vector<int64_t>{n};
-        variable_list out{fresh(need_x, at::IntArrayRef(d).slice(14)), fresh(need_w, {n, k}), fresh(need_b, {n}),
+        variable_list out{fresh(need_x, at::IntArrayRef(d).slice(15)), fresh(need_w, {n, k}), fresh(need_b, {n}),
                           need_r ? dy : Tensor(), fresh(need_g, gate_shape), Tensor()};
         if (m && n && (need_x || need_w || need_b || need_g)) {
             const at::AutoGradMode off(false);
@@ -192,12 +205,24 @@ struct LinearNode : public torch::autograd::Function<LinearNode> {
             wf_linear_grad_args a = {};
             a.workspace_bytes = wf_linear_backward_workspace(m, n, rpg);
             const Tensor work = at::empty({a.workspace_bytes}, opt.dtype(at::kByte));
-            const Tensor gate = saved[2].defined() ? saved[2].contiguous() : Tensor();
-            a.dy = dy2.const_data_ptr(), a.x = ptr(saved[0]), a.w = ptr(saved[1]), a.z = ptr(saved[3]), a.gate = ptr(gate);
+            const at::ScalarType type = dy.scalar_type();
+            Tensor gate, z;
+            if (saved[0].defined()) check_saved("linear: x", saved[0], {m, d[5]}, type, dy.device());
+            if (saved[1].defined()) check_saved("linear: weight", saved[1], {n, d[6]}, type, dy.device());
+            if (saved[2].defined()) {
+                check_saved("linear: gate", saved[2], gate_shape, type, dy.device());
+                gate = saved[2].contiguous();
+            }
+            if (saved[3].defined()) {
+                check_saved("linear: the pre-activation", saved[3], {m, up8(n)}, static_cast<at::ScalarType>(d[14]), dy.device());
+                std::tie(z, a.ldz) = as_rows(saved[3]);
+            }
+            const auto [xo, wo] = as_operands(saved[0], saved[1]);
+            a.dy = dy2.const_data_ptr(), a.x = ptr(xo.t), a.w = ptr(wo.t), a.z = ptr(z), a.gate = ptr(gate);
             a.dx = mut(out[0]), a.dw = mut(out[1]), a.db = mut(out[2]), a.dg = mut(out[4]), a.workspace = work.mutable_data_ptr();
-            a.lddy = lddy, a.ldx = d[5], a.ldw = d[6], a.ldz = up8(n), a.lddx = k, a.lddw = k, a.rows_per_group = rpg;
-            a.m = m, a.n = n, a.k = k, a.act = static_cast<int32_t>(act), a.type = code_of(dy.scalar_type());
-            a.z_type = saved[3].defined() ? code_of(saved[3].scalar_type()) : 0;
+            a.lddy = lddy, a.ldx = xo.ld, a.ldw = wo.ld, a.lddx = k, a.lddw = k, a.rows_per_group = rpg;
+            a.m = m, a.n = n, a.k = k, a.act = static_cast<int32_t>(act), a.type = code_of(type);
+            a.z_type = z.defined() ? code_of(z.scalar_type()) : 0;
             check(wf_linear_backward(&a, stream_of(dy)), "wf_linear_backward");
         }
         only_once(out);
@@ -253,8 +278,7 @@ struct NormCall {
 };
 
 struct Stats {
-    Tensor x, stats;  // x's rows; mean and rstd [2, m]
-    int64_t ldx = 0;
+    Tensor x, stats;  // x's rows [m, d]; mean and rstd [2, m]
 };
 
 Tensor norm_forward(const Tensor &x, const MaybeTensor &weight, const MaybeTensor &bias, const NormCall &c, Stats *kept) {
@@ -270,7 +294,7 @@ Tensor norm_forward(const Tensor &x, const MaybeTensor &weight, const MaybeTenso
         stats = at::empty({2, c.m}, x.options().dtype(at::kFloat));
         a.mean = stats.mutable_data_ptr<float>();
         a.rstd = a.mean + c.m;
-        *kept = Stats{x2, stats, ldx};
+        *kept = Stats{x2, stats};
     }
     a.x = x2.const_data_ptr(), a.w = ptr(w), a.b = ptr(b), a.y = y.mutable_data_ptr();
     a.ldx = ldx, a.ldy = c.d, a.rows = c.m, a.d = c.d, a.rows_per_group = c.rpg, a.eps = static_cast<float>(c.eps);
@@ -285,7 +309,7 @@ struct NormNode : public torch::autograd::Function<NormNode> {
         Tensor y = norm_forward(x, weight, bias, c, &kept);
         ctx->save_for_backward({kept.x, weight ? *weight : Tensor(), kept.stats});
         const Tensor p = weight ? *weight : bias ? *bias : Tensor();
-        std::vector<int64_t> d{c.rpg, c.m, c.d, kept.ldx, x.requires_grad(), wants_grad(weight), wants_grad(bias),
+        std::vector<int64_t> d{c.rpg, c.m, c.d, x.requires_grad(), wants_grad(weight), wants_grad(bias),
                                p.defined() ? static_cast<int64_t>(p.scalar_type()) : 0, p.defined() ? p.dim() : 0};
         if (p.defined()) d.insert(d.end(), p.sizes().begin(), p.sizes().end());
         d.insert(d.end(), x.sizes().begin(), x.sizes().end());
@@ -300,28 +324,33 @@ struct NormNode : public torch::autograd::Function<NormNode> {
         const variable_list saved = ctx->get_saved_variables();
         const c10::cuda::CUDAGuard guard(dy.device());
         const auto opt = dy.options();
-        const auto p_opt = opt.dtype(static_cast<at::ScalarType>(v[7]));
-        const at::IntArrayRef p_shape = at::IntArrayRef(v).slice(9, v[8]), x_shape = at::IntArrayRef(v).slice(9 + v[8]);
+        const auto p_opt = opt.dtype(static_cast<at::ScalarType>(v[6]));
+        const at::IntArrayRef p_shape = at::IntArrayRef(v).slice(8, v[7]), x_shape = at::IntArrayRef(v).slice(8 + v[7]);
         auto fresh = [&](bool need, at::IntArrayRef shape, const at::TensorOptions &o) {
             return !need ? Tensor() : m ? at::empty(shape, o) : at::zeros(shape, o);
         };
-        variable_list out{fresh(v[4], x_shape, opt), fresh(v[5], p_shape, p_opt), fresh(v[6], p_shape, p_opt), Tensor()};
-        if (m && (v[4] || v[5] || v[6])) {
+        variable_list out{fresh(v[3], x_shape, opt), fresh(v[4], p_shape, p_opt), fresh(v[5], p_shape, p_opt), Tensor()};
+        if (m && (v[3] || v[4] || v[5])) {
             const at::AutoGradMode off(false);
             const auto [dy2, lddy] = as_rows(dy.dim() == 2 ? dy : dy.reshape({m, d}));
             wf_layer_norm_grad_args a = {};
             a.type = code_of(dy.scalar_type());
-            a.w_type = v[8] ? code_of(static_cast<at::ScalarType>(v[7])) : a.type;
+            a.w_type = v[7] ? code_of(static_cast<at::ScalarType>(v[6])) : a.type;
             Tensor work;
-            if (v[5] || v[6]) {
+            if (v[4] || v[5]) {
                 a.workspace_bytes = wf_layer_norm_backward_workspace(m, d, rpg, a.type);
                 work = at::empty({a.workspace_bytes}, opt.dtype(at::kByte));
             }
-            const Tensor w = saved[1].defined() ? saved[1].contiguous() : Tensor();
-            a.dy = dy2.const_data_ptr(), a.x = saved[0].const_data_ptr(), a.w = ptr(w);
-            a.mean = saved[2].const_data_ptr<float>(), a.rstd = a.mean + m;
+            check_saved("layer_norm: x", saved[0], {m, d}, dy.scalar_type(), dy.device());
+            check_saved("layer_norm: the statistics", saved[2], {2, m}, at::kFloat, dy.device());
+            if (saved[1].defined())
+                check_saved("layer_norm: weight", saved[1], p_shape, static_cast<at::ScalarType>(v[6]), dy.device());
+            const Tensor w = saved[1].defined() ? saved[1].contiguous() : Tensor(), stats = saved[2].contiguous();
+            const auto [x2, ldx] = as_rows(saved[0]);
+            a.dy = dy2.const_data_ptr(), a.x = x2.const_data_ptr(), a.w = ptr(w);
+            a.mean = stats.const_data_ptr<float>(), a.rstd = a.mean + m;
             a.dx = mut(out[0]), a.dw = mut(out[1]), a.db = mut(out[2]), a.workspace = mut(work);
-            a.lddy = lddy, a.ldx = v[3], a.lddx = d, a.rows = m, a.d = d, a.rows_per_group = rpg;
+            a.lddy = lddy, a.ldx = ldx, a.lddx = d, a.rows = m, a.d = d, a.rows_per_group = rpg;
             check(wf_layer_norm_backward(&a, stream_of(dy)), "wf_layer_norm_backward");
         }
         only_once(out);
