@@ -125,8 +125,13 @@ struct Epilogue {
 };
 
 // float32 -> f16, clamped to f16's range: the kept z is read by the slopes alone, which are constant out there, and
-// f16's 11 bits keep a bf16 layer's gradients as exact as their own rounding
-__device__ __forceinline__ uint32_t pack2_sat(float a, float b) {
+// f16's 11 bits keep a bf16 layer's gradients as exact as their own rounding. relu's slope steps at 0, so there no positive z
+// may round to 0 (f16 ends at 2^-24, bf16 layers reach much further down).
+__device__ __forceinline__ uint32_t pack2_sat(float a, float b, bool relu) {
+    if (relu) {
+        a = a > 0.f ? fmaxf(a, 0x1p-24f) : a;
+        b = b > 0.f ? fmaxf(b, 0x1p-24f) : b;
+    }
     uint32_t w;
     asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(w) : "f"(b), "f"(a));
     return w;
@@ -194,7 +199,8 @@ __device__ __forceinline__ void finish4(const Epilogue &e, float (&v)[R][4], int
             const int at = row + r * step;
             if (at >= row_end) continue;
             if (e.keep == KEEP_F16) {
-                const uint32_t w[2] = {pack2_sat(v[r][0], v[r][1]), pack2_sat(v[r][2], v[r][3])};
+                const bool relu = e.act == WF_ACT_RELU;
+                const uint32_t w[2] = {pack2_sat(v[r][0], v[r][1], relu), pack2_sat(v[r][2], v[r][3], relu)};
                 uint16_t *dst = static_cast<uint16_t *>(e.kept) + at * e.ld_kept + col;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
@@ -591,7 +597,7 @@ __device__ __forceinline__ void finish_half(float (&v)[32], Warp32 &w, const Epi
             } else {
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    p[i] = e.keep == KEEP_F16 ? pack2_sat(v[2 * i], v[2 * i + 1]) : pack2<T>(v[2 * i], v[2 * i + 1]);
+                    p[i] = e.keep == KEEP_F16 ? pack2_sat(v[2 * i], v[2 * i + 1], e.act == WF_ACT_RELU) : pack2<T>(v[2 * i], v[2 * i + 1]);
                 // z's last store has been read; y's may go on, and is the last one where y leaves by TMA at all
                 if (w.lane == 0) w.y.tma ? bulk_wait_read1() : bulk_wait_read_all();
                 __syncwarp();

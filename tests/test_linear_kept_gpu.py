@@ -57,3 +57,30 @@ def test_kept_values_in_every_layout(cuda, m, n, k, kind, z_name):
             else:
                 assert torch.equal(y[:, :n], first[0][:, :n]) and torch.equal(z[:, :n], first[1][:, :n]), (ldy, ldz)
     assert wf("enhancers.fused_linear").status() == 0
+
+
+def _exact_step(torch, dtype, kind, m, k, n, xs, ws, ds):
+    """A training step on small integers times powers of two (x: xs, weight: ws, dy: ds), whose products and sums float32 holds
+    exactly: (z, dy, dx, dw) in float64 for a slope that is 1 above 0, 0 below, and half of both at 0 but for relu; and the
+    step's own dx and dw."""
+    g = torch.Generator(device="cuda").manual_seed(m + n)
+
+    def integers(*shape, s):
+        return (torch.randint(-3, 4, shape, device="cuda", generator=g) * s).to(dtype)
+    x, w, dy = integers(m, k, s=xs).requires_grad_(), integers(n, k, s=ws).requires_grad_(), integers(m, n, s=ds)
+    y = wf("enhancers.fused_linear").linear(x, w, activation=kind)
+    got = torch.autograd.grad(y, (x, w), dy)
+    x, w, dy = x.detach().double(), w.detach().double(), dy.double()
+    z = x @ w.t()
+    dz = dy * torch.where(z > 0, 1.0, torch.where(z < 0, 0.0, 0.0 if kind == "relu" else 0.5)).double()
+    return z, (dz @ w, dz.t() @ x), got
+
+
+@pytest.mark.parametrize("m,n", [(24, 512), (300, 61), (3000, 2048), (3000, 2041)])
+def test_relu_of_small_values(cuda, m, n):
+    """z of a few steps of 2^-40, far below what f16 holds: the slope is 1 wherever z is above 0."""
+    import torch
+    z, want, got = _exact_step(torch, torch.bfloat16, "relu", m, 72, n, 2.0 ** -20, 2.0 ** -20, 1.0)
+    assert bool((z.abs() < 2.0 ** -25).all())
+    for nm, a, b in zip(("dx", "dw"), got, want):
+        assert torch.equal(a, b.to(torch.bfloat16)), nm
