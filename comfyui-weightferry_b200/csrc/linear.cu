@@ -1082,7 +1082,9 @@ extern "C" WF_API int wf_linear(const wf_linear_args *args, wf_stream_t stream) 
     if (a.z != nullptr) {
         if (a.z_type != WF_F32 && a.z_type != WF_F16 && a.z_type != a.type) return WF_ERR_UNSUPPORTED;
         if (a.ldz < a.n || !aligned_to(a.z, dtype_size(a.z_type))) return WF_ERR_ARG;
-        keep = a.z_type == WF_F32 ? KEEP_F32 : a.z_type == WF_F16 && a.type != WF_F16 ? KEEP_F16 : KEEP_SAME;
+        // an f16 layer's own type is the slope's f16 too, where there is an activation: z past f16's range would be infinite
+        // otherwise, and the slope of infinity NaN
+        keep = a.z_type == WF_F32 ? KEEP_F32 : a.z_type == WF_F16 && (a.type != WF_F16 || a.act != WF_ACT_NONE) ? KEEP_F16 : KEEP_SAME;
     }
     const Product p{a.x, a.w, a.ldx, a.ldw, a.m, a.n, a.k};
     const Epilogue e{a.bias, a.gate, a.resid, a.y, a.z, a.ld_resid, a.ldy, a.ldz, a.rows_per_group, a.act, keep, false};

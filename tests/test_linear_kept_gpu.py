@@ -84,3 +84,40 @@ def test_relu_of_small_values(cuda, m, n):
     assert bool((z.abs() < 2.0 ** -25).all())
     for nm, a, b in zip(("dx", "dw"), got, want):
         assert torch.equal(a, b.to(torch.bfloat16)), nm
+
+
+@pytest.mark.parametrize("kind", ["relu", "silu", "gelu", "gelu_tanh"])
+@pytest.mark.parametrize("m,n", [(24, 512), (300, 61), (3000, 2048), (3000, 2041)])
+def test_f16_values_past_its_range(cuda, kind, m, n):
+    """An f16 layer whose z are multiples of 2^13, most of them past 65504: the slopes are 0 and 1 out there (1/2 at 0), and
+    the gradients finite."""
+    import torch
+    z, want, got = _exact_step(torch, torch.float16, kind, m, 72, n, 2.0 ** 8, 2.0 ** 5, 2.0 ** -8)
+    assert bool((z > 65504).any()) and bool((z < -65504).any())
+    for nm, a, b in zip(("dx", "dw"), got, want):
+        assert torch.equal(a, b.to(torch.float16)), nm
+
+
+@pytest.mark.parametrize("m,n", [(24, 512), (300, 61), (3000, 2048), (3000, 2041)])
+def test_f16_relu_of_small_values(cuda, m, n):
+    """z of a few steps of 2^-28 in an f16 layer, which itself rounds most of them to 0: their slope is 1 all the same."""
+    import torch
+    z, want, got = _exact_step(torch, torch.float16, "relu", m, 72, n, 2.0 ** -14, 2.0 ** -14, 1.0)
+    assert bool((z[z > 0] <= 2.0 ** -25).any())
+    for nm, a, b in zip(("dx", "dw"), got, want):
+        assert torch.equal(a, b.to(torch.float16)), nm
+
+
+def test_nan_stays_nan(cuda):
+    """A NaN on the way into z is one in the gradient of its row and of its inputs' column, for every smooth slope."""
+    import torch
+    for dtype in (torch.bfloat16, torch.float16):
+        for m, n in ((24, 512), (3000, 2048)):
+            for kind in ("silu", "gelu", "gelu_tanh"):
+                x = torch.ones((m, 72), device="cuda", dtype=dtype)
+                x[5, 3] = float("nan")
+                w = torch.ones((n, 72), device="cuda", dtype=dtype)
+                x.requires_grad_(), w.requires_grad_()
+                y = wf("enhancers.fused_linear").linear(x, w, activation=kind)
+                dx, dw = torch.autograd.grad(y, (x, w), torch.ones_like(y))
+                assert bool(torch.isnan(dx[5]).all()) and bool(torch.isfinite(dx[6]).all()) and bool(torch.isnan(dw).all())
