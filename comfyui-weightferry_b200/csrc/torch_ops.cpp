@@ -168,10 +168,11 @@ struct LinearNode : public torch::autograd::Function<LinearNode> {
                           const MaybeTensor &resid, const MaybeTensor &gate, const LinearCall &c) {
         const bool need_x = x.requires_grad(), need_w = w.requires_grad(), need_b = wants_grad(bias), need_g = wants_grad(gate);
         // How z is kept. The activation's slope is constant where f16 ends, so f16 (clamped, 11 bits) keeps it more exactly
-        // than bf16 would; the gate's gradient reads activation(z) itself: exactly (f32), or as the layer rounds it where
-        // there is no activation.
+        // than bf16 would. The gate's gradient reads activation(z) itself: exactly (f32), or in a bf16 layer without an
+        // activation as that layer rounds it (two bytes a value less to write and read). f16 does not hold every z of a finite
+        // gate * z.
         std::optional<at::ScalarType> z_type;
-        if (need_g) z_type = c.act ? at::kFloat : x.scalar_type();
+        if (need_g) z_type = c.act || x.scalar_type() == at::kHalf ? at::kFloat : x.scalar_type();
         else if (c.act && (need_x || need_w || need_b)) z_type = at::kHalf;
         Kept kept;
         Tensor y = linear_forward(x, w, bias, resid, gate, c, z_type, &kept);

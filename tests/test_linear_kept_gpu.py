@@ -121,3 +121,23 @@ def test_nan_stays_nan(cuda):
                 y = wf("enhancers.fused_linear").linear(x, w, activation=kind)
                 dx, dw = torch.autograd.grad(y, (x, w), torch.ones_like(y))
                 assert bool(torch.isnan(dx[5]).all()) and bool(torch.isfinite(dx[6]).all()) and bool(torch.isnan(dw).all())
+
+
+@pytest.mark.parametrize("m,n", [(24, 512), (300, 61), (3000, 2048), (3000, 2041)])
+def test_f16_gate_of_values_past_its_range(cuda, m, n):
+    """residual + gate * z is finite where z is not, in f16: so is the gate's gradient, the sum of dy z, and rows of dy = 0
+    count nothing in it."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(m + n)
+
+    def integers(*shape, s):
+        return (torch.randint(-3, 4, shape, device="cuda", generator=g) * s).half()
+    x, w, dy = integers(m, 72, s=2.0 ** 8), integers(n, 72, s=2.0 ** 5), integers(m, n, s=2.0 ** -12)
+    dy[m // 2:] = 0
+    residual = integers(m, n, s=1.0)
+    gate = torch.full((n,), 2.0 ** -10, device="cuda", dtype=torch.float16, requires_grad=True)
+    y = wf("enhancers.fused_linear").linear(x, w, residual=residual, gate=gate)
+    dg, = torch.autograd.grad(y, gate, dy)
+    z = x.double() @ w.double().t()
+    assert bool((z.abs() > 65504).any()) and bool(torch.isfinite(y).all())
+    assert torch.equal(dg, (dy.double() * z).sum(0).half())  # the float32 sums are exact: multiples of 2, below 2^25
