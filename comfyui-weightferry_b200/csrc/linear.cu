@@ -949,8 +949,11 @@ int launch_pair(const Product &p, const Epilogue &e0, int dev, cudaStream_t stre
     // 16-byte accesses to the bias, the gate and the residual
     e.vec_bias = vec8_ok(e.bias, 0);
     e.vec = p.n % 8 == 0 && vec8_ok(e.bias, 0) && vec8_ok(e.gate, p.n) && vec8_ok(e.resid, e.ld_resid);
-    const bool tma_out = vec8_ok(e.out, e.ld_out);
-    const bool tma_kept = (e.keep == KEEP_F16 || e.keep == KEEP_SAME) && vec8_ok(e.kept, e.ld_kept);
+    // A TMA store clips at whole 16-byte pieces: behind a row of n values it writes zeros up to the next multiple of 8 (as
+    // measured). y's neighbours are the caller's; z's rows have room for it where their pitch is that multiple.
+    const bool tma_out = p.n % 8 == 0 && vec8_ok(e.out, e.ld_out);
+    const bool tma_kept = (e.keep == KEEP_F16 || e.keep == KEEP_SAME) && vec8_ok(e.kept, e.ld_kept) &&
+                          (p.n % 8 == 0 || e.ld_kept == (p.n + 7) / 8 * 8);
     CUtensorMap ma, mb, mo = {}, mk = {};
     int rc = A_ROWS ? operand_map(&ma, p.a, p.c, p.m, p.lda, BC) : operand_map(&ma, p.a, p.m, p.c, p.lda, 128);
     if (rc == WF_OK) rc = B_ROWS ? operand_map(&mb, p.b, p.c, p.n, p.ldb, BC) : operand_map(&mb, p.b, p.n, p.c, p.ldb, BN / 2);

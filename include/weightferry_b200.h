@@ -202,7 +202,8 @@ enum { WF_ACT_NONE = 0, WF_ACT_RELU = 1, WF_ACT_SILU = 2, WF_ACT_GELU = 3 /* erf
  * gate [ceil(m / rows_per_group), n] contiguous, resid and y [m, n]; bias, gate and resid may be NULL (0, 1, 0). float32
  * throughout, one rounding to y. z (may be NULL) keeps the pre-activation for the backward pass as z_type: WF_F32,
  * `type` or WF_F16. Under bf16, or an activation, WF_F16 is for the slope only: clamped to f16's range, and no positive z
- * rounds to 0 under WF_ACT_RELU. y may be resid. m, n >= 0, k >= 1. */
+ * rounds to 0 under WF_ACT_RELU. z holds m * ldz values, and where ldz is n rounded up to a multiple of 8 those behind a row
+ * may be written too. y may be resid. m, n >= 0, k >= 1. */
 typedef struct wf_linear_args {
     const void *x, *w, *bias, *gate, *resid;
     void *y, *z;

@@ -141,3 +141,29 @@ def test_f16_gate_of_values_past_its_range(cuda, m, n):
     z = x.double() @ w.double().t()
     assert bool((z.abs() > 65504).any()) and bool(torch.isfinite(y).all())
     assert torch.equal(dg, (dy.double() * z).sum(0).half())  # the float32 sums are exact: multiples of 2, below 2^25
+
+
+@pytest.mark.parametrize("m,n,k", [(5001, 2041, 72), (5001, 2044, 72), (700, 61, 64), (3, 61, 64)])
+def test_columns_behind_the_rows_are_left_alone(cuda, m, n, k):
+    """Widths that are no multiple of 8 at pitches that are: y, z past its next multiple of 8, dx and dw write nothing else."""
+    import torch
+    x = torch.ones((m, k), device="cuda", dtype=torch.bfloat16)
+    w = torch.ones((n, k), device="cuda", dtype=torch.bfloat16)
+    up = (n + 7) // 8 * 8
+    for ld in (up, up + 8, up + 64):
+        for z_type in (torch.float16, torch.float32):
+            y, z = _forward(torch, x, w, "relu", z_type, ld, ld)
+            assert bool((y[:, :n] == k).all()) and bool((y[:, n:] == -7).all()), ld
+            assert bool((z[:, :n] == k).all()) and bool((z[:, n if ld > up else up:] == -7).all()), ld
+        # a product of m x n and n x k with the widths' parts exchanged: dx [m, n] = dy [m, k] w [k, n], dw [k, n]
+        xw = torch.ones((m, up), device="cuda", dtype=torch.bfloat16)
+        wk = torch.ones((k, up), device="cuda", dtype=torch.bfloat16)
+        dx = torch.full((m, ld), -7.0, device="cuda", dtype=torch.bfloat16)
+        dw = torch.full((k, ld), -7.0, device="cuda", dtype=torch.bfloat16)
+        size = wf("_ext").lib().wf_linear_backward_workspace(m, k, m)
+        work = torch.empty((size,), device="cuda", dtype=torch.uint8)
+        dense_cabi.launch("wf_linear_backward", dense_cabi.LINEAR_GRAD_ARGS.pack(
+            x.data_ptr(), xw.data_ptr(), wk.data_ptr(), 0, 0, dx.data_ptr(), dw.data_ptr(), 0, 0, work.data_ptr(), k, up, up, 0, ld,
+            ld, m, size, m, k, n, 0, 1, 0, 0))
+        assert bool((dx[:, :n] == k).all()) and bool((dx[:, n:] == -7).all()), ld
+        assert bool((dw[:, :n] == float(torch.tensor(float(m)).bfloat16())).all()) and bool((dw[:, n:] == -7).all()), ld
