@@ -73,6 +73,7 @@ SIGNATURES = {
     "wf_linear_backward_workspace": (ctypes.c_int64, [ctypes.c_int64] * 3),
     "wf_linear_backward": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
     "wf_linear_status": (ctypes.c_int, [ctypes.POINTER(ctypes.c_int)]),
+    "wf_linear_set_wait_limit": (ctypes.c_int, [ctypes.c_uint64]),
     "wf_copy_rows16": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]),
     "wf_layer_norm": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
     "wf_layer_norm_backward_workspace": (ctypes.c_int64, [ctypes.c_int64] * 3 + [ctypes.c_int]),

@@ -26,18 +26,28 @@ constexpr int BC = 64;  // contraction values of a stage: 128 bytes of 16-bit va
 
 __device__ int g_linear_status;  // 0 ok; 1 producer wait expired; 2 MMA wait expired; 3 epilogue wait expired
 
-// Wait for the phase of the given parity, at most kWaitLimitNs; gives up early when another role aborted.
-__device__ __forceinline__ bool pipe_wait(uint32_t a, uint32_t parity, volatile int *abort_flag, int code) {
+// What a pipeline wait needs to know beside its barrier: the CTA's abort flag, a word in mapped host memory that tells the
+// host's next call, and the time limit.
+struct Waits {
+    volatile int *abort_flag, *alarm;
+    uint64_t limit_ns;
+};
+
+// Wait for the phase of the given parity, at most limit_ns; gives up early when another role aborted. A try suspends for some
+// microseconds, so that a limit shortened by a test is looked at after each.
+__device__ __forceinline__ bool pipe_wait(uint32_t a, uint32_t parity, const Waits &w, int code) {
     if (mbar_try(a, parity)) return true;
     const uint64_t t0 = global_ns();
+    const int tries = w.limit_ns < 1000000u ? 1 : 32;
     while (true) {
 #pragma unroll 1
-        for (int i = 0; i < 32; ++i)
+        for (int i = 0; i < tries; ++i)
             if (mbar_try(a, parity)) return true;
-        if (*abort_flag) return false;
-        if (global_ns() - t0 > kWaitLimitNs) {
-            *abort_flag = 1;
+        if (*w.abort_flag) return false;
+        if (global_ns() - t0 > w.limit_ns) {
+            *w.abort_flag = 1;
             atomicCAS(&g_linear_status, 0, code);
+            *w.alarm = code;
             return false;
         }
     }
@@ -118,6 +128,8 @@ struct Epilogue {
     const void *resid;  // [m, ld_resid] or null
     void *out;          // [m, ld_out]
     void *kept;         // [m, ld_kept] or null
+    int *alarm;         // set when a wait runs out of time ...
+    uint64_t wait_ns;   // ... and when that is
     int64_t ld_resid, ld_out, ld_kept, rows_per_group;
     int act, keep;
     bool vec;  // every pointer 8-byte aligned and every row pitch (n too, where it is one) a multiple of 4 values
@@ -314,14 +326,14 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_const
     fence_after();
     const uint32_t tmem = s_tmem_base;
     wait_prior_grid();
-    volatile int *abort_flag = &s_abort;
+    const Waits waits{&s_abort, epi.alarm, epi.wait_ns};
 
     if (warp == 4) {
         int stage = 0;
         uint32_t phase = 0;
         int issued = 0;
         for (int s = c_lo; s < c_hi; ++s, ++issued) {
-            if (!__all_sync(0xFFFFFFFFu, pipe_wait(empty0 + 8 * stage, phase ^ 1u, abort_flag, 1))) break;
+            if (!__all_sync(0xFFFFFFFFu, pipe_wait(empty0 + 8 * stage, phase ^ 1u, waits, 1))) break;
             const uint32_t bar = full0 + 8 * stage, p = ring0 + stage * S::stage, q = p + S::p_bytes;
             if (elect_one()) {
                 mbar_expect_tx(bar, S::stage);
@@ -349,7 +361,7 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_const
         int stage = 0;
         uint32_t phase = 0;
         for (int s = c_lo; s < c_hi; ++s) {
-            if (!__all_sync(0xFFFFFFFFu, pipe_wait(full0 + 8 * stage, phase, abort_flag, 2))) break;
+            if (!__all_sync(0xFFFFFFFFu, pipe_wait(full0 + 8 * stage, phase, waits, 2))) break;
             const uint32_t p = p0 + stage * (S::stage >> 4), q = q0 + stage * (S::stage >> 4);
             if (elect_one()) {
 #pragma unroll
@@ -366,7 +378,7 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_const
         __syncwarp();
     } else if (warp < 4) {
         // lane w * 32 + l of tensor memory is column j0 + 32 w + l
-        const bool ok = __all_sync(0xFFFFFFFFu, pipe_wait(done, 0, abort_flag, 3) && !*abort_flag);
+        const bool ok = __all_sync(0xFFFFFFFFu, pipe_wait(done, 0, waits, 3) && !*waits.abort_flag);
         fence_after();
         if (ok) {  // the NT rows to part[row][column]
             float *part = reinterpret_cast<float *>(ring) + warp * 32 + lane;
@@ -387,6 +399,10 @@ linear_tile_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_const
     }
     fence_before();
     __syncthreads();
+    if (*waits.abort_flag) {  // settled: every role has stopped. The tile's sums become NaN, here and in the CTAs that add these parts
+        for (int i = threadIdx.x; i < NT * TILE_J; i += TILE_THREADS) reinterpret_cast<float *>(ring)[i] = __int_as_float(0x7FFFFFFF);
+        __syncthreads();
+    }
     if (split > 1) cluster_sync();
     fence_after();
     if (warp == 5)
@@ -646,6 +662,19 @@ __device__ __forceinline__ void finish_half(float (&v)[32], Warp32 &w, const Epi
     }
 }
 
+// After a wait that ran out of time: NaN in an epilogue warp's rows of every tile that it has not written.
+__device__ __noinline__ void fill_nan(const Epilogue &e, int tile, int n_clusters, int m, int n, int band, int rank, int quarter, int half) {
+    const int tiles_m = (m + 255) / 256, tiles_n = (n + BN - 1) / BN, lane = threadIdx.x & 31;
+    for (; tile < tiles_m * tiles_n; tile += n_clusters) {
+        int mi, ni;
+        tile_coords(tile, tiles_m, tiles_n, band, mi, ni);
+        const int row0 = mi * 256 + rank * 128 + quarter * 32, col0 = ni * BN + half * (BN / 2);
+        for (int row = row0; row < min(row0 + 32, m); ++row)
+            for (int col = col0 + lane; col < min(col0 + BN / 2, n); col += 32)
+                static_cast<uint16_t *>(e.out)[row * e.ld_out + col] = 0x7FFF;  // bf16's and f16's
+    }
+}
+
 // FULL: the forward pass's epilogue; else D is rounded and stored. KEEP: z is kept
 template <bool A_ROWS, bool B_ROWS, int T, bool FULL, bool KEEP>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
@@ -694,7 +723,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
     fence_after();
     const uint32_t tmem = s_tmem_base;
     wait_prior_grid();
-    volatile int *abort_flag = &s_abort;
+    const Waits waits{&s_abort, epi.alarm, epi.wait_ns};
 
     if (warp == 8) {
         if (elect_one()) {
@@ -710,7 +739,7 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
             tile_coords(tile, tiles_m, tiles_n, band, mi, ni);
             const int i0 = mi * 256 + static_cast<int>(rank) * 128, j0 = ni * BN + static_cast<int>(rank) * (BN / 2);
             for (int s = 0; s < steps; ++s) {
-                if (!__all_sync(0xFFFFFFFFu, pipe_wait(empty0 + 8 * stage, phase ^ 1u, abort_flag, 1))) { ok = false; break; }
+                if (!__all_sync(0xFFFFFFFFu, pipe_wait(empty0 + 8 * stage, phase ^ 1u, waits, 1))) { ok = false; break; }
                 const uint32_t bar = (full0 + 8 * stage) & kPeerBitMask;  // the even CTA's
                 const uint32_t a = ring0 + stage * PAIR_STAGE, b = a + PAIR_HALF;
                 if (elect_one()) {
@@ -751,11 +780,11 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
             uint32_t phase = 0, acc_phase = 0;
             bool ok = true;
             for (int tile = cluster_id; tile < n_tiles && ok; tile += n_clusters) {
-                if (!__all_sync(0xFFFFFFFFu, pipe_wait(tempty0 + 8 * acc, acc_phase ^ 1u, abort_flag, 2))) break;
+                if (!__all_sync(0xFFFFFFFFu, pipe_wait(tempty0 + 8 * acc, acc_phase ^ 1u, waits, 2))) break;
                 fence_after();
                 const uint32_t d = tmem + static_cast<uint32_t>(acc * BN);
                 for (int s = 0; s < steps; ++s) {
-                    if (!__all_sync(0xFFFFFFFFu, pipe_wait(full0 + 8 * stage, phase, abort_flag, 2))) { ok = false; break; }
+                    if (!__all_sync(0xFFFFFFFFu, pipe_wait(full0 + 8 * stage, phase, waits, 2))) { ok = false; break; }
                     const uint32_t a = a0 + stage * (PAIR_STAGE >> 4), b = b0 + stage * (PAIR_STAGE >> 4);
                     if (elect_one()) {
 #pragma unroll
@@ -801,7 +830,10 @@ linear_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
                 asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;"
                              ::"l"(static_cast<const uint16_t *>(w.resid) + col0), "r"(static_cast<uint32_t>(min(BN / 2, n - col0)) * 2u)
                              : "memory");
-            if (!__all_sync(0xFFFFFFFFu, pipe_wait(tfull0 + 8 * acc, acc_phase, abort_flag, 3))) break;
+            if (!__all_sync(0xFFFFFFFFu, pipe_wait(tfull0 + 8 * acc, acc_phase, waits, 3))) {
+                fill_nan(epi, tile, n_clusters, m, n, band, static_cast<int>(rank), quarter, half);
+                break;
+            }
             fence_after();
             const uint32_t taddr = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * BN + half * (BN / 2));
             uint32_t r[32], b[16], g[16], res[16];
@@ -1054,15 +1086,47 @@ bool vec4_ok(const void *p, int64_t ld) { return p == nullptr || (aligned_to(p, 
 int64_t dz_bytes(int64_t m, int64_t n) { return m * ((n + 7) / 8 * 8) * 2; }
 
 Epilogue plain_epilogue(void *out, int64_t ld) {
-    return Epilogue{nullptr, nullptr, nullptr, out, nullptr, 0, ld, 0, 1, WF_ACT_NONE, KEEP_NONE, false};
+    return Epilogue{nullptr, nullptr, nullptr, out, nullptr, nullptr, 0, 0, ld, 0, 1, WF_ACT_NONE, KEEP_NONE, false};
+}
+
+// A word of each device in mapped host memory, set by a kernel whose wait ran out of time and looked at by every call: no
+// call is needed to learn of it. Allocated by the first call, which a stream capture may surround.
+int *alarm_words() {
+    static int *words = [] {
+        int *p = nullptr;
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        if (cudaHostAlloc(reinterpret_cast<void **>(&p), 64 * sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped) != cudaSuccess) {
+            cudaGetLastError();
+            p = nullptr;
+        }
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        if (p != nullptr) std::fill(p, p + 64, 0);
+        return p;
+    }();
+    return words;
+}
+
+std::atomic<uint64_t> g_wait_ns{kWaitLimitNs};  // wf_linear_set_wait_limit
+
+// the current device's word, or the status that refuses the call
+int alarm_of_device(int **word) {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    int *words = alarm_words();
+    if (dev < 0 || dev >= 64 || words == nullptr) return WF_ERR_DEVICE;
+    *word = words + dev;
+    return *static_cast<volatile int *>(*word) != 0 ? WF_ERR_EXPIRED : WF_OK;
 }
 
 template <bool A_ROWS, bool B_ROWS>
 int run_product(const Product &p, Epilogue e, int type, cudaStream_t stream) {
     e.vec = vec4_ok(e.bias, 0) && vec4_ok(e.gate, p.n) && vec4_ok(e.resid, e.ld_resid) && vec4_ok(e.out, e.ld_out) &&
             (e.keep != KEEP_SAME || vec4_ok(e.kept, e.ld_kept));
-    const int rc = check_device();
+    int rc = check_device();
+    if (rc == WF_OK) rc = alarm_of_device(&e.alarm);
     if (rc != WF_OK) return rc;
+    e.wait_ns = g_wait_ns.load(std::memory_order_relaxed);
     return type == WF_BF16 ? dispatch<A_ROWS, B_ROWS, WF_BF16>(p, e, stream) : dispatch<A_ROWS, B_ROWS, WF_F16>(p, e, stream);
 }
 
@@ -1090,7 +1154,7 @@ extern "C" WF_API int wf_linear(const wf_linear_args *args, wf_stream_t stream) 
         keep = a.z_type == WF_F32 ? KEEP_F32 : a.z_type == WF_F16 && (a.type != WF_F16 || a.act != WF_ACT_NONE) ? KEEP_F16 : KEEP_SAME;
     }
     const Product p{a.x, a.w, a.ldx, a.ldw, a.m, a.n, a.k};
-    const Epilogue e{a.bias, a.gate, a.resid, a.y, a.z, a.ld_resid, a.ldy, a.ldz, a.rows_per_group, a.act, keep, false};
+    const Epilogue e{a.bias, a.gate, a.resid, a.y, a.z, nullptr, 0, a.ld_resid, a.ldy, a.ldz, a.rows_per_group, a.act, keep, false};
     return run_product<false, false>(p, e, a.type, reinterpret_cast<cudaStream_t>(stream));
 }
 
@@ -1120,6 +1184,8 @@ extern "C" WF_API int wf_linear_backward(const wf_linear_grad_args *args, wf_str
                                       a.workspace_bytes < wf_linear_backward_workspace(a.m, a.n, a.rows_per_group)))
         return WF_ERR_ARG;
     int rc = check_device();
+    int *word = nullptr;
+    if (rc == WF_OK) rc = alarm_of_device(&word);  // before the first launch, not between two
     if (rc != WF_OK) return rc;
     const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     const void *dz = a.dy;
@@ -1145,6 +1211,11 @@ extern "C" WF_API int wf_linear_backward(const wf_linear_grad_args *args, wf_str
     return rc;
 }
 
+extern "C" WF_API int wf_linear_set_wait_limit(uint64_t limit_ns) {
+    wf::g_wait_ns.store(limit_ns == 0 ? wf::kWaitLimitNs : std::min<uint64_t>(limit_ns, wf::kWaitLimitNs));
+    return WF_OK;
+}
+
 extern "C" WF_API int wf_linear_status(int *status) {
     if (status == nullptr) return WF_ERR_ARG;
     int v = 0;
@@ -1153,6 +1224,8 @@ extern "C" WF_API int wf_linear_status(int *status) {
     if (v != 0) {
         const int zero = 0;
         cudaMemcpyToSymbol(wf::g_linear_status, &zero, sizeof(int));
+        int *word = nullptr;
+        if (wf::alarm_of_device(&word) == WF_ERR_EXPIRED) *word = 0;
     }
     *status = v;
     return WF_OK;

@@ -59,6 +59,7 @@ extern "C" WF_API const char *wf_status_string(int status) {
         case WF_ERR_UNSUPPORTED: return "unsupported type or mode";
         case WF_ERR_SHAPE: return "byte count and value count disagree for this format";
         case WF_ERR_DEVICE: return "no usable sm_100 device is current";
+        case WF_ERR_EXPIRED: return "a wait of an earlier dense linear call ran out of time; its output is NaN (wf_linear_status clears this)";
         case WF_ERR_TOO_LARGE: return "problem larger than the library's fixed buffer (no-allocation entry point)";
         default: break;
     }

@@ -27,8 +27,8 @@ def linear(x, weight, bias=None, activation="none", residual=None, gate=None, ro
 
 
 def status():
-    """0, or the code of a pipeline wait of the linear kernels that ran out of time (their output is then incomplete);
-    synchronises and clears it."""
+    """0, or the code of a pipeline wait of the linear kernels that ran out of time: what they could not compute is NaN, and
+    further calls on the device raise RuntimeError until this has been read. Synchronises and clears it."""
     v = ctypes.c_int()
     _ext.check(_ext.lib().wf_linear_status(ctypes.byref(v)), "wf_linear_status")
     return v.value

@@ -34,7 +34,8 @@ enum {
     WF_ERR_UNSUPPORTED = -2, /* a GGML type id (or mode) this library does not decode */
     WF_ERR_SHAPE = -3,       /* byte count and value count disagree for the format */
     WF_ERR_DEVICE = -4,      /* the current device is not an sm_100 part, or no device */
-    WF_ERR_TOO_LARGE = -5    /* the problem exceeds a fixed-size buffer of the library */
+    WF_ERR_TOO_LARGE = -5,   /* the problem exceeds a fixed-size buffer of the library */
+    WF_ERR_EXPIRED = -6      /* a kernel of an earlier call ran out of time in a wait and left NaN (wf_linear_status) */
 };
 
 enum { WF_F16 = 0, WF_BF16 = 1, WF_F32 = 2 };
@@ -227,8 +228,13 @@ typedef struct wf_linear_grad_args {
 WF_API int64_t wf_linear_backward_workspace(int64_t m, int64_t n, int64_t rows_per_group);
 WF_API int wf_linear_backward(const wf_linear_grad_args *args, wf_stream_t stream);
 
-/* Status word of the dense linear layer's kernels, as wf_w8a8_gemm_status. Reading it synchronises and clears it. */
+/* Status word of the dense linear layer's kernels, as wf_w8a8_gemm_status. A kernel whose wait ran out of time fills what it
+ * could not compute with NaN, and every call after it on the device is refused with WF_ERR_EXPIRED until the word has been
+ * read. Reading it synchronises and clears it. */
 WF_API int wf_linear_status(int *status);
+
+/* Test hook, as wf_w8a8_gemm_set_wait_limit: the time limit of these kernels' pipeline waits in nanoseconds (0: 2 s). */
+WF_API int wf_linear_set_wait_limit(uint64_t limit_ns);
 
 /* One or two copies of rows x cols 16-bit values to another row pitch (any 2-byte alignment) in one launch. */
 typedef struct wf_copy_rows {
