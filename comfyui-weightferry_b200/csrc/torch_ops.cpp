@@ -5,13 +5,16 @@
 //
 // Every call runs on x's device and PyTorch's current stream there (the backward pass on the forward pass's, as PyTorch's
 // engine sets it) and allocates with PyTorch's allocator, workspaces too, so calls may overlap on several streams and be
-// captured into CUDA graphs. Refused arguments raise ValueError or TypeError, a refused launch RuntimeError.
+// captured into CUDA graphs. Refused arguments raise ValueError or TypeError, forward-mode tangents and traces
+// NotImplementedError, a refused launch RuntimeError.
 
 #include <torch/extension.h>
 
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <c10/core/AutogradState.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <optional>
 #include <string>
@@ -125,6 +128,14 @@ void only_once(variable_list &grads) {
     size_t i = 0;
     for (Tensor &g : grads)
         if (g.defined()) g = live[i++];
+}
+
+// Tangents and traces, which the operations would drop without a word: their outputs come out of kernels that neither sees.
+void refuse_unseen(const char *what, std::initializer_list<const Tensor *> tensors) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing(), what, ": a call cannot be traced");
+    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+    for (const Tensor *t : tensors)
+        TORCH_CHECK_NOT_IMPLEMENTED(t == nullptr || !t->_fw_grad(0).defined(), what, ": no forward-mode derivatives");
 }
 
 // ------------------------------------------------------------------------------------------------ dense linear layer
@@ -264,6 +275,7 @@ Tensor linear(const Tensor &x, const Tensor &weight, const MaybeTensor &bias, co
     }
     for (const auto &[name, p] : rest)
         if (p != nullptr && p->device() != x.device()) refuse_value("linear: ", name, " is on ", p->device(), ", x on ", x.device());
+    refuse_unseen("linear", {&x, &weight, rest[1].second, rest[2].second, rest[3].second});
     if (!x.is_cuda()) refuse_value("linear: x is on ", x.device(), "; a CUDA device is needed");
     const c10::cuda::CUDAGuard guard(x.device());
     if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() || wants_grad(bias) || wants_grad(residual) ||
@@ -384,6 +396,7 @@ Tensor layer_norm(const Tensor &x, const MaybeTensor &weight, const MaybeTensor 
     } else if (rows_per_group) {
         refuse_value("layer_norm: rows_per_group without weight or bias");
     }
+    refuse_unseen("layer_norm", {&x, weight ? &*weight : nullptr, bias ? &*bias : nullptr});
     if (!x.is_cuda()) refuse_value("layer_norm: x is on ", x.device(), "; a CUDA device is needed");
     const c10::cuda::CUDAGuard guard(x.device());
     if (at::GradMode::is_enabled() && (x.requires_grad() || wants_grad(weight) || wants_grad(bias)))

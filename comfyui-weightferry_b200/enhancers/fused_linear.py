@@ -22,7 +22,7 @@ def linear(x, weight, bias=None, activation="none", residual=None, gate=None, ro
     holds for rows g * rows_per_group .. of x (rows_per_group: all rows divided evenly where it is not given; the last
     group may be short). All of one type, bfloat16 or float16, on one CUDA device; any strides (rows whose pitch is a
     multiple of 8 values are read in place, others are copied first). activation: a name of ``ACTIVATIONS``. Returns a
-    new contiguous [..., n]. Differentiable once in every tensor."""
+    new contiguous [..., n]. Differentiable once in every tensor, in reverse mode; tangents and traces raise NotImplementedError."""
     return (_ext._ops or _ext.ops()).linear(x, weight, bias, activation, residual, gate, rows_per_group)
 
 

@@ -16,5 +16,6 @@ def layer_norm(x, weight=None, bias=None, eps=1e-6, rows_per_group=None):
 
     weight and bias: None, [d], or [groups, d] whose row g holds for rows g * rows_per_group .. of x (rows_per_group: all
     rows divided evenly where it is not given; the last group may be short); of x's type or float32, both alike. Returns a
-    new contiguous tensor of x's shape and type. Differentiable once in x, weight and bias."""
+    new contiguous tensor of x's shape and type. Differentiable once in x, weight and bias, in reverse mode; tangents and traces
+    raise NotImplementedError."""
     return (_ext._ops or _ext.ops()).layer_norm(x, weight, bias, eps, rows_per_group)
