@@ -71,6 +71,7 @@ SIGNATURES = {
     "wf_w8a8_linear_noalloc": (ctypes.c_int, [ctypes.c_void_p] * 4 + [ctypes.c_int64] * 3 + [ctypes.c_void_p]),
     "wf_linear": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
     "wf_linear_backward_workspace": (ctypes.c_int64, [ctypes.c_int64] * 3),
+    "wf_linear_backward_needs": (ctypes.c_int64, [ctypes.c_void_p]),
     "wf_linear_backward": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
     "wf_linear_status": (ctypes.c_int, [ctypes.POINTER(ctypes.c_int)]),
     "wf_linear_set_wait_limit": (ctypes.c_int, [ctypes.c_uint64]),

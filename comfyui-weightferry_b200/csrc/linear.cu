@@ -1158,10 +1158,26 @@ extern "C" WF_API int wf_linear(const wf_linear_args *args, wf_stream_t stream) 
     return run_product<false, false>(p, e, a.type, reinterpret_cast<cudaStream_t>(stream));
 }
 
+namespace wf {
+namespace {
+// Whether a backward pass writes dz: the products read dy itself where dz is dy and TMA can read it.
+bool makes_dz(const wf_linear_grad_args &a) {
+    return (a.dx || a.dw) && (a.act != WF_ACT_NONE || a.gate || !operand_ok(a.dy, a.n, a.lddy));
+}
+int64_t backward_bytes(const wf_linear_grad_args &a) { return (makes_dz(a) ? dz_bytes(a.m, a.n) : 0) + linear_grad_bytes(a); }
+}  // namespace
+}  // namespace wf
+
 extern "C" WF_API int64_t wf_linear_backward_workspace(int64_t m, int64_t n, int64_t rows_per_group) {
     using namespace wf;
     if (!sizes_ok(m, n, 1) || m < 1 || n < 1 || rows_per_group < 1) return 0;
-    return dz_bytes(m, n) + linear_grad_workspace(m, n, rows_per_group);
+    return dz_bytes(m, n) + linear_grad_most_bytes(m, n, rows_per_group);
+}
+
+extern "C" WF_API int64_t wf_linear_backward_needs(const wf_linear_grad_args *args) {
+    using namespace wf;
+    if (args == nullptr || !sizes_ok(args->m, args->n, 1) || args->m < 1 || args->n < 1 || args->rows_per_group < 1) return 0;
+    return backward_bytes(*args);
 }
 
 extern "C" WF_API int wf_linear_backward(const wf_linear_grad_args *args, wf_stream_t stream) {
@@ -1178,10 +1194,8 @@ extern "C" WF_API int wf_linear_backward(const wf_linear_grad_args *args, wf_str
     if (a.dx && (!operand_ok(a.w, a.k, a.ldw) || a.lddx < a.k || !aligned_to(a.dx, 2))) return WF_ERR_ARG;
     if (a.dw && (!operand_ok(a.x, a.k, a.ldx) || a.lddw < a.k || !aligned_to(a.dw, 2))) return WF_ERR_ARG;
     if (!a.dx && !a.dw && !a.db && !a.dg) return WF_OK;
-    // the products read dy itself where dz is dy and TMA can read it
-    const bool make_dz = (a.dx || a.dw) && (a.act != WF_ACT_NONE || a.gate || !operand_ok(a.dy, a.n, a.lddy));
-    if ((make_dz || a.db || a.dg) && (!a.workspace || !aligned_to(a.workspace, 16) ||
-                                      a.workspace_bytes < wf_linear_backward_workspace(a.m, a.n, a.rows_per_group)))
+    const bool make_dz = makes_dz(a);
+    if ((make_dz || a.db || a.dg) && (!a.workspace || !aligned_to(a.workspace, 16) || a.workspace_bytes < backward_bytes(a)))
         return WF_ERR_ARG;
     int rc = check_device();
     int *word = nullptr;
@@ -1195,7 +1209,7 @@ extern "C" WF_API int wf_linear_backward(const wf_linear_grad_args *args, wf_str
             dz = a.workspace;
             lddz = (a.n + 7) / 8 * 8;
         }
-        float *part = reinterpret_cast<float *>(static_cast<char *>(a.workspace) + dz_bytes(a.m, a.n));
+        float *part = reinterpret_cast<float *>(static_cast<char *>(a.workspace) + (make_dz ? dz_bytes(a.m, a.n) : 0));
         rc = linear_grad(a, make_dz ? a.workspace : nullptr, lddz, part, st);
         if (rc != WF_OK) return rc;
     }

@@ -256,16 +256,21 @@ int dispatch_grad_type(const LinearGradArgs &a, int act, int z_type, cudaStream_
 // rows of a group as the kernel takes them: all of them where no group matters
 static int64_t grad_group(const wf_linear_grad_args &g) { return g.gate || g.dg ? g.rows_per_group : g.m; }
 
-int64_t linear_grad_workspace(int64_t m, int64_t n, int64_t rows_per_group) {
-    const RowSplit s = grad_split(m, n, rows_per_group);
-    return (s.blocks() + s.partial_rows()) * n * static_cast<int64_t>(sizeof(float));
+int64_t linear_grad_bytes(const wf_linear_grad_args &g) {
+    const RowSplit s = grad_split(g.m, g.n, grad_group(g));
+    return ((g.db ? s.blocks() : 0) + (g.dg ? s.partial_rows() : 0)) * g.n * static_cast<int64_t>(sizeof(float));
+}
+
+int64_t linear_grad_most_bytes(int64_t m, int64_t n, int64_t rows_per_group) {
+    const RowSplit grouped = grad_split(m, n, rows_per_group), plain = grad_split(m, n, m);
+    return std::max(grouped.blocks() + grouped.partial_rows(), plain.blocks()) * n * static_cast<int64_t>(sizeof(float));
 }
 
 int linear_grad(const wf_linear_grad_args &g, void *dz, int64_t lddz, float *part, cudaStream_t stream) {
     const RowSplit split = grad_split(g.m, g.n, grad_group(g));
     const bool vec = g.n % 8 == 0 && aligned_to(g.dy, 16) && g.lddy % 8 == 0 && (!dz || (aligned_to(dz, 16) && lddz % 8 == 0)) &&
                      (!g.z || (aligned_to(g.z, 16) && g.ldz % 8 == 0));
-    LinearGradArgs a{g.dy, g.z, g.gate, dz, g.db ? part : nullptr, g.dg ? part + split.blocks() * g.n : nullptr, g.lddy,
+    LinearGradArgs a{g.dy, g.z, g.gate, dz, g.db ? part : nullptr, g.dg ? part + (g.db ? split.blocks() * g.n : 0) : nullptr, g.lddy,
                      g.ldz, lddz, g.n, split, vec};
     const int rc = g.type == WF_BF16 ? dispatch_grad_type<WF_BF16>(a, g.act, g.z_type, stream)
                                      : dispatch_grad_type<WF_F16>(a, g.act, g.z_type, stream);

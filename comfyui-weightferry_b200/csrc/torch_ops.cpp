@@ -215,8 +215,6 @@ struct LinearNode : public torch::autograd::Function<LinearNode> {
             const at::AutoGradMode off(false);
             const auto [dy2, lddy] = as_rows(dy.dim() == 2 ? dy : dy.reshape({m, n}));
             wf_linear_grad_args a = {};
-            a.workspace_bytes = wf_linear_backward_workspace(m, n, rpg);
-            const Tensor work = at::empty({a.workspace_bytes}, opt.dtype(at::kByte));
             const at::ScalarType type = dy.scalar_type();
             Tensor gate, z;
             if (saved[0].defined()) check_saved("linear: x", saved[0], {m, d[5]}, type, dy.device());
@@ -231,10 +229,13 @@ struct LinearNode : public torch::autograd::Function<LinearNode> {
             }
             const auto [xo, wo] = as_operands(saved[0], saved[1]);
             a.dy = dy2.const_data_ptr(), a.x = ptr(xo.t), a.w = ptr(wo.t), a.z = ptr(z), a.gate = ptr(gate);
-            a.dx = mut(out[0]), a.dw = mut(out[1]), a.db = mut(out[2]), a.dg = mut(out[4]), a.workspace = work.mutable_data_ptr();
+            a.dx = mut(out[0]), a.dw = mut(out[1]), a.db = mut(out[2]), a.dg = mut(out[4]);
             a.lddy = lddy, a.ldx = xo.ld, a.ldw = wo.ld, a.lddx = k, a.lddw = k, a.rows_per_group = rpg;
             a.m = m, a.n = n, a.k = k, a.act = static_cast<int32_t>(act), a.type = code_of(type);
             a.z_type = z.defined() ? code_of(z.scalar_type()) : 0;
+            a.workspace_bytes = wf_linear_backward_needs(&a);
+            const Tensor work = a.workspace_bytes ? at::empty({a.workspace_bytes}, opt.dtype(at::kByte)) : Tensor();
+            a.workspace = mut(work);
             check(wf_linear_backward(&a, stream_of(dy)), "wf_linear_backward");
         }
         only_once(out);

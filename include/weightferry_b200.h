@@ -217,8 +217,9 @@ WF_API int wf_linear(const wf_linear_args *args, wf_stream_t stream);
  *   dx [m, k] = dz w,  dw [n, k] = dz^T x,  db [n] = sum of dz over the rows,  dg [groups, n] = sum of dy * act(z) over
  * each group's rows. Each result may be NULL, and so may what it does not need (x without dw, w without dx, z where act
  * is WF_ACT_NONE and dg NULL). dz is rounded to `type` for the two products; the sums are float32, of unrounded values,
- * in a fixed order. m, n, k >= 1. workspace (16-byte aligned) holds wf_linear_backward_workspace bytes for the duration
- * of the call's work on the stream: dz, unless the products can read dy itself, and partial sums. */
+ * in a fixed order. m, n, k >= 1. workspace (16-byte aligned) is used for the duration of the call's work on the stream: dz,
+ * unless the products can read dy itself, and partial sums. wf_linear_backward_needs(args) is what it takes (all but
+ * workspace and workspace_bytes set; 0: no workspace); wf_linear_backward_workspace, for sizes alone, the most of any call. */
 typedef struct wf_linear_grad_args {
     const void *dy, *x, *w, *z, *gate;
     void *dx, *dw, *db, *dg, *workspace;
@@ -226,6 +227,7 @@ typedef struct wf_linear_grad_args {
     int32_t act, type, z_type, reserved;
 } wf_linear_grad_args;
 WF_API int64_t wf_linear_backward_workspace(int64_t m, int64_t n, int64_t rows_per_group);
+WF_API int64_t wf_linear_backward_needs(const wf_linear_grad_args *args);
 WF_API int wf_linear_backward(const wf_linear_grad_args *args, wf_stream_t stream);
 
 /* Status word of the dense linear layer's kernels, as wf_w8a8_gemm_status. A kernel whose wait ran out of time fills what it
