@@ -6,12 +6,15 @@ library's status string. Every launch takes the caller's current CUDA stream, as
 
 import ctypes
 import importlib.util
+import json
 import os
+import sysconfig
 import threading
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "_lib", "libweightferry_b200.so")
 OPS_PATH = os.path.join(HERE, "_lib", "wf_torch.so")
+ABI_PATH = os.path.join(HERE, "_lib", "wf_torch.abi")  # what the module was built for (csrc/build.py)
 
 WF_F16, WF_BF16, WF_F32 = 0, 1, 2
 
@@ -105,6 +108,20 @@ def _load():
     return _lib
 
 
+def _check_abi():
+    """Raise rather than load a module that was built for another PyTorch or Python."""
+    import torch
+    try:
+        with open(ABI_PATH) as f:
+            built = json.load(f)
+    except (OSError, ValueError):
+        return  # not written down
+    here = {"torch": torch.__version__, "python": sysconfig.get_config_var("EXT_SUFFIX")}
+    if any(built.get(k) != v for k, v in here.items()):
+        raise ExtensionMissing(f"weightferry_b200 operations were built for {built}, this process is {here} "
+                               "(run __graft_entry__.build())")
+
+
 def ops():
     """The module of the differentiable operations (csrc/torch_ops.cpp; raises ExtensionMissing when it is not built)."""
     global _ops
@@ -116,6 +133,7 @@ def ops():
             if not os.path.exists(OPS_PATH):
                 raise ExtensionMissing(f"weightferry_b200 operations not built: {OPS_PATH} is missing "
                                        "(run __graft_entry__.build())")
+            _check_abi()
             spec = importlib.util.spec_from_file_location("wf_torch", OPS_PATH)
             mod = importlib.util.module_from_spec(spec)
             spec.loader.exec_module(mod)

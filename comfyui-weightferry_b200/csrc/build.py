@@ -4,7 +4,8 @@ Every .cu file of this folder is compiled for sm_100a only (``-gencode arch=comp
 into one shared library with the CUDA runtime linked dynamically, so that the process shares one runtime (and one
 stream namespace) with PyTorch. Objects go to ``csrc/_build/``, the library to ``<package>/_lib/``. A file is
 recompiled only when it, or a header, is newer than its object. torch_ops.cpp (the operations with autograd nodes) becomes
-a Python module of its own beside the library, which it links; it is host code against PyTorch's headers.
+a Python module of its own beside the library, which it links; it is host code against PyTorch's headers, and rebuilt as well
+when the PyTorch, the Python or the C++ ABI that it was built for (written down beside it) is another.
 
     python comfyui-weightferry_b200/csrc/build.py [--force] [-j N]
 """
@@ -14,6 +15,7 @@ import glob
 import os
 import shutil
 import importlib.util
+import json
 import subprocess
 import sys
 import sysconfig
@@ -27,6 +29,7 @@ OBJ_DIR = os.path.join(HERE, "_build")
 LIB_DIR = os.path.join(PKG, "_lib")
 LIB_NAME = "libweightferry_b200.so"
 OPS_NAME = "wf_torch.so"
+ABI_NAME = "wf_torch.abi"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -53,11 +56,27 @@ def _torch_dir():
     return os.path.dirname(spec.origin)
 
 
+def _ops_abi():
+    """What the module is bound to beside its sources."""
+    import torch
+    return {"torch": torch.__version__, "python": sysconfig.get_config_var("EXT_SUFFIX"),
+            "cxx11_abi": int(torch.compiled_with_cxx11_abi())}
+
+
+def _other_abi(path):
+    """The module was built for another PyTorch, Python or C++ ABI than this process's, or for none that is known."""
+    try:
+        with open(path) as f:
+            return json.load(f) != _ops_abi()
+    except (OSError, ValueError):
+        return True
+
+
 def _cxx_cmd(nvcc, src, obj):
     torch = _torch_dir()
     inc = [os.path.join(torch, "include"), os.path.join(torch, "include", "torch", "csrc", "api", "include"),
            sysconfig.get_paths()["include"], os.path.join(_cuda_home(nvcc), "include")]
-    cmd = ["g++", "-c", src, "-o", obj, "-fPIC", "-O2", "-std=c++17", "-fvisibility=hidden", "-D_GLIBCXX_USE_CXX11_ABI=1",
+    cmd = ["g++", "-c", src, "-o", obj, "-fPIC", "-O2", "-std=c++17", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={_ops_abi()['cxx11_abi']}",
            "-I", INCLUDE]
     for d in inc:
         cmd += ["-isystem", d]
@@ -92,7 +111,8 @@ def build(force=False, jobs=None, verbose=False):
 
     ops_src, ops_obj = os.path.join(HERE, "torch_ops.cpp"), os.path.join(OBJ_DIR, "torch_ops.o")
     api_header = os.path.getmtime(os.path.join(INCLUDE, "weightferry_b200.h"))
-    if force or _stale(ops_src, ops_obj, api_header):
+    abi_path = os.path.join(LIB_DIR, ABI_NAME)
+    if force or _stale(ops_src, ops_obj, api_header) or _other_abi(abi_path):
         todo.insert(0, (ops_src, ops_obj))
 
     def compile_one(pair):
@@ -128,6 +148,8 @@ def build(force=False, jobs=None, verbose=False):
         if res.returncode != 0:
             raise RuntimeError(f"link of {OPS_NAME} failed:\n{res.stdout}\n{res.stderr}")
         os.replace(ops + ".tmp", ops)
+        with open(abi_path, "w") as f:
+            json.dump(_ops_abi(), f)
     return lib
 
 
