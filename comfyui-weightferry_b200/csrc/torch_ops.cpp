@@ -13,7 +13,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <c10/core/AutogradState.h>
-#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
 #include <optional>
@@ -116,18 +116,25 @@ int64_t group_rows(const char *what, const Tensor &p, int64_t m, const std::opti
     return *given;
 }
 
-// Inside a backward pass that is itself recorded (create_graph): gradients that raise when they are differentiated.
-void only_once(variable_list &grads) {
+// What a gradient depends on, when it is itself recorded (create_graph): raises for whoever asks how.
+struct Refusal : public torch::autograd::Node {
+    explicit Refusal(torch::autograd::edge_list &&next) : Node(std::move(next)) {}
+    variable_list apply(variable_list &&) override { TORCH_CHECK(false, "this gradient cannot be differentiated again"); }
+};
+
+// Ties the fresh gradients of a recorded backward pass to dy and to everything that the forward pass was given, so that no way
+// of differentiating them finds them constant.
+void only_once(variable_list &grads, const Tensor &dy) {
     if (!at::GradMode::is_enabled()) return;
-    variable_list live;
-    for (const Tensor &g : grads)
-        if (g.defined()) live.push_back(g.detach().set_requires_grad(true));
-    auto error = std::make_shared<torch::autograd::DelayedError>("this gradient cannot be differentiated again",
-                                                                 static_cast<int64_t>(live.size()));
-    live = (*error)(std::move(live));
-    size_t i = 0;
-    for (Tensor &g : grads)
-        if (g.defined()) g = live[i++];
+    torch::autograd::edge_list next{torch::autograd::impl::gradient_edge(dy)};
+    if (const auto node = torch::autograd::get_current_node())
+        next.insert(next.end(), node->next_edges().begin(), node->next_edges().end());
+    std::shared_ptr<Refusal> refusal;
+    for (const Tensor &g : grads) {
+        if (!g.defined() || g.is_same(dy)) continue;  // the residual's gradient is dy
+        if (refusal == nullptr) refusal = std::shared_ptr<Refusal>(new Refusal(std::move(next)), torch::autograd::deleteNode);
+        torch::autograd::set_history(g, refusal);
+    }
 }
 
 // Tangents and traces, which the operations would drop without a word: their outputs come out of kernels that neither sees.
@@ -238,7 +245,7 @@ struct LinearNode : public torch::autograd::Function<LinearNode> {
             a.workspace = mut(work);
             check(wf_linear_backward(&a, stream_of(dy)), "wf_linear_backward");
         }
-        only_once(out);
+        only_once(out, dy);
         return out;
     }
 };
@@ -367,7 +374,7 @@ struct NormNode : public torch::autograd::Function<NormNode> {
             a.lddy = lddy, a.ldx = ldx, a.lddx = d, a.rows = m, a.d = d, a.rows_per_group = rpg;
             check(wf_layer_norm_backward(&a, stream_of(dy)), "wf_layer_norm_backward");
         }
-        only_once(out);
+        only_once(out, dy);
         return out;
     }
 };
