@@ -13,6 +13,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <c10/core/AutogradState.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
@@ -139,7 +140,10 @@ void only_once(variable_list &grads, const Tensor &dy) {
 
 // Tangents and traces, which the operations would drop without a word: their outputs come out of kernels that neither sees.
 void refuse_unseen(const char *what, std::initializer_list<const Tensor *> tensors) {
-    TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing(), what, ": a call cannot be traced");
+    using Modes = c10::impl::TorchDispatchModeTLS;
+    using Key = c10::impl::TorchDispatchModeKey;
+    TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing() && !Modes::get_mode(Key::PROXY) && !Modes::get_mode(Key::FAKE), what,
+                                ": a call cannot be traced");
     if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
     for (const Tensor *t : tensors)
         TORCH_CHECK_NOT_IMPLEMENTED(t == nullptr || !t->_fw_grad(0).defined(), what, ": no forward-mode derivatives");
@@ -254,6 +258,7 @@ constexpr const char *kActivations[] = {"none", "relu", "silu", "gelu", "gelu_ta
 
 Tensor linear(const Tensor &x, const Tensor &weight, const MaybeTensor &bias, const std::string &activation,
               const MaybeTensor &residual, const MaybeTensor &gate, const std::optional<int64_t> &rows_per_group) {
+    refuse_unseen("linear", {&x, &weight, bias ? &*bias : nullptr, residual ? &*residual : nullptr, gate ? &*gate : nullptr});
     const at::ScalarType t = x.scalar_type();
     if (t != at::kBFloat16 && t != at::kHalf) refuse_type("linear: x is ", t, "; bfloat16 or float16 is needed");
     int64_t act = 0;
@@ -283,7 +288,6 @@ Tensor linear(const Tensor &x, const Tensor &weight, const MaybeTensor &bias, co
     }
     for (const auto &[name, p] : rest)
         if (p != nullptr && p->device() != x.device()) refuse_value("linear: ", name, " is on ", p->device(), ", x on ", x.device());
-    refuse_unseen("linear", {&x, &weight, rest[1].second, rest[2].second, rest[3].second});
     if (!x.is_cuda()) refuse_value("linear: x is on ", x.device(), "; a CUDA device is needed");
     const c10::cuda::CUDAGuard guard(x.device());
     if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() || wants_grad(bias) || wants_grad(residual) ||
@@ -381,6 +385,7 @@ struct NormNode : public torch::autograd::Function<NormNode> {
 
 Tensor layer_norm(const Tensor &x, const MaybeTensor &weight, const MaybeTensor &bias, double eps,
                   const std::optional<int64_t> &rows_per_group) {
+    refuse_unseen("layer_norm", {&x, weight ? &*weight : nullptr, bias ? &*bias : nullptr});
     const at::ScalarType t = x.scalar_type();
     if (t != at::kBFloat16 && t != at::kHalf && t != at::kFloat)
         refuse_type("layer_norm: x is ", t, "; bfloat16, float16 or float32 is needed");
@@ -404,7 +409,6 @@ Tensor layer_norm(const Tensor &x, const MaybeTensor &weight, const MaybeTensor 
     } else if (rows_per_group) {
         refuse_value("layer_norm: rows_per_group without weight or bias");
     }
-    refuse_unseen("layer_norm", {&x, weight ? &*weight : nullptr, bias ? &*bias : nullptr});
     if (!x.is_cuda()) refuse_value("layer_norm: x is on ", x.device(), "; a CUDA device is needed");
     const c10::cuda::CUDAGuard guard(x.device());
     if (at::GradMode::is_enabled() && (x.requires_grad() || wants_grad(weight) || wants_grad(bias)))
