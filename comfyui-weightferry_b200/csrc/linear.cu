@@ -662,7 +662,7 @@ __device__ __forceinline__ void finish_half(float (&v)[32], Warp32 &w, const Epi
     }
 }
 
-// After a wait that ran out of time: NaN in an epilogue warp's rows of every tile that it has not written.
+// After a wait that ran out of time: NaN in an epilogue warp's rows of every tile that it has not written, and in the kept z's.
 __device__ __noinline__ void fill_nan(const Epilogue &e, int tile, int n_clusters, int m, int n, int band, int rank, int quarter, int half) {
     const int tiles_m = (m + 255) / 256, tiles_n = (n + BN - 1) / BN, lane = threadIdx.x & 31;
     for (; tile < tiles_m * tiles_n; tile += n_clusters) {
@@ -670,8 +670,11 @@ __device__ __noinline__ void fill_nan(const Epilogue &e, int tile, int n_cluster
         tile_coords(tile, tiles_m, tiles_n, band, mi, ni);
         const int row0 = mi * 256 + rank * 128 + quarter * 32, col0 = ni * BN + half * (BN / 2);
         for (int row = row0; row < min(row0 + 32, m); ++row)
-            for (int col = col0 + lane; col < min(col0 + BN / 2, n); col += 32)
+            for (int col = col0 + lane; col < min(col0 + BN / 2, n); col += 32) {
                 static_cast<uint16_t *>(e.out)[row * e.ld_out + col] = 0x7FFF;  // bf16's and f16's
+                if (e.keep == KEEP_F32) static_cast<uint32_t *>(e.kept)[row * e.ld_kept + col] = 0x7FFFFFFFu;
+                else if (e.keep != KEEP_NONE) static_cast<uint16_t *>(e.kept)[row * e.ld_kept + col] = 0x7FFF;
+            }
     }
 }
 

@@ -86,3 +86,33 @@ print("ok")
     res = subprocess.run(["timeout", "-k", "10", "200", sys.executable, "-c", code], cwd=REPO, capture_output=True, text=True,
                          env=dict(os.environ))
     assert res.returncode == 0 and res.stdout.endswith("ok\n"), res.stdout[-1000:] + res.stderr[-2000:]
+
+
+@pytest.mark.parametrize("m,k,n", [(24, 32768, 1024), (4096, 8192, 2048), (4096, 8192, 2041)])
+@pytest.mark.parametrize("z_name", ["float16", "float32"])
+def test_expired_waits_leave_nan_in_the_kept_values(cuda, m, k, n, z_name):
+    """z, too, is what a whole run leaves or NaN."""
+    import torch
+    import dense_cabi
+    x = torch.randn((m, k), device="cuda").bfloat16()
+    w = (torch.randn((n, k), device="cuda") * 0.02).bfloat16()
+    up = (n + 7) // 8 * 8
+
+    def run():
+        y = torch.full((m, n), -7.0, device="cuda", dtype=torch.bfloat16)
+        z = torch.full((m, up), -7.0, device="cuda", dtype=getattr(torch, z_name))
+        dense_cabi.launch("wf_linear", dense_cabi.LINEAR_ARGS.pack(
+            x.data_ptr(), w.data_ptr(), 0, 0, 0, y.data_ptr(), z.data_ptr(), k, k, 0, n, up, 1, m, n, k, 3, 1,
+            {"float16": 0, "float32": 2}[z_name], 0))
+        torch.cuda.synchronize()
+        return y, z[:, :n]
+    want = run()
+    _limit(1)
+    try:
+        got = run()
+    finally:
+        _limit(0)
+    assert wf("enhancers.fused_linear").status() in (1, 2, 3)
+    for a, b in zip(got, want):
+        bad = torch.isnan(a)
+        assert bool(bad.any()) and torch.equal(a[~bad], b[~bad])
